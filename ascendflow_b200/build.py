@@ -17,7 +17,9 @@ from .diagnostics import ErrorKind, require
 
 PACKAGE = Path(__file__).resolve().parent
 ROOT = PACKAGE.parent
-SOURCES = (PACKAGE / "csrc" / "sparse_mla_abi.cu", PACKAGE / "csrc" / "sparse_mla_neighbours.cu")
+SOURCES = tuple(PACKAGE / "csrc" / name for name in (
+    "sparse_mla_abi.cu", "sparse_mla_neighbours.cu", "latent_rotary.cu", "latent_attention.cu", "latent_prefill.cu"))
+HEADERS = (ROOT / "include" / "sparse_mla.h", ROOT / "include" / "latent.h")
 LIBRARY = PACKAGE / "lib" / "libsparse_mla_sm100a.so"
 STAMP = LIBRARY.with_suffix(".stamp")
 FLAGS = (
@@ -28,7 +30,7 @@ FLAGS = (
 
 def _identity():
     digest = hashlib.sha256(" ".join(FLAGS).encode())
-    for path in sorted((PACKAGE / "csrc").glob("*")) + [ROOT / "include" / "sparse_mla.h"]:
+    for path in [*sorted((PACKAGE / "csrc").glob("*")), *HEADERS]:
         digest.update(path.name.encode())
         digest.update(path.read_bytes())
     return digest.hexdigest()
@@ -50,7 +52,7 @@ def build_library(force=False, verbose=False):
     require(compiler is not None, "nvcc not found; cannot build the sm_100a library",
             kind=ErrorKind.RESOURCE)
     LIBRARY.parent.mkdir(parents=True, exist_ok=True)
-    command = [compiler, *FLAGS, *(["-Xptxas", "-v"] if verbose else []), "-o", str(LIBRARY),
+    command = [compiler, *FLAGS, "--threads", "0", *(["-Xptxas", "-v"] if verbose else []), "-o", str(LIBRARY),
                *map(str, SOURCES)]
     result = subprocess.run(command, capture_output=True, text=True)
     require(result.returncode == 0, "nvcc failed:\n" + result.stderr[-4000:], kind=ErrorKind.RESOURCE)
@@ -63,7 +65,7 @@ def build_library(force=False, verbose=False):
     return LIBRARY
 
 
-HOST_SOURCE = PACKAGE / "csrc" / "host_calls.cpp"
+HOST_SOURCES = (PACKAGE / "csrc" / "host_calls.cpp", PACKAGE / "csrc" / "latent_calls.cpp")
 HOST_LIBRARY = PACKAGE / "lib" / "_host_calls.so"
 HOST_STAMP = HOST_LIBRARY.with_suffix(".stamp")
 
@@ -82,7 +84,7 @@ def _host_command(output):
     abi = f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}"
     includes = [f"-I{path}" for path in (*cpp_extension.include_paths("cuda"), sysconfig.get_paths()["include"])]
     libraries = [f"-L{path}" for path in cpp_extension.library_paths("cuda")]
-    return [os.environ.get("CXX", "g++"), *HOST_FLAGS, abi, *includes, "-o", str(output), str(HOST_SOURCE), *libraries, *HOST_LINKED]
+    return [os.environ.get("CXX", "g++"), *HOST_FLAGS, abi, *includes, "-o", str(output), *map(str, HOST_SOURCES), *libraries, *HOST_LINKED]
 
 
 def _host_identity():
@@ -93,7 +95,7 @@ def _host_identity():
 
     parts = (torch.__version__, torch.__file__, sys.version, *HOST_FLAGS, *HOST_LINKED)
     digest = hashlib.sha256("\n".join(parts).encode())
-    for path in (HOST_SOURCE, ROOT / "include" / "sparse_mla.h"):
+    for path in (*HOST_SOURCES, PACKAGE / "csrc" / "host_calls.h", *HEADERS):
         digest.update(path.read_bytes())
     return digest.hexdigest()
 

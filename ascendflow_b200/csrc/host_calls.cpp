@@ -31,6 +31,7 @@
 #include <vector>
 
 #include "../../include/sparse_mla.h"
+#include "host_calls.h"
 
 namespace {
 
@@ -489,4 +490,16 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host_calls", nullptr, -1, methods
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__host_calls() { return PyModule_Create(&module); }
+cudaError_t ascendflow_host::status_block(const c10::cuda::CUDAStream& stream, at::Tensor* kept, void** block) {
+  bool capturing = false;
+  if (const cudaError_t error = is_capturing(stream.stream(), &capturing)) return error;
+  if (capturing) return captured_block(stream.device_index(), block);
+  *block = (*kept = workspace_for(stream)).mutable_data_ptr();
+  return cudaSuccess;
+}
+
+PyMODINIT_FUNC PyInit__host_calls() {
+  PyObject* created = PyModule_Create(&module);
+  if (created != nullptr && PyModule_AddFunctions(created, ascendflow_host::latent_methods) != 0) Py_CLEAR(created);
+  return created;
+}

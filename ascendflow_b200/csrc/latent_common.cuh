@@ -1,0 +1,68 @@
+// What the kernels around dense latent attention share: storage types, the turn of a pair of features, reports.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/latent.h"
+#include "../../include/sparse_mla.h"
+#include "tcgen05_ptx.cuh"
+
+namespace latent {
+
+__device__ __forceinline__ void report(int32_t* status, int code, int token, int detail) {
+  if (atomicCAS(status, SPARSE_MLA_STATUS_OK, code) == SPARSE_MLA_STATUS_OK) {
+    status[1] = token;
+    status[2] = detail;
+  }
+}
+
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_float(float v) { return v; }
+template <typename T> __device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ float from_float(float v) { return v; }
+
+// Radians per position as a fraction of a turn, times 2^64: an angle is then a 64-bit product whose overflow is whole
+// turns, exact for every position (the fraction is rounded once, to 53 bits). A frequency that is no number is none.
+__device__ __forceinline__ uint64_t turns_of(double radians) {
+  double turns = radians * 0.15915494309189533577;  // 1 / (2 pi)
+  turns -= floor(turns);
+  return turns >= 0.0 && turns < 1.0 ? uint64_t(turns * 18446744073709551616.0) : 0;
+}
+// (cos, sin) of `position` such fractions, times `amplitude`. The signed upper word is the angle in 2^-32 turns, within half a turn.
+__device__ __forceinline__ float2 turn_of(int64_t position, uint64_t turns, float amplitude) {
+  const int32_t fraction = int32_t((uint64_t(position) * turns + (uint64_t(1) << 31)) >> 32);
+  float sine, cosine;
+  sincospif(float(fraction) * 4.656612873077393e-10f, &sine, &cosine);  // 2^-31: half turns
+  return make_float2(cosine * amplitude, sine * amplitude);
+}
+
+// The request that owns `token` (binary search; empty requests are skipped), or -1 in front of the first and behind the last.
+__device__ __forceinline__ int request_of(const int32_t* cu, int batches, int token) {
+  if (token < __ldg(cu) || token >= __ldg(cu + batches)) return -1;
+  int lo = 0, hi = batches;  // cu[lo] <= token < cu[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (__ldg(cu + mid) <= token) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+inline int multiprocessors() {
+  static int cached[64] = {0};  // plain words written with the same value by whoever gets there first
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return 148;
+  if (cached[device] == 0) {
+    int count = 0;
+    if (cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || count <= 0) count = 148;
+    cached[device] = count;
+  }
+  return cached[device];
+}
+
+}  // namespace latent

@@ -1,0 +1,177 @@
+// Rotary positions: the queries' rope part, and a step's new rows on their way into the paged cache.
+//
+// y1 = a (x1 cos t - x2 sin t), y2 = a (x1 sin t + x2 cos t) with t = position * inv_freq[pair], in FP32, rounded once.
+// Angles are formed as fractions of a turn in 64-bit whole numbers (`turns_of`), so far positions cost nothing
+// and lose nothing; cosine and sine come from the fraction directly.
+#include "latent_common.cuh"
+
+namespace latent {
+namespace {
+
+constexpr int kThreads = 256;
+
+template <typename T> struct Vector { static constexpr int kElements = 16 / int(sizeof(T)); };
+
+// Eight elements as FP32 from 16-byte aligned memory, and back.
+template <typename T>
+__device__ __forceinline__ void load8(const T* at, float (&v)[8]) {
+  uint4 words[8 * sizeof(T) / 16];
+#pragma unroll
+  for (int i = 0; i < int(8 * sizeof(T) / 16); ++i) words[i] = *reinterpret_cast<const uint4*>(at + i * Vector<T>::kElements);
+  const T* values = reinterpret_cast<const T*>(words);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = to_float(values[i]);
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* at, const float (&v)[8]) {
+  uint4 words[8 * sizeof(T) / 16];
+  T* values = reinterpret_cast<T*>(words);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) values[i] = from_float<T>(v[i]);
+#pragma unroll
+  for (int i = 0; i < int(8 * sizeof(T) / 16); ++i) *reinterpret_cast<uint4*>(at + i * Vector<T>::kElements) = words[i];
+}
+
+struct RotaryParams {
+  latent_rotary_call c;
+  int tokens_per_block, rotated_units, units;  // of a head: units of eight pairs, and besides of eight copied features
+};
+
+// A block takes a few whole tokens: their angles are worked out once for all heads. A thread turns eight pairs of a
+// head, or copies eight features of its part in front.
+template <typename T, bool kHalves>
+__global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p) {
+  extern __shared__ float2 turn[];  // [tokens_per_block][pairs]
+  const latent_rotary_call& c = p.c;
+  const int pairs = int(c.pairs), heads = int(c.heads);
+  sm100::wait_for_predecessor();
+  sm100::let_successor_start();
+  const int64_t first = int64_t(blockIdx.x) * p.tokens_per_block;
+  const int tokens = int(min(int64_t(p.tokens_per_block), c.tokens - first));
+  for (int i = threadIdx.x; i < tokens * pairs; i += kThreads) {
+    const int64_t token = first + i / pairs;
+    const int64_t position = c.positions64 ? static_cast<const int64_t*>(c.positions)[token] : static_cast<const int32_t*>(c.positions)[token];
+    const uint64_t turns = turns_of(__ldg(c.inv_freq + i % pairs));
+    turn[i] = turn_of(c.inverse ? -position : position, turns, float(c.amplitude));
+  }
+  __syncthreads();
+  const int per_token = heads * p.units;
+  const int front = int(c.features) - 2 * pairs;
+  for (int i = threadIdx.x; i < tokens * per_token; i += kThreads) {
+    const int token = i / per_token, rest = i - token * per_token, head = rest / p.units, unit = rest - head * p.units;
+    const T* x = static_cast<const T*>(c.x) + (first + token) * c.x_token + head * c.x_head;
+    T* out = static_cast<T*>(c.out) + (first + token) * c.out_token + head * c.out_head;
+    if (unit >= p.rotated_units) {
+      const int at = (unit - p.rotated_units) * 8;
+#pragma unroll
+      for (int k = 0; k < int(8 * sizeof(T) / 16); ++k)
+        reinterpret_cast<uint4*>(out + at)[k] = reinterpret_cast<const uint4*>(x + at)[k];
+      continue;
+    }
+    const float2* angle = turn + token * pairs + unit * 8;
+    const int low = front + (kHalves ? unit * 8 : unit * 16), high = low + (kHalves ? pairs : 8);
+    float a[8], b[8];
+    load8(x + low, a);
+    load8(x + high, b);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      // halves: pair k is (a[k], b[k]); neighbours: pairs 0-3 lie in a, 4-7 in b
+      float& u = kHalves ? a[k] : k < 4 ? a[2 * k] : b[2 * k - 8];
+      float& v = kHalves ? b[k] : k < 4 ? a[2 * k + 1] : b[2 * k - 7];
+      const float2 t = angle[k];
+      const float turned_u = u * t.x - v * t.y, turned_v = u * t.y + v * t.x;
+      u = turned_u;
+      v = turned_v;
+    }
+    store8(out + low, a);
+    store8(out + high, b);
+  }
+}
+
+// One warp per new row.
+template <typename T, bool kHalves>
+__global__ void __launch_bounds__(kThreads) append_kernel(const latent_append_call c) {
+  const int lane = threadIdx.x & 31;
+  sm100::wait_for_predecessor();
+  sm100::let_successor_start();
+  const int64_t token = int64_t(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
+  if (token >= c.tokens) return;
+  const int request = request_of(c.cu_seqlens_q, int(c.batches), int(token));
+  if (request < 0) return;
+  const int begin = __ldg(c.cu_seqlens_q + request), count = __ldg(c.cu_seqlens_q + request + 1) - begin;
+  const int64_t position = int64_t(__ldg(c.seqused_kv + request)) - count + (token - begin);
+  const int64_t column = position / c.page_rows;
+  int64_t page = -1;
+  if (position >= 0 && column < c.pages) page = __ldg(c.block_table + request * c.pages + column);
+  if (page < 0 || page >= c.blocks) {  // nowhere to put it: reported, not written
+    if (lane == 0) report(c.status, SPARSE_MLA_STATUS_BAD_PAGE, int(token), int(position));
+    return;
+  }
+  const int pairs = int(c.pairs), front = int(c.width) - 2 * pairs;
+  T* target = static_cast<T*>(c.cache) + (page * c.page_rows + position % c.page_rows) * c.width;
+  const T* latent = static_cast<const T*>(c.latent) + token * c.latent_token;
+  for (int at = lane * 8; at < front; at += 256) *reinterpret_cast<uint4*>(target + at) = *reinterpret_cast<const uint4*>(latent + at);
+  const T* rope = static_cast<const T*>(c.rope) + token * c.rope_token;
+  for (int i = lane; i < pairs; i += 32) {
+    const float2 t = turn_of(position, turns_of(__ldg(c.inv_freq + i)), float(c.amplitude));
+    const int low = kHalves ? i : 2 * i, high = kHalves ? i + pairs : 2 * i + 1;
+    const float u = to_float(rope[low]), v = to_float(rope[high]);
+    target[front + low] = from_float<T>(u * t.x - v * t.y);
+    target[front + high] = from_float<T>(u * t.y + v * t.x);
+  }
+}
+
+template <typename T>
+int launch_rotary(const RotaryParams& p, cudaStream_t stream) {
+  const int64_t blocks = (p.c.tokens + p.tokens_per_block - 1) / p.tokens_per_block;
+  const size_t bytes = size_t(p.tokens_per_block) * size_t(p.c.pairs) * sizeof(float2);
+  auto* kernel = p.c.layout ? rotary_kernel<T, true> : rotary_kernel<T, false>;
+  return int(sm100::launch_overlapped(kernel, int(blocks), kThreads, bytes, stream, p));
+}
+
+template <typename T>
+int launch_append(const latent_append_call& c, cudaStream_t stream) {
+  const int64_t blocks = (c.tokens + kThreads / 32 - 1) / (kThreads / 32);
+  return int(sm100::launch_overlapped(c.layout ? append_kernel<T, true> : append_kernel<T, false>, int(blocks), kThreads, 0, stream, c));
+}
+
+bool pairs_fit(int64_t pairs) { return pairs >= 8 && pairs <= LATENT_MOST_PAIRS && pairs % 8 == 0; }
+bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+}  // namespace
+}  // namespace latent
+
+extern "C" {
+
+int launch_latent_rotary(void* stream, const latent_rotary_call* call) {
+  using namespace latent;
+  const latent_rotary_call& c = *call;
+  const int size = c.type == LATENT_F32 ? 4 : 2;
+  if (c.type < LATENT_F16 || c.type > LATENT_F32 || !pairs_fit(c.pairs) || c.features < 2 * c.pairs || c.features % 8 != 0) return -1;
+  if (c.tokens < 0 || c.tokens > INT32_MAX || c.heads < 0 || c.heads > 65536 || c.features > 65536) return -1;
+  for (const int64_t stride : {c.x_token, c.x_head, c.out_token, c.out_head})
+    if (stride * size % 16 != 0) return -1;
+  if (!aligned(c.x) || !aligned(c.out)) return -1;
+  if (c.tokens == 0 || c.heads == 0) return 0;
+  RotaryParams p = {c, 1, int(c.pairs / 8), 0};
+  p.units = p.rotated_units + (c.x == c.out ? 0 : int(c.features - 2 * c.pairs) / 8);
+  const int64_t per_token = c.heads * p.units;
+  if (per_token * 32 > INT32_MAX) return -1;
+  // A block's threads take a unit each where a token has few; the angles of 32 tokens are 32 KiB at most.
+  p.tokens_per_block = int(per_token >= kThreads ? 1 : per_token * 32 >= kThreads ? kThreads / per_token : 32);
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return c.type == LATENT_F32 ? launch_rotary<float>(p, s) : c.type == LATENT_BF16 ? launch_rotary<__nv_bfloat16>(p, s) : launch_rotary<__half>(p, s);
+}
+
+int launch_latent_append(void* stream, const latent_append_call* call) {
+  using namespace latent;
+  const latent_append_call& c = *call;
+  if ((c.type != LATENT_F16 && c.type != LATENT_BF16) || !pairs_fit(c.pairs) || c.width < 2 * c.pairs || c.width % 8 != 0 || c.width > 65536) return -1;
+  if (c.batches < 0 || c.batches >= INT32_MAX || c.tokens < 0 || c.tokens > INT32_MAX || c.pages < 0 || c.blocks < 0 || c.page_rows < 1) return -1;
+  if (!aligned(c.latent) || c.latent_token % 8 != 0 || !aligned(c.cache) || c.status == nullptr) return -1;
+  if (c.tokens == 0 || c.batches == 0) return 0;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return c.type == LATENT_BF16 ? launch_append<__nv_bfloat16>(c, s) : launch_append<__half>(c, s);
+}
+
+}  // extern "C"

@@ -51,6 +51,11 @@ class _Unavailable:
     def cache_append(self, *arguments):
         return None
 
+    def rotary(self, *arguments):
+        return False
+
+    latent_append = latent_attention = latent_prefill = rotary
+
     def read_status(self):
         raise RuntimeError("the native host side is not available") from self.error
 
@@ -68,6 +73,7 @@ except (CompileError, ImportError, OSError) as error:
     calls = _Unavailable(error)
 _fallback = None
 _connected = False
+_latent_connected = False
 
 
 def set_fallback(function):
@@ -93,4 +99,21 @@ def connect():
         "launch_sparse_mla_kept_status", "launch_sparse_mla_topk_indices", "launch_sparse_mla_cache_append_flagged"))
     calls.configure(*addresses, _fallback)
     _connected = True
+    return True
+
+
+def connect_latent():
+    """The same for the operators around dense latent attention."""
+    global _latent_connected
+    if _latent_connected:
+        return False
+    if isinstance(calls, _Unavailable):
+        raise RuntimeError("the native host side is not available") from calls.error
+    from .build import library_path
+    from .runtime.torch import _library
+
+    library = _library(library_path())
+    calls.configure_latent(*(ct.cast(getattr(library, name), ct.c_void_p).value for name in (
+        "launch_latent_rotary", "launch_latent_append", "launch_latent_attention", "launch_latent_prefill", "workspace_size_latent_attention")))
+    _latent_connected = True
     return True
