@@ -1,60 +1,468 @@
 // Attention of prompts in expanded form: keys and values per head, and one rope key per token for all heads.
+//
+// out = softmax(scale [q] . [k | k_rope]) v per head, causal or not, over ragged requests. One block takes 256 query rows of a
+// head as two tiles of 128 and walks the keys in tiles of 128. All products run on tcgen05 with M = 128, N = 128: S = Q K^T from shared
+// memory (K = 192), O += P V with P from tensor memory (K = 128). While the softmax warps of one tile work, the products of
+// the other run.
+//
+//   warps 0-3, 4-7  softmax of tile 0 and 1: a thread owns a query row. Scores out of tensor memory, running reference and
+//                   sum in FP32, P (16 bits) over the scores' columns, output.
+//   warp 8          one thread issues the products.
+//   warp 9          one thread brings boxes of 64 features x 128 rows (16 KiB) by tensor copies into a ring of eight:
+//                   three of a key tile (128 features of the head, 64 of rope), two of a value tile, in the order of their use.
+//
+// Tensor memory: scores (P over their first half) of tile t in columns 128 t .. + 127, O of tile t in 256 + 128 t .. + 127.
+//
+// Rows of a value box behind the request's last key are cleared before they are multiplied: their weights are zero, but they
+// belong to other requests (or to nobody) and 0 x infinity would be a NaN. Scores of such keys are replaced, whatever they are.
 #include "latent_common.cuh"
+#include "latent_ptx.cuh"
 
 namespace latent {
-namespace {
+namespace prefill {
 
-// One warp per token and head: running maximum and sum, a key at a time.
-template <typename T>
-__global__ void __launch_bounds__(256) prefill_kernel(const latent_prefill_call c) {
-  const int lane = threadIdx.x & 31;
-  const int64_t row = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  if (row >= c.tokens * c.heads) return;
-  const int token = int(row % c.tokens), head = int(row / c.tokens);
-  const int request = request_of(c.cu_seqlens_q, int(c.batches), token);
-  if (request < 0) return;
-  const int begin = c.cu_seqlens_q[request], count = c.cu_seqlens_q[request + 1] - begin;
-  const int first = c.cu_seqlens_k[request], length = c.cu_seqlens_k[request + 1] - first;
-  const int keys = c.causal ? length - count + (token - begin) + 1 : length;
-  const float scale = float(c.scale) * 1.4426950408889634f;
-  float q[6], o[4] = {};
-#pragma unroll
-  for (int i = 0; i < 6; ++i) q[i] = to_float(static_cast<const T*>(c.q)[token * c.q_token + head * c.q_head + i * 32 + lane]) * scale;
-  float most = -INFINITY, sum = 0.f;
-  for (int64_t key = first; key < first + keys; ++key) {
-    const T* k = static_cast<const T*>(c.k) + key * c.k_token + head * c.k_head + lane;
-    const T* v = static_cast<const T*>(c.v) + key * c.v_token + head * c.v_head + lane;
-    const T* rope = static_cast<const T*>(c.k_rope) + key * c.rope_token + lane;
-    float score = q[4] * to_float(rope[0]) + q[5] * to_float(rope[32]);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) score += q[i] * to_float(k[i * 32]);
-#pragma unroll
-    for (int i = 16; i > 0; i >>= 1) score += __shfl_xor_sync(0xffffffffu, score, i);
-    const float next = fmaxf(most, score), alpha = exp2f(most - next), weight = exp2f(score - next);
-    most = next;
-    sum = sum * alpha + weight;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = o[i] * alpha + weight * to_float(v[i * 32]);
-  }
-  const float inverse = sum > 0.f ? 1.f / sum : 0.f;
-  T* out = static_cast<T*>(c.out) + (int64_t(token) * c.heads + head) * LATENT_NOPE + lane;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) out[i * 32] = from_float<T>(o[i] * inverse);
-  if (c.lse != nullptr && lane == 0) c.lse[int64_t(token) * c.heads + head] = sum > 0.f ? (most + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+using namespace sm100;
+
+constexpr int kTile = 128;                    // query rows of a tile, keys of a step
+constexpr int kFeatures = LATENT_NOPE + LATENT_ROPE;
+constexpr int kThreads = 320;
+constexpr int kProductWarp = 8, kCopyWarp = 9;
+constexpr int kBoxBytes = kTile * 128;        // 64 features of 128 rows
+constexpr int kQBoxes = kFeatures / 64, kKeyBoxes = 3, kValueBoxes = 2, kRing = 8;
+
+constexpr int kSmemQ = 0;                                       // two tiles of three boxes; the output on its way out in the end
+constexpr int kSmemRing = kSmemQ + 2 * kQBoxes * kBoxBytes;
+constexpr int kSmemBars = kSmemRing + kRing * kBoxBytes;
+constexpr int kSmemEnd = kSmemBars + 256;
+constexpr int kSmemBytes = kSmemEnd + 1024;                     // the tiles are aligned to 1024 bytes
+
+constexpr uint32_t kColumnsO = 256;
+
+enum Bar { kFull0 = 0, kFree0 = kRing, kQFull = 2 * kRing, kScores0, kScores1, kWeights0, kWeights1, kOut0, kOut1, kMended, kBarCount };
+static_assert(kBarCount * 8 + 16 <= 256, "barriers, tensor-memory slot and abort flag");
+
+struct Params {
+  CUtensorMap q, k, v, rope;
+  const int32_t *cu_q, *cu_k;
+  void* out;
+  float* lse;
+  int32_t* status;
+  int32_t batches, tokens, keys, heads, q_head, k_head, v_head;  // *_head: 0 where all heads share memory
+  int32_t causal;
+  float scale_log2;
+};
+
+struct Shared {
+  uint32_t base;
+  unsigned char* ptr;
+  __device__ __forceinline__ uint32_t bar(int which) const { return base + kSmemBars + which * 8; }
+  __device__ __forceinline__ uint32_t* slot() const { return reinterpret_cast<uint32_t*>(ptr + kSmemBars + 240); }
+  __device__ __forceinline__ volatile int* abort_flag() const { return reinterpret_cast<volatile int*>(ptr + kSmemBars + 244); }
+};
+
+// 256 query rows of a head.
+struct Item {
+  int head;
+  int row;    // first query token
+  int rows;   // query rows
+  int first;  // first key of the request
+  int keys;   // keys that the request has
+  int offset; // row i sees keys below offset + i + 1 (causal)
+};
+
+// Keys that the first `rows` rows of the item see, at most.
+__device__ __forceinline__ int reach(const Params& p, const Item& item, int rows) {
+  if (rows <= 0) return 0;
+  return p.causal ? min(item.keys, max(0, item.offset + rows)) : item.keys;
 }
 
-}  // namespace
+__device__ __forceinline__ int bounded(int value, int most) { return min(max(value, 0), most); }
+
+// The item of this block, by whole warps; false when there are fewer. Items: heads, of each all requests, of each request blocks of
+// 256 rows from its end (where causal rows see most keys) to its beginning.
+__device__ __forceinline__ bool find_item(const Params& p, int index, Item& item) {
+  const int lane = threadIdx.x & 31;
+  int per_head = 0;
+  for (int b = lane; b < p.batches; b += 32)
+    per_head += (max(bounded(__ldg(p.cu_q + b + 1), p.tokens) - bounded(__ldg(p.cu_q + b), p.tokens), 0) + 255) >> 8;
+  per_head = __reduce_add_sync(0xffffffffu, per_head);
+  if (per_head == 0 || index / per_head >= p.heads) return false;
+  item.head = index / per_head;
+  int left = index - item.head * per_head;
+  for (int first = 0;; first += 32) {  // (ends: left < per_head)
+    const int b = first + lane;
+    const int begin = b < p.batches ? bounded(__ldg(p.cu_q + b), p.tokens) : 0;
+    const int count = b < p.batches ? max(bounded(__ldg(p.cu_q + b + 1), p.tokens) - begin, 0) : 0;
+    const int blocks = (count + 255) >> 8;
+    int before = blocks;  // inclusive prefix sum
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int other = __shfl_up_sync(0xffffffffu, before, d);
+      if (lane >= d) before += other;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, left < before);
+    if (hit == 0) {
+      left -= __shfl_sync(0xffffffffu, before, 31);
+      continue;
+    }
+    const int owner = __ffs(hit) - 1;
+    const int k_begin = b < p.batches ? bounded(__ldg(p.cu_k + b), p.keys) : 0;
+    const int k_count = b < p.batches ? max(bounded(__ldg(p.cu_k + b + 1), p.keys) - k_begin, 0) : 0;
+    const int block = __shfl_sync(0xffffffffu, before - 1 - left, owner);  // from the request's end
+    const int request_count = __shfl_sync(0xffffffffu, count, owner), start = block << 8;
+    item.row = __shfl_sync(0xffffffffu, begin, owner) + start;
+    item.rows = min(256, request_count - start);
+    item.first = __shfl_sync(0xffffffffu, k_begin, owner);
+    item.keys = __shfl_sync(0xffffffffu, k_count, owner);
+    item.offset = item.keys - request_count + start;
+    return true;
+  }
+}
+
+// Key steps of tile t.
+__device__ __forceinline__ int steps_of(const Params& p, const Item& item, int t) {
+  return item.rows <= t * kTile ? 0 : (reach(p, item, min(item.rows, (t + 1) * kTile)) + kTile - 1) / kTile;
+}
+
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+}
+
+// ---- copies ---------------------------------------------------------------------------------------------------------
+
+// By the whole warp; lane 0 issues.
+__device__ void copy_role(const Params& p, const Shared& sm, const Item& item) {
+  const int lane = threadIdx.x & 31;
+  volatile int* abort_flag = sm.abort_flag();
+  const int steps = max(steps_of(p, item, 0), steps_of(p, item, 1));
+  if (steps == 0) return;
+  if (lane == 0) {
+    mbar_arrive_expect(sm.bar(kQFull), 2 * kQBoxes * kBoxBytes);
+#pragma unroll
+    for (int box = 0; box < 2 * kQBoxes; ++box)  // (rows behind the item are multiplied and thrown away)
+      copy_box(sm.base + kSmemQ + box * kBoxBytes, &p.q, box % kQBoxes * 64, item.head * p.q_head, item.row + box / kQBoxes * kTile, sm.bar(kQFull));
+  }
+  uint32_t count = 0, mended = 0;  // boxes so far; those that were cleared in part
+  bool given_up = false;
+  // Claims the next slot of the ring and lets its copy be started by lane 0.
+  auto bring = [&](auto start, int valid_rows) {
+    const uint32_t slot = count % kRing, use = count / kRing, target = sm.base + kSmemRing + slot * kBoxBytes;
+    if (use > 0 && !warp_wait(sm.bar(kFree0 + slot), (use - 1) & 1, abort_flag)) { given_up = true; return; }
+    const bool mend = valid_rows < kTile;
+    const uint32_t bar = sm.bar(mend ? int(kMended) : int(kFull0 + slot));
+    if (lane == 0) {
+      mbar_arrive_expect(bar, kBoxBytes);
+      start(target, bar);
+    }
+    __syncwarp();
+    if (mend) {
+      if (!warp_wait(bar, mended++ & 1, abort_flag)) { given_up = true; return; }
+      // (the swizzle stays within a row)
+      for (int at = valid_rows * 128 + lane * 16; at < kBoxBytes; at += 512)
+        *reinterpret_cast<uint4*>(sm.ptr + kSmemRing + slot * kBoxBytes + at) = make_uint4(0, 0, 0, 0);
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(sm.bar(kFull0 + slot));
+    }
+    ++count;
+  };
+  for (int step = 0; step < steps && !given_up; ++step) {
+    const int key = item.first + step * kTile;
+    for (int box = 0; box < 2 && !given_up; ++box)
+      bring([&](uint32_t target, uint32_t bar) { copy_box(target, &p.k, box * 64, item.head * p.k_head, key, bar); }, kTile);
+    if (!given_up) bring([&](uint32_t target, uint32_t bar) { copy_box(target, &p.rope, 0, key, bar); }, kTile);
+    const int valid = min(kTile, item.keys - step * kTile);
+    for (int box = 0; box < kValueBoxes && !given_up; ++box)
+      bring([&](uint32_t target, uint32_t bar) { copy_box(target, &p.v, box * 64, item.head * p.v_head, key, bar); }, valid);
+  }
+  if (*abort_flag != 0) {  // nothing of this block may be written behind its end
+    int never = 0;
+    mbar_wait(sm.bar(kQFull), 0, &never);
+    for (uint32_t i = count > kRing ? count - kRing : 0; i < count; ++i) mbar_wait(sm.bar(kFull0 + i % kRing), (i / kRing) & 1, &never);
+    if (mended > 0) mbar_wait(sm.bar(kMended), (mended - 1) & 1, &never);
+  }
+}
+
+// ---- products (one thread) -------------------------------------------------------------------------------------------
+
+template <int kFormat> constexpr uint32_t kIdescScores = idesc_f16(128, 128, kFormat, 0, 0);
+template <int kFormat, int kColumns> constexpr uint32_t kIdescValues = idesc_f16(128, kColumns, kFormat, 0, 1);
+
+template <int kFormat>
+__device__ void product_role(const Params& p, const Shared& sm, const Item& item, uint32_t tmem) {
+  volatile int* abort_flag = sm.abort_flag();
+  const int steps[2] = {steps_of(p, item, 0), steps_of(p, item, 1)};
+  const int most = max(steps[0], steps[1]);
+  if (most == 0) return;
+  uint32_t count = 0;  // boxes used
+  auto box_at = [&](uint32_t box) { return sm.base + kSmemRing + box % kRing * kBoxBytes; };
+  auto landed = [&](uint32_t box) { return mbar_wait(sm.bar(kFull0 + box % kRing), (box / kRing) & 1, abort_flag); };
+  auto release = [&](uint32_t first, int boxes) {
+    for (int i = 0; i < boxes; ++i) mma_commit(sm.bar(kFree0 + (first + i) % kRing));
+  };
+  auto scores = [&](int t, uint32_t keys) {
+#pragma unroll
+    for (int box = 0; box < kKeyBoxes; ++box) {
+      const uint64_t a = smem_desc_sw128(sm.base + kSmemQ + (t * kQBoxes + box) * kBoxBytes, 16, 1024);
+      const uint64_t b = smem_desc_sw128(box_at(keys + box), 16, 1024);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (box == 0 && k == 0) mma_ss_c<false>(tmem + t * kTile, a, b, kIdescScores<kFormat>);
+        else mma_ss_c<true>(tmem + t * kTile, a + k * 2, b + k * 2, kIdescScores<kFormat>);
+      }
+    }
+    mma_commit(sm.bar(kScores0 + t));
+  };
+  auto keys_landed = [&](uint32_t keys) { return landed(keys) && landed(keys + 1) && landed(keys + 2); };
+  if (!mbar_wait(sm.bar(kQFull), 0, abort_flag) || !keys_landed(0)) return;
+  for (int t = 0; t < 2; ++t)
+    if (steps[t] > 0) scores(t, 0);
+  release(0, kKeyBoxes);
+  count = kKeyBoxes;
+  for (int step = 0; step < most; ++step) {
+    const uint32_t values = count, keys = count + kValueBoxes;
+    const bool more = step + 1 < most;
+    if (!landed(values) || !landed(values + 1)) return;
+    for (int t = 0; t < 2; ++t) {
+      if (step < steps[t]) {
+        if (!mbar_wait(sm.bar(kWeights0 + t), step & 1, abort_flag)) return;
+        tc_fence_after_sync();
+        const uint32_t o = tmem + kColumnsO + t * kTile, weights = tmem + t * kTile;
+        const uint64_t b = smem_desc_sw128(box_at(values), kBoxBytes, 1024);
+        if (box_at(values + 1) > box_at(values)) {
+#pragma unroll
+          for (int k = 0; k < kTile / 16; ++k) mma_ts(o, weights + k * 8, b + k * 128, kIdescValues<kFormat, 128>, step > 0 || k > 0);
+        } else {  // every eighth time the second box is at the ring's beginning: 64 features each, which takes half as long again
+          const uint64_t b1 = smem_desc_sw128(box_at(values + 1), kBoxBytes, 1024);
+#pragma unroll
+          for (int k = 0; k < kTile / 16; ++k) mma_ts(o, weights + k * 8, b + k * 128, kIdescValues<kFormat, 64>, step > 0 || k > 0);
+#pragma unroll
+          for (int k = 0; k < kTile / 16; ++k) mma_ts(o + 64, weights + k * 8, b1 + k * 128, kIdescValues<kFormat, 64>, step > 0 || k > 0);
+        }
+        if (step + 1 == steps[t]) mma_commit(sm.bar(kOut0 + t));
+      }
+      if (t == 1) release(values, kValueBoxes);
+      if (step + 1 < steps[t]) {
+        if (!keys_landed(keys)) return;
+        scores(t, keys);
+      }
+    }
+    if (more) release(keys, kKeyBoxes);
+    count += kValueBoxes + kKeyBoxes;
+  }
+}
+
+// ---- softmax ----------------------------------------------------------------------------------------------------------
+
+// A row's reference (log2) starts at the maximum of its first scores and moves when others exceed it by more than kRoom, to kStep below
+// them: weights of up to 2^15 fit IEEE half, and the accumulator is rarely rescaled.
+constexpr float kRoom = 15.f, kStep = 8.f;
+
+template <int kFormat>
+__device__ void softmax_role(const Params& p, const Shared& sm, const Item& item, uint32_t tmem) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, t = warp >> 2;
+  volatile int* abort_flag = sm.abort_flag();
+  const int row = t * kTile + (warp & 3) * 32 + lane;  // of the item
+  const int steps = steps_of(p, item, t);
+  const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
+  const uint32_t s_tmem = tmem + t * kTile + lanes, o_tmem = tmem + kColumnsO + t * kTile + lanes;
+  const int end = p.causal ? min(item.keys, item.offset + row + 1) : item.keys;  // this row sees keys below
+  const int warp_end = p.causal ? min(item.keys, item.offset + (row & ~31) + 1) : item.keys;  // all rows of the warp see keys below
+  float reference = -INFINITY, sum = 0.f;
+  for (int step = 0; step < steps; ++step) {
+    if (!warp_wait(sm.bar(kScores0 + t), step & 1, abort_flag)) return;
+    tc_fence_after_sync();
+    float2 s[kTile / 2];
+#pragma unroll
+    for (int c = 0; c < kTile; c += 32) tmem_ld32(s_tmem + c, reinterpret_cast<uint32_t*>(&s[c / 2]));
+    tmem_wait_ld();
+    const int key = step * kTile;
+    if (key + kTile > warp_end) {
+#pragma unroll
+      for (int i = 0; i < kTile / 2; ++i) {
+        if (key + 2 * i >= end) s[i].x = -INFINITY;
+        if (key + 2 * i + 1 >= end) s[i].y = -INFINITY;
+      }
+    }
+    float most[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      most[k] = fmaxf(s[16 * k].x, s[16 * k].y);
+#pragma unroll
+      for (int i = 1; i < 16; ++i) most[k] = greatest(most[k], s[16 * k + i].x, s[16 * k + i].y);
+    }
+    const float top = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * p.scale_log2;  // scale > 0
+    const bool moves = top > reference + kRoom;
+    if (__any_sync(0xffffffffu, moves)) {
+      float alpha = 1.f;
+      if (moves) {
+        const float next = reference == -INFINITY ? top : top - kStep;
+        alpha = exp2f(reference - next);
+        reference = next;
+      }
+      sum *= alpha;
+      if (step > 0) {  // (scores of this step are there: the products of the one before have ended)
+#pragma unroll 1
+        for (int c = 0; c < kTile; c += 32) {
+          uint32_t o[32];
+          tmem_ld32(o_tmem + c, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+          tmem_st32(o_tmem + c, o);
+        }
+        tmem_wait_st();
+      }
+    }
+    const float shift = reference == -INFINITY ? 0.f : -reference;
+    const float2 scale = make_float2(p.scale_log2, p.scale_log2), shifts = make_float2(shift, shift);
+    float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      uint32_t words[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        float2 weight = fma2(s[half * 32 + i], scale, shifts);
+        weight.x = exp2f(weight.x);
+        weight.y = exp2f(weight.y);
+        sums[i & 1] = add2(sums[i & 1], weight);
+        words[i] = pack2<kFormat>(weight.x, weight.y);
+      }
+      tmem_st32(s_tmem + half * 32, words);
+    }
+    sum += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
+    tmem_wait_st();
+    tc_fence_before_sync();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(sm.bar(kWeights0 + t));
+  }
+  // Output: through this tile's part of Q's memory, which nothing reads any more, so that whole lines are written.
+  const bool live = row < item.rows;
+  if (p.lse != nullptr && live)
+    p.lse[size_t(item.row + row) * p.heads + item.head] = sum > 0.f ? (reference + log2f(sum)) * 0.6931471805599453f : (sum == 0.f ? -INFINITY : sum);
+  const float inverse = sum == 0.f ? 0.f : 1.f / sum;
+  unsigned char* staged = sm.ptr + kSmemQ + t * kQBoxes * kBoxBytes + (warp & 3) * 8192;
+  if (steps > 0) {
+    if (!warp_wait(sm.bar(kOut0 + t), 0, abort_flag)) return;
+    tc_fence_after_sync();
+  } else if (steps_of(p, item, t ^ 1) > 0) {
+    if (!warp_wait(sm.bar(kQFull), 0, abort_flag)) return;  // Q is still on its way to the memory that the output goes through
+  }
+#pragma unroll 1
+  for (int c = 0; c < kTile; c += 32) {
+    uint32_t o[32];
+    if (steps > 0) {
+      tmem_ld32(o_tmem + c, o);
+      tmem_wait_ld();
+    }
+#pragma unroll
+    for (int unit = 0; unit < 4; ++unit) {
+      uint32_t words[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        words[i] = sum == 0.f ? 0u : pack2<kFormat>(__uint_as_float(o[unit * 8 + 2 * i]) * inverse, __uint_as_float(o[unit * 8 + 2 * i + 1]) * inverse);
+      const int place = c / 8 + unit;  // of the row's sixteen
+      *reinterpret_cast<uint4*>(staged + lane * 256 + ((place ^ (lane & 7)) << 4)) = make_uint4(words[0], words[1], words[2], words[3]);
+    }
+  }
+  __syncwarp();
+  const int first_row = t * kTile + (warp & 3) * 32;
+#pragma unroll 4
+  for (int i = 0; i < 16; ++i) {
+    const int r = i * 2 + (lane >> 4), place = lane & 15;
+    const uint4 v = *reinterpret_cast<const uint4*>(staged + r * 256 + ((place ^ (r & 7)) << 4));
+    if (first_row + r < item.rows)
+      *reinterpret_cast<uint4*>(static_cast<char*>(p.out) + (size_t(item.row + first_row + r) * p.heads + item.head) * (LATENT_NOPE * 2) + place * 16) = v;
+  }
+}
+
+template <int kFormat>
+__global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_constant__ Params p) {
+  extern __shared__ unsigned char smem_raw[];
+  Shared sm;
+  const uint32_t raw = smem_u32(smem_raw), pad = (1024u - (raw & 1023u)) & 1023u;
+  sm.base = raw + pad;
+  sm.ptr = smem_raw + pad;
+  const int warp = threadIdx.x >> 5;
+  wait_for_predecessor();
+  let_successor_start();
+  Item item;
+  if (!find_item(p, blockIdx.x, item)) return;  // the whole block
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kBarCount; ++i) mbar_init(sm.bar(i), i == kWeights0 || i == kWeights1 ? 4 : 1);
+    mbar_fence_init();
+    *sm.abort_flag() = 0;
+  }
+  if (warp == kProductWarp) { tmem_alloc(smem_u32(sm.slot()), 512); tmem_relinquish(); }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = *sm.slot();
+  if (warp < kProductWarp) {
+    softmax_role<kFormat>(p, sm, item, tmem);
+  } else if (warp == kProductWarp) {
+    if (elect_one()) product_role<kFormat>(p, sm, item, tmem);
+    __syncwarp();
+  } else {
+    copy_role(p, sm, item);
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (threadIdx.x == 0 && *sm.abort_flag() != 0) report(p.status, SPARSE_MLA_STATUS_WAIT_EXPIRED, item.row, item.head);
+  if (warp == kProductWarp) tmem_dealloc(tmem, 512);
+}
+
+// The map of [rows, heads, features] with boxes of 128 rows of a head; *step: what a head adds to its coordinate (0: all share memory).
+int map_heads(CUtensorMap* map, int format, const void* base, int64_t rows, int64_t heads, int64_t features, int64_t row_stride, int64_t head_stride, int32_t* step) {
+  *step = heads > 1 && head_stride != 0;
+  const int64_t sizes[3] = {features, *step ? heads : 1, rows};
+  const int64_t strides[2] = {*step ? head_stride : features, rows > 1 ? row_stride : features};
+  return encode_map(map, format, 3, base, sizes, strides, 2, kTile);
+}
+
+template <int kFormat>
+int launch(const Params& p, int blocks, cudaStream_t stream) {
+  static bool configured[64] = {false};  // a per-device setting: plain words written with the same value by whoever gets there first
+  int device = 0;
+  if (const cudaError_t error = cudaGetDevice(&device)) return int(error);
+  if (device < 0 || device >= 64) return -1;
+  if (!configured[device]) {
+    if (const cudaError_t error = cudaFuncSetAttribute(prefill_kernel<kFormat>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes)) return int(error);
+    configured[device] = true;
+  }
+  return int(launch_overlapped(prefill_kernel<kFormat>, blocks, kThreads, kSmemBytes, stream, p));
+}
+
+}  // namespace prefill
 }  // namespace latent
 
 extern "C" int launch_latent_prefill(void* stream, const latent_prefill_call* call) {
   using namespace latent;
   const latent_prefill_call& c = *call;
-  if (c.type != LATENT_F16 && c.type != LATENT_BF16) return -1;
-  if (c.batches < 0 || c.tokens < 0 || c.keys < 0 || c.heads < 1) return -1;
+  if ((c.type != LATENT_F16 && c.type != LATENT_BF16) || !(c.scale > 0) || c.status == nullptr) return -1;
+  if (c.batches < 0 || c.batches >= INT32_MAX || c.tokens < 0 || c.tokens > INT32_MAX - 256 || c.keys < 0 || c.keys > INT32_MAX - 256 || c.heads < 1 || c.heads > 65535) return -1;
+  const int64_t blocks = (c.tokens / 256 + c.batches) * c.heads;  // at least as many as there are items
+  if (blocks > INT32_MAX) return -1;
   if (c.tokens == 0 || c.batches == 0) return 0;
-  const unsigned blocks = unsigned((c.tokens * c.heads + 7) / 8);
+  prefill::Params p = {};
+  const int64_t keys = c.keys > 0 ? c.keys : 1;  // (without keys nothing is copied)
+  const void* any = c.q;
+  if (const int e = prefill::map_heads(&p.q, c.type, c.q, c.tokens, c.heads, prefill::kFeatures, c.q_token, c.q_head, &p.q_head)) return e;
+  if (const int e = prefill::map_heads(&p.k, c.type, c.keys > 0 ? c.k : any, keys, c.keys > 0 ? c.heads : 1, LATENT_NOPE, c.k_token, c.k_head, &p.k_head)) return e;
+  if (const int e = prefill::map_heads(&p.v, c.type, c.keys > 0 ? c.v : any, keys, c.keys > 0 ? c.heads : 1, LATENT_NOPE, c.v_token, c.v_head, &p.v_head)) return e;
+  const int64_t sizes[2] = {LATENT_ROPE, keys}, strides[1] = {keys > 1 ? c.rope_token : LATENT_ROPE};
+  if (const int e = sm100::encode_map(&p.rope, c.type, 2, c.keys > 0 ? c.k_rope : any, sizes, strides, 1, prefill::kTile)) return e;
+  p.cu_q = c.cu_seqlens_q;
+  p.cu_k = c.cu_seqlens_k;
+  p.out = c.out;
+  p.lse = c.lse;
+  p.status = c.status;
+  p.batches = int32_t(c.batches);
+  p.tokens = int32_t(c.tokens);
+  p.keys = int32_t(c.keys);
+  p.heads = int32_t(c.heads);
+  p.causal = c.causal;
+  p.scale_log2 = float(c.scale * 1.4426950408889634);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (c.type == LATENT_BF16) prefill_kernel<__nv_bfloat16><<<blocks, 256, 0, s>>>(c);
-  else prefill_kernel<__half><<<blocks, 256, 0, s>>>(c);
-  return int(cudaGetLastError());
+  return c.type == LATENT_BF16 ? prefill::launch<1>(p, int(blocks), s) : prefill::launch<0>(p, int(blocks), s);
 }
