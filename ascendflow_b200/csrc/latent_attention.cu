@@ -1,79 +1,861 @@
 // Attention over the paged latent cache in absorbed form: one row per token is key and value of all heads.
+//
+// out = softmax(scale Q X^T) X[:, :512] per request, Q the queries of all heads (row j * H + h), X the cached rows, row j * H + h seeing
+// the first L - n + j + 1 of them. Rows of a request are dealt in tiles of 64, whatever the number of heads, and cached rows in
+// chunks of 64 (pages are multiples). A block works on a stretch of the call's (tile, chunk) pairs, tile by tile: all blocks get
+// stretches of the same cost (`Plan`), so a tile may be shared by several blocks; their unnormalised sums then go to the
+// workspace in FP32 and `combine_kernel` adds them up, in the order of the chunks.
+//
+//   warps 0-3   softmax: scores out of tensor memory, running reference and sum in FP32, P (16 bits) to shared memory, rescaling of
+//               the accumulator, output.
+//   warp 4      one thread issues S = Q X^T: Q from tensor memory, X K-major from the chunk's tile. 64 rows fill half of the 128 lanes
+//               that the tensor core wants, so the features of a row are split between two lanes: lanes 0-15 of every subpartition
+//               hold the even pairs of features of 16 rows, lanes 16-31 the odd pairs. Either is a 2:4 sparse row: W / 32 sparse
+//               instructions M = 128, N = 64, K = 32 give every lane the partial scores of its pairs.
+//   warp 5      one thread issues O += P X: weight-stationary M = 64, N = 256, X MN-major from the same tile.
+//   warp 6      brings chunks by tensor copies (boxes of 64 features x 64 rows) into a ring of three tiles.
+//   warp 7      works out the block's pieces (a tile and a stretch of its chunks) ahead of everybody.
+//   warps 8-15  Q of the next piece from global to tensor memory, through registers.
+//
+// Tensor memory: columns 0-255 O (lane l: row l % 64, accumulators of features 128 (l / 64) .. + 127 and 256 more), 256-383 Q's first 512
+// features, 384-447 scores, 448-463 the sparse products' metadata, 464-479 Q's other 64 features.
+//
+// Rows of a chunk behind the request's length are cleared in the tile's value part (a zero weight times infinity is a
+// NaN) and their scores replaced; so are whole chunks whose page is not in the cache, which are reported.
 #include "latent_common.cuh"
+#include "latent_ptx.cuh"
 
 namespace latent {
-namespace {
+namespace absorbed {
 
-// One warp per token and head: running maximum and sum, a key at a time.
-template <typename T, int kWidth>
-__global__ void __launch_bounds__(256) attention_kernel(const latent_attention_call c) {
-  constexpr int kOwn = kWidth / 32, kOwnValues = LATENT_VALUES / 32;
-  const int lane = threadIdx.x & 31;
-  const int64_t row = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  if (row >= c.tokens * c.heads) return;
-  const int token = int(row / c.heads), head = int(row % c.heads);
-  const int request = request_of(c.cu_seqlens_q, int(c.batches), token);
-  if (request < 0) return;
-  const int begin = c.cu_seqlens_q[request], count = c.cu_seqlens_q[request + 1] - begin;
-  const int keys = c.seqused_kv[request] - count + (token - begin) + 1;
-  const float scale = float(c.scale) * 1.4426950408889634f;
-  float q[kOwn], o[kOwnValues] = {};
-#pragma unroll
-  for (int i = 0; i < kOwn; ++i) q[i] = to_float(static_cast<const T*>(c.q)[row * kWidth + i * 32 + lane]) * scale;
-  float most = -INFINITY, sum = 0.f;
-  for (int key = 0; key < keys; ++key) {
-    const int64_t column = key / c.page_rows;
-    const int64_t page = column < c.pages ? c.block_table[request * c.pages + column] : -1;
-    if (page < 0 || page >= c.blocks) {
-      if (lane == 0) report(c.status, SPARSE_MLA_STATUS_BAD_PAGE, token, key);
-      continue;
-    }
-    const T* k = static_cast<const T*>(c.cache) + (page * c.page_rows + key % c.page_rows) * kWidth + lane;
-    float values[kOwn], score = 0.f;
-#pragma unroll
-    for (int i = 0; i < kOwn; ++i) score += q[i] * (values[i] = to_float(k[i * 32]));
-#pragma unroll
-    for (int i = 16; i > 0; i >>= 1) score += __shfl_xor_sync(0xffffffffu, score, i);
-    const float next = fmaxf(most, score), alpha = exp2f(most - next), weight = exp2f(score - next);
-    most = next;
-    sum = sum * alpha + weight;
-#pragma unroll
-    for (int i = 0; i < kOwnValues; ++i) o[i] = o[i] * alpha + weight * values[i];
-  }
-  float inverse = sum > 0.f ? 1.f / sum : 0.f, log_sum = sum > 0.f ? most + log2f(sum) : -INFINITY;
-  const float sink = c.sinks != nullptr ? c.sinks[head] * 1.4426950408889634f : -INFINITY, top = fmaxf(log_sum, sink);
-  if (sink > -INFINITY) {
-    const float total = exp2f(log_sum - top) + exp2f(sink - top);
-    inverse = sum > 0.f ? inverse * exp2f(log_sum - top) / total : 0.f;
-    log_sum = top + log2f(total);
-  }
-  T* out = static_cast<T*>(c.out) + row * LATENT_VALUES + lane;
-#pragma unroll
-  for (int i = 0; i < kOwnValues; ++i) out[i * 32] = from_float<T>(o[i] * inverse);
-  if (c.lse != nullptr && lane == 0) c.lse[row] = log_sum * 0.6931471805599453f;
+using namespace sm100;
+
+constexpr int kRows = 64, kChunk = 64;
+constexpr int kSoftmaxWarps = 4, kScoreWarp = 4, kValueWarp = 5, kCopyWarp = 6, kPlanWarp = 7, kQueryWarp0 = 8, kQueryWarps = 8;
+constexpr int kThreads = 32 * (kQueryWarp0 + kQueryWarps);
+constexpr int kBoxBytes = kChunk * 128;  // 64 features of a chunk
+constexpr int kStages = 3;
+constexpr int kPieces = 4;               // pieces announced ahead
+
+constexpr uint32_t kColumnsQ = 256, kColumnsScores = 384, kColumnsPlaces = 448, kColumnsQRest = 464;
+constexpr uint32_t kHighLanes = 16u << 16;
+
+// What a block does next: rows of one request's tile and a stretch of chunks.
+struct Piece {
+  int64_t row;      // first row of q and out
+  int rows;         // 1 .. 64
+  int request;
+  int token;        // the tile's first row's token within the request
+  int head;         // ... and head
+  int base;         // keys that the request's first token sees: L - n + 1
+  int length;       // keys of the request that may be read
+  int first, last;  // chunks [first, last); first < 0: no more pieces
+  int slot;         // of the workspace, or -1: the piece is all of its tile
+};
+static_assert(sizeof(Piece) <= 64, "the piece ring holds 64-byte entries");
+
+template <int kWidth>
+struct Layout {
+  static constexpr int kBoxes = kWidth / 64;
+  static constexpr int kTileBytes = kBoxes * kBoxBytes;
+  static constexpr int kSmemP = kStages * kTileBytes;            // 64 rows x 64 weights; the output on its way out
+  static constexpr int kSmemPieces = kSmemP + kRows * 128;
+  static constexpr int kSmemBars = kSmemPieces + kPieces * 64;
+  static constexpr int kSmemAlpha = kSmemBars + 256;             // float[2][64]
+  static constexpr int kSmemInverse = kSmemAlpha + 2 * kRows * 4;  // float[64]
+  static constexpr int kSmemMisc = kSmemInverse + kRows * 4;
+  static constexpr int kSmemBytes = kSmemMisc + 128 + 1024;      // the tiles are aligned to 1024 bytes
+};
+static_assert(Layout<576>::kSmemBytes <= 232448, "one block per SM");
+
+enum Bar {
+  kFull0 = 0, kFree0 = kFull0 + kStages, kPieceReady0 = kFree0 + kStages, kPieceDone0 = kPieceReady0 + kPieces, kQFull = kPieceDone0 + kPieces,
+  kQFree, kPlaces, kScoresFull, kScoresFree, kWeightsFull, kWeightsFree, kMended, kBarCount
+};
+static_assert(kBarCount <= 32, "the barrier area");
+
+// Workspace: per block a record, statistics and sums of two slots (2 i: a tile that begins in an earlier block; 2 i + 1: one that begins here and
+// ends in a later one).
+struct Record {
+  int64_t row;
+  int rows, head;
+  int last;       // block that has the tile's end; -1: no tile begins here that ends elsewhere
+  int continued;  // slot 2 i holds a part of the tile before
+  int pad[2];
+};
+constexpr int kSlotFloats = LATENT_VALUES * kRows;  // [feature][row]
+inline size_t statistics_offset(int blocks) { return size_t(blocks) * sizeof(Record); }
+inline size_t sums_offset(int blocks) { return (statistics_offset(blocks) + size_t(blocks) * 2 * kRows * sizeof(float2) + 511) / 512 * 512; }
+inline size_t workspace_bytes(int blocks) { return sums_offset(blocks) + size_t(blocks) * 2 * kSlotFloats * sizeof(float); }
+
+struct Params {
+  CUtensorMap cache;
+  const char* q;
+  const int32_t *table, *cu, *lengths;
+  const float* sinks;
+  char* out;
+  float* lse;
+  Record* records;
+  float2* statistics;
+  float* sums;
+  int32_t* status;
+  int32_t batches, tokens, heads, pages, blocks, page_rows;
+  float scale_log2;
+};
+
+struct Shared {
+  uint32_t base;
+  unsigned char* ptr;
+  int bars, pieces, misc;
+  __device__ __forceinline__ uint32_t bar(int which) const { return base + bars + which * 8; }
+  __device__ __forceinline__ Piece* piece(uint32_t index) const { return reinterpret_cast<Piece*>(ptr + pieces + (index % kPieces) * 64); }
+  __device__ __forceinline__ uint32_t* tmem_slot() const { return reinterpret_cast<uint32_t*>(ptr + misc); }
+  __device__ __forceinline__ volatile int* abort_flag() const { return reinterpret_cast<volatile int*>(ptr + misc + 4); }
+  __device__ __forceinline__ volatile int* live(uint32_t stage) const { return reinterpret_cast<volatile int*>(ptr + misc + 8 + stage * 4); }
+  __device__ __forceinline__ int64_t* scan() const { return reinterpret_cast<int64_t*>(ptr); }  // (before the first tile lands)
+};
+
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
 }
 
-}  // namespace
+// ---- the plan -----------------------------------------------------------------------------------------------------
+
+// A request's tiles and what they cost, in cached rows: the tiles' rows see from `near` keys on up to `far`, a piece costs kFixed more.
+constexpr int kFixed = 128;
+struct Request {
+  int begin, count;  // tokens
+  int length;        // keys
+  int rows, tiles;
+  int near, far;
+  // Cost of the first `t` tiles. (Any function will do that everybody evaluates alike and that grows; in doubles it cannot overflow.)
+  __device__ __forceinline__ int64_t cost(int t) const {
+    const double ramp = tiles > 1 ? double(far - near) * (double(t) * double(t - 1)) / (2.0 * double(tiles - 1)) : 0.0;
+    return int64_t(t) * (kFixed + near) + int64_t(ramp);
+  }
+};
+
+__device__ __forceinline__ Request request_at(const Params& p, int b) {
+  Request r;
+  r.begin = min(max(__ldg(p.cu + b), 0), p.tokens);
+  r.count = max(min(max(__ldg(p.cu + b + 1), 0), p.tokens) - r.begin, 0);
+  r.length = max(__ldg(p.lengths + b), 0);
+  r.rows = r.count * p.heads;
+  r.tiles = (r.rows + kRows - 1) / kRows;
+  // (one key behind the table is enough to report a length that does not fit)
+  r.far = int(min(int64_t(r.length), int64_t(p.pages) * p.page_rows + 1));
+  r.near = int(min(int64_t(r.far), max(int64_t(r.length) - r.count, int64_t(0)) + kRows / p.heads + 1));
+  return r;
+}
+
+// Chunks that tile t's rows see.
+__device__ __forceinline__ int chunks_of(const Params& p, const Request& r, int t) {
+  const int last_token = (min((t + 1) * kRows, r.rows) - 1) / p.heads;
+  const int64_t seen = int64_t(r.length) - r.count + last_token + 1;
+  return int((min(max(seen, int64_t(0)), int64_t(r.far)) + kChunk - 1) / kChunk);
+}
+
+// Stretch [border(i), border(i + 1)) of the total cost is block i's.
+struct Borders {
+  int64_t total;
+  int blocks;  // that get a stretch
+  __device__ __forceinline__ int64_t at(int i) const { return total / blocks * i + total % blocks * i / blocks; }
+};
+// A block with fewer chunks than these loses more with its start and with its part of the sums than it takes off the others.
+constexpr int kLeastChunks = 4;
+
+// By all threads of the block: the total, and the request that cost `border(blockIdx.x)` lies in (with the cost in front of it).
+__device__ __forceinline__ Borders plan_block(const Params& p, int64_t* scan, int* request, int64_t* before) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int kWarps = kThreads / 32;
+  Borders borders = {0, 1};
+  int64_t own = 0, inclusive = 0;
+  auto sum_up = [&](int first) {  // costs of kThreads requests: own, and with all in front of them; returns their sum
+    const int b = first + int(threadIdx.x);
+    own = 0;
+    if (b < p.batches) {
+      const Request r = request_at(p, b);
+      own = r.cost(r.tiles);
+    }
+    inclusive = own;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t other = __shfl_up_sync(0xffffffffu, inclusive, d);
+      if (lane >= d) inclusive += other;
+    }
+    __syncthreads();
+    if (lane == 31) scan[warp] = inclusive;
+    __syncthreads();
+    int64_t sum = 0;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w == warp) inclusive += sum;
+      sum += scan[w];
+    }
+    return sum;
+  };
+  for (int first = 0; first < p.batches; first += kThreads) borders.total += sum_up(first);
+  const int64_t most = borders.total / (kLeastChunks * kChunk);
+  borders.blocks = int(min(max(most, int64_t(1)), int64_t(gridDim.x)));
+  if (int(blockIdx.x) >= borders.blocks || borders.total == 0) { borders.blocks = 0; return borders; }
+  const int64_t mine = borders.at(blockIdx.x);
+  int64_t passed = 0;
+  for (int first = 0; first < p.batches; first += kThreads) {
+    const int64_t sum = p.batches <= kThreads ? borders.total : sum_up(first);  // (one round: the values are still there)
+    const int64_t start = passed + inclusive - own;
+    if (own > 0 && start <= mine && mine < start + own) {
+      scan[kWarps] = first + int(threadIdx.x);
+      scan[kWarps + 1] = start;
+    }
+    passed += sum;
+  }
+  __syncthreads();
+  *request = int(scan[kWarps]);
+  *before = scan[kWarps + 1];
+  return borders;
+}
+
+// The pieces of this block, announced one after the other (by one warp; all lanes work out the same).
+__device__ void plan_role(const Params& p, const Shared& sm, const Borders& borders, int request, int64_t before) {
+  const int lane = threadIdx.x & 31;
+  volatile int* abort_flag = sm.abort_flag();
+  Record record = {0, 0, 0, -1, 0, {0, 0}};
+  uint32_t announced = 0;
+  // A free entry of the ring; false when somebody has given up.
+  auto claim = [&]() { return announced < kPieces || warp_wait(sm.bar(kPieceDone0 + announced % kPieces), (announced / kPieces - 1) & 1, abort_flag); };
+  auto announce = [&](const Piece& piece) {
+    if (lane == 0) {
+      *sm.piece(announced) = piece;
+      mbar_arrive(sm.bar(kPieceReady0 + announced % kPieces));
+    }
+    ++announced;
+  };
+  if (borders.blocks > 0) {
+    const int64_t end = borders.at(blockIdx.x + 1);
+    int64_t at = borders.at(blockIdx.x);
+    Request r = request_at(p, request);
+    int tile = 0;
+    for (int low = 0, high = r.tiles; high - low > 1;) {  // cost(low) <= at - before < cost(high)
+      const int middle = (low + high) >> 1;
+      if (r.cost(middle) <= at - before) low = middle; else high = middle;
+      tile = low;
+    }
+    while (at < end) {
+      const int64_t start = before + r.cost(tile), past = before + r.cost(tile + 1), cost = past - start;
+      const int chunks = chunks_of(p, r, tile);
+      Piece piece;
+      piece.first = int((at - start) * chunks / cost);
+      piece.last = past <= end ? chunks : int((end - start) * chunks / cost);
+      if (piece.first < piece.last || (chunks == 0 && at == start)) {
+        const int row = tile * kRows;
+        piece.row = int64_t(r.begin) * p.heads + row;
+        piece.rows = min(kRows, r.rows - row);
+        piece.request = request;
+        piece.token = row / p.heads;
+        piece.head = row % p.heads;
+        piece.base = r.length - r.count + 1;
+        piece.length = r.far;
+        const bool whole = piece.first == 0 && piece.last == chunks;
+        piece.slot = whole ? -1 : 2 * int(blockIdx.x) + (piece.first == 0);
+        if (!whole && piece.first == 0) {
+          record.row = piece.row;
+          record.rows = piece.rows;
+          record.head = piece.head;
+          int last = int(double(past) / double(borders.total) * borders.blocks);  // the block that has the tile's end, or next to it
+          last = min(max(last, int(blockIdx.x)), borders.blocks - 1);
+          while (last > int(blockIdx.x) && borders.at(last) >= past) --last;
+          while (last + 1 < borders.blocks && borders.at(last + 1) < past) ++last;
+          record.last = last;
+        } else if (!whole) {
+          record.continued = 1;
+        }
+        if (!claim()) break;
+        announce(piece);
+      }
+      at = min(past, end);
+      if (past <= end && ++tile >= r.tiles) {
+        before = past;
+        if (at >= end) break;
+        // The next request that has rows. (There is one: cost is left.)
+        tile = 0;
+        unsigned hit = 0;
+        for (int b = request + 1; hit == 0 && b < p.batches; b += 32) {
+          hit = __ballot_sync(0xffffffffu, b + lane < p.batches && request_at(p, b + lane).rows > 0);
+          request = b + __ffs(hit) - 1;
+        }
+        if (hit == 0) break;
+        r = request_at(p, request);
+      }
+    }
+  }
+  if (lane == 0) p.records[blockIdx.x] = record;
+  if (!claim()) return;
+  Piece none = {};
+  none.first = -1;
+  announce(none);
+}
+
+// Everybody's way through the pieces. `next` waits for one and returns false behind the last (or when a wait gave up); `done` gives its entry back.
+struct Walk {
+  const Shared& sm;
+  uint32_t index = 0;
+  Piece piece;
+  __device__ __forceinline__ explicit Walk(const Shared& shared) : sm(shared) {}
+  __device__ __forceinline__ bool next_of_warp() { return warp_wait(sm.bar(kPieceReady0 + index % kPieces), (index / kPieces) & 1, sm.abort_flag()) && read(); }
+  __device__ __forceinline__ bool next_of_thread() { return mbar_wait(sm.bar(kPieceReady0 + index % kPieces), (index / kPieces) & 1, sm.abort_flag()) && read(); }
+  __device__ __forceinline__ bool read() { piece = *sm.piece(index); return piece.first >= 0; }
+  __device__ __forceinline__ void done() { mbar_arrive(sm.bar(kPieceDone0 + index % kPieces)); ++index; }  // one thread
+  __device__ __forceinline__ void done_of_warp() {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(sm.bar(kPieceDone0 + index % kPieces));
+    ++index;
+  }
+};
+
+// ---- copies ---------------------------------------------------------------------------------------------------------
+
+template <int kWidth>
+__device__ void copy_role(const Params& p, const Shared& sm) {
+  using L = Layout<kWidth>;
+  const int lane = threadIdx.x & 31;
+  volatile int* abort_flag = sm.abort_flag();
+  uint32_t count = 0, mended = 0;
+  bool given_up = false;
+  Walk walk(sm);
+  for (; !given_up && walk.next_of_warp(); walk.done_of_warp()) {
+    const Piece& piece = walk.piece;
+    if (piece.first == piece.last) continue;  // sees nothing
+    const int32_t* table = p.table + size_t(piece.request) * p.pages;
+    auto page_of = [&](int chunk) {  // lane l: the page of chunk `chunk + l`, or -1
+      const int column = min(chunk + lane, piece.last - 1) * kChunk / p.page_rows;
+      return column < p.pages ? __ldg(table + column) : -1;
+    };
+    int pages = 0, next_pages = page_of(piece.first);  // of 32 chunks; of the next 32
+    for (int chunk = piece.first; chunk < piece.last; ++chunk, ++count) {
+      const int place = (chunk - piece.first) & 31;
+      if (place == 0) {
+        pages = next_pages;
+        if (chunk + 32 < piece.last) next_pages = page_of(chunk + 32);
+      }
+      const int page = __shfl_sync(0xffffffffu, pages, place);
+      const uint32_t stage = count % kStages, use = count / kStages, target = sm.base + stage * L::kTileBytes;
+      if (use > 0 && !warp_wait(sm.bar(kFree0 + stage), (use - 1) & 1, abort_flag)) { given_up = true; break; }
+      const bool legal = unsigned(page) < unsigned(p.blocks);
+      const int valid = legal ? min(kChunk, piece.length - chunk * kChunk) : 0;
+      const bool mend = valid < kChunk;
+      const uint32_t bar = sm.bar(mend ? int(kMended) : int(kFull0 + stage));
+      if (lane == 0) {
+        *sm.live(stage) = valid;
+        if (legal) {
+          mbar_arrive_expect(bar, L::kTileBytes);
+          const int row = page * p.page_rows + chunk * kChunk % p.page_rows;
+#pragma unroll
+          for (int box = 0; box < L::kBoxes; ++box) copy_box(target + box * kBoxBytes, &p.cache, box * 64, row, bar);
+        } else {
+          report(p.status, SPARSE_MLA_STATUS_BAD_PAGE, int(piece.row / p.heads), chunk * kChunk);
+        }
+      }
+      __syncwarp();
+      if (mend) {
+        if (legal && !warp_wait(bar, mended++ & 1, abort_flag)) { given_up = true; break; }
+        for (int box = 0; box < LATENT_VALUES / 64; ++box)  // (the swizzle stays within a row)
+          for (int at = valid * 128 + lane * 16; at < kBoxBytes; at += 512)
+            *reinterpret_cast<uint4*>(sm.ptr + stage * L::kTileBytes + box * kBoxBytes + at) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(sm.bar(kFull0 + stage));
+      }
+    }
+  }
+  if (*abort_flag != 0) {  // nothing of this block may be written behind its end
+    int never = 0;
+    for (uint32_t i = count > kStages ? count - kStages : 0; i < count; ++i) mbar_wait(sm.bar(kFull0 + i % kStages), (i / kStages) & 1, &never);
+    if (mended > 0) mbar_wait(sm.bar(kMended), (mended - 1) & 1, &never);
+  }
+}
+
+// ---- queries --------------------------------------------------------------------------------------------------------
+
+// Columns of 16 lanes (`taddr`'s lane field is the warp's lane base + 0 or + 16), see tmem_st_16x256b; eight columns.
+__device__ __forceinline__ void tmem_st_8(uint32_t taddr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("tcgen05.st.sync.aligned.16x256b.x1.b32 [%0], {%1,%2,%3,%4};\n" ::"r"(taddr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+// A subpartition's 16 rows are shared by two warps: eight segments of 64 bytes each, and one of Q's last two. A thread loads 16 bytes of rows
+// t / 4 and t / 4 + 8 of every segment; even words go to the low lanes and odd words to the high lanes as they are.
+template <int kWidth>
+__device__ void query_role(const Params& p, const Shared& sm, uint32_t tmem) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile int* abort_flag = sm.abort_flag();
+  const int subpartition = warp & 3, part = (warp - kQueryWarp0) >> 2;
+  const uint32_t lanes = uint32_t(subpartition * 32) << 16;
+  constexpr int kOwn = kWidth / 64;  // segments of this warp
+  uint32_t loads = 0;
+  Walk walk(sm);
+  for (; walk.next_of_warp(); walk.done_of_warp()) {
+    const Piece& piece = walk.piece;
+    if (piece.first == piece.last) continue;  // sees nothing
+    uint4 words[2 * kOwn];
+#pragma unroll
+    for (int s = 0; s < kOwn; ++s) {
+      const int segment = s < 8 ? part * 8 + s : 16 + part;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int row = subpartition * 16 + (lane >> 2) + 8 * k;
+        words[2 * s + k] = make_uint4(0, 0, 0, 0);
+        if (row < piece.rows) words[2 * s + k] = __ldg(reinterpret_cast<const uint4*>(p.q + (piece.row + row) * (kWidth * 2) + segment * 64 + (lane & 3) * 16));
+      }
+    }
+    if (loads > 0 && !warp_wait(sm.bar(kQFree), (loads - 1) & 1, abort_flag)) return;
+    tc_fence_after_sync();
+#pragma unroll
+    for (int s = 0; s < kOwn; ++s) {
+      const uint32_t at = tmem + lanes + (s < 8 ? kColumnsQ + (part * 8 + s) * 8 : kColumnsQRest + part * 8);
+      const uint4 a = words[2 * s], b = words[2 * s + 1];
+      tmem_st_8(at, a.x, a.z, b.x, b.z);
+      tmem_st_8(at + kHighLanes, a.y, a.w, b.y, b.w);
+    }
+    tmem_wait_st();
+    tc_fence_before_sync();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(sm.bar(kQFull));
+    ++loads;
+  }
+}
+
+// ---- products (one thread each) --------------------------------------------------------------------------------------
+
+template <int kFormat> constexpr uint32_t kIdescScores = idesc_f16(128, kChunk, kFormat, 0, 0) | kSparseA;
+template <int kFormat> constexpr uint32_t kIdescValues = idesc_f16(64, 256, kFormat, 0, 1);  // issued as .ws
+
+template <int kFormat, int kSteps, int K = 0>
+__device__ __forceinline__ void issue_scores(uint32_t tmem, uint64_t x_desc) {
+  if constexpr (K < kSteps) {
+    constexpr uint32_t offset = (K >> 1) * kBoxBytes + (K & 1) * 64;
+    constexpr uint32_t q = K < 16 ? kColumnsQ + K * 8 : kColumnsQRest + (K - 16) * 8;
+    mma_sparse_ts_c<K != 0>(tmem + kColumnsScores, tmem + q, x_desc + (offset >> 4), tmem + kColumnsPlaces, kIdescScores<kFormat>);
+    issue_scores<kFormat, kSteps, K + 1>(tmem, x_desc);
+  }
+}
+template <int kFormat, bool kFirst, int I = 0>
+__device__ __forceinline__ void issue_values(uint32_t tmem, uint64_t p_desc, uint64_t x_desc) {
+  if constexpr (I < 2 * (kChunk / 16)) {
+    constexpr int half = I % 2, k = I / 2;
+    constexpr uint32_t offset = half * 4 * kBoxBytes + k * 2048;
+    mma_ws_ss_c<!(kFirst && k == 0)>(tmem + half * 128, p_desc + ((k * 32) >> 4), x_desc + (offset >> 4), kIdescValues<kFormat>);
+    issue_values<kFormat, kFirst, I + 1>(tmem, p_desc, x_desc);
+  }
+}
+
+template <int kFormat, int kWidth>
+__device__ void score_role(const Shared& sm, uint32_t tmem) {
+  volatile int* abort_flag = sm.abort_flag();
+  uint32_t count = 0, loads = 0;
+  Walk walk(sm);
+  if (!mbar_wait(sm.bar(kPlaces), 0, abort_flag)) return;
+  for (; walk.next_of_thread(); walk.done()) {
+    const int chunks = walk.piece.last - walk.piece.first;
+    if (chunks == 0) continue;
+    if (!mbar_wait(sm.bar(kQFull), loads++ & 1, abort_flag)) return;
+    for (int i = 0; i < chunks; ++i, ++count) {
+      const uint32_t stage = count % kStages;
+      if (!mbar_wait(sm.bar(kFull0 + stage), (count / kStages) & 1, abort_flag)) return;
+      if (!mbar_wait(sm.bar(kScoresFree), (count & 1) ^ 1, abort_flag)) return;
+      tc_fence_after_sync();
+      issue_scores<kFormat, kWidth / 32>(tmem, smem_desc_sw128(sm.base + stage * Layout<kWidth>::kTileBytes, 16, 1024));
+      mma_commit(sm.bar(kScoresFull));
+    }
+    mma_commit(sm.bar(kQFree));
+  }
+}
+
+template <int kFormat, int kWidth>
+__device__ void value_role(const Shared& sm, uint32_t tmem) {
+  volatile int* abort_flag = sm.abort_flag();
+  uint32_t count = 0;
+  Walk walk(sm);
+  const uint64_t p_desc = smem_desc_sw128(sm.base + Layout<kWidth>::kSmemP, 16, 1024);
+  for (; walk.next_of_thread(); walk.done()) {
+    const int chunks = walk.piece.last - walk.piece.first;
+    for (int i = 0; i < chunks; ++i, ++count) {
+      const uint32_t stage = count % kStages;
+      if (!mbar_wait(sm.bar(kWeightsFull), count & 1, abort_flag)) return;
+      tc_fence_after_sync();
+      const uint64_t x_desc = smem_desc_sw128(sm.base + stage * Layout<kWidth>::kTileBytes, kBoxBytes, 1024);
+      if (i == 0) issue_values<kFormat, true>(tmem, p_desc, x_desc);
+      else issue_values<kFormat, false>(tmem, p_desc, x_desc);
+      mma_commit(sm.bar(kWeightsFree));
+      mma_commit(sm.bar(kFree0 + stage));
+    }
+  }
+}
+
+// ---- softmax ----------------------------------------------------------------------------------------------------------
+
+// A row's reference (log2) starts at the maximum of its first scores and moves when others exceed it by more than kRoom, to kStep below
+// them: weights of up to 2^15 fit IEEE half, and the accumulator is rarely rescaled.
+constexpr float kRoom = 15.f, kStep = 8.f;
+constexpr float kLog2E = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// 1 / denominator and the log (log2) of it, from a row's reference and sum and its sink (log2; -infinity: none).
+__device__ __forceinline__ float inverse_of(float reference, float sum, float sink, float* log_sum) {
+  const float own = sum == 0.f ? -INFINITY : reference + log2f(sum);
+  if (sink == -INFINITY) {
+    *log_sum = own;
+    return sum == 0.f ? 0.f : 1.f / sum;
+  }
+  const float top = fmaxf(own, sink), share = exp2f(own - top), total = share + exp2f(sink - top);
+  *log_sum = top + log2f(total);
+  return sum == 0.f ? 0.f : share / (total * sum);
+}
+
+template <int kFormat, int kWidth>
+__device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
+  using L = Layout<kWidth>;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = lane >> 4;
+  volatile int* abort_flag = sm.abort_flag();
+  const uint32_t lanes = uint32_t(warp * 32) << 16, scores = tmem + kColumnsScores + lanes;
+  // This thread works out weights of row `row`, of keys 32 half .. + 31 of a chunk; the accumulator's lane that it reads belongs to another row.
+  const int row = warp * 16 + (lane & 15), o_row = (warp & 1) * 32 + lane, o_feature = (warp >> 1) * 128;
+  float* alphas = reinterpret_cast<float*>(sm.ptr + L::kSmemAlpha);
+  float* inverses = reinterpret_cast<float*>(sm.ptr + L::kSmemInverse);
+  unsigned char* weights = sm.ptr + L::kSmemP;
+  {
+    uint32_t columns[16];  // which pairs a lane of Q holds: numbers 0 and 1 of every four features, or 2 and 3
+#pragma unroll
+    for (int e = 0; e < 16; ++e) columns[e] = half ? 0xeeeeeeeeu : 0x44444444u;
+    tmem_st16(tmem + kColumnsPlaces + lanes, columns);
+    tmem_wait_st();
+    tc_fence_before_sync();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(sm.bar(kPlaces));
+  }
+  // The four warps meet once a chunk. One whose wait gave up says so there, and all leave behind it.
+  bool failed = false;
+  constexpr uint32_t kGivenUp = 32;
+  auto meet = [&](bool flag) { return named_barrier_count(1, 32 * kSoftmaxWarps, failed || (flag && lane == 0)); };
+  uint32_t count = 0;
+  Walk walk(sm);
+  for (; walk.next_of_warp(); walk.done_of_warp()) {
+    const Piece& piece = walk.piece;
+    const int chunks = piece.last - piece.first;
+    const int end = row < piece.rows ? piece.base + (piece.head + row) / p.heads + piece.token : INT32_MAX;  // this row sees keys below
+    const int warp_end = __reduce_min_sync(0xffffffffu, end);
+    float reference = -INFINITY, sum = 0.f;
+    for (int i = 0; i < chunks; ++i, ++count) {
+      const uint32_t stage = count % kStages;
+      // (the tile has landed when its scores are there; this wait makes what was written about it visible)
+      if (!warp_wait(sm.bar(kScoresFull), count & 1, abort_flag) || !warp_wait(sm.bar(kFull0 + stage), (count / kStages) & 1, abort_flag)) { failed = true; meet(true); return; }
+      tc_fence_after_sync();
+      const int key = (piece.first + i) * kChunk, live = *sm.live(stage);
+      float2 s[16];
+      {
+        // Both partial sums of a score come straight to the thread that owns it.
+        uint32_t low_a[16], low_b[16], high_a[16], high_b[16];
+        tmem_ld16_halves<32>(scores, low_a);
+        tmem_ld16_halves<32>(scores + 16, low_b);
+        tmem_ld16_halves<32>(scores + kHighLanes, high_a);
+        tmem_ld16_halves<32>(scores + kHighLanes + 16, high_b);
+        tmem_wait_ld();
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(sm.bar(kScoresFree));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          s[e] = add2(make_float2(__uint_as_float(low_a[2 * e]), __uint_as_float(low_a[2 * e + 1])),
+                      make_float2(__uint_as_float(high_a[2 * e]), __uint_as_float(high_a[2 * e + 1])));
+          s[8 + e] = add2(make_float2(__uint_as_float(low_b[2 * e]), __uint_as_float(low_b[2 * e + 1])),
+                          make_float2(__uint_as_float(high_b[2 * e]), __uint_as_float(high_b[2 * e + 1])));
+        }
+      }
+      if (live < kChunk || key + kChunk > warp_end) {
+        const int seen = min(end - key, live) - half * 32;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          if (2 * e >= seen) s[e].x = -INFINITY;
+          if (2 * e + 1 >= seen) s[e].y = -INFINITY;
+        }
+      }
+      float most[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        most[k] = fmaxf(s[4 * k].x, s[4 * k].y);
+#pragma unroll
+        for (int e = 1; e < 4; ++e) most[k] = greatest(most[k], s[4 * k + e].x, s[4 * k + e].y);
+      }
+      const float own = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * p.scale_log2;  // scale > 0
+      const bool look = __any_sync(0xffffffffu, own > reference + kRoom);
+      float alpha = 1.f;
+      if (look) {
+        const float top = fmaxf(own, __shfl_xor_sync(0xffffffffu, own, 16));
+        if (top > reference + kRoom) {
+          const float next = reference == -INFINITY ? top : top - kStep;
+          alpha = exp2f(reference - next);
+          reference = next;
+        }
+      }
+      float* factors = alphas + (count & 1) * kRows;
+      if (half == 0) factors[row] = alpha;
+      const float shift = reference == -INFINITY ? 0.f : -reference;
+      const float2 scale = make_float2(p.scale_log2, p.scale_log2), shifts = make_float2(shift, shift);
+      float2 sum_a = make_float2(0.f, 0.f), sum_b = sum_a;
+      uint4 packed[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        uint32_t words[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const int e = 4 * u + w;
+          float2 weight = fma2(s[e], scale, shifts);
+          weight.x = exp2f(weight.x);
+          weight.y = exp2f(weight.y);
+          if (e & 1) sum_b = add2(sum_b, weight); else sum_a = add2(sum_a, weight);
+          words[w] = pack2<kFormat>(weight.x, weight.y);
+        }
+        packed[u] = make_uint4(words[0], words[1], words[2], words[3]);
+      }
+      sum = sum * alpha + ((sum_a.x + sum_a.y) + (sum_b.x + sum_b.y));
+      // The product of the chunk before has ended: its weights may be overwritten, the accumulator rescaled.
+      if (count > 0 && !warp_wait(sm.bar(kWeightsFree), (count - 1) & 1, abort_flag)) { failed = true; meet(true); return; }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) *reinterpret_cast<uint4*>(weights + row * 128 + (((half * 4 + u) ^ (row & 7)) << 4)) = packed[u];
+      const uint32_t met = meet(look && i > 0);
+      if (met >= kGivenUp) return;
+      if (met != 0) {
+        tc_fence_after_sync();
+        const float o_alpha = factors[o_row];
+#pragma unroll 1
+        for (int c = 0; c < 256; c += 32) {
+          uint32_t o[32];
+          tmem_ld32(tmem + c + lanes, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * o_alpha);
+          tmem_st32(tmem + c + lanes, o);
+        }
+        tmem_wait_st();
+      }
+      fence_proxy_async();  // the product reads the weights through the async proxy
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(sm.bar(kWeightsFull));
+    }
+    sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+    // ---- output
+    if (chunks > 0) {
+      if (!warp_wait(sm.bar(kWeightsFree), (count - 1) & 1, abort_flag)) { failed = true; meet(true); return; }
+      tc_fence_after_sync();
+    }
+    if (piece.slot >= 0) {  // a part of a tile: sums as they are, [feature][row]
+      if (half == 0 && row < piece.rows) p.statistics[size_t(piece.slot) * kRows + row] = make_float2(reference, sum);
+      float* sums = p.sums + size_t(piece.slot) * kSlotFloats + o_row;
+#pragma unroll 1
+      for (int c = 0; c < 256; c += 32) {
+        uint32_t o[32];
+        tmem_ld32(tmem + c + lanes, o);
+        tmem_wait_ld();
+        if (o_row < piece.rows) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) sums[size_t((c >> 7) * 256 + o_feature + (c & 127) + e) * kRows] = __uint_as_float(o[e]);
+        }
+      }
+      continue;
+    }
+    float log_sum;
+    const float sink = p.sinks != nullptr && row < piece.rows ? __ldg(p.sinks + (piece.head + row) % p.heads) * kLog2E : -INFINITY;
+    const float inverse = inverse_of(reference, sum, sink, &log_sum);
+    if (half == 0) {
+      inverses[row] = inverse;
+      if (p.lse != nullptr && row < piece.rows) p.lse[piece.row + row] = log_sum * kLn2;
+    }
+    if (meet(false) != 0) return;
+    const float o_inverse = inverses[o_row];
+    // 32 rows x 64 bytes per warp and pass, through the warp's quarter of the weights' tile.
+    unsigned char* staged = weights + warp * 2048;
+#pragma unroll 1
+    for (int c = 0; c < 256; c += 32) {
+      uint32_t o[32];
+      if (chunks > 0) {
+        tmem_ld32(tmem + c + lanes, o);
+        tmem_wait_ld();
+      }
+#pragma unroll
+      for (int unit = 0; unit < 4; ++unit) {
+        uint32_t words[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          words[k] = chunks == 0 || o_inverse == 0.f ? 0u : pack2<kFormat>(__uint_as_float(o[unit * 8 + 2 * k]) * o_inverse, __uint_as_float(o[unit * 8 + 2 * k + 1]) * o_inverse);
+        *reinterpret_cast<uint4*>(staged + lane * 64 + ((unit ^ ((lane >> 1) & 3)) << 4)) = make_uint4(words[0], words[1], words[2], words[3]);
+      }
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = i * 8 + (lane >> 2), unit = lane & 3, target = (warp & 1) * 32 + r;
+        const uint4 v = *reinterpret_cast<const uint4*>(staged + r * 64 + ((unit ^ ((r >> 1) & 3)) << 4));
+        if (target < piece.rows)
+          *reinterpret_cast<uint4*>(p.out + ((piece.row + target) * LATENT_VALUES + (c >> 7) * 256 + o_feature + (c & 127) + unit * 8) * 2) = v;
+      }
+      __syncwarp();
+    }
+    if (meet(false) != 0) return;  // the inverses and the weights' tile are free again
+  }
+  if (*abort_flag != 0) failed = true;
+  meet(false);  // with a warp that has given up since the last time
+}
+
+// ---- kernels and launch ------------------------------------------------------------------------------------------------
+
+template <int kFormat, int kWidth>
+__global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_constant__ Params p) {
+  using L = Layout<kWidth>;
+  extern __shared__ unsigned char smem_raw[];
+  Shared sm;
+  const uint32_t raw = smem_u32(smem_raw), pad = (1024u - (raw & 1023u)) & 1023u;
+  sm.base = raw + pad;
+  sm.ptr = smem_raw + pad;
+  sm.bars = L::kSmemBars;
+  sm.pieces = L::kSmemPieces;
+  sm.misc = L::kSmemMisc;
+  const int warp = threadIdx.x >> 5;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kBarCount; ++i) {
+      int arrivals = 1;
+      if (i >= kPieceDone0 && i < kPieceDone0 + kPieces) arrivals = kSoftmaxWarps + 3 + kQueryWarps;
+      else if (i == kQFull) arrivals = kQueryWarps;
+      else if (i == kScoresFree || i == kWeightsFull || i == kPlaces) arrivals = kSoftmaxWarps;
+      mbar_init(sm.bar(i), arrivals);
+    }
+    mbar_fence_init();
+    *sm.abort_flag() = 0;
+  }
+  if (warp == kScoreWarp) { tmem_alloc(smem_u32(sm.tmem_slot()), 512); tmem_relinquish(); }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = *sm.tmem_slot();
+  wait_for_predecessor();
+  let_successor_start();
+  int request = 0;
+  int64_t before = 0;
+  const Borders borders = plan_block(p, sm.scan(), &request, &before);
+  fence_proxy_async();  // the plan's scratch is the first tile's memory
+  __syncthreads();
+  if (warp < kSoftmaxWarps) softmax_role<kFormat, kWidth>(p, sm, tmem);
+  else if (warp == kScoreWarp) { if (elect_one()) score_role<kFormat, kWidth>(sm, tmem); __syncwarp(); }
+  else if (warp == kValueWarp) { if (elect_one()) value_role<kFormat, kWidth>(sm, tmem); __syncwarp(); }
+  else if (warp == kCopyWarp) copy_role<kWidth>(p, sm);
+  else if (warp == kPlanWarp) plan_role(p, sm, borders, request, before);
+  else query_role<kWidth>(p, sm, tmem);
+  tc_fence_before_sync();
+  __syncthreads();
+  if (threadIdx.x == 0 && *sm.abort_flag() != 0) report(p.status, SPARSE_MLA_STATUS_WAIT_EXPIRED, blockIdx.x, 0);
+  if (warp == kScoreWarp) tmem_dealloc(tmem, 512);
+}
+
+// Tiles that several blocks worked on: block (i, y) adds up features 16 y .. + 15 of the tile that begins in block i, four per thread.
+constexpr int kCombineThreads = 256, kCombineFeatures = 16;
+template <int kFormat>
+__global__ void __launch_bounds__(kCombineThreads) combine_kernel(const __grid_constant__ Params p) {
+  wait_for_predecessor();
+  let_successor_start();
+  const Record record = p.records[blockIdx.x];
+  if (record.last < 0) return;
+  const int row = threadIdx.x & 63, group = threadIdx.x >> 6, first = int(blockIdx.x);
+  if (row >= record.rows) return;
+  auto slot_of = [&](int i) { return i == first ? 2 * i + 1 : 2 * i; };
+  float reference = -INFINITY;
+  for (int i = first; i <= record.last; ++i)
+    if (i == first || p.records[i].continued) reference = fmaxf(reference, p.statistics[size_t(slot_of(i)) * kRows + row].x);
+  const int feature = blockIdx.y * kCombineFeatures + group * 4;
+  float sum = 0.f, total[4] = {};
+  for (int i = first; i <= record.last; ++i) {
+    if (i != first && !p.records[i].continued) continue;
+    const float2 part = p.statistics[size_t(slot_of(i)) * kRows + row];
+    const float factor = part.x == -INFINITY ? 0.f : exp2f(part.x - reference);
+    sum += part.y * factor;
+    const float* values = p.sums + size_t(slot_of(i)) * kSlotFloats + size_t(feature) * kRows + row;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) total[k] += values[k * kRows] * factor;
+  }
+  float log_sum;
+  const float sink = p.sinks != nullptr ? __ldg(p.sinks + (record.head + row) % p.heads) * kLog2E : -INFINITY;
+  const float inverse = inverse_of(reference, sum, sink, &log_sum);
+  if (p.lse != nullptr && feature == 0) p.lse[record.row + row] = log_sum * kLn2;
+  uint2 words = make_uint2(0, 0);
+  if (inverse != 0.f) words = make_uint2(pack2<kFormat>(total[0] * inverse, total[1] * inverse), pack2<kFormat>(total[2] * inverse, total[3] * inverse));
+  *reinterpret_cast<uint2*>(p.out + ((record.row + row) * LATENT_VALUES + feature) * 2) = words;
+}
+
+template <int kFormat, int kWidth>
+int launch(const Params& p, int blocks, cudaStream_t stream) {
+  using L = Layout<kWidth>;
+  static bool configured[64] = {false};  // a per-device setting: plain words written with the same value by whoever gets there first
+  int device = 0;
+  if (const cudaError_t error = cudaGetDevice(&device)) return int(error);
+  if (device < 0 || device >= 64) return -1;
+  if (!configured[device]) {
+    if (const cudaError_t error = cudaFuncSetAttribute(attention_kernel<kFormat, kWidth>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmemBytes)) return int(error);
+    configured[device] = true;
+  }
+  if (const cudaError_t error = launch_overlapped(attention_kernel<kFormat, kWidth>, blocks, kThreads, L::kSmemBytes, stream, p)) return int(error);
+  cudaLaunchAttribute overlap = {};
+  overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  overlap.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(unsigned(blocks), LATENT_VALUES / kCombineFeatures);
+  config.blockDim = dim3(kCombineThreads);
+  config.stream = stream;
+  config.attrs = &overlap;
+  config.numAttrs = 1;
+  return int(cudaLaunchKernelEx(&config, combine_kernel<kFormat>, p));
+}
+
+}  // namespace absorbed
 }  // namespace latent
 
 extern "C" {
 
 int workspace_size_latent_attention(uint64_t* bytes) {
+  using namespace latent;
   if (bytes == nullptr) return -1;
-  *bytes = 512;
+  *bytes = absorbed::workspace_bytes(multiprocessors());
   return 0;
 }
 
 int launch_latent_attention(void* stream, const latent_attention_call* call) {
   using namespace latent;
   const latent_attention_call& c = *call;
-  if ((c.type != LATENT_F16 && c.type != LATENT_BF16) || (c.width != 512 && c.width != 576)) return -1;
-  if (c.batches < 0 || c.tokens < 0 || c.heads < 1 || c.pages < 0 || c.blocks < 0 || c.page_rows < 64 || c.page_rows % 64 != 0) return -1;
+  if ((c.type != LATENT_F16 && c.type != LATENT_BF16) || (c.width != 512 && c.width != 576) || !(c.scale > 0)) return -1;
+  if (c.batches < 0 || c.batches > INT32_MAX / 2 || c.tokens < 0 || c.heads < 1 || c.tokens > (int64_t(1) << 30) / c.heads) return -1;
+  if (c.pages < 0 || c.blocks < 0 || c.page_rows < 64 || c.page_rows % 64 != 0 || c.pages > (INT32_MAX - 128) / c.page_rows || c.blocks > INT32_MAX / c.page_rows) return -1;
   if (c.tokens == 0 || c.batches == 0) return 0;
-  auto* kernel = c.type == LATENT_BF16 ? (c.width == 576 ? attention_kernel<__nv_bfloat16, 576> : attention_kernel<__nv_bfloat16, 512>)
-                                       : (c.width == 576 ? attention_kernel<__half, 576> : attention_kernel<__half, 512>);
-  kernel<<<unsigned((c.tokens * c.heads + 7) / 8), 256, 0, static_cast<cudaStream_t>(stream)>>>(c);
-  return int(cudaGetLastError());
+  if (c.workspace == nullptr || c.status == nullptr) return -1;
+  const int blocks = multiprocessors();
+  absorbed::Params p = {};
+  // (without pages nothing is copied)
+  const int64_t sizes[2] = {c.width, c.blocks > 0 ? c.blocks * c.page_rows : 1}, strides[1] = {c.width};
+  if (const int e = sm100::encode_map(&p.cache, c.type, 2, c.blocks > 0 ? c.cache : c.q, sizes, strides, 1, absorbed::kChunk)) return e;
+  char* workspace = static_cast<char*>(c.workspace);
+  p.q = static_cast<const char*>(c.q);
+  p.table = c.block_table;
+  p.cu = c.cu_seqlens_q;
+  p.lengths = c.seqused_kv;
+  p.sinks = c.sinks;
+  p.out = static_cast<char*>(c.out);
+  p.lse = c.lse;
+  p.records = reinterpret_cast<absorbed::Record*>(workspace);
+  p.statistics = reinterpret_cast<float2*>(workspace + absorbed::statistics_offset(blocks));
+  p.sums = reinterpret_cast<float*>(workspace + absorbed::sums_offset(blocks));
+  p.status = c.status;
+  p.batches = int32_t(c.batches);
+  p.tokens = int32_t(c.tokens);
+  p.heads = int32_t(c.heads);
+  p.pages = int32_t(c.pages);
+  p.blocks = int32_t(c.blocks);
+  p.page_rows = int32_t(c.page_rows);
+  p.scale_log2 = float(c.scale * 1.4426950408889634);
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (c.type == LATENT_BF16) return c.width == 576 ? absorbed::launch<1, 576>(p, blocks, s) : absorbed::launch<1, 512>(p, blocks, s);
+  return c.width == 576 ? absorbed::launch<0, 576>(p, blocks, s) : absorbed::launch<0, 512>(p, blocks, s);
 }
 
 }  // extern "C"

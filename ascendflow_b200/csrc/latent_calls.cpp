@@ -167,7 +167,7 @@ struct Paged {
 bool paged(const Tensor& cache, const Tensor& table, const Tensor& cu, const Tensor& lengths, int device, at::ScalarType type, Paged* p) {
   if (cache.dim() != 4 || table.dim() != 2) return false;
   *p = {table.size(0), table.size(1), cache.size(0), cache.size(1), cache.size(3)};
-  if (p->page_rows < 64 || p->page_rows % 64 != 0 || p->blocks > INT32_MAX / p->page_rows || p->batches > INT32_MAX / 2 || p->pages > INT32_MAX / p->page_rows) return false;
+  if (p->page_rows < 64 || p->page_rows % 64 != 0 || p->blocks > (INT32_MAX - 128) / p->page_rows || p->batches > INT32_MAX / 2 || p->pages > (INT32_MAX - 128) / p->page_rows) return false;
   return plain(cache, device, type, {p->blocks, p->page_rows, 1, p->width}) && rows_aligned(cache) && plain(table, device, at::kInt, {p->batches, p->pages}) &&
          plain(cu, device, at::kInt, {p->batches + 1}) && plain(lengths, device, at::kInt, {p->batches});
 }

@@ -215,7 +215,7 @@ def _check_paged(cache, block_table, cu_seqlens_q, seqused_kv, dtype):
     require(isinstance(block_table, torch.Tensor) and block_table.dim() == 2, "block_table: expected [B, PAGES]")
     batches, pages = block_table.shape
     _tensor(block_table, "block_table", (torch.int32,), (batches, pages))
-    require(max(cache.shape[0], pages) * cache.shape[1] < 1 << 31, "cache and block_table: positions must fit 31 bits")
+    require(max(cache.shape[0], pages) * cache.shape[1] < (1 << 31) - 128, "cache and block_table: positions must fit 31 bits")
     _tensor(cu_seqlens_q, "cu_seqlens_q", (torch.int32,), (batches + 1,))
     _tensor(seqused_kv, "seqused_kv", (torch.int32,), (batches,))
 
