@@ -80,10 +80,9 @@ struct Record {
   int64_t row;
   int rows, head;
   int last;       // block that has the tile's end; -1: no tile begins here that ends elsewhere
-  int continued;  // slot 2 i holds a part of the tile before
-  int pad[2];
+  int pad[3];
 };
-constexpr int kSlotFloats = LATENT_VALUES * kRows;  // [feature][row]
+constexpr int kSlotFloats = kRows * LATENT_VALUES;
 inline size_t statistics_offset(int blocks) { return size_t(blocks) * sizeof(Record); }
 inline size_t sums_offset(int blocks) { return (statistics_offset(blocks) + size_t(blocks) * 2 * kRows * sizeof(float2) + 511) / 512 * 512; }
 inline size_t workspace_bytes(int blocks) { return sums_offset(blocks) + size_t(blocks) * 2 * kSlotFloats * sizeof(float); }
@@ -164,61 +163,121 @@ struct Borders {
 // A block with fewer chunks than these loses more with its start and with its part of the sums than it takes off the others.
 constexpr int kLeastChunks = 4;
 
-// By all threads of the block: the total, and the request that cost `border(blockIdx.x)` lies in (with the cost in front of it).
-__device__ __forceinline__ Borders plan_block(const Params& p, int64_t* scan, int* request, int64_t* before) {
+// Where a stretch begins: a request's tile and the cost in front of that.
+struct Place {
+  int request, tile;
+  int64_t start;
+};
+
+// Sum over the block's threads, for all of them.
+__device__ __forceinline__ int64_t block_sum(int64_t value, int64_t* scratch) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) value += __shfl_xor_sync(0xffffffffu, value, d);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = value;
+  __syncthreads();
+  int64_t sum = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) sum += scratch[w];
+  return sum;
+}
+
+// By all threads of the block: the stretches, and where this block's begins.
+//
+// The order of the tiles: the first tile of every request, then the second ones, and so on. Where requests have as many tiles each, and
+// the blocks are a multiple of that, the blocks that work on a request's tiles go through its chunks side by side: a chunk comes from
+// memory once and from L2 for the others. (Tile after tile they would be chunks apart: 32 requests of 6 tiles and 256 chunks then
+// read 3.6 GB instead of 0.6.) Up to a sixteenth of the blocks is given up for that.
+__device__ __forceinline__ Borders plan_block(const Params& p, int64_t* scratch, Place* place) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int kWarps = kThreads / 32;
-  Borders borders = {0, 1};
-  int64_t own = 0, inclusive = 0;
-  auto sum_up = [&](int first) {  // costs of kThreads requests: own, and with all in front of them; returns their sum
-    const int b = first + int(threadIdx.x);
-    own = 0;
-    if (b < p.batches) {
-      const Request r = request_at(p, b);
-      own = r.cost(r.tiles);
+  const int rounds = (p.batches + kThreads - 1) / kThreads;
+  Request none = {};
+  const Request own = int(threadIdx.x) < p.batches ? request_at(p, threadIdx.x) : none;
+  auto of_round = [&](int round) {
+    const int b = round * kThreads + int(threadIdx.x);
+    return round == 0 ? own : b < p.batches ? request_at(p, b) : none;
+  };
+  Borders borders = {0, 0};
+  int64_t cost = 0;
+  int most_tiles = 0, least_tiles = INT32_MAX;
+  for (int round = 0; round < rounds; ++round) {
+    const Request r = of_round(round);
+    cost += r.cost(r.tiles);
+    most_tiles = max(most_tiles, r.tiles);
+    if (r.tiles > 0) least_tiles = min(least_tiles, r.tiles);
+  }
+  most_tiles = __reduce_max_sync(0xffffffffu, most_tiles);
+  least_tiles = __reduce_min_sync(0xffffffffu, least_tiles);
+  if (lane == 0) scratch[kWarps + warp] = int64_t(most_tiles) << 32 | uint32_t(least_tiles);
+  borders.total = block_sum(cost, scratch);
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    most_tiles = max(most_tiles, int(scratch[kWarps + w] >> 32));
+    least_tiles = min(least_tiles, int(uint32_t(scratch[kWarps + w])));
+  }
+  if (borders.total == 0) return borders;
+  const int grid = int(gridDim.x);
+  int blocks = int(min(max(borders.total / (kLeastChunks * kChunk), int64_t(1)), int64_t(grid)));
+  if (most_tiles == least_tiles && blocks % most_tiles <= blocks / 16) blocks -= blocks % most_tiles;
+  if (int(blockIdx.x) >= blocks) return borders;
+  borders.blocks = blocks;
+  const int64_t mine = borders.at(blockIdx.x);
+  // The tile: the last whose predecessors cost no more.
+  int tile = 0;
+  int64_t passed = 0;
+  for (int high = most_tiles; high - tile > 1;) {
+    const int middle = (tile + high) >> 1;
+    int64_t before = 0;
+    for (int round = 0; round < rounds; ++round) {
+      const Request r = of_round(round);
+      before += r.cost(min(middle, r.tiles));
     }
-    inclusive = own;
+    before = block_sum(before, scratch);
+    if (before <= mine) {
+      tile = middle;
+      passed = before;
+    } else {
+      high = middle;
+    }
+  }
+  // The request.
+  for (int round = 0; round < rounds; ++round) {
+    const Request r = of_round(round);
+    const int64_t value = r.tiles > tile ? r.cost(tile + 1) - r.cost(tile) : 0;
+    int64_t inclusive = value;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const int64_t other = __shfl_up_sync(0xffffffffu, inclusive, d);
       if (lane >= d) inclusive += other;
     }
     __syncthreads();
-    if (lane == 31) scan[warp] = inclusive;
+    if (lane == 31) scratch[warp] = inclusive;
     __syncthreads();
-    int64_t sum = 0;
+    int64_t sum = 0, in_front = 0;
+#pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      if (w == warp) inclusive += sum;
-      sum += scan[w];
+      if (w == warp) in_front = sum;
+      sum += scratch[w];
     }
-    return sum;
-  };
-  for (int first = 0; first < p.batches; first += kThreads) borders.total += sum_up(first);
-  const int64_t most = borders.total / (kLeastChunks * kChunk);
-  borders.blocks = int(min(max(most, int64_t(1)), int64_t(gridDim.x)));
-  if (int(blockIdx.x) >= borders.blocks || borders.total == 0) { borders.blocks = 0; return borders; }
-  const int64_t mine = borders.at(blockIdx.x);
-  int64_t passed = 0;
-  for (int first = 0; first < p.batches; first += kThreads) {
-    const int64_t sum = p.batches <= kThreads ? borders.total : sum_up(first);  // (one round: the values are still there)
-    const int64_t start = passed + inclusive - own;
-    if (own > 0 && start <= mine && mine < start + own) {
-      scan[kWarps] = first + int(threadIdx.x);
-      scan[kWarps + 1] = start;
+    const int64_t start = passed + in_front + inclusive - value;
+    if (value > 0 && start <= mine && mine < start + value) {
+      scratch[2 * kWarps] = round * kThreads + int(threadIdx.x);
+      scratch[2 * kWarps + 1] = start;
     }
     passed += sum;
   }
   __syncthreads();
-  *request = int(scan[kWarps]);
-  *before = scan[kWarps + 1];
+  *place = {int(scratch[2 * kWarps]), tile, scratch[2 * kWarps + 1]};
   return borders;
 }
 
 // The pieces of this block, announced one after the other (by one warp; all lanes work out the same).
-__device__ void plan_role(const Params& p, const Shared& sm, const Borders& borders, int request, int64_t before) {
+__device__ void plan_role(const Params& p, const Shared& sm, const Borders& borders, const Place& place) {
   const int lane = threadIdx.x & 31;
   volatile int* abort_flag = sm.abort_flag();
-  Record record = {0, 0, 0, -1, 0, {0, 0}};
+  Record record = {0, 0, 0, -1, {0, 0, 0}};
+  bool continued = false;  // slot 2 i holds a part of the tile before
   uint32_t announced = 0;
   // A free entry of the ring; false when somebody has given up.
   auto claim = [&]() { return announced < kPieces || warp_wait(sm.bar(kPieceDone0 + announced % kPieces), (announced / kPieces - 1) & 1, abort_flag); };
@@ -232,15 +291,11 @@ __device__ void plan_role(const Params& p, const Shared& sm, const Borders& bord
   if (borders.blocks > 0) {
     const int64_t end = borders.at(blockIdx.x + 1);
     int64_t at = borders.at(blockIdx.x);
-    Request r = request_at(p, request);
-    int tile = 0;
-    for (int low = 0, high = r.tiles; high - low > 1;) {  // cost(low) <= at - before < cost(high)
-      const int middle = (low + high) >> 1;
-      if (r.cost(middle) <= at - before) low = middle; else high = middle;
-      tile = low;
-    }
+    int request = place.request, tile = place.tile;
+    int64_t start = place.start;
     while (at < end) {
-      const int64_t start = before + r.cost(tile), past = before + r.cost(tile + 1), cost = past - start;
+      const Request r = request_at(p, request);
+      const int64_t cost = r.cost(tile + 1) - r.cost(tile), past = start + cost;
       const int chunks = chunks_of(p, r, tile);
       Piece piece;
       piece.first = int((at - start) * chunks / cost);
@@ -266,28 +321,29 @@ __device__ void plan_role(const Params& p, const Shared& sm, const Borders& bord
           while (last + 1 < borders.blocks && borders.at(last + 1) < past) ++last;
           record.last = last;
         } else if (!whole) {
-          record.continued = 1;
+          continued = true;
         }
         if (!claim()) break;
         announce(piece);
       }
       at = min(past, end);
-      if (past <= end && ++tile >= r.tiles) {
-        before = past;
-        if (at >= end) break;
-        // The next request that has rows. (There is one: cost is left.)
-        tile = 0;
-        unsigned hit = 0;
-        for (int b = request + 1; hit == 0 && b < p.batches; b += 32) {
-          hit = __ballot_sync(0xffffffffu, b + lane < p.batches && request_at(p, b + lane).rows > 0);
-          request = b + __ffs(hit) - 1;
+      if (at >= end) break;
+      // The next request that has such a tile, or the first that has one more.
+      start = past;
+      unsigned hit = 0;
+      for (int turn = 0; turn < 2 && hit == 0; ++turn) {
+        for (int b = turn == 0 ? request + 1 : 0; hit == 0 && b < p.batches; b += 32) {
+          hit = __ballot_sync(0xffffffffu, b + lane < p.batches && request_at(p, b + lane).tiles > tile);
+          if (hit != 0) request = b + __ffs(hit) - 1;
         }
-        if (hit == 0) break;
-        r = request_at(p, request);
+        if (hit == 0) ++tile;
       }
+      if (hit == 0) break;  // (does not happen: there is cost left)
     }
   }
   if (lane == 0) p.records[blockIdx.x] = record;
+  if (!continued)
+    for (int row = lane; row < kRows; row += 32) p.statistics[size_t(2 * blockIdx.x) * kRows + row] = make_float2(-INFINITY, 0.f);
   if (!claim()) return;
   Piece none = {};
   none.first = -1;
@@ -508,6 +564,12 @@ __device__ __forceinline__ float inverse_of(float reference, float sum, float si
   return sum == 0.f ? 0.f : share / (total * sum);
 }
 
+// 32 bytes (aligned) in one store: a whole sector of a lane's own row.
+__device__ __forceinline__ void store32(float* at, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n"
+               ::"l"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+}
+
 template <int kFormat, int kWidth>
 __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
   using L = Layout<kWidth>;
@@ -645,9 +707,9 @@ __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
       if (!warp_wait(sm.bar(kWeightsFree), (count - 1) & 1, abort_flag)) { failed = true; meet(true); return; }
       tc_fence_after_sync();
     }
-    if (piece.slot >= 0) {  // a part of a tile: sums as they are, [feature][row]
+    if (piece.slot >= 0) {  // a part of a tile: sums as they are
       if (half == 0 && row < piece.rows) p.statistics[size_t(piece.slot) * kRows + row] = make_float2(reference, sum);
-      float* sums = p.sums + size_t(piece.slot) * kSlotFloats + o_row;
+      float* sums = p.sums + size_t(piece.slot) * kSlotFloats + o_row * LATENT_VALUES + o_feature;
 #pragma unroll 1
       for (int c = 0; c < 256; c += 32) {
         uint32_t o[32];
@@ -655,7 +717,7 @@ __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
         tmem_wait_ld();
         if (o_row < piece.rows) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) sums[size_t((c >> 7) * 256 + o_feature + (c & 127) + e) * kRows] = __uint_as_float(o[e]);
+          for (int e = 0; e < 32; e += 8) store32(sums + (c >> 7) * 256 + (c & 127) + e, o + e);
         }
       }
       continue;
@@ -734,16 +796,15 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
   const uint32_t tmem = *sm.tmem_slot();
   wait_for_predecessor();
   let_successor_start();
-  int request = 0;
-  int64_t before = 0;
-  const Borders borders = plan_block(p, sm.scan(), &request, &before);
+  Place place = {};
+  const Borders borders = plan_block(p, sm.scan(), &place);
   fence_proxy_async();  // the plan's scratch is the first tile's memory
   __syncthreads();
   if (warp < kSoftmaxWarps) softmax_role<kFormat, kWidth>(p, sm, tmem);
   else if (warp == kScoreWarp) { if (elect_one()) score_role<kFormat, kWidth>(sm, tmem); __syncwarp(); }
   else if (warp == kValueWarp) { if (elect_one()) value_role<kFormat, kWidth>(sm, tmem); __syncwarp(); }
   else if (warp == kCopyWarp) copy_role<kWidth>(p, sm);
-  else if (warp == kPlanWarp) plan_role(p, sm, borders, request, before);
+  else if (warp == kPlanWarp) plan_role(p, sm, borders, place);
   else query_role<kWidth>(p, sm, tmem);
   tc_fence_before_sync();
   __syncthreads();
@@ -751,39 +812,65 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
   if (warp == kScoreWarp) tmem_dealloc(tmem, 512);
 }
 
-// Tiles that several blocks worked on: block (i, y) adds up features 16 y .. + 15 of the tile that begins in block i, four per thread.
-constexpr int kCombineThreads = 256, kCombineFeatures = 16;
+// Tiles that several blocks worked on: block (i, y) adds up rows 4 y .. + 3 of the tile that begins in block i, a row by two warps. A lane has
+// the factors of every 32nd part.
+constexpr int kCombineThreads = 256, kCombineRows = 4, kMostParts = 8;  // of 32
 template <int kFormat>
 __global__ void __launch_bounds__(kCombineThreads) combine_kernel(const __grid_constant__ Params p) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   wait_for_predecessor();
   let_successor_start();
   const Record record = p.records[blockIdx.x];
-  if (record.last < 0) return;
-  const int row = threadIdx.x & 63, group = threadIdx.x >> 6, first = int(blockIdx.x);
-  if (row >= record.rows) return;
-  auto slot_of = [&](int i) { return i == first ? 2 * i + 1 : 2 * i; };
+  const int row = int(blockIdx.y) * kCombineRows + (warp >> 1), first = int(blockIdx.x);
+  if (record.last < 0 || row >= record.rows) return;
+  const int parts = record.last - first + 1;
+  auto slot_of = [&](int part) { return size_t(part == 0 ? 2 * first + 1 : 2 * (first + part)); };
+  // (a block that had none of the tile's chunks has said so: reference -infinity)
+  float2 own[kMostParts];
   float reference = -INFINITY;
-  for (int i = first; i <= record.last; ++i)
-    if (i == first || p.records[i].continued) reference = fmaxf(reference, p.statistics[size_t(slot_of(i)) * kRows + row].x);
-  const int feature = blockIdx.y * kCombineFeatures + group * 4;
-  float sum = 0.f, total[4] = {};
-  for (int i = first; i <= record.last; ++i) {
-    if (i != first && !p.records[i].continued) continue;
-    const float2 part = p.statistics[size_t(slot_of(i)) * kRows + row];
-    const float factor = part.x == -INFINITY ? 0.f : exp2f(part.x - reference);
-    sum += part.y * factor;
-    const float* values = p.sums + size_t(slot_of(i)) * kSlotFloats + size_t(feature) * kRows + row;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) total[k] += values[k * kRows] * factor;
+  for (int k = 0; k < kMostParts; ++k) {
+    own[k] = k * 32 + lane < parts ? p.statistics[slot_of(k * 32 + lane) * kRows + row] : make_float2(-INFINITY, 0.f);
+    reference = fmaxf(reference, own[k].x);
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) reference = fmaxf(reference, __shfl_xor_sync(0xffffffffu, reference, d));
+  float sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < kMostParts; ++k) {
+    own[k].x = own[k].x == -INFINITY ? 0.f : exp2f(own[k].x - reference);
+    sum += own[k].x * own[k].y;
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  const int feature = (warp & 1) * 256 + lane * 8;
+  float total[8] = {};
+#pragma unroll
+  for (int k = 0; k < kMostParts; ++k) {
+    const int here = min(parts - k * 32, 32);
+#pragma unroll 8
+    for (int m = 0; m < here; ++m) {
+      const float factor = __shfl_sync(0xffffffffu, own[k].x, m);
+      if (factor == 0.f) continue;  // (its sums may be anything)
+      const float4* values = reinterpret_cast<const float4*>(p.sums + slot_of(k * 32 + m) * kSlotFloats + size_t(row) * LATENT_VALUES + feature);
+      const float4 a = __ldg(values), b = __ldg(values + 1);
+      total[0] += a.x * factor; total[1] += a.y * factor; total[2] += a.z * factor; total[3] += a.w * factor;
+      total[4] += b.x * factor; total[5] += b.y * factor; total[6] += b.z * factor; total[7] += b.w * factor;
+    }
   }
   float log_sum;
   const float sink = p.sinks != nullptr ? __ldg(p.sinks + (record.head + row) % p.heads) * kLog2E : -INFINITY;
   const float inverse = inverse_of(reference, sum, sink, &log_sum);
-  if (p.lse != nullptr && feature == 0) p.lse[record.row + row] = log_sum * kLn2;
-  uint2 words = make_uint2(0, 0);
-  if (inverse != 0.f) words = make_uint2(pack2<kFormat>(total[0] * inverse, total[1] * inverse), pack2<kFormat>(total[2] * inverse, total[3] * inverse));
-  *reinterpret_cast<uint2*>(p.out + ((record.row + row) * LATENT_VALUES + feature) * 2) = words;
+  if (p.lse != nullptr && (threadIdx.x & 63) == 0) p.lse[record.row + row] = log_sum * kLn2;
+  uint4 words = make_uint4(0, 0, 0, 0);
+  if (inverse != 0.f)
+    words = make_uint4(pack2<kFormat>(total[0] * inverse, total[1] * inverse), pack2<kFormat>(total[2] * inverse, total[3] * inverse),
+                       pack2<kFormat>(total[4] * inverse, total[5] * inverse), pack2<kFormat>(total[6] * inverse, total[7] * inverse));
+  *reinterpret_cast<uint4*>(p.out + ((record.row + row) * LATENT_VALUES + feature) * 2) = words;
 }
+
+// One block per SM; no more than `combine_kernel` has room for.
+int grid() { const int count = multiprocessors(); return count < kMostParts * 32 ? count : kMostParts * 32; }
 
 template <int kFormat, int kWidth>
 int launch(const Params& p, int blocks, cudaStream_t stream) {
@@ -801,7 +888,7 @@ int launch(const Params& p, int blocks, cudaStream_t stream) {
   overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   overlap.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(unsigned(blocks), LATENT_VALUES / kCombineFeatures);
+  config.gridDim = dim3(unsigned(blocks), kRows / kCombineRows);
   config.blockDim = dim3(kCombineThreads);
   config.stream = stream;
   config.attrs = &overlap;
@@ -817,7 +904,7 @@ extern "C" {
 int workspace_size_latent_attention(uint64_t* bytes) {
   using namespace latent;
   if (bytes == nullptr) return -1;
-  *bytes = absorbed::workspace_bytes(multiprocessors());
+  *bytes = absorbed::workspace_bytes(absorbed::grid());
   return 0;
 }
 
@@ -829,7 +916,7 @@ int launch_latent_attention(void* stream, const latent_attention_call* call) {
   if (c.pages < 0 || c.blocks < 0 || c.page_rows < 64 || c.page_rows % 64 != 0 || c.pages > (INT32_MAX - 128) / c.page_rows || c.blocks > INT32_MAX / c.page_rows) return -1;
   if (c.tokens == 0 || c.batches == 0) return 0;
   if (c.workspace == nullptr || c.status == nullptr) return -1;
-  const int blocks = multiprocessors();
+  const int blocks = latent::absorbed::grid();
   absorbed::Params p = {};
   // (without pages nothing is copied)
   const int64_t sizes[2] = {c.width, c.blocks > 0 ? c.blocks * c.page_rows : 1}, strides[1] = {c.width};
