@@ -564,12 +564,6 @@ __device__ __forceinline__ float inverse_of(float reference, float sum, float si
   return sum == 0.f ? 0.f : share / (total * sum);
 }
 
-// 32 bytes (aligned) in one store: a whole sector of a lane's own row.
-__device__ __forceinline__ void store32(float* at, const uint32_t* v) {
-  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n"
-               ::"l"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
-}
-
 template <int kFormat, int kWidth>
 __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
   using L = Layout<kWidth>;
@@ -717,7 +711,7 @@ __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
         tmem_wait_ld();
         if (o_row < piece.rows) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 8) store32(sums + (c >> 7) * 256 + (c & 127) + e, o + e);
+          for (int e = 0; e < 32; e += 8) store_sector(sums + (c >> 7) * 256 + (c & 127) + e, o + e);
         }
       }
       continue;

@@ -10,6 +10,8 @@
 //   warp 8          one thread issues the products.
 //   warp 9          one thread brings boxes of 64 features x 128 rows (16 KiB) by tensor copies into a ring of eight:
 //                   three of a key tile (128 features of the head, 64 of rope), two of a value tile, in the order of their use.
+//   warp 10         finds out what the block does next: blocks that have not started yet are taken over, one after the other, by those
+//                   that run (cluster launch control). The copies and first products of the next 256 rows run beside the output of the last.
 //
 // Tensor memory: scores (P over their first half) of tile t in columns 128 t .. + 127, O of tile t in 256 + 128 t .. + 127.
 //
@@ -25,21 +27,26 @@ using namespace sm100;
 
 constexpr int kTile = 128;                    // query rows of a tile, keys of a step
 constexpr int kFeatures = LATENT_NOPE + LATENT_ROPE;
-constexpr int kThreads = 320;
-constexpr int kProductWarp = 8, kCopyWarp = 9;
+constexpr int kThreads = 384;  // (the last warp has nothing to do but to give registers away)
+constexpr int kSoftmaxWarps = 8, kProductWarp = 8, kCopyWarp = 9, kPlanWarp = 10;
 constexpr int kBoxBytes = kTile * 128;        // 64 features of 128 rows
 constexpr int kQBoxes = kFeatures / 64, kKeyBoxes = 3, kValueBoxes = 2, kRing = 8;
+constexpr int kItems = 2;                     // announced ahead
 
-constexpr int kSmemQ = 0;                                       // two tiles of three boxes; the output on its way out in the end
+constexpr int kSmemQ = 0;                                       // two tiles of three boxes
 constexpr int kSmemRing = kSmemQ + 2 * kQBoxes * kBoxBytes;
 constexpr int kSmemBars = kSmemRing + kRing * kBoxBytes;
-constexpr int kSmemEnd = kSmemBars + 256;
+constexpr int kSmemMisc = kSmemBars + 320;                       // tensor-memory slot, abort flag; 32: answer of the launch control; 64: items
+constexpr int kSmemEnd = kSmemMisc + 64 + kItems * 32;
 constexpr int kSmemBytes = kSmemEnd + 1024;                     // the tiles are aligned to 1024 bytes
 
 constexpr uint32_t kColumnsO = 256;
 
-enum Bar { kFull0 = 0, kFree0 = kRing, kQFull = 2 * kRing, kScores0, kScores1, kWeights0, kWeights1, kOut0, kOut1, kMended, kBarCount };
-static_assert(kBarCount * 8 + 16 <= 256, "barriers, tensor-memory slot and abort flag");
+enum Bar {
+  kFull0 = 0, kFree0 = kRing, kQFull0 = 2 * kRing, kQFree0 = kQFull0 + 2, kScores0 = kQFree0 + 2, kWeights0 = kScores0 + 2, kOut0 = kWeights0 + 2,
+  kMended = kOut0 + 2, kAnswer, kLastStep, kItemReady0, kItemDone0 = kItemReady0 + kItems, kBarCount = kItemDone0 + kItems
+};
+static_assert(kBarCount <= 40, "the barrier area");
 
 struct Params {
   CUtensorMap q, k, v, rope;
@@ -56,8 +63,10 @@ struct Shared {
   uint32_t base;
   unsigned char* ptr;
   __device__ __forceinline__ uint32_t bar(int which) const { return base + kSmemBars + which * 8; }
-  __device__ __forceinline__ uint32_t* slot() const { return reinterpret_cast<uint32_t*>(ptr + kSmemBars + 240); }
-  __device__ __forceinline__ volatile int* abort_flag() const { return reinterpret_cast<volatile int*>(ptr + kSmemBars + 244); }
+  __device__ __forceinline__ uint32_t* slot() const { return reinterpret_cast<uint32_t*>(ptr + kSmemMisc); }
+  __device__ __forceinline__ volatile int* abort_flag() const { return reinterpret_cast<volatile int*>(ptr + kSmemMisc + 4); }
+  __device__ __forceinline__ uint32_t answer() const { return base + kSmemMisc + 32; }
+  __device__ __forceinline__ struct Item* item(uint32_t index) const;
 };
 
 // 256 query rows of a head.
@@ -69,6 +78,8 @@ struct Item {
   int keys;   // keys that the request has
   int offset; // row i sees keys below offset + i + 1 (causal)
 };
+static_assert(sizeof(Item) <= 32, "the item ring holds 32-byte entries");
+__device__ __forceinline__ Item* Shared::item(uint32_t index) const { return reinterpret_cast<Item*>(ptr + kSmemMisc + 64 + index % kItems * 32); }
 
 // Keys that the first `rows` rows of the item see, at most.
 __device__ __forceinline__ int reach(const Params& p, const Item& item, int rows) {
@@ -78,7 +89,7 @@ __device__ __forceinline__ int reach(const Params& p, const Item& item, int rows
 
 __device__ __forceinline__ int bounded(int value, int most) { return min(max(value, 0), most); }
 
-// The item of this block, by whole warps; false when there are fewer. Items: heads, of each all requests, of each request blocks of
+// Item number `index`, by whole warps; false when there are fewer. Items: heads, of each all requests, of each request blocks of
 // 256 rows from its end (where causal rows see most keys) to its beginning.
 __device__ __forceinline__ bool find_item(const Params& p, int index, Item& item) {
   const int lane = threadIdx.x & 31;
@@ -128,21 +139,100 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
 }
 
+// ---- what to do next ------------------------------------------------------------------------------------------------
+
+// Asks for a block of the launch that has not started; 16 bytes at `answer` and on `bar` in time. Not after a refusal.
+__device__ __forceinline__ void ask_for_block(uint32_t answer, uint32_t bar) {
+  mbar_arrive_expect(bar, 16);
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];\n" ::"r"(answer), "r"(bar) : "memory");
+}
+// The block that was given (it will not start), or -1.
+__device__ __forceinline__ int block_given(uint32_t answer) {
+  uint32_t given, index;
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      ".reg .b128 r;\n"
+      "ld.shared.b128 r, [%2];\n"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n"
+      "selp.u32 %0, 1, 0, p;\n"
+      "mov.u32 %1, 0;\n"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, _, _, _}, r;\n"
+      "}\n"
+      : "=r"(given), "=r"(index) : "r"(answer) : "memory");
+  return given != 0 ? int(index) : -1;
+}
+
+// By a whole warp. `item` is the first.
+__device__ void plan_role(const Params& p, const Shared& sm, Item item) {
+  const int lane = threadIdx.x & 31;
+  volatile int* abort_flag = sm.abort_flag();
+  uint32_t announced = 0, asked = 0;
+  for (bool has = true;; ) {
+    if (announced >= kItems && !warp_wait(sm.bar(kItemDone0 + announced % kItems), (announced / kItems - 1) & 1, abort_flag)) return;
+    if (lane == 0) {
+      Item* target = sm.item(announced);
+      *target = item;
+      if (!has) target->rows = 0;  // no more
+      mbar_arrive(sm.bar(kItemReady0 + announced % kItems));
+    }
+    ++announced;
+    if (!has) return;
+    // The next block is asked for when the copies of this item's last step begin: early enough for the answer to come in time, no earlier, so
+    // that the last items go to whoever is free (8192 x 8192 tokens, 64 heads: asked for with the item's announcement 1389 us, so 1289).
+    if (!warp_wait(sm.bar(kLastStep), asked & 1, abort_flag)) return;
+    if (lane == 0) {
+      fence_proxy_async();  // (the answer before was read through the generic proxy)
+      ask_for_block(sm.answer(), sm.bar(kAnswer));
+    }
+    // (also where a wait has given up: the answer is still to come)
+    int never = 0;
+    if (!__all_sync(0xffffffffu, mbar_wait(sm.bar(kAnswer), asked & 1, &never))) *abort_flag = 1;
+    ++asked;
+    if (*abort_flag != 0) return;
+    int index = block_given(sm.answer());
+    __syncwarp();
+    has = index >= 0 && find_item(p, index, item);
+    if (!has) {
+      // Numbers grow: the blocks behind this one have nothing to do either. They are taken over so that they need not start.
+      while (index >= 0) {
+        if (lane == 0) {
+          fence_proxy_async();
+          ask_for_block(sm.answer(), sm.bar(kAnswer));
+        }
+        if (!__all_sync(0xffffffffu, mbar_wait(sm.bar(kAnswer), asked & 1, &never))) { *abort_flag = 1; return; }
+        ++asked;
+        index = block_given(sm.answer());
+        __syncwarp();
+      }
+    }
+  }
+}
+
+// Everybody's way through the items.
+struct Walk {
+  const Shared& sm;
+  uint32_t index = 0;
+  Item item;
+  __device__ __forceinline__ explicit Walk(const Shared& shared) : sm(shared) {}
+  __device__ __forceinline__ bool read() { item = *sm.item(index); return item.rows > 0; }
+  __device__ __forceinline__ bool next_of_warp() { return warp_wait(sm.bar(kItemReady0 + index % kItems), (index / kItems) & 1, sm.abort_flag()) && read(); }
+  __device__ __forceinline__ bool next_of_thread() { return mbar_wait(sm.bar(kItemReady0 + index % kItems), (index / kItems) & 1, sm.abort_flag()) && read(); }
+  __device__ __forceinline__ void done() { mbar_arrive(sm.bar(kItemDone0 + index % kItems)); ++index; }
+  __device__ __forceinline__ void done_of_warp() {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(sm.bar(kItemDone0 + index % kItems));
+    ++index;
+  }
+};
+
 // ---- copies ---------------------------------------------------------------------------------------------------------
 
 // By the whole warp; lane 0 issues.
-__device__ void copy_role(const Params& p, const Shared& sm, const Item& item) {
+__device__ void copy_role(const Params& p, const Shared& sm) {
   const int lane = threadIdx.x & 31;
   volatile int* abort_flag = sm.abort_flag();
-  const int steps = max(steps_of(p, item, 0), steps_of(p, item, 1));
-  if (steps == 0) return;
-  if (lane == 0) {
-    mbar_arrive_expect(sm.bar(kQFull), 2 * kQBoxes * kBoxBytes);
-#pragma unroll
-    for (int box = 0; box < 2 * kQBoxes; ++box)  // (rows behind the item are multiplied and thrown away)
-      copy_box(sm.base + kSmemQ + box * kBoxBytes, &p.q, box % kQBoxes * 64, item.head * p.q_head, item.row + box / kQBoxes * kTile, sm.bar(kQFull));
-  }
-  uint32_t count = 0, mended = 0;  // boxes so far; those that were cleared in part
+  uint32_t count = 0, mended = 0, loads[2] = {0, 0};  // boxes so far; those that were cleared in part; tiles of Q
   bool given_up = false;
   // Claims the next slot of the ring and lets its copy be started by lane 0.
   auto bring = [&](auto start, int valid_rows) {
@@ -166,18 +256,40 @@ __device__ void copy_role(const Params& p, const Shared& sm, const Item& item) {
     }
     ++count;
   };
-  for (int step = 0; step < steps && !given_up; ++step) {
-    const int key = item.first + step * kTile;
-    for (int box = 0; box < 2 && !given_up; ++box)
-      bring([&](uint32_t target, uint32_t bar) { copy_box(target, &p.k, box * 64, item.head * p.k_head, key, bar); }, kTile);
-    if (!given_up) bring([&](uint32_t target, uint32_t bar) { copy_box(target, &p.rope, 0, key, bar); }, kTile);
-    const int valid = min(kTile, item.keys - step * kTile);
-    for (int box = 0; box < kValueBoxes && !given_up; ++box)
-      bring([&](uint32_t target, uint32_t bar) { copy_box(target, &p.v, box * 64, item.head * p.v_head, key, bar); }, valid);
+  Walk walk(sm);
+  for (; !given_up && walk.next_of_warp(); walk.done_of_warp()) {
+    const Item& item = walk.item;
+    const int steps_0 = steps_of(p, item, 0), steps_1 = steps_of(p, item, 1), steps = max(steps_0, steps_1);
+    if (steps == 0 && lane == 0) mbar_arrive(sm.bar(kLastStep));
+    for (int step = 0; step < steps && !given_up; ++step) {
+      if (step + 1 == steps && lane == 0) mbar_arrive(sm.bar(kLastStep));
+      const int key = item.first + step * kTile;
+      for (int box = 0; box < 2 && !given_up; ++box)
+        bring([&](uint32_t target, uint32_t bar) { copy_box(target, &p.k, box * 64, item.head * p.k_head, key, bar); }, kTile);
+      if (!given_up) bring([&](uint32_t target, uint32_t bar) { copy_box(target, &p.rope, 0, key, bar); }, kTile);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {  // (rows behind the item are multiplied and thrown away)
+        if (step > 0 || given_up || (t == 0 ? steps_0 : steps_1) == 0) continue;
+        if (loads[t] > 0 && !warp_wait(sm.bar(kQFree0 + t), (loads[t] - 1) & 1, abort_flag)) { given_up = true; continue; }
+        if (lane == 0) {
+          mbar_arrive_expect(sm.bar(kQFull0 + t), kQBoxes * kBoxBytes);
+#pragma unroll
+          for (int box = 0; box < kQBoxes; ++box)
+            copy_box(sm.base + kSmemQ + (t * kQBoxes + box) * kBoxBytes, &p.q, box * 64, item.head * p.q_head, item.row + t * kTile, sm.bar(kQFull0 + t));
+        }
+        __syncwarp();
+        ++loads[t];
+      }
+      const int valid = min(kTile, item.keys - step * kTile);
+      for (int box = 0; box < kValueBoxes && !given_up; ++box)
+        bring([&](uint32_t target, uint32_t bar) { copy_box(target, &p.v, box * 64, item.head * p.v_head, key, bar); }, valid);
+    }
   }
   if (*abort_flag != 0) {  // nothing of this block may be written behind its end
     int never = 0;
-    mbar_wait(sm.bar(kQFull), 0, &never);
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+      if (loads[t] > 0) mbar_wait(sm.bar(kQFull0 + t), (loads[t] - 1) & 1, &never);
     for (uint32_t i = count > kRing ? count - kRing : 0; i < count; ++i) mbar_wait(sm.bar(kFull0 + i % kRing), (i / kRing) & 1, &never);
     if (mended > 0) mbar_wait(sm.bar(kMended), (mended - 1) & 1, &never);
   }
@@ -189,12 +301,9 @@ template <int kFormat> constexpr uint32_t kIdescScores = idesc_f16(128, 128, kFo
 template <int kFormat, int kColumns> constexpr uint32_t kIdescValues = idesc_f16(128, kColumns, kFormat, 0, 1);
 
 template <int kFormat>
-__device__ void product_role(const Params& p, const Shared& sm, const Item& item, uint32_t tmem) {
+__device__ void product_role(const Params& p, const Shared& sm, uint32_t tmem) {
   volatile int* abort_flag = sm.abort_flag();
-  const int steps[2] = {steps_of(p, item, 0), steps_of(p, item, 1)};
-  const int most = max(steps[0], steps[1]);
-  if (most == 0) return;
-  uint32_t count = 0;  // boxes used
+  uint32_t count = 0, loads[2] = {0, 0}, weights_seen[2] = {0, 0};  // boxes used; tiles of Q; weights
   auto box_at = [&](uint32_t box) { return sm.base + kSmemRing + box % kRing * kBoxBytes; };
   auto landed = [&](uint32_t box) { return mbar_wait(sm.bar(kFull0 + box % kRing), (box / kRing) & 1, abort_flag); };
   auto release = [&](uint32_t first, int boxes) {
@@ -214,41 +323,55 @@ __device__ void product_role(const Params& p, const Shared& sm, const Item& item
     mma_commit(sm.bar(kScores0 + t));
   };
   auto keys_landed = [&](uint32_t keys) { return landed(keys) && landed(keys + 1) && landed(keys + 2); };
-  if (!mbar_wait(sm.bar(kQFull), 0, abort_flag) || !keys_landed(0)) return;
-  for (int t = 0; t < 2; ++t)
-    if (steps[t] > 0) scores(t, 0);
-  release(0, kKeyBoxes);
-  count = kKeyBoxes;
-  for (int step = 0; step < most; ++step) {
-    const uint32_t values = count, keys = count + kValueBoxes;
-    const bool more = step + 1 < most;
-    if (!landed(values) || !landed(values + 1)) return;
+  Walk walk(sm);
+  for (; walk.next_of_thread(); walk.done()) {
+    const int steps[2] = {steps_of(p, walk.item, 0), steps_of(p, walk.item, 1)};
+    const int most = max(steps[0], steps[1]);
+    if (most == 0) continue;
+    if (!keys_landed(count)) return;
+#pragma unroll
     for (int t = 0; t < 2; ++t) {
-      if (step < steps[t]) {
-        if (!mbar_wait(sm.bar(kWeights0 + t), step & 1, abort_flag)) return;
-        tc_fence_after_sync();
-        const uint32_t o = tmem + kColumnsO + t * kTile, weights = tmem + t * kTile;
-        const uint64_t b = smem_desc_sw128(box_at(values), kBoxBytes, 1024);
-        if (box_at(values + 1) > box_at(values)) {
-#pragma unroll
-          for (int k = 0; k < kTile / 16; ++k) mma_ts(o, weights + k * 8, b + k * 128, kIdescValues<kFormat, 128>, step > 0 || k > 0);
-        } else {  // every eighth time the second box is at the ring's beginning: 64 features each, which takes half as long again
-          const uint64_t b1 = smem_desc_sw128(box_at(values + 1), kBoxBytes, 1024);
-#pragma unroll
-          for (int k = 0; k < kTile / 16; ++k) mma_ts(o, weights + k * 8, b + k * 128, kIdescValues<kFormat, 64>, step > 0 || k > 0);
-#pragma unroll
-          for (int k = 0; k < kTile / 16; ++k) mma_ts(o + 64, weights + k * 8, b1 + k * 128, kIdescValues<kFormat, 64>, step > 0 || k > 0);
-        }
-        if (step + 1 == steps[t]) mma_commit(sm.bar(kOut0 + t));
-      }
-      if (t == 1) release(values, kValueBoxes);
-      if (step + 1 < steps[t]) {
-        if (!keys_landed(keys)) return;
-        scores(t, keys);
-      }
+      if (steps[t] == 0) continue;
+      if (!mbar_wait(sm.bar(kQFull0 + t), loads[t]++ & 1, abort_flag)) return;
+      tc_fence_after_sync();
+      scores(t, count);
+      if (steps[t] == 1) mma_commit(sm.bar(kQFree0 + t));
     }
-    if (more) release(keys, kKeyBoxes);
-    count += kValueBoxes + kKeyBoxes;
+    release(count, kKeyBoxes);
+    count += kKeyBoxes;
+    for (int step = 0; step < most; ++step) {
+      const uint32_t values = count, keys = count + kValueBoxes;
+      const bool more = step + 1 < most;
+      if (!landed(values) || !landed(values + 1)) return;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if (step < steps[t]) {
+          if (!mbar_wait(sm.bar(kWeights0 + t), weights_seen[t]++ & 1, abort_flag)) return;
+          tc_fence_after_sync();
+          const uint32_t o = tmem + kColumnsO + t * kTile, weights = tmem + t * kTile;
+          const uint64_t b = smem_desc_sw128(box_at(values), kBoxBytes, 1024);
+          if (box_at(values + 1) > box_at(values)) {
+#pragma unroll
+            for (int k = 0; k < kTile / 16; ++k) mma_ts(o, weights + k * 8, b + k * 128, kIdescValues<kFormat, 128>, step > 0 || k > 0);
+          } else {  // every eighth time the second box is at the ring's beginning: 64 features each, which takes half as long again
+            const uint64_t b1 = smem_desc_sw128(box_at(values + 1), kBoxBytes, 1024);
+#pragma unroll
+            for (int k = 0; k < kTile / 16; ++k) mma_ts(o, weights + k * 8, b + k * 128, kIdescValues<kFormat, 64>, step > 0 || k > 0);
+#pragma unroll
+            for (int k = 0; k < kTile / 16; ++k) mma_ts(o + 64, weights + k * 8, b1 + k * 128, kIdescValues<kFormat, 64>, step > 0 || k > 0);
+          }
+          if (step + 1 == steps[t]) mma_commit(sm.bar(kOut0 + t));
+        }
+        if (t == 1) release(values, kValueBoxes);
+        if (step + 1 < steps[t]) {
+          if (!keys_landed(keys)) return;
+          scores(t, keys);
+          if (step + 2 == steps[t]) mma_commit(sm.bar(kQFree0 + t));
+        }
+      }
+      if (more) release(keys, kKeyBoxes);
+      count += kValueBoxes + (more ? kKeyBoxes : 0);
+    }
   }
 }
 
@@ -259,120 +382,128 @@ __device__ void product_role(const Params& p, const Shared& sm, const Item& item
 constexpr float kRoom = 15.f, kStep = 8.f;
 
 template <int kFormat>
-__device__ void softmax_role(const Params& p, const Shared& sm, const Item& item, uint32_t tmem) {
+__device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, t = warp >> 2;
   volatile int* abort_flag = sm.abort_flag();
-  const int row = t * kTile + (warp & 3) * 32 + lane;  // of the item
-  const int steps = steps_of(p, item, t);
+  const int row = t * kTile + (warp & 3) * 32 + lane;  // of an item
   const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
   const uint32_t s_tmem = tmem + t * kTile + lanes, o_tmem = tmem + kColumnsO + t * kTile + lanes;
-  const int end = p.causal ? min(item.keys, item.offset + row + 1) : item.keys;  // this row sees keys below
-  const int warp_end = p.causal ? min(item.keys, item.offset + (row & ~31) + 1) : item.keys;  // all rows of the warp see keys below
-  float reference = -INFINITY, sum = 0.f;
-  for (int step = 0; step < steps; ++step) {
-    if (!warp_wait(sm.bar(kScores0 + t), step & 1, abort_flag)) return;
-    tc_fence_after_sync();
-    float2 s[kTile / 2];
+  uint32_t scores_seen = 0, outputs = 0;
+  Walk walk(sm);
+  for (; walk.next_of_warp(); walk.done_of_warp()) {
+    const Item& item = walk.item;
+    const int steps = steps_of(p, item, t);
+    const int end = p.causal ? min(item.keys, item.offset + row + 1) : item.keys;  // this row sees keys below
+    const int warp_end = p.causal ? min(item.keys, item.offset + (row & ~31) + 1) : item.keys;  // all rows of the warp see keys below
+    float reference = -INFINITY, sum = 0.f;
+    for (int step = 0; step < steps; ++step) {
+      if (!warp_wait(sm.bar(kScores0 + t), scores_seen++ & 1, abort_flag)) return;
+      tc_fence_after_sync();
+      const int key = step * kTile;
+      const bool masked = key + kTile > warp_end;
+      uint32_t words[kTile / 2];
+      float own;
+      // Weights are worked out with the reference as it is, without looking for the maximum: as long as their sum stays below 2^kRoom so does each of
+      // them. Where it does not (for some row of the warp), and in a row's first step, the scores are read again and the reference may move.
+      for (bool look = step == 0;; look = true) {
+        float2 s[2][16];  // 32 scores, and the next 32 on their way
+        auto load = [&](int part) { tmem_ld32(s_tmem + part * 32, reinterpret_cast<uint32_t*>(&s[part & 1][0])); };
+        auto mask = [&](int part) {
+          const int seen = end - key - part * 32;
 #pragma unroll
-    for (int c = 0; c < kTile; c += 32) tmem_ld32(s_tmem + c, reinterpret_cast<uint32_t*>(&s[c / 2]));
-    tmem_wait_ld();
-    const int key = step * kTile;
-    if (key + kTile > warp_end) {
+          for (int i = 0; i < 16; ++i) {
+            if (2 * i >= seen) s[part & 1][i].x = -INFINITY;
+            if (2 * i + 1 >= seen) s[part & 1][i].y = -INFINITY;
+          }
+        };
+        if (look) {
+          float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int i = 0; i < kTile / 2; ++i) {
-        if (key + 2 * i >= end) s[i].x = -INFINITY;
-        if (key + 2 * i + 1 >= end) s[i].y = -INFINITY;
-      }
-    }
-    float most[4];
+          for (int part = 0; part < 4; ++part) {
+            load(part);
+            tmem_wait_ld();
+            if (masked) mask(part);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      most[k] = fmaxf(s[16 * k].x, s[16 * k].y);
-#pragma unroll
-      for (int i = 1; i < 16; ++i) most[k] = greatest(most[k], s[16 * k + i].x, s[16 * k + i].y);
-    }
-    const float top = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * p.scale_log2;  // scale > 0
-    const bool moves = top > reference + kRoom;
-    if (__any_sync(0xffffffffu, moves)) {
-      float alpha = 1.f;
-      if (moves) {
-        const float next = reference == -INFINITY ? top : top - kStep;
-        alpha = exp2f(reference - next);
-        reference = next;
-      }
-      sum *= alpha;
-      if (step > 0) {  // (scores of this step are there: the products of the one before have ended)
+            for (int i = 0; i < 16; ++i) most[i & 3] = greatest(most[i & 3], s[part & 1][i].x, s[part & 1][i].y);
+          }
+          const float top = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * p.scale_log2;  // scale > 0
+          const bool moves = top > reference + kRoom;
+          float alpha = 1.f;
+          if (moves) {
+            const float next = reference == -INFINITY ? top : top - kStep;
+            alpha = exp2f(reference - next);
+            reference = next;
+          }
+          sum *= alpha;
+          if (step > 0 && __any_sync(0xffffffffu, moves)) {  // (scores of this step are there: the products of the one before have ended)
 #pragma unroll 1
-        for (int c = 0; c < kTile; c += 32) {
-          uint32_t o[32];
-          tmem_ld32(o_tmem + c, o);
-          tmem_wait_ld();
+            for (int c = 0; c < kTile; c += 32) {
+              uint32_t o[32];
+              tmem_ld32(o_tmem + c, o);
+              tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-          tmem_st32(o_tmem + c, o);
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              tmem_st32(o_tmem + c, o);
+            }
+            tmem_wait_st();
+          }
         }
-        tmem_wait_st();
-      }
-    }
-    const float shift = reference == -INFINITY ? 0.f : -reference;
-    const float2 scale = make_float2(p.scale_log2, p.scale_log2), shifts = make_float2(shift, shift);
-    float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        const float shift = reference == -INFINITY ? 0.f : -reference;
+        const float2 scale = make_float2(p.scale_log2, p.scale_log2), shifts = make_float2(shift, shift);
+        float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        load(0);
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      uint32_t words[32];
+        for (int part = 0; part < 4; ++part) {
+          tmem_wait_ld();
+          if (part < 3) load(part + 1);
+          if (masked) mask(part);
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        float2 weight = fma2(s[half * 32 + i], scale, shifts);
-        weight.x = exp2f(weight.x);
-        weight.y = exp2f(weight.y);
-        sums[i & 1] = add2(sums[i & 1], weight);
-        words[i] = pack2<kFormat>(weight.x, weight.y);
+          for (int i = 0; i < 16; ++i) {
+            float2 weight = fma2(s[part & 1][i], scale, shifts);
+            weight.x = exp2f(weight.x);
+            weight.y = exp2f(weight.y);
+            sums[i & 1] = add2(sums[i & 1], weight);
+            words[part * 16 + i] = pack2<kFormat>(weight.x, weight.y);
+          }
+        }
+        own = (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
+        if (look || !__any_sync(0xffffffffu, own > 32768.f)) break;
       }
-      tmem_st32(s_tmem + half * 32, words);
+      sum += own;
+      tmem_st32(s_tmem, words);
+      tmem_st32(s_tmem + 32, words + 32);
+      tmem_wait_st();
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(sm.bar(kWeights0 + t));
     }
-    sum += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
-    tmem_wait_st();
-    tc_fence_before_sync();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(sm.bar(kWeights0 + t));
-  }
-  // Output: through this tile's part of Q's memory, which nothing reads any more, so that whole lines are written.
-  const bool live = row < item.rows;
-  if (p.lse != nullptr && live)
-    p.lse[size_t(item.row + row) * p.heads + item.head] = sum > 0.f ? (reference + log2f(sum)) * 0.6931471805599453f : (sum == 0.f ? -INFINITY : sum);
-  const float inverse = sum == 0.f ? 0.f : 1.f / sum;
-  unsigned char* staged = sm.ptr + kSmemQ + t * kQBoxes * kBoxBytes + (warp & 3) * 8192;
-  if (steps > 0) {
-    if (!warp_wait(sm.bar(kOut0 + t), 0, abort_flag)) return;
-    tc_fence_after_sync();
-  } else if (steps_of(p, item, t ^ 1) > 0) {
-    if (!warp_wait(sm.bar(kQFull), 0, abort_flag)) return;  // Q is still on its way to the memory that the output goes through
-  }
-#pragma unroll 1
-  for (int c = 0; c < kTile; c += 32) {
-    uint32_t o[32];
+    // Output: a row's 256 bytes by its own thread, in whole sectors.
+    const bool live = row < item.rows;
+    if (p.lse != nullptr && live)
+      p.lse[size_t(item.row + row) * p.heads + item.head] = sum > 0.f ? (reference + log2f(sum)) * 0.6931471805599453f : (sum == 0.f ? -INFINITY : sum);
+    const float inverse = sum == 0.f ? 0.f : 1.f / sum;
+    char* out = static_cast<char*>(p.out) + (size_t(item.row + row) * p.heads + item.head) * (LATENT_NOPE * 2);
     if (steps > 0) {
-      tmem_ld32(o_tmem + c, o);
-      tmem_wait_ld();
+      if (!warp_wait(sm.bar(kOut0 + t), outputs++ & 1, abort_flag)) return;
+      tc_fence_after_sync();
     }
+#pragma unroll 1
+    for (int c = 0; c < kTile; c += 32) {
+      uint32_t o[32];
+      if (steps > 0) {
+        tmem_ld32(o_tmem + c, o);
+        tmem_wait_ld();
+      }
+      uint32_t words[16];
 #pragma unroll
-    for (int unit = 0; unit < 4; ++unit) {
-      uint32_t words[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        words[i] = sum == 0.f ? 0u : pack2<kFormat>(__uint_as_float(o[unit * 8 + 2 * i]) * inverse, __uint_as_float(o[unit * 8 + 2 * i + 1]) * inverse);
-      const int place = c / 8 + unit;  // of the row's sixteen
-      *reinterpret_cast<uint4*>(staged + lane * 256 + ((place ^ (lane & 7)) << 4)) = make_uint4(words[0], words[1], words[2], words[3]);
+      for (int i = 0; i < 16; ++i)
+        words[i] = sum == 0.f ? 0u : pack2<kFormat>(__uint_as_float(o[2 * i]) * inverse, __uint_as_float(o[2 * i + 1]) * inverse);
+      if (live) {
+        store_sector(out + c * 2, words);
+        store_sector(out + c * 2 + 32, words + 8);
+      }
     }
-  }
-  __syncwarp();
-  const int first_row = t * kTile + (warp & 3) * 32;
-#pragma unroll 4
-  for (int i = 0; i < 16; ++i) {
-    const int r = i * 2 + (lane >> 4), place = lane & 15;
-    const uint4 v = *reinterpret_cast<const uint4*>(staged + r * 256 + ((place ^ (r & 7)) << 4));
-    if (first_row + r < item.rows)
-      *reinterpret_cast<uint4*>(static_cast<char*>(p.out) + (size_t(item.row + first_row + r) * p.heads + item.head) * (LATENT_NOPE * 2) + place * 16) = v;
+    tc_fence_before_sync();  // (the accumulator may be overwritten when this warp's next weights are there)
   }
 }
 
@@ -389,7 +520,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
   Item item;
   if (!find_item(p, blockIdx.x, item)) return;  // the whole block
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kBarCount; ++i) mbar_init(sm.bar(i), i == kWeights0 || i == kWeights1 ? 4 : 1);
+    for (int i = 0; i < kBarCount; ++i)
+      mbar_init(sm.bar(i), i >= kWeights0 && i < kWeights0 + 2 ? 4 : i >= kItemDone0 ? kSoftmaxWarps + 2 : 1);
     mbar_fence_init();
     *sm.abort_flag() = 0;
   }
@@ -398,13 +530,20 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = *sm.slot();
-  if (warp < kProductWarp) {
-    softmax_role<kFormat>(p, sm, item, tmem);
-  } else if (warp == kProductWarp) {
-    if (elect_one()) product_role<kFormat>(p, sm, item, tmem);
-    __syncwarp();
+  // A softmax thread holds a row's 128 scores: the third warpgroup's registers go to the first two (200 + 200 + 104 of 3 x 168).
+  if (warp < kSoftmaxWarps) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;\n");
+    softmax_role<kFormat>(p, sm, tmem);
   } else {
-    copy_role(p, sm, item);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;\n");
+    if (warp == kProductWarp) {
+      if (elect_one()) product_role<kFormat>(p, sm, tmem);
+      __syncwarp();
+    } else if (warp == kCopyWarp) {
+      copy_role(p, sm);
+    } else if (warp == kPlanWarp) {
+      plan_role(p, sm, item);
+    }
   }
   tc_fence_before_sync();
   __syncthreads();

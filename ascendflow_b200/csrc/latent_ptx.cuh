@@ -91,6 +91,12 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
       : "memory");
 }
 
+// 32 bytes (aligned) in one store: a whole sector of a lane's own row.
+__device__ __forceinline__ void store_sector(void* at, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n"
+               ::"l"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+}
+
 // ---- arithmetic on pairs -------------------------------------------------------------------------------------------
 
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
