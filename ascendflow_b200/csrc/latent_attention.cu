@@ -154,14 +154,22 @@ __device__ __forceinline__ int chunks_of(const Params& p, const Request& r, int 
   return int((min(max(seen, int64_t(0)), int64_t(r.far)) + kChunk - 1) / kChunk);
 }
 
-// Stretch [border(i), border(i + 1)) of the total cost is block i's.
+// Stretch [at(i), at(i + 1)) of the total cost is block i's.
 struct Borders {
-  int64_t total;
-  int blocks;  // that get a stretch
-  __device__ __forceinline__ int64_t at(int i) const { return total / blocks * i + total % blocks * i / blocks; }
+  int64_t total, each;
+  uint32_t rest, blocks;  // that get a stretch (at most 255)
+  __device__ __forceinline__ int64_t at(uint32_t i) const { return each * i + rest * i / blocks; }
 };
-// A block with fewer chunks than these loses more with its start and with its part of the sums than it takes off the others.
-constexpr int kLeastChunks = 4;
+// value * factor / divisor, rounded down: everybody who asks gets the same.
+__device__ __forceinline__ int share_of(int64_t value, int factor, int64_t divisor) {
+  const uint64_t product = uint64_t(value) * uint32_t(factor);
+  if ((product | uint64_t(divisor)) >> 32 == 0) return int(uint32_t(product) / uint32_t(divisor));  // (a 64-bit division takes several times as long)
+  return int(product / uint64_t(divisor));
+}
+// A block with fewer chunks than these loses more with its start and with its part of the sums than it takes off the others (64 heads, one
+// token; 1, 2, 3, 4 chunks: 2048 keys 18.6, 18.3, 18.8, 22.8 us, 8192 26.2, 22.1, 21.4, 21.2, four requests of 8192 24.1, 24.0, 24.0, 26.2,
+// four of 1024 with six tokens 26.4, 26.2, 31.2, 30.8).
+constexpr int kLeastChunks = 2;
 
 // Where a stretch begins: a request's tile and the cost in front of that.
 struct Place {
@@ -198,7 +206,7 @@ __device__ __forceinline__ Borders plan_block(const Params& p, int64_t* scratch,
     const int b = round * kThreads + int(threadIdx.x);
     return round == 0 ? own : b < p.batches ? request_at(p, b) : none;
   };
-  Borders borders = {0, 0};
+  Borders borders = {0, 0, 0, 0};
   int64_t cost = 0;
   int most_tiles = 0, least_tiles = INT32_MAX;
   for (int round = 0; round < rounds; ++round) {
@@ -221,7 +229,9 @@ __device__ __forceinline__ Borders plan_block(const Params& p, int64_t* scratch,
   int blocks = int(min(max(borders.total / (kLeastChunks * kChunk), int64_t(1)), int64_t(grid)));
   if (most_tiles == least_tiles && blocks % most_tiles <= blocks / 16) blocks -= blocks % most_tiles;
   if (int(blockIdx.x) >= blocks) return borders;
-  borders.blocks = blocks;
+  borders.blocks = uint32_t(blocks);
+  borders.each = borders.total / blocks;
+  borders.rest = uint32_t(borders.total - borders.each * blocks);
   const int64_t mine = borders.at(blockIdx.x);
   // The tile: the last whose predecessors cost no more.
   int tile = 0;
@@ -298,8 +308,8 @@ __device__ void plan_role(const Params& p, const Shared& sm, const Borders& bord
       const int64_t cost = r.cost(tile + 1) - r.cost(tile), past = start + cost;
       const int chunks = chunks_of(p, r, tile);
       Piece piece;
-      piece.first = int((at - start) * chunks / cost);
-      piece.last = past <= end ? chunks : int((end - start) * chunks / cost);
+      piece.first = at == start ? 0 : share_of(at - start, chunks, cost);
+      piece.last = past <= end ? chunks : share_of(end - start, chunks, cost);
       if (piece.first < piece.last || (chunks == 0 && at == start)) {
         const int row = tile * kRows;
         piece.row = int64_t(r.begin) * p.heads + row;
@@ -311,20 +321,22 @@ __device__ void plan_role(const Params& p, const Shared& sm, const Borders& bord
         piece.length = r.far;
         const bool whole = piece.first == 0 && piece.last == chunks;
         piece.slot = whole ? -1 : 2 * int(blockIdx.x) + (piece.first == 0);
+        if (!claim()) break;
+        announce(piece);
         if (!whole && piece.first == 0) {
           record.row = piece.row;
           record.rows = piece.rows;
           record.head = piece.head;
-          int last = int(double(past) / double(borders.total) * borders.blocks);  // the block that has the tile's end, or next to it
-          last = min(max(last, int(blockIdx.x)), borders.blocks - 1);
-          while (last > int(blockIdx.x) && borders.at(last) >= past) --last;
-          while (last + 1 < borders.blocks && borders.at(last + 1) < past) ++last;
+          // The block that has the tile's end: the last that begins in front of it.
+          int last = blockIdx.x;
+          for (int high = int(borders.blocks); high - last > 1;) {
+            const int middle = (last + high) >> 1;
+            if (borders.at(middle) < past) last = middle; else high = middle;
+          }
           record.last = last;
         } else if (!whole) {
           continued = true;
         }
-        if (!claim()) break;
-        announce(piece);
       }
       at = min(past, end);
       if (at >= end) break;
@@ -705,13 +717,14 @@ __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
       if (half == 0 && row < piece.rows) p.statistics[size_t(piece.slot) * kRows + row] = make_float2(reference, sum);
       float* sums = p.sums + size_t(piece.slot) * kSlotFloats + o_row * LATENT_VALUES + o_feature;
 #pragma unroll 1
-      for (int c = 0; c < 256; c += 32) {
-        uint32_t o[32];
+      for (int c = 0; c < 256; c += 64) {
+        uint32_t o[64];
         tmem_ld32(tmem + c + lanes, o);
+        tmem_ld32(tmem + c + 32 + lanes, o + 32);
         tmem_wait_ld();
         if (o_row < piece.rows) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 8) store_sector(sums + (c >> 7) * 256 + (c & 127) + e, o + e);
+          for (int e = 0; e < 64; e += 8) store_sector(sums + (c >> 7) * 256 + (c & 127) + e, o + e);
         }
       }
       continue;
@@ -806,65 +819,121 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
   if (warp == kScoreWarp) tmem_dealloc(tmem, 512);
 }
 
-// Tiles that several blocks worked on: block (i, y) adds up rows 4 y .. + 3 of the tile that begins in block i, a row by two warps. A lane has
-// the factors of every 32nd part.
-constexpr int kCombineThreads = 256, kCombineRows = 4, kMostParts = 8;  // of 32
+// Tiles that several blocks worked on. Every block makes the list of them, with what there is to do for each: a tile of few parts by groups of
+// eight rows, a warp each; of many parts by half rows, the parts shared out over eight warps. Sums are added in the order of the parts (of the
+// warps' shares), whatever block does it.
+constexpr int kCombineThreads = 256, kCombineWarps = kCombineThreads / 32, kMostBlocks = 256, kFewParts = 8;
+
 template <int kFormat>
-__global__ void __launch_bounds__(kCombineThreads) combine_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kCombineThreads) combine_kernel(const __grid_constant__ Params p, int blocks) {
+  __shared__ int ends[kCombineWarps];
+  __shared__ struct { int block, parts, items; } list[kMostBlocks];  // tiles; `items`: with those in front of it
+  __shared__ float shared_sums[kCombineWarps][LATENT_VALUES / 2];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   wait_for_predecessor();
   let_successor_start();
-  const Record record = p.records[blockIdx.x];
-  const int row = int(blockIdx.y) * kCombineRows + (warp >> 1), first = int(blockIdx.x);
-  if (record.last < 0 || row >= record.rows) return;
-  const int parts = record.last - first + 1;
-  auto slot_of = [&](int part) { return size_t(part == 0 ? 2 * first + 1 : 2 * (first + part)); };
-  // (a block that had none of the tile's chunks has said so: reference -infinity)
-  float2 own[kMostParts];
-  float reference = -INFINITY;
+  // The tiles, packed.
+  const int last = int(threadIdx.x) < blocks ? __ldg(&p.records[threadIdx.x].last) : -1;
+  const int parts_here = last >= 0 ? last - int(threadIdx.x) + 1 : 0;
+  const int items_here = parts_here == 0 ? 0 : parts_here <= kFewParts ? kRows / 8 : 2 * kRows;
+  int packed = items_here << 8 | (parts_here > 0);  // both sums at once: items below 2^15, tiles below 2^8
 #pragma unroll
-  for (int k = 0; k < kMostParts; ++k) {
-    own[k] = k * 32 + lane < parts ? p.statistics[slot_of(k * 32 + lane) * kRows + row] : make_float2(-INFINITY, 0.f);
-    reference = fmaxf(reference, own[k].x);
+  for (int d = 1; d < 32; d <<= 1) {
+    const int other = __shfl_up_sync(0xffffffffu, packed, d);
+    if (lane >= d) packed += other;
   }
+  if (lane == 31) ends[warp] = packed;
+  __syncthreads();
+  int all = 0;
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) reference = fmaxf(reference, __shfl_xor_sync(0xffffffffu, reference, d));
-  float sum = 0.f;
-#pragma unroll
-  for (int k = 0; k < kMostParts; ++k) {
-    own[k].x = own[k].x == -INFINITY ? 0.f : exp2f(own[k].x - reference);
-    sum += own[k].x * own[k].y;
+  for (int w = 0; w < kCombineWarps; ++w) {
+    if (w < warp) packed += ends[w];
+    all += ends[w];
   }
+  if (parts_here > 0) list[(packed & 255) - 1] = {int(threadIdx.x), parts_here, packed >> 8};
+  __syncthreads();
+  const int items = all >> 8;
+  int tile = 0;
+  for (int item = blockIdx.x; item < items; item += gridDim.x) {
+    while (list[tile].items <= item) ++tile;
+    const int first = list[tile].block, parts = list[tile].parts, in_front = tile > 0 ? list[tile - 1].items : 0;
+    const Record record = p.records[first];
+    auto slot_of = [&](int part) { return size_t(part == 0 ? 2 * first + 1 : 2 * (first + part)); };
+    const bool few = parts <= kFewParts;
+    const int row = few ? (item - in_front) * 8 + warp : (item - in_front) >> 1, half = few ? 0 : (item - in_front) & 1;
+    if (row >= record.rows && !few) continue;  // the whole block
+    const bool live = row < record.rows;
+    // Factors: lane l has those of parts l, l + 32, ... (a block that had none of the tile's chunks has said so: reference -infinity).
+    float2 own[kMostBlocks / 32];
+    float reference = -INFINITY, sum = 0.f;
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-  const int feature = (warp & 1) * 256 + lane * 8;
-  float total[8] = {};
-#pragma unroll
-  for (int k = 0; k < kMostParts; ++k) {
-    const int here = min(parts - k * 32, 32);
-#pragma unroll 8
-    for (int m = 0; m < here; ++m) {
-      const float factor = __shfl_sync(0xffffffffu, own[k].x, m);
-      if (factor == 0.f) continue;  // (its sums may be anything)
-      const float4* values = reinterpret_cast<const float4*>(p.sums + slot_of(k * 32 + m) * kSlotFloats + size_t(row) * LATENT_VALUES + feature);
-      const float4 a = __ldg(values), b = __ldg(values + 1);
-      total[0] += a.x * factor; total[1] += a.y * factor; total[2] += a.z * factor; total[3] += a.w * factor;
-      total[4] += b.x * factor; total[5] += b.y * factor; total[6] += b.z * factor; total[7] += b.w * factor;
+    for (int k = 0; k < kMostBlocks / 32; ++k) {
+      own[k] = live && k * 32 + lane < parts ? __ldg(p.statistics + slot_of(k * 32 + lane) * kRows + row) : make_float2(-INFINITY, 0.f);
+      reference = fmaxf(reference, own[k].x);
     }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) reference = fmaxf(reference, __shfl_xor_sync(0xffffffffu, reference, d));
+#pragma unroll
+    for (int k = 0; k < kMostBlocks / 32; ++k) {
+      own[k].x = own[k].x == -INFINITY ? 0.f : exp2f(own[k].x - reference);
+      sum += own[k].x * own[k].y;
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    // This warp's parts: lane l adds up features 4 l .. + 3 of every 128.
+    float4 total[4] = {};
+    const int step = few ? 1 : kCombineWarps;
+    const float* sums = p.sums + size_t(row) * LATENT_VALUES + half * 256 + lane * 4;
+    auto add = [&](int k) {
+#pragma unroll 4
+      for (int part = k * 32 + (few ? 0 : warp); part < min(parts, k * 32 + 32); part += step) {
+        const float factor = __shfl_sync(0xffffffffu, own[k].x, part & 31);
+        if (factor == 0.f) continue;  // (its sums may be anything)
+        const float4* values = reinterpret_cast<const float4*>(sums + slot_of(part) * kSlotFloats);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (i >= 2 && !few) continue;
+          const float4 v = __ldg(values + i * 32);
+          total[i].x += v.x * factor; total[i].y += v.y * factor; total[i].z += v.z * factor; total[i].w += v.w * factor;
+        }
+      }
+    };
+#pragma unroll
+    for (int k = 0; k < kMostBlocks / 32; ++k)
+      if (k * 32 < parts) add(k);
+    float log_sum;
+    const float sink = live && p.sinks != nullptr ? __ldg(p.sinks + (record.head + row) % p.heads) * kLog2E : -INFINITY;
+    const float inverse = inverse_of(reference, sum, sink, &log_sum);
+    if (live && p.lse != nullptr && lane == 0 && (few || (warp == 0 && half == 0))) p.lse[record.row + row] = log_sum * kLn2;
+    char* out = p.out + (record.row + row) * (LATENT_VALUES * 2);
+    if (few) {
+      if (live) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          reinterpret_cast<uint2*>(out)[i * 32 + lane] = inverse == 0.f ? make_uint2(0, 0)
+              : make_uint2(pack2<kFormat>(total[i].x * inverse, total[i].y * inverse), pack2<kFormat>(total[i].z * inverse, total[i].w * inverse));
+      }
+      continue;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) reinterpret_cast<float4*>(shared_sums[warp])[i * 32 + lane] = total[i];
+    __syncthreads();
+    if (threadIdx.x < 128) {
+      float2 v = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kCombineWarps; ++w) {
+        const float2 share = reinterpret_cast<const float2*>(shared_sums[w])[threadIdx.x];
+        v.x += share.x;
+        v.y += share.y;
+      }
+      reinterpret_cast<uint32_t*>(out)[half * 128 + threadIdx.x] = inverse == 0.f ? 0u : pack2<kFormat>(v.x * inverse, v.y * inverse);
+    }
+    __syncthreads();  // the shares may be overwritten
   }
-  float log_sum;
-  const float sink = p.sinks != nullptr ? __ldg(p.sinks + (record.head + row) % p.heads) * kLog2E : -INFINITY;
-  const float inverse = inverse_of(reference, sum, sink, &log_sum);
-  if (p.lse != nullptr && (threadIdx.x & 63) == 0) p.lse[record.row + row] = log_sum * kLn2;
-  uint4 words = make_uint4(0, 0, 0, 0);
-  if (inverse != 0.f)
-    words = make_uint4(pack2<kFormat>(total[0] * inverse, total[1] * inverse), pack2<kFormat>(total[2] * inverse, total[3] * inverse),
-                       pack2<kFormat>(total[4] * inverse, total[5] * inverse), pack2<kFormat>(total[6] * inverse, total[7] * inverse));
-  *reinterpret_cast<uint4*>(p.out + ((record.row + row) * LATENT_VALUES + feature) * 2) = words;
 }
 
 // One block per SM; no more than `combine_kernel` has room for.
-int grid() { const int count = multiprocessors(); return count < kMostParts * 32 ? count : kMostParts * 32; }
+int grid() { const int count = multiprocessors(); return count < kMostBlocks ? count : kMostBlocks - 1; }
 
 template <int kFormat, int kWidth>
 int launch(const Params& p, int blocks, cudaStream_t stream) {
@@ -882,12 +951,12 @@ int launch(const Params& p, int blocks, cudaStream_t stream) {
   overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   overlap.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(unsigned(blocks), kRows / kCombineRows);
+  config.gridDim = dim3(unsigned(blocks) * 4);
   config.blockDim = dim3(kCombineThreads);
   config.stream = stream;
   config.attrs = &overlap;
   config.numAttrs = 1;
-  return int(cudaLaunchKernelEx(&config, combine_kernel<kFormat>, p));
+  return int(cudaLaunchKernelEx(&config, combine_kernel<kFormat>, p, blocks));
 }
 
 }  // namespace absorbed
