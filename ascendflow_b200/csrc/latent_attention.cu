@@ -126,11 +126,13 @@ struct Request {
   int begin, count;  // tokens
   int length;        // keys
   int rows, tiles;
+  int seen;          // keys that may be read, and one behind the table where the length does not fit
   int near, far;
-  // Cost of the first `t` tiles. (Any function will do that everybody evaluates alike and that grows; in doubles it cannot overflow.)
+  // Cost of the first `t` tiles: any function will do that everybody evaluates alike and that grows.
   __device__ __forceinline__ int64_t cost(int t) const {
-    const double ramp = tiles > 1 ? double(far - near) * (double(t) * double(t - 1)) / (2.0 * double(tiles - 1)) : 0.0;
-    return int64_t(t) * (kFixed + near) + int64_t(ramp);
+    int64_t sum = int64_t(t) * (kFixed + near);
+    if (far != near) sum += int64_t(far - near) * (int64_t(t) * (t - 1) / 2) / (tiles - 1);  // (below 2^31 x 2^31; more than one tile)
+    return sum;
   }
 };
 
@@ -142,8 +144,11 @@ __device__ __forceinline__ Request request_at(const Params& p, int b) {
   r.rows = r.count * p.heads;
   r.tiles = (r.rows + kRows - 1) / kRows;
   // (one key behind the table is enough to report a length that does not fit)
-  r.far = int(min(int64_t(r.length), int64_t(p.pages) * p.page_rows + 1));
+  r.seen = r.far = int(min(int64_t(r.length), int64_t(p.pages) * p.page_rows + 1));
   r.near = int(min(int64_t(r.far), max(int64_t(r.length) - r.count, int64_t(0)) + kRows / p.heads + 1));
+  // Nearly alike (as where tokens are decoded), or too many for the product in `cost`: taken to be alike, which spares a division.
+  if (r.far - r.near <= kChunk) r.near = r.far;
+  else if (r.tiles > 65536) r.near = r.far = (r.near >> 1) + (r.far >> 1);
   return r;
 }
 
@@ -151,7 +156,7 @@ __device__ __forceinline__ Request request_at(const Params& p, int b) {
 __device__ __forceinline__ int chunks_of(const Params& p, const Request& r, int t) {
   const int last_token = (min((t + 1) * kRows, r.rows) - 1) / p.heads;
   const int64_t seen = int64_t(r.length) - r.count + last_token + 1;
-  return int((min(max(seen, int64_t(0)), int64_t(r.far)) + kChunk - 1) / kChunk);
+  return int((min(max(seen, int64_t(0)), int64_t(r.seen)) + kChunk - 1) / kChunk);
 }
 
 // Stretch [at(i), at(i + 1)) of the total cost is block i's.
@@ -318,7 +323,7 @@ __device__ void plan_role(const Params& p, const Shared& sm, const Borders& bord
         piece.token = row / p.heads;
         piece.head = row % p.heads;
         piece.base = r.length - r.count + 1;
-        piece.length = r.far;
+        piece.length = r.seen;
         const bool whole = piece.first == 0 && piece.last == chunks;
         piece.slot = whole ? -1 : 2 * int(blockIdx.x) + (piece.first == 0);
         if (!claim()) break;
@@ -819,114 +824,123 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
   if (warp == kScoreWarp) tmem_dealloc(tmem, 512);
 }
 
-// Tiles that several blocks worked on. Every block makes the list of them, with what there is to do for each: a tile of few parts by groups of
-// eight rows, a warp each; of many parts by half rows, the parts shared out over eight warps. Sums are added in the order of the parts (of the
-// warps' shares), whatever block does it.
-constexpr int kCombineThreads = 256, kCombineWarps = kCombineThreads / 32, kMostBlocks = 256, kFewParts = 8;
+// Tiles that several blocks worked on. Every block makes the list of them, with what there is to do for each: half a row by one warp where
+// the parts are few, by the eight warps of a block together where they are many. Sums are added in the order of the parts (of the
+// warps' shares), whatever block does it. Bound by latency: the list, statistics, and eight parts' sums at a time.
+constexpr int kCombineThreads = 256, kCombineWarps = kCombineThreads / 32, kMostBlocks = 256, kFewParts = 16, kPartsInFlight = 8;
 
 template <int kFormat>
-__global__ void __launch_bounds__(kCombineThreads) combine_kernel(const __grid_constant__ Params p, int blocks) {
+__global__ void __launch_bounds__(kCombineThreads, 2) combine_kernel(const __grid_constant__ Params p, int blocks) {
+  struct Tile {
+    int64_t row;
+    int rows, head, block, parts, items;  // `items`: with those in front of it
+  };
   __shared__ int ends[kCombineWarps];
-  __shared__ struct { int block, parts, items; } list[kMostBlocks];  // tiles; `items`: with those in front of it
-  __shared__ float shared_sums[kCombineWarps][LATENT_VALUES / 2];
+  __shared__ Tile list[kMostBlocks];
+  __shared__ float factors[kCombineWarps][kMostBlocks], shares[kCombineWarps][LATENT_VALUES / 2];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   wait_for_predecessor();
   let_successor_start();
-  // The tiles, packed.
-  const int last = int(threadIdx.x) < blocks ? __ldg(&p.records[threadIdx.x].last) : -1;
-  const int parts_here = last >= 0 ? last - int(threadIdx.x) + 1 : 0;
-  const int items_here = parts_here == 0 ? 0 : parts_here <= kFewParts ? kRows / 8 : 2 * kRows;
-  int packed = items_here << 8 | (parts_here > 0);  // both sums at once: items below 2^15, tiles below 2^8
+  {
+    const int own = threadIdx.x;
+    Record record = {0, 0, 0, -1, {0, 0, 0}};
+    if (own < blocks) record = p.records[own];
+    const int parts = record.last >= 0 ? record.last - own + 1 : 0;
+    const int items = parts == 0 ? 0 : parts <= kFewParts ? (2 * record.rows + kCombineWarps - 1) / kCombineWarps : 2 * record.rows;
+    int packed = items << 8 | (parts > 0);  // both sums at once: items below 2^16, tiles below 2^8
 #pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int other = __shfl_up_sync(0xffffffffu, packed, d);
-    if (lane >= d) packed += other;
-  }
-  if (lane == 31) ends[warp] = packed;
-  __syncthreads();
-  int all = 0;
+    for (int d = 1; d < 32; d <<= 1) {
+      const int other = __shfl_up_sync(0xffffffffu, packed, d);
+      if (lane >= d) packed += other;
+    }
+    if (lane == 31) ends[warp] = packed;
+    __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kCombineWarps; ++w) {
-    if (w < warp) packed += ends[w];
-    all += ends[w];
+    for (int w = 0; w < kCombineWarps; ++w)
+      if (w < warp) packed += ends[w];
+    if (parts > 0) list[(packed & 255) - 1] = {record.row, record.rows, record.head, own, parts, packed >> 8};
+    __syncthreads();
   }
-  if (parts_here > 0) list[(packed & 255) - 1] = {int(threadIdx.x), parts_here, packed >> 8};
-  __syncthreads();
-  const int items = all >> 8;
-  int tile = 0;
+  int items = 0;
+#pragma unroll
+  for (int w = 0; w < kCombineWarps; ++w) items += ends[w] >> 8;
+  int index = 0;
   for (int item = blockIdx.x; item < items; item += gridDim.x) {
-    while (list[tile].items <= item) ++tile;
-    const int first = list[tile].block, parts = list[tile].parts, in_front = tile > 0 ? list[tile - 1].items : 0;
-    const Record record = p.records[first];
-    auto slot_of = [&](int part) { return size_t(part == 0 ? 2 * first + 1 : 2 * (first + part)); };
-    const bool few = parts <= kFewParts;
-    const int row = few ? (item - in_front) * 8 + warp : (item - in_front) >> 1, half = few ? 0 : (item - in_front) & 1;
-    if (row >= record.rows && !few) continue;  // the whole block
-    const bool live = row < record.rows;
-    // Factors: lane l has those of parts l, l + 32, ... (a block that had none of the tile's chunks has said so: reference -infinity).
-    float2 own[kMostBlocks / 32];
+    while (list[index].items <= item) ++index;
+    const Tile tile = list[index];
+    const int place = item - (index > 0 ? list[index - 1].items : 0);
+    const bool few = tile.parts <= kFewParts;
+    const int unit = few ? place * kCombineWarps + warp : place, row = unit >> 1, half = unit & 1;
+    if (few && row >= tile.rows) continue;  // (no barrier in this branch)
+    auto slot_of = [&](int part) { return size_t(part == 0 ? 2 * tile.block + 1 : 2 * (tile.block + part)); };
+    // Factors of the parts (a block that had none of the tile's chunks has said so: reference -infinity).
     float reference = -INFINITY, sum = 0.f;
-#pragma unroll
-    for (int k = 0; k < kMostBlocks / 32; ++k) {
-      own[k] = live && k * 32 + lane < parts ? __ldg(p.statistics + slot_of(k * 32 + lane) * kRows + row) : make_float2(-INFINITY, 0.f);
-      reference = fmaxf(reference, own[k].x);
+    for (int part = lane; part < tile.parts; part += 32) {
+      const float own = __ldg(&p.statistics[slot_of(part) * kRows + row].x);
+      factors[warp][part] = own;
+      reference = fmaxf(reference, own);
     }
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) reference = fmaxf(reference, __shfl_xor_sync(0xffffffffu, reference, d));
-#pragma unroll
-    for (int k = 0; k < kMostBlocks / 32; ++k) {
-      own[k].x = own[k].x == -INFINITY ? 0.f : exp2f(own[k].x - reference);
-      sum += own[k].x * own[k].y;
+    for (int part = lane; part < tile.parts; part += 32) {
+      const float own = factors[warp][part], factor = own == -INFINITY ? 0.f : exp2f(own - reference);
+      factors[warp][part] = factor;
+      sum += factor * __ldg(&p.statistics[slot_of(part) * kRows + row].y);
     }
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    // This warp's parts: lane l adds up features 4 l .. + 3 of every 128.
-    float4 total[4] = {};
-    const int step = few ? 1 : kCombineWarps;
+    __syncwarp();
+    // This warp's parts: lane l adds up features 4 l .. + 3 and 128 + 4 l .. + 3 of the half.
+    float4 total[2] = {};
+    const int step = few ? 1 : kCombineWarps, first = few ? 0 : warp;
     const float* sums = p.sums + size_t(row) * LATENT_VALUES + half * 256 + lane * 4;
-    auto add = [&](int k) {
-#pragma unroll 4
-      for (int part = k * 32 + (few ? 0 : warp); part < min(parts, k * 32 + 32); part += step) {
-        const float factor = __shfl_sync(0xffffffffu, own[k].x, part & 31);
-        if (factor == 0.f) continue;  // (its sums may be anything)
-        const float4* values = reinterpret_cast<const float4*>(sums + slot_of(part) * kSlotFloats);
+    for (int part = first; part < tile.parts; part += step * kPartsInFlight) {
+      float4 v[kPartsInFlight][2];
+      float factor[kPartsInFlight];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (i >= 2 && !few) continue;
-          const float4 v = __ldg(values + i * 32);
-          total[i].x += v.x * factor; total[i].y += v.y * factor; total[i].z += v.z * factor; total[i].w += v.w * factor;
+      for (int n = 0; n < kPartsInFlight; ++n) {
+        const int at = part + n * step, here = min(at, tile.parts - 1);
+        const float4* values = reinterpret_cast<const float4*>(sums + slot_of(here) * kSlotFloats);
+        v[n][0] = __ldg(values);
+        v[n][1] = __ldg(values + 32);
+        factor[n] = factors[warp][here];
+        if (at >= tile.parts) factor[n] = 0.f;
+      }
+#pragma unroll
+      for (int n = 0; n < kPartsInFlight; ++n) {
+        if (factor[n] == 0.f) continue;  // (what a block without chunks of the tile has there may be anything)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          total[i].x += v[n][i].x * factor[n]; total[i].y += v[n][i].y * factor[n];
+          total[i].z += v[n][i].z * factor[n]; total[i].w += v[n][i].w * factor[n];
         }
       }
-    };
-#pragma unroll
-    for (int k = 0; k < kMostBlocks / 32; ++k)
-      if (k * 32 < parts) add(k);
+    }
+    __syncwarp();  // the factors may be overwritten
     float log_sum;
-    const float sink = live && p.sinks != nullptr ? __ldg(p.sinks + (record.head + row) % p.heads) * kLog2E : -INFINITY;
+    const float sink = p.sinks != nullptr ? __ldg(p.sinks + (tile.head + row) % p.heads) * kLog2E : -INFINITY;
     const float inverse = inverse_of(reference, sum, sink, &log_sum);
-    if (live && p.lse != nullptr && lane == 0 && (few || (warp == 0 && half == 0))) p.lse[record.row + row] = log_sum * kLn2;
-    char* out = p.out + (record.row + row) * (LATENT_VALUES * 2);
+    if (p.lse != nullptr && half == 0 && lane == 0 && (few || warp == 0)) p.lse[tile.row + row] = log_sum * kLn2;
+    char* out = p.out + ((tile.row + row) * LATENT_VALUES + half * 256) * 2;
     if (few) {
-      if (live) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          reinterpret_cast<uint2*>(out)[i * 32 + lane] = inverse == 0.f ? make_uint2(0, 0)
-              : make_uint2(pack2<kFormat>(total[i].x * inverse, total[i].y * inverse), pack2<kFormat>(total[i].z * inverse, total[i].w * inverse));
-      }
+      for (int i = 0; i < 2; ++i)
+        reinterpret_cast<uint2*>(out)[i * 32 + lane] = inverse == 0.f ? make_uint2(0, 0)
+            : make_uint2(pack2<kFormat>(total[i].x * inverse, total[i].y * inverse), pack2<kFormat>(total[i].z * inverse, total[i].w * inverse));
       continue;
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i) reinterpret_cast<float4*>(shared_sums[warp])[i * 32 + lane] = total[i];
+    for (int i = 0; i < 2; ++i) reinterpret_cast<float4*>(shares[warp])[i * 32 + lane] = total[i];
     __syncthreads();
     if (threadIdx.x < 128) {
       float2 v = make_float2(0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < kCombineWarps; ++w) {
-        const float2 share = reinterpret_cast<const float2*>(shared_sums[w])[threadIdx.x];
+        const float2 share = reinterpret_cast<const float2*>(shares[w])[threadIdx.x];
         v.x += share.x;
         v.y += share.y;
       }
-      reinterpret_cast<uint32_t*>(out)[half * 128 + threadIdx.x] = inverse == 0.f ? 0u : pack2<kFormat>(v.x * inverse, v.y * inverse);
+      reinterpret_cast<uint32_t*>(out)[threadIdx.x] = inverse == 0.f ? 0u : pack2<kFormat>(v.x * inverse, v.y * inverse);
     }
     __syncthreads();  // the shares may be overwritten
   }
@@ -951,7 +965,7 @@ int launch(const Params& p, int blocks, cudaStream_t stream) {
   overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   overlap.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(unsigned(blocks) * 4);
+  config.gridDim = dim3(unsigned(blocks) * 2);
   config.blockDim = dim3(kCombineThreads);
   config.stream = stream;
   config.attrs = &overlap;
