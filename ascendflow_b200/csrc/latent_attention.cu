@@ -163,6 +163,7 @@ __device__ __forceinline__ int chunks_of(const Params& p, const Request& r, int 
 struct Borders {
   int64_t total, each;
   uint32_t rest, blocks;  // that get a stretch (at most 255)
+  bool whole;             // stretches end between tiles
   __device__ __forceinline__ int64_t at(uint32_t i) const { return each * i + rest * i / blocks; }
 };
 // value * factor / divisor, rounded down: everybody who asks gets the same.
@@ -171,6 +172,9 @@ __device__ __forceinline__ int share_of(int64_t value, int factor, int64_t divis
   if ((product | uint64_t(divisor)) >> 32 == 0) return int(uint32_t(product) / uint32_t(divisor));  // (a 64-bit division takes several times as long)
   return int(product / uint64_t(divisor));
 }
+// What sharing tiles costs a call, in cached rows: the parts' way through memory and `combine_kernel`, the more of both the more tiles there are to share.
+// Where giving every tile to one block makes no block's stretch longer than that, none is shared: the borders move to the nearest tile's.
+constexpr int kSharing = 10 * kChunk, kSharingMany = 27 * kChunk;
 // A block with fewer chunks than these loses more with its start and with its part of the sums than it takes off the others (64 heads, one
 // token; 1, 2, 3, 4 chunks: 2048 keys 18.6, 18.3, 18.8, 22.8 us, 8192 26.2, 22.1, 21.4, 21.2, four requests of 8192 24.1, 24.0, 24.0, 26.2,
 // four of 1024 with six tokens 26.4, 26.2, 31.2, 30.8).
@@ -211,27 +215,42 @@ __device__ __forceinline__ Borders plan_block(const Params& p, int64_t* scratch,
     const int b = round * kThreads + int(threadIdx.x);
     return round == 0 ? own : b < p.batches ? request_at(p, b) : none;
   };
-  Borders borders = {0, 0, 0, 0};
+  Borders borders = {0, 0, 0, 0, false};
   int64_t cost = 0;
-  int most_tiles = 0, least_tiles = INT32_MAX;
+  int most_tiles = 0, least_tiles = INT32_MAX, most_cost = 0, least_cost = INT32_MAX;
   for (int round = 0; round < rounds; ++round) {
     const Request r = of_round(round);
     cost += r.cost(r.tiles);
     most_tiles = max(most_tiles, r.tiles);
-    if (r.tiles > 0) least_tiles = min(least_tiles, r.tiles);
+    if (r.tiles > 0) {
+      least_tiles = min(least_tiles, r.tiles);
+      most_cost = max(most_cost, r.far);
+      least_cost = min(least_cost, r.near);
+    }
   }
   most_tiles = __reduce_max_sync(0xffffffffu, most_tiles);
   least_tiles = __reduce_min_sync(0xffffffffu, least_tiles);
-  if (lane == 0) scratch[kWarps + warp] = int64_t(most_tiles) << 32 | uint32_t(least_tiles);
+  most_cost = __reduce_max_sync(0xffffffffu, most_cost);
+  least_cost = __reduce_min_sync(0xffffffffu, least_cost);
+  if (lane == 0) {
+    scratch[kWarps + warp] = int64_t(most_tiles) << 32 | uint32_t(least_tiles);
+    scratch[2 * kWarps + warp] = int64_t(most_cost) << 32 | uint32_t(least_cost);
+  }
   borders.total = block_sum(cost, scratch);
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) {
     most_tiles = max(most_tiles, int(scratch[kWarps + w] >> 32));
     least_tiles = min(least_tiles, int(uint32_t(scratch[kWarps + w])));
+    most_cost = max(most_cost, int(scratch[2 * kWarps + w] >> 32));
+    least_cost = min(least_cost, int(uint32_t(scratch[2 * kWarps + w])));
   }
   if (borders.total == 0) return borders;
-  const int grid = int(gridDim.x);
+  const int grid = int(gridDim.x), most = most_cost + kFixed;
   int blocks = int(min(max(borders.total / (kLeastChunks * kChunk), int64_t(1)), int64_t(grid)));
+  // The longest stretch if no tile is shared: whole rounds where all cost the same, otherwise half a tile more than the mean, and a tile at least.
+  const int64_t tiles = borders.total / most;  // (where all cost the same)
+  const int64_t longest = most_cost == least_cost ? (tiles + grid - 1) / grid * most : max(int64_t(most), borders.total / grid + most / 2);
+  borders.whole = longest <= borders.total / blocks + kSharing + kSharingMany * min(tiles, int64_t(grid)) / grid;
   if (most_tiles == least_tiles && blocks % most_tiles <= blocks / 16) blocks -= blocks % most_tiles;
   if (int(blockIdx.x) >= blocks) return borders;
   borders.blocks = uint32_t(blocks);
@@ -277,13 +296,13 @@ __device__ __forceinline__ Borders plan_block(const Params& p, int64_t* scratch,
     }
     const int64_t start = passed + in_front + inclusive - value;
     if (value > 0 && start <= mine && mine < start + value) {
-      scratch[2 * kWarps] = round * kThreads + int(threadIdx.x);
-      scratch[2 * kWarps + 1] = start;
+      scratch[3 * kWarps] = round * kThreads + int(threadIdx.x);
+      scratch[3 * kWarps + 1] = start;
     }
     passed += sum;
   }
   __syncthreads();
-  *place = {int(scratch[2 * kWarps]), tile, scratch[2 * kWarps + 1]};
+  *place = {int(scratch[3 * kWarps]), tile, scratch[3 * kWarps + 1]};
   return borders;
 }
 
@@ -313,8 +332,16 @@ __device__ void plan_role(const Params& p, const Shared& sm, const Borders& bord
       const int64_t cost = r.cost(tile + 1) - r.cost(tile), past = start + cost;
       const int chunks = chunks_of(p, r, tile);
       Piece piece;
-      piece.first = at == start ? 0 : share_of(at - start, chunks, cost);
-      piece.last = past <= end ? chunks : share_of(end - start, chunks, cost);
+      if (borders.whole) {  // a border belongs to the tile's nearer end
+        const bool begins = 2 * (at - start) < cost, ends = past <= end || 2 * (end - start) >= cost;
+        piece.first = begins ? 0 : chunks;
+        piece.last = begins && ends ? chunks : 0;
+        if (begins && ends) at = start;
+        else if (chunks == 0) at = start + 1;
+      } else {
+        piece.first = at == start ? 0 : share_of(at - start, chunks, cost);
+        piece.last = past <= end ? chunks : share_of(end - start, chunks, cost);
+      }
       if (piece.first < piece.last || (chunks == 0 && at == start)) {
         const int row = tile * kRows;
         piece.row = int64_t(r.begin) * p.heads + row;
