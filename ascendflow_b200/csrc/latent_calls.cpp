@@ -308,12 +308,14 @@ PyObject* call_prefill(PyObject*, PyObject* const* arguments, Py_ssize_t count) 
   c.heads = q.size(1);
   c.keys = k.size(0);
   c.batches = t[4]->size(0) - 1;
-  if (c.heads < 1 || c.heads > 65535 || c.batches < 0 || c.batches > INT32_MAX / 2 || c.tokens > kMostRows / c.heads || c.keys > kMostRows) Py_RETURN_FALSE;
+  if (c.heads < 1 || c.heads > 65535 || c.batches < 0 || c.batches > INT32_MAX / 2 || c.tokens > kMostRows / c.heads || c.keys > kMostRows ||
+      (c.tokens / 256 + c.batches) * c.heads > INT32_MAX)
+    Py_RETURN_FALSE;
   if (!shaped(q, {c.tokens, c.heads, LATENT_NOPE + LATENT_ROPE}) || !shaped(k, {c.keys, c.heads, LATENT_NOPE}) || !shaped(v, {c.keys, c.heads, LATENT_NOPE}) ||
       !shaped(rope, {c.keys, LATENT_ROPE}))
     Py_RETURN_FALSE;
   for (int i = 0; i < 4; ++i)
-    if (!on_device(*t[i], device, type) || !rows_aligned(*t[i])) Py_RETURN_FALSE;
+    if (!on_device(*t[i], device, type) || !rows_aligned(*t[i]) || (t[i]->size(0) > 1 && t[i]->stride(0) == 0)) Py_RETURN_FALSE;
   if (!plain(*t[4], device, at::kInt, {c.batches + 1}) || !plain(*t[5], device, at::kInt, {c.batches + 1}) ||
       !plain(*out, device, type, {c.tokens, c.heads, LATENT_NOPE}) || !rows_aligned(*out))
     Py_RETURN_FALSE;

@@ -1,6 +1,6 @@
 // Attention of prompts in expanded form: keys and values per head, and one rope key per token for all heads.
 //
-// out = softmax(scale [q] . [k | k_rope]) v per head, causal or not, over ragged requests. One block takes 256 query rows of a
+// out = softmax(scale q . [k | k_rope]) v per head, causal or not, over ragged requests. One block takes 256 query rows of a
 // head as two tiles of 128 and walks the keys in tiles of 128. All products run on tcgen05 with M = 128, N = 128: S = Q K^T from shared
 // memory (K = 192), O += P V with P from tensor memory (K = 128). While the softmax warps of one tile work, the products of
 // the other run.

@@ -271,8 +271,10 @@ def _check_prefill(q, k, v, k_rope, cu_seqlens_q, cu_seqlens_k, scale, causal, o
         _tensor(tensor, name, (q.dtype,))
         require(tuple(tensor.shape) == tuple(shape), f"{name}: expected shape {list(shape)}")
         _rows(tensor, name)
+        require(tensor.shape[0] <= 1 or tensor.stride(0) > 0, f"{name}: tokens must not share memory")
     require(q.shape[:2].numel() <= MOST_ROWS and keys <= MOST_ROWS, "too many rows")
     require(isinstance(cu_seqlens_q, torch.Tensor) and cu_seqlens_q.dim() == 1 and cu_seqlens_q.shape[0] >= 1, "cu_seqlens_q: expected [B + 1]")
+    require((q.shape[0] // 256 + cu_seqlens_q.shape[0] - 1) * heads < 1 << 31, "too many requests and heads")
     for tensor, name in ((cu_seqlens_q, "cu_seqlens_q"), (cu_seqlens_k, "cu_seqlens_k")):
         _tensor(tensor, name, (torch.int32,), cu_seqlens_q.shape)
     _tensor(out, "out", (q.dtype,), (*q.shape[:2], NOPE))

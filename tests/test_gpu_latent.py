@@ -294,6 +294,27 @@ def test_attention_long_and_many(heads, requests, queries, length):
     check_attention(normal(2, requests * queries, heads, 576), cache, table, [queries] * requests, lengths, 192 ** -0.5)
 
 
+@pytest.mark.parametrize("requests,heads", [(600, 16), (1100, 3), (40, 64), (150, 64), (300, 64)])
+def test_attention_ragged_batches(requests, heads):
+    """Requests of every kind in one call, more than a block has threads among them: without tokens, without keys, of many tiles. What one block
+    does alone and what several share follows from the whole batch, so two batches of each."""
+    generator = torch.Generator().manual_seed(requests)
+    for longest in (300, 4000):
+        counts = torch.randint(-1, 4, (requests,), generator=generator).clamp(min=0).tolist()
+        lengths = (torch.rand(requests, generator=generator) ** 4 * longest).int().tolist()
+        counts[requests // 2] = 50
+        cache, table = paged(requests, lengths, 576, 64, BF16)
+        check_attention(normal(2, sum(counts), heads, 576), cache, table, counts, lengths, 192 ** -0.5)
+
+
+@pytest.mark.parametrize("heads,queries,lengths", [
+    (64, 1, [1000] * 149), (64, 2, [640] * 74), (64, 1, [130] * 148), (64, 3, [2000] * 50), (128, 1, [700] * 75), (16, 9, [3000, 3000, 64]), (64, 200, [200, 900]),
+])
+def test_attention_batches_between_sharing_and_not(heads, queries, lengths):
+    cache, table = paged(1, lengths, 576, 128, BF16)
+    check_attention(normal(2, queries * len(lengths), heads, 576), cache, table, [queries] * len(lengths), lengths, 192 ** -0.5)
+
+
 def test_attention_offsets_beyond_32_bits():
     """A cache of more than 2^32 bytes and 2^31 features, its last pages in use."""
     blocks = 4_000_000 // 64
@@ -353,6 +374,37 @@ def test_attention_of_nothing():
     latent.latent_attention(normal(0, 2, 4, 576), cache, table[:0], i32([0]), i32([]), scale=1.0, out=empty)
     assert (empty == 7).all()
     check_attention(normal(2, 2, 4, 576), cache[:0], torch.zeros((1, 0), dtype=torch.int32, device="cuda"), [2], [0], 1.0)
+
+
+@pytest.mark.parametrize("call", ["attention", "prefill", "append"])
+def test_first_call_of_a_process_may_be_captured(call):
+    """A fresh process whose first call of an operator is made while a graph is captured."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    program = """
+import torch
+from ascendflow_b200 import latent
+cache, table = torch.randn((4, 64, 1, 576), device="cuda").half(), torch.arange(4, dtype=torch.int32, device="cuda").view(1, 4)
+cu, seq = torch.tensor([0, 3], dtype=torch.int32, device="cuda"), torch.tensor([200], dtype=torch.int32, device="cuda")
+q, kv = torch.randn((3, 8, 576), device="cuda").half(), torch.randn((3, 8, 256), device="cuda").half()
+frequencies = latent.rotary_frequencies(64)
+calls = {
+    "attention": lambda: latent.latent_attention(q, cache, table, cu, seq, scale=0.1),
+    "prefill": lambda: latent.latent_prefill(q[..., :192], kv[..., :128], kv[..., 128:], q[:, 0, 512:], cu, cu, scale=0.1),
+    "append": lambda: latent.rotary_append(q[:, 0, :512], q[:, 0, 512:], cache, table, cu, seq, frequencies),
+}
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = calls["CALL"]()
+graph.replay()
+replayed = out.clone()
+assert torch.equal(replayed, calls["CALL"]()) and replayed.isfinite().all()
+print("done")
+""".replace("CALL", call)
+    result = subprocess.run([sys.executable, "-c", program], cwd=Path(__file__).resolve().parents[1], capture_output=True, text=True, timeout=120)
+    assert result.stdout.strip() == "done", result.stderr[-2000:]
 
 
 def test_attention_refusals():
@@ -418,6 +470,17 @@ def test_prefill(dtype, causal, heads, counts, lengths):
     check_prefill(normal(1, sum(counts), heads, 192, dtype=dtype), normal(2, keys, heads, 256, dtype=dtype), normal(3, keys, 64, dtype=dtype), counts, lengths, 192 ** -0.5, causal)
 
 
+@pytest.mark.parametrize("heads", [1, 5])
+def test_prefill_ragged_batches(heads):
+    """More requests than a warp has threads, without tokens and without keys among them, and more items than blocks run at a time."""
+    generator = torch.Generator().manual_seed(heads)
+    counts = torch.randint(-3, 40, (170,), generator=generator).clamp(min=0).tolist()
+    lengths = (torch.rand(170, generator=generator) ** 3 * 400).int().tolist()
+    counts[33], lengths[33] = 700, 900
+    counts[64:100] = [0] * 36
+    check_prefill(normal(1, sum(counts), heads, 192), normal(2, sum(lengths), heads, 256), normal(3, sum(lengths), 64), counts, lengths, 192 ** -0.5)
+
+
 @pytest.mark.parametrize("causal", [True, False])
 def test_prefill_rows_that_see_nothing_and_padding(causal):
     """Requests without keys, with fewer keys than queries, and buffers with NaN in front of, between and behind the sequences' ends."""
@@ -480,6 +543,7 @@ def test_prefill_refusals():
         ("k_rope", dict(rope=rope[:, :32])), ("16-byte", dict(k=odd[..., 2:130])), ("int32", dict(cu_k=cu.long())), ("shape", dict(cu_k=i32([0]))),
         ("expected torch.bfloat16", dict(rope=rope.half())), ("overlap", dict(out=kv.view(-1)[: 8 * 2 * 128].view(8, 2, 128))), ("lse", dict(lse=normal(1, 8, 2))),
         ("gradient", dict(v=kv[..., 128:].clone().requires_grad_())), ("out", dict(out=normal(1, 8, 2, 256)[..., :128])),
+        ("share memory", dict(rope=rope[:1].expand(8, 64))), ("share memory", dict(q=q[:1].expand(8, 2, 192))),
     ):
         with pytest.raises(CompileError, match=message):
             call(**change)
