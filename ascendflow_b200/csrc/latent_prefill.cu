@@ -377,9 +377,11 @@ __device__ void product_role(const Params& p, const Shared& sm, uint32_t tmem) {
 
 // ---- softmax ----------------------------------------------------------------------------------------------------------
 
-// A row's reference (log2) starts at the maximum of its first scores and moves when others exceed it by more than kRoom, to kStep below
-// them: weights of up to 2^15 fit IEEE half, and the accumulator is rarely rescaled.
-constexpr float kRoom = 15.f, kStep = 8.f;
+// A row's reference (log2) starts at the maximum of its first scores. It moves, to kStep below the maximum of a step, where the step's weights
+// sum up to more than kMostWeight: weights fit IEEE half, and the accumulator is rarely rescaled. (A sum that large has a weight of
+// more than 2^kStep in it, so that it does move.)
+constexpr float kStep = 8.f, kMostWeight = 32768.f;
+static_assert(kTile * 256 <= kMostWeight, "the smallest sum that is looked into");
 
 template <int kFormat>
 __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
@@ -403,8 +405,8 @@ __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
       const bool masked = key + kTile > warp_end;
       uint32_t words[kTile / 2];
       float own;
-      // Weights are worked out with the reference as it is, without looking for the maximum: as long as their sum stays below 2^kRoom so does each of
-      // them. Where it does not (for some row of the warp), and in a row's first step, the scores are read again and the reference may move.
+      // Weights are worked out with the reference as it is, without looking for the maximum: as long as their sum stays below kMostWeight so does
+      // each of them. Where it does not (for some row of the warp), and in a row's first step, the scores are read again and the reference may move.
       for (bool look = step == 0;; look = true) {
         float2 s[2][16];  // 32 scores, and the next 32 on their way
         auto load = [&](int part) { tmem_ld32(s_tmem + part * 32, reinterpret_cast<uint32_t*>(&s[part & 1][0])); };
@@ -427,7 +429,7 @@ __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
             for (int i = 0; i < 16; ++i) most[i & 3] = greatest(most[i & 3], s[part & 1][i].x, s[part & 1][i].y);
           }
           const float top = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * p.scale_log2;  // scale > 0
-          const bool moves = top > reference + kRoom;
+          const bool moves = top > reference + kStep;
           float alpha = 1.f;
           if (moves) {
             const float next = reference == -INFINITY ? top : top - kStep;
@@ -467,7 +469,7 @@ __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
           }
         }
         own = (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
-        if (look || !__any_sync(0xffffffffu, own > 32768.f)) break;
+        if (look || !__any_sync(0xffffffffu, own > kMostWeight)) break;
       }
       sum += own;
       tmem_st32(s_tmem, words);
