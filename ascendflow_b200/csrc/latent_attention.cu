@@ -20,6 +20,15 @@
 // Tensor memory: columns 0-255 O (lane l: row l % 64, accumulators of features 128 (l / 64) .. + 127 and 256 more), 256-383 Q's first 512
 // features, 384-447 scores, 448-463 the sparse products' metadata, 464-479 Q's other 64 features.
 //
+// What bounds it: memory where a request brings one token (64 requests of 64 heads at 32K: 2.42 GB in 380 us in a few calls after a pause, 6.4 TB/s;
+// in a long loop 410-465 us at 1.0 GHz, since reading random data at that rate takes the board's 1000 W by itself: a plain reduction of as
+// many bytes takes 393 us there), products where it brings several (32 requests of six tokens at 16K: 475-490 us, 0.9 PFLOP/s, 1.0 where all
+// requests share their pages). A chunk takes 2.0 k cycles, 1.43 k of them the two products' own; shared memory's ports are busy for
+// two thirds of it. Two tiles of weights (room for them by a ring of its own for the last 64 features), weights without looking for the
+// maximum, and fewer barriers per chunk were each built and slower by 2 to 12 per cent in loops.
+// A call of few chunks is a chain of 21 us: plan 2.5, pieces and page 2.4, copy 1.6, chunks 0.8 each, sums to memory 3.6 (128 KiB
+// per block at the SM's 32 bytes per cycle), the next kernel's start 1.0, their sum 3 to 4.
+//
 // Rows of a chunk behind the request's length are cleared in the tile's value part (a zero weight times infinity is a
 // NaN) and their scores replaced; so are whole chunks whose page is not in the cache, which are reported.
 #include "latent_common.cuh"

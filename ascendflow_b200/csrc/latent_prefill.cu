@@ -15,6 +15,14 @@
 //
 // Tensor memory: scores (P over their first half) of tile t in columns 128 t .. + 127, O of tile t in 256 + 128 t .. + 127.
 //
+// What paces it: a tile's chain of scores to weights (about 1.9 k cycles: 128 exponentials per thread at 8 cycles a warp are 1.0 k of them) and products
+// (1.6 k, of which 1.3 k are the tensor core's), 3.8 k per step of both tiles against 2.6 k of products. In a loop of large calls the
+// board's power limit, not the chain, decides: 8192 x 8192 tokens of 64 heads, causal, take 1.13 ms in a few calls after a pause (1.22 PFLOP/s) and
+// 1.20 ms in a long loop (1.14 PFLOP/s, 1.6 GHz), and what shortens the chain gives a third of that there. Before: one block per 256 rows and
+// a maximum for every step 1.29 ms; a quarter of the exponentials by a polynomial, weights handed over in halves, and the rows of two heads
+// in a block where a request has no more than 128 were no faster or slowed the large calls down. Registers decide: 160 bytes of spills in the softmax
+// loop make 1.39 ms of it.
+//
 // Rows of a value box behind the request's last key are cleared before they are multiplied: their weights are zero, but they
 // belong to other requests (or to nobody) and 0 x infinity would be a NaN. Scores of such keys are replaced, whatever they are.
 #include "latent_common.cuh"
@@ -44,7 +52,7 @@ constexpr uint32_t kColumnsO = 256;
 
 enum Bar {
   kFull0 = 0, kFree0 = kRing, kQFull0 = 2 * kRing, kQFree0 = kQFull0 + 2, kScores0 = kQFree0 + 2, kWeights0 = kScores0 + 2, kOut0 = kWeights0 + 2,
-  kMended = kOut0 + 2, kAnswer, kLastStep, kItemReady0, kItemDone0 = kItemReady0 + kItems, kBarCount = kItemDone0 + kItems
+  kMended = kOut0 + 2, kAnswer, kNearlyDone, kItemReady0, kItemDone0 = kItemReady0 + kItems, kBarCount = kItemDone0 + kItems
 };
 static_assert(kBarCount <= 40, "the barrier area");
 
@@ -178,9 +186,9 @@ __device__ void plan_role(const Params& p, const Shared& sm, Item item) {
     }
     ++announced;
     if (!has) return;
-    // The next block is asked for when the copies of this item's last step begin: early enough for the answer to come in time, no earlier, so
+    // The next block is asked for when the copies of this item's last step but one begin: early enough for the answer to come in time, no earlier, so
     // that the last items go to whoever is free (8192 x 8192 tokens, 64 heads: asked for with the item's announcement 1389 us, so 1289).
-    if (!warp_wait(sm.bar(kLastStep), asked & 1, abort_flag)) return;
+    if (!warp_wait(sm.bar(kNearlyDone), asked & 1, abort_flag)) return;
     if (lane == 0) {
       fence_proxy_async();  // (the answer before was read through the generic proxy)
       ask_for_block(sm.answer(), sm.bar(kAnswer));
@@ -260,9 +268,9 @@ __device__ void copy_role(const Params& p, const Shared& sm) {
   for (; !given_up && walk.next_of_warp(); walk.done_of_warp()) {
     const Item& item = walk.item;
     const int steps_0 = steps_of(p, item, 0), steps_1 = steps_of(p, item, 1), steps = max(steps_0, steps_1);
-    if (steps == 0 && lane == 0) mbar_arrive(sm.bar(kLastStep));
+    if (steps == 0 && lane == 0) mbar_arrive(sm.bar(kNearlyDone));
     for (int step = 0; step < steps && !given_up; ++step) {
-      if (step + 1 == steps && lane == 0) mbar_arrive(sm.bar(kLastStep));
+      if (step == max(steps - 2, 0) && lane == 0) mbar_arrive(sm.bar(kNearlyDone));
       const int key = item.first + step * kTile;
       for (int box = 0; box < 2 && !given_up; ++box)
         bring([&](uint32_t target, uint32_t bar) { copy_box(target, &p.k, box * 64, item.head * p.k_head, key, bar); }, kTile);
@@ -406,8 +414,9 @@ __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
       uint32_t words[kTile / 2];
       float own;
       // Weights are worked out with the reference as it is, without looking for the maximum: as long as their sum stays below kMostWeight so does
-      // each of them. Where it does not (for some row of the warp), and in a row's first step, the scores are read again and the reference may move.
-      for (bool look = step == 0;; look = true) {
+      // each of them. Where it does not (for some row of the warp) the reference may move, and they are worked out again. A row's first reference is
+      // the maximum of its first 32 scores.
+      for (int look = step == 0 ? 1 : 0;; look = 4) {  // parts of 32 scores to look at
         float2 s[2][16];  // 32 scores, and the next 32 on their way
         auto load = [&](int part) { tmem_ld32(s_tmem + part * 32, reinterpret_cast<uint32_t*>(&s[part & 1][0])); };
         auto mask = [&](int part) {
@@ -418,10 +427,11 @@ __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
             if (2 * i + 1 >= seen) s[part & 1][i].y = -INFINITY;
           }
         };
-        if (look) {
+        if (look > 0) {
           float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
           for (int part = 0; part < 4; ++part) {
+            if (part >= look) break;
             load(part);
             tmem_wait_ld();
             if (masked) mask(part);
@@ -469,7 +479,7 @@ __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
           }
         }
         own = (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
-        if (look || !__any_sync(0xffffffffu, own > kMostWeight)) break;
+        if (look == 4 || !__any_sync(0xffffffffu, own > kMostWeight)) break;
       }
       sum += own;
       tmem_st32(s_tmem, words);
