@@ -79,7 +79,7 @@ static_assert(Layout<576>::kSmemBytes <= 232448, "one block per SM");
 
 enum Bar {
   kFull0 = 0, kFree0 = kFull0 + kStages, kPieceReady0 = kFree0 + kStages, kPieceDone0 = kPieceReady0 + kPieces, kQFull = kPieceDone0 + kPieces,
-  kQFree, kPlaces, kScoresFull, kScoresFree, kWeightsFull, kWeightsFree, kMended, kBarCount
+  kQFree, kPlaces, kScoresFull, kScoresFree, kWeightsFull, kWeightsFree, kMended, kGivenUp0, kGivenUp1, kBarCount
 };
 static_assert(kBarCount <= 32, "the barrier area");
 
@@ -849,8 +849,14 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
   fence_proxy_async();  // the plan's scratch is the first tile's memory
   __syncthreads();
   if (warp < kSoftmaxWarps) softmax_role<kFormat, kWidth>(p, sm, tmem);
-  else if (warp == kScoreWarp) { if (elect_one()) score_role<kFormat, kWidth>(sm, tmem); __syncwarp(); }
-  else if (warp == kValueWarp) { if (elect_one()) value_role<kFormat, kWidth>(sm, tmem); __syncwarp(); }
+  else if (warp == kScoreWarp || warp == kValueWarp) {
+    if (elect_one()) {
+      if (warp == kScoreWarp) score_role<kFormat, kWidth>(sm, tmem);
+      else value_role<kFormat, kWidth>(sm, tmem);
+      if (*sm.abort_flag() != 0) wait_for_products(sm.bar(warp == kScoreWarp ? kGivenUp0 : kGivenUp1));
+    }
+    __syncwarp();
+  }
   else if (warp == kCopyWarp) copy_role<kWidth>(p, sm);
   else if (warp == kPlanWarp) plan_role(p, sm, borders, place);
   else query_role<kWidth>(p, sm, tmem);
@@ -1028,7 +1034,7 @@ int launch_latent_attention(void* stream, const latent_attention_call* call) {
   if (c.batches < 0 || c.batches > INT32_MAX / 2 || c.tokens < 0 || c.heads < 1 || c.tokens > (int64_t(1) << 30) / c.heads) return -1;
   if (c.pages < 0 || c.blocks < 0 || c.page_rows < 64 || c.page_rows % 64 != 0 || c.pages > (INT32_MAX - 128) / c.page_rows || c.blocks > INT32_MAX / c.page_rows) return -1;
   if (c.tokens == 0 || c.batches == 0) return 0;
-  if (c.workspace == nullptr || c.status == nullptr) return -1;
+  if (c.workspace == nullptr || reinterpret_cast<uintptr_t>(c.workspace) % 32 != 0 || c.status == nullptr) return -1;
   const int blocks = latent::absorbed::grid();
   absorbed::Params p = {};
   // (without pages nothing is copied)

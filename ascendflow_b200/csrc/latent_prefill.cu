@@ -52,7 +52,7 @@ constexpr uint32_t kColumnsO = 256;
 
 enum Bar {
   kFull0 = 0, kFree0 = kRing, kQFull0 = 2 * kRing, kQFree0 = kQFull0 + 2, kScores0 = kQFree0 + 2, kWeights0 = kScores0 + 2, kOut0 = kWeights0 + 2,
-  kMended = kOut0 + 2, kAnswer, kNearlyDone, kItemReady0, kItemDone0 = kItemReady0 + kItems, kBarCount = kItemDone0 + kItems
+  kMended = kOut0 + 2, kAnswer, kNearlyDone, kItemReady0, kGivenUp = kItemReady0 + kItems, kItemDone0, kBarCount = kItemDone0 + kItems
 };
 static_assert(kBarCount <= 40, "the barrier area");
 
@@ -549,7 +549,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 104;\n");
     if (warp == kProductWarp) {
-      if (elect_one()) product_role<kFormat>(p, sm, tmem);
+      if (elect_one()) {
+        product_role<kFormat>(p, sm, tmem);
+        if (*sm.abort_flag() != 0) wait_for_products(sm.bar(kGivenUp));
+      }
       __syncwarp();
     } else if (warp == kCopyWarp) {
       copy_role(p, sm);

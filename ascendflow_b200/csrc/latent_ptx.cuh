@@ -70,6 +70,13 @@ __device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_
       "}\n" ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(uint32_t(accumulate)) : "memory");
 }
 
+// For a role that has given up: waits (with the usual limit) for the products that this thread has issued, so that tensor memory can be given back.
+__device__ __forceinline__ void wait_for_products(uint32_t unused_bar) {
+  int never = 0;
+  mma_commit(unused_bar);
+  mbar_wait(unused_bar, 0, &never);
+}
+
 // ---- tensor memory -------------------------------------------------------------------------------------------------
 
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {

@@ -85,7 +85,7 @@ typedef struct {
   int64_t batches, tokens, heads, width, pages, blocks, page_rows;
   double scale;
 } latent_attention_call;
-/* Bytes of `workspace` on the current device; its contents matter to nobody between calls, but calls that may run at the same time need one each. */
+/* Bytes of `workspace` (32-byte aligned) on the current device; its contents matter to nobody between calls, but calls that may run at the same time need one each. */
 int workspace_size_latent_attention(uint64_t* bytes);
 int launch_latent_attention(void* stream, const latent_attention_call* call);
 
