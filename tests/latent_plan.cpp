@@ -58,6 +58,7 @@ inline const int64_t* meet(int64_t mine) {
   return warp.value[generation & 1];
 }
 template <typename T> inline T __shfl_up_sync(unsigned, T v, int d) { const int lane = threadIdx.x & 31; return T(meet(v)[lane >= d ? lane - d : lane]); }
+template <typename T> inline T __shfl_sync(unsigned, T v, int from) { return T(meet(v)[from]); }
 template <typename T> inline T __shfl_xor_sync(unsigned, T v, int d) { const int lane = threadIdx.x & 31; return T(meet(v)[lane ^ d]); }
 inline unsigned __ballot_sync(unsigned, bool v) {
   const int64_t* all = meet(v);
@@ -132,9 +133,14 @@ int main() {
     statistics[size_t(2 * block) * kRows] = {1.f, 1.f};
     body = [&] {
       Place place = {};
-      const Borders borders = plan_block(p, reinterpret_cast<int64_t*>(memory.data()), &place);
-      __syncthreads();
-      if (threadIdx.x >> 5 == kPlanWarp) plan_role(p, sm, borders, place);
+      Borders borders = {};
+      if (batches > 32) {
+        borders = plan_block<kBlockThreads / 32>(p, reinterpret_cast<int64_t*>(memory.data()), &place);
+        __syncthreads();
+      }
+      if (threadIdx.x >> 5 != kPlanWarp) return;
+      if (batches <= 32) borders = plan_block<1>(p, nullptr, &place);
+      plan_role(p, sm, borders, place);
     };
     if (!run_block()) { fprintf(stderr, "block %d: somebody waits for ever\n", block); return 2; }
     for (const Piece& q : pieces) {
