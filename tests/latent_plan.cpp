@@ -127,7 +127,7 @@ int main() {
     sm.ptr = memory.data();
     sm.bars = 0;
     sm.pieces = 2048;
-    sm.misc = 3072;
+    sm.misc = 3328;
     current = &sm;
     pieces.clear();
     statistics[size_t(2 * block) * kRows] = {1.f, 1.f};
