@@ -3,7 +3,7 @@
 // out = softmax(scale Q X^T) X[:, :512] per request, Q the queries of all heads (row j * H + h), X the cached rows, row j * H + h seeing
 // the first L - n + j + 1 of them. Rows of a request are dealt in tiles of 64, whatever the number of heads, and cached rows in
 // chunks of 64 (pages are multiples). A block works on a stretch of the call's (tile, chunk) pairs, tile by tile: all blocks get
-// stretches of the same cost (`Plan`), so a tile may be shared by several blocks; their unnormalised sums then go to the
+// stretches of the same cost (`plan_block`), so a tile may be shared by several blocks; their unnormalised sums then go to the
 // workspace in FP32 and `combine_kernel` adds them up, in the order of the chunks.
 //
 //   warps 0-3   softmax: scores out of tensor memory, running reference and sum in FP32, P (16 bits) to shared memory, rescaling of
@@ -123,8 +123,8 @@ struct Shared {
   __device__ __forceinline__ int64_t* scan() const { return reinterpret_cast<int64_t*>(ptr); }  // (before the first tile lands)
 };
 
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, long long limit = 1ll << 31) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, limit));
 }
 
 // ---- the plan -----------------------------------------------------------------------------------------------------
@@ -337,7 +337,7 @@ __device__ void plan_role(const Params& p, const Shared& sm, const Borders& bord
   bool continued = false;  // slot 2 i holds a part of the tile before
   uint32_t announced = 0;
   // A free entry of the ring; false when somebody has given up.
-  auto claim = [&]() { return announced < kPieces || warp_wait(sm.bar(kPieceDone0 + announced % kPieces), (announced / kPieces - 1) & 1, abort_flag); };
+  auto claim = [&]() { return announced < kPieces || warp_wait(sm.bar(kPieceDone0 + announced % kPieces), (announced / kPieces - 1) & 1, abort_flag, kLongWait); };
   auto announce = [&](const Piece& piece) {
     if (lane == 0) {
       *sm.piece(announced) = piece;
@@ -423,8 +423,8 @@ struct Walk {
   uint32_t index = 0;
   Piece piece;
   __device__ __forceinline__ explicit Walk(const Shared& shared) : sm(shared) {}
-  __device__ __forceinline__ bool next_of_warp() { return warp_wait(sm.bar(kPieceReady0 + index % kPieces), (index / kPieces) & 1, sm.abort_flag()) && read(); }
-  __device__ __forceinline__ bool next_of_thread() { return mbar_wait(sm.bar(kPieceReady0 + index % kPieces), (index / kPieces) & 1, sm.abort_flag()) && read(); }
+  __device__ __forceinline__ bool next_of_warp() { return warp_wait(sm.bar(kPieceReady0 + index % kPieces), (index / kPieces) & 1, sm.abort_flag(), kLongWait) && read(); }
+  __device__ __forceinline__ bool next_of_thread() { return mbar_wait(sm.bar(kPieceReady0 + index % kPieces), (index / kPieces) & 1, sm.abort_flag(), kLongWait) && read(); }
   __device__ __forceinline__ bool read() { piece = *sm.piece(index); return piece.first >= 0; }
   __device__ __forceinline__ void done() { mbar_arrive(sm.bar(kPieceDone0 + index % kPieces)); ++index; }  // one thread
   __device__ __forceinline__ void done_of_warp() {
@@ -528,7 +528,7 @@ __device__ void query_role(const Params& p, const Shared& sm, uint32_t tmem) {
         if (row < piece.rows) words[2 * s + k] = __ldg(reinterpret_cast<const uint4*>(p.q + (piece.row + row) * (kWidth * 2) + segment * 64 + (lane & 3) * 16));
       }
     }
-    if (loads > 0 && !warp_wait(sm.bar(kQFree), (loads - 1) & 1, abort_flag)) return;
+    if (loads > 0 && !warp_wait(sm.bar(kQFree), (loads - 1) & 1, abort_flag, kLongWait)) return;
     tc_fence_after_sync();
 #pragma unroll
     for (int s = 0; s < kOwn; ++s) {
@@ -1049,13 +1049,14 @@ int workspace_size_latent_attention(uint64_t* bytes) {
 
 int launch_latent_attention(void* stream, const latent_attention_call* call) {
   using namespace latent;
+  if (call == nullptr) return -1;
   const latent_attention_call& c = *call;
   if ((c.type != LATENT_F16 && c.type != LATENT_BF16) || (c.width != 512 && c.width != 576) || !(c.scale > 0)) return -1;
   if (c.batches < 0 || c.batches > INT32_MAX / 2 || c.tokens < 0 || c.heads < 1 || c.tokens > (int64_t(1) << 30) / c.heads) return -1;
   if (c.pages < 0 || c.blocks < 0 || c.page_rows < 64 || c.page_rows % 64 != 0 || c.pages > (INT32_MAX - 128) / c.page_rows || c.blocks > INT32_MAX / c.page_rows) return -1;
   if (c.tokens == 0 || c.batches == 0) return 0;
   if (c.workspace == nullptr || reinterpret_cast<uintptr_t>(c.workspace) % 32 != 0 || c.status == nullptr) return -1;
-  const int blocks = latent::absorbed::grid();
+  const int blocks = absorbed::grid();
   absorbed::Params p = {};
   // (without pages nothing is copied)
   const int64_t sizes[2] = {c.width, c.blocks > 0 ? c.blocks * c.page_rows : 1}, strides[1] = {c.width};

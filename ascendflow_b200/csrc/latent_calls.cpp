@@ -26,6 +26,7 @@ decltype(&launch_latent_attention) launch_attention = nullptr;
 decltype(&launch_latent_prefill) launch_prefill = nullptr;
 decltype(&workspace_size_latent_attention) workspace_size = nullptr;
 
+constexpr double kLeastScale = 1e-30, kMostScale = 1e30;  // what FP32 holds with room to spare
 constexpr int64_t kMostRows = int64_t(1) << 30;  // tokens x heads
 
 // A plain torch.Tensor argument, or nullptr.
@@ -234,7 +235,7 @@ PyObject* call_attention(PyObject*, PyObject* const* arguments, Py_ssize_t count
     if ((t[i] = tensor_of(arguments[i])) == nullptr) Py_RETURN_FALSE;
   const Tensor *sinks, *out = tensor_of(arguments[7]), *lse;
   latent_attention_call c = {};
-  if (!number_of(arguments[5], &c.scale) || c.scale <= 0 || out == nullptr || !optional_of(arguments[6], &sinks) || !optional_of(arguments[8], &lse) ||
+  if (!number_of(arguments[5], &c.scale) || c.scale < kLeastScale || c.scale > kMostScale || out == nullptr || !optional_of(arguments[6], &sinks) || !optional_of(arguments[8], &lse) ||
       !t[0]->is_cuda())
     Py_RETURN_FALSE;
   const Tensor &q = *t[0], &cache = *t[1];
@@ -296,7 +297,7 @@ PyObject* call_prefill(PyObject*, PyObject* const* arguments, Py_ssize_t count) 
     if ((t[i] = tensor_of(arguments[i])) == nullptr) Py_RETURN_FALSE;
   const Tensor *out = tensor_of(arguments[8]), *lse;
   latent_prefill_call c = {};
-  if (!number_of(arguments[6], &c.scale) || c.scale <= 0 || !flag_of(arguments[7], &c.causal) || out == nullptr || !optional_of(arguments[9], &lse) ||
+  if (!number_of(arguments[6], &c.scale) || c.scale < kLeastScale || c.scale > kMostScale || !flag_of(arguments[7], &c.causal) || out == nullptr || !optional_of(arguments[9], &lse) ||
       !t[0]->is_cuda())
     Py_RETURN_FALSE;
   const Tensor &q = *t[0], &k = *t[1], &v = *t[2], &rope = *t[3];

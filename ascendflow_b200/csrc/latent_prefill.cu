@@ -143,8 +143,8 @@ __device__ __forceinline__ int steps_of(const Params& p, const Item& item, int t
   return item.rows <= t * kTile ? 0 : (reach(p, item, min(item.rows, (t + 1) * kTile)) + kTile - 1) / kTile;
 }
 
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, long long limit = 1ll << 31) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, limit));
 }
 
 // ---- what to do next ------------------------------------------------------------------------------------------------
@@ -177,7 +177,7 @@ __device__ void plan_role(const Params& p, const Shared& sm, Item item) {
   volatile int* abort_flag = sm.abort_flag();
   uint32_t announced = 0, asked = 0;
   for (bool has = true;; ) {
-    if (announced >= kItems && !warp_wait(sm.bar(kItemDone0 + announced % kItems), (announced / kItems - 1) & 1, abort_flag)) return;
+    if (announced >= kItems && !warp_wait(sm.bar(kItemDone0 + announced % kItems), (announced / kItems - 1) & 1, abort_flag, kLongWait)) return;
     if (lane == 0) {
       Item* target = sm.item(announced);
       *target = item;
@@ -188,7 +188,7 @@ __device__ void plan_role(const Params& p, const Shared& sm, Item item) {
     if (!has) return;
     // The next block is asked for when the copies of this item's last step but one begin: early enough for the answer to come in time, no earlier, so
     // that the last items go to whoever is free (8192 x 8192 tokens, 64 heads: asked for with the item's announcement 1389 us, so 1289).
-    if (!warp_wait(sm.bar(kNearlyDone), asked & 1, abort_flag)) return;
+    if (!warp_wait(sm.bar(kNearlyDone), asked & 1, abort_flag, kLongWait)) return;
     if (lane == 0) {
       fence_proxy_async();  // (the answer before was read through the generic proxy)
       ask_for_block(sm.answer(), sm.bar(kAnswer));
@@ -224,8 +224,8 @@ struct Walk {
   Item item;
   __device__ __forceinline__ explicit Walk(const Shared& shared) : sm(shared) {}
   __device__ __forceinline__ bool read() { item = *sm.item(index); return item.rows > 0; }
-  __device__ __forceinline__ bool next_of_warp() { return warp_wait(sm.bar(kItemReady0 + index % kItems), (index / kItems) & 1, sm.abort_flag()) && read(); }
-  __device__ __forceinline__ bool next_of_thread() { return mbar_wait(sm.bar(kItemReady0 + index % kItems), (index / kItems) & 1, sm.abort_flag()) && read(); }
+  __device__ __forceinline__ bool next_of_warp() { return warp_wait(sm.bar(kItemReady0 + index % kItems), (index / kItems) & 1, sm.abort_flag(), kLongWait) && read(); }
+  __device__ __forceinline__ bool next_of_thread() { return mbar_wait(sm.bar(kItemReady0 + index % kItems), (index / kItems) & 1, sm.abort_flag(), kLongWait) && read(); }
   __device__ __forceinline__ void done() { mbar_arrive(sm.bar(kItemDone0 + index % kItems)); ++index; }
   __device__ __forceinline__ void done_of_warp() {
     __syncwarp();
@@ -592,6 +592,7 @@ int launch(const Params& p, int blocks, cudaStream_t stream) {
 
 extern "C" int launch_latent_prefill(void* stream, const latent_prefill_call* call) {
   using namespace latent;
+  if (call == nullptr) return -1;
   const latent_prefill_call& c = *call;
   if ((c.type != LATENT_F16 && c.type != LATENT_BF16) || !(c.scale > 0) || c.status == nullptr) return -1;
   if (c.batches < 0 || c.batches >= INT32_MAX || c.tokens < 0 || c.tokens > INT32_MAX - 256 || c.keys < 0 || c.keys > INT32_MAX - 256 || c.heads < 1 || c.heads > 65535) return -1;

@@ -12,9 +12,6 @@ namespace sm100 {
 
 // ---- tensor copies ------------------------------------------------------------------------------------------------
 
-__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
-  asm volatile("prefetch.tensormap [%0];\n" ::"l"(map) : "memory");
-}
 // A box to shared memory; counts its bytes on `bar`. The first coordinate is a multiple of 16 bytes. What lies outside of the tensor is zero.
 __device__ __forceinline__ void copy_box(uint32_t target, const CUtensorMap* map, int x, int y, uint32_t bar) {
   asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n"
@@ -69,6 +66,10 @@ __device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
       "}\n" ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(uint32_t(accumulate)) : "memory");
 }
+
+// Limit (SM clocks, half a minute) of a wait that lasts as long as others work through many tiles; what they wait for by themselves has the usual one of a
+// second, and whoever gives up ends all waits of the block.
+constexpr long long kLongWait = 1ll << 36;
 
 // For a role that has given up: waits (with the usual limit) for the products that this thread has issued, so that tensor memory can be given back.
 __device__ __forceinline__ void wait_for_products(uint32_t unused_bar) {

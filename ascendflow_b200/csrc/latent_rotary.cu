@@ -159,6 +159,7 @@ extern "C" {
 
 int launch_latent_rotary(void* stream, const latent_rotary_call* call) {
   using namespace latent;
+  if (call == nullptr) return -1;
   const latent_rotary_call& c = *call;
   const int size = c.type == LATENT_F32 ? 4 : 2;
   if (c.type < LATENT_F16 || c.type > LATENT_F32 || !pairs_fit(c.pairs) || c.features < 2 * c.pairs || c.features % 8 != 0) return -1;
@@ -180,6 +181,7 @@ int launch_latent_rotary(void* stream, const latent_rotary_call* call) {
 
 int launch_latent_append(void* stream, const latent_append_call* call) {
   using namespace latent;
+  if (call == nullptr) return -1;
   const latent_append_call& c = *call;
   if ((c.type != LATENT_F16 && c.type != LATENT_BF16) || !pairs_fit(c.pairs) || c.width < 2 * c.pairs || c.width % 8 != 0 || c.width > 65536) return -1;
   if (c.batches < 0 || c.batches >= INT32_MAX || c.tokens < 0 || c.tokens > INT32_MAX || c.pages < 0 || c.blocks < 0 || c.page_rows < 1) return -1;

@@ -243,7 +243,7 @@ def _check_written(out, lse, inputs):
 
 def _check_attention(q, cache, block_table, cu_seqlens_q, seqused_kv, scale, sinks, out, lse):
     _number(scale, "scale")
-    require(scale > 0, "scale must be above 0")
+    require(1e-30 <= scale <= 1e30, "scale must be a positive float32 number")
     _tensor(q, "q", _STORED)
     require(q.dim() == 3 and q.shape[2] in (512, 576) and q.shape[1] >= 1 and q.is_contiguous(), "q: expected contiguous [T, H, 512] or [T, H, 576]")
     require(q.shape[:2].numel() <= MOST_ROWS, "q: too many rows")
@@ -261,7 +261,7 @@ def _check_attention(q, cache, block_table, cu_seqlens_q, seqused_kv, scale, sin
 
 def _check_prefill(q, k, v, k_rope, cu_seqlens_q, cu_seqlens_k, scale, causal, out, lse):
     _number(scale, "scale")
-    require(scale > 0, "scale must be above 0")
+    require(1e-30 <= scale <= 1e30, "scale must be a positive float32 number")
     require(isinstance(causal, bool), "causal: expected True or False")
     _tensor(q, "q", _STORED)
     require(q.dim() == 3 and q.shape[2] == NOPE + ROPE and 1 <= q.shape[1] <= 65535, "q: expected [T, H, 192]")

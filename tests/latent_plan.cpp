@@ -93,7 +93,8 @@ inline bool run_block() {
 void announced_on(uint32_t bar);
 inline void mbar_arrive(uint32_t bar) { announced_on(bar); }
 struct Shared;
-inline bool warp_wait(uint32_t, uint32_t, volatile int*) { meet(0); return true; }
+constexpr long long kLongWait = 1ll << 36;
+inline bool warp_wait(uint32_t, uint32_t, volatile int*, long long) { meet(0); return true; }
 
 #include "plan.inc"
 

@@ -415,7 +415,7 @@ def test_attention_refusals():
     call()
     big = normal(3, 3, 8, 1024)
     for message, change in (
-        ("scale", dict(scale=-1.0)), ("scale", dict(scale="1")), ("576", dict(q=normal(2, 3, 8, 640))), ("contiguous", dict(q=big[..., :576])),
+        ("scale", dict(scale=-1.0)), ("scale", dict(scale="1")), ("scale", dict(scale=1e300)), ("576", dict(q=normal(2, 3, 8, 640))), ("contiguous", dict(q=big[..., :576])),
         ("as wide", dict(q=big[..., :512].contiguous())), ("expected torch.bfloat16", dict(q=q, cache=cache.half())), ("float16", dict(q=q.float())),
         ("multiple of 64 rows", dict(cache=cache.view(-1, 32, 1, 576))), ("int32", dict(seq=seq.long())), ("shape", dict(cu=i32([0, 1, 3]))),
         ("sinks", dict(sinks=normal(1, 7, dtype=F32))), ("sinks", dict(sinks=normal(1, 8))), ("lse", dict(lse=normal(1, 3, 8))),
