@@ -129,23 +129,30 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
 
 // ---- the plan -----------------------------------------------------------------------------------------------------
 
-// A request's tiles and what they cost, in cached rows: the tiles' rows see from `near` keys on up to `far`, a piece costs kFixed more.
+// A request's tiles and what they cost, in cached rows: the tiles' rows see from `near` keys on up to `far`, a tile costs kFixed more.
 constexpr int kFixed = 128;
 struct Request {
   int begin, count;  // tokens
   int length;        // keys
   int rows, tiles;
   int seen;          // keys that may be read, and one behind the table where the length does not fit
-  int near, far;
+  int near, far, fixed;
   // Cost of the first `t` tiles: any function will do that everybody evaluates alike and that grows.
   __device__ __forceinline__ int64_t cost(int t) const {
-    int64_t sum = int64_t(t) * (kFixed + near);
+    int64_t sum = int64_t(t) * (fixed + near);
     if (far != near) sum += int64_t(far - near) * (int64_t(t) * (t - 1) / 2) / (tiles - 1);  // (below 2^31 x 2^31; more than one tile)
     return sum;
   }
+  // Blocks that a tile gets if each takes 1 / `density` rows or a little less (rounded somehow: only everybody has to get the same).
+  __device__ __forceinline__ int blocks(float density) const { return max(1, int(ceilf(float(far) * density))); }
+  // From here on a tile costs the blocks that it gets.
+  __device__ __forceinline__ void dealt(float density) {
+    near = far = blocks(density);
+    fixed = 0;
+  }
 };
 
-__device__ __forceinline__ Request request_at(const Params& p, int b) {
+__device__ __forceinline__ Request request_at(const Params& p, int b, float density = 0.f) {
   Request r;
   r.begin = min(max(__ldg(p.cu + b), 0), p.tokens);
   r.count = max(min(max(__ldg(p.cu + b + 1), 0), p.tokens) - r.begin, 0);
@@ -158,6 +165,8 @@ __device__ __forceinline__ Request request_at(const Params& p, int b) {
   // Nearly alike (as where tokens are decoded), or too many for the product in `cost`: taken to be alike, which spares a division.
   if (r.far - r.near <= kChunk) r.near = r.far;
   else if (r.tiles > 65536) r.near = r.far = (r.near >> 1) + (r.far >> 1);
+  r.fixed = kFixed;
+  if (density > 0.f) r.dealt(density);
   return r;
 }
 
@@ -173,17 +182,26 @@ struct Borders {
   int64_t total, each;
   uint32_t rest, blocks;  // that get a stretch (at most 255)
   bool whole;             // stretches end between tiles
+  float density;          // > 0: every tile has blocks of its own, so many per row; costs are numbers of blocks
   __device__ __forceinline__ int64_t at(uint32_t i) const { return each * i + rest * i / blocks; }
 };
+// Quotients of numbers that are not negative (a 64-bit division takes several times as long as one of 32 bits).
+__device__ __forceinline__ int64_t quotient(int64_t value, int64_t divisor) {
+  if ((uint64_t(value) | uint64_t(divisor)) >> 32 == 0) return uint32_t(value) / uint32_t(divisor);
+  return value / divisor;
+}
 // value * factor / divisor, rounded down: everybody who asks gets the same.
 __device__ __forceinline__ int share_of(int64_t value, int factor, int64_t divisor) {
-  const uint64_t product = uint64_t(value) * uint32_t(factor);
-  if ((product | uint64_t(divisor)) >> 32 == 0) return int(uint32_t(product) / uint32_t(divisor));  // (a 64-bit division takes several times as long)
-  return int(product / uint64_t(divisor));
+  return int(quotient(value * factor, divisor));
 }
 // What sharing tiles costs a call, in cached rows: the parts' way through memory and `combine_kernel`, the more of both the more tiles there are to share.
-// Where giving every tile to one block makes no block's stretch longer than that, none is shared: the borders move to the nearest tile's.
-constexpr int kSharing = 10 * kChunk, kSharingMany = 27 * kChunk;
+// Where giving every tile to one block makes no block's stretch longer than that, none is shared: the borders move to the nearest tile's. (64 heads, one
+// token; whole / shared: 512 keys 16.7 / 16.1 us, 32 requests of 1024 25.4 / 23.9, 64 of 1024 28.1 / 30, 64 of 2048 49.7 / 52.5.)
+constexpr int kSharing = 6 * kChunk, kSharingMany = 32 * kChunk;
+// A block that ends one tile and begins another writes sums twice, and all wait for it. Where every tile can have blocks of its own without making the
+// stretches longer than by this (for 64 rows), it has: 64 heads, one token, 3, 8, 16, 32 requests of 8192 keys 27.1, 36.6, 48.2, 76.5 us with borders anywhere,
+// 24.3, 33.4, 45.9, 73.4 so; 32 requests of 512 to 4096 keys 38.0 and 34.1.
+constexpr int kTwoTiles = 10 * kChunk;
 // A block with fewer chunks than these loses more with its start and with its part of the sums than it takes off the others (64 heads, one
 // token; 1, 2, 3, 4 chunks: 2048 keys 18.6, 18.3, 18.8, 22.8 us, 8192 26.2, 22.1, 21.4, 21.2, four requests of 8192 24.1, 24.0, 24.0, 26.2,
 // four of 1024 with six tokens 26.4, 26.2, 31.2, 30.8).
@@ -210,6 +228,20 @@ __device__ __forceinline__ int64_t plan_sum(int64_t value, int64_t* scratch) {
   return sum;
 }
 
+// The same for numbers whose sum fits.
+template <int kWarps>
+__device__ __forceinline__ int plan_count(int value, int64_t* scratch) {
+  value = __reduce_add_sync(0xffffffffu, value);
+  if constexpr (kWarps == 1) return value;
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = value;
+  __syncthreads();
+  int sum = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) sum += int(scratch[w]);
+  return sum;
+}
+
 // The stretches, and where this block's begins; by all threads of the block, or, for up to 32 requests, by one warp (which saves the others' barriers:
 // 1.1 of 21.5 us of a call of one token).
 //
@@ -223,12 +255,12 @@ __device__ __forceinline__ Borders plan_block(const Params& p, int64_t* scratch,
   const int warp = kWarps == 1 ? 0 : int(threadIdx.x >> 5), lane = threadIdx.x & 31, thread = warp * 32 + lane;
   const int rounds = (p.batches + kRound - 1) / kRound;
   Request none = {};
-  const Request own = thread < p.batches ? request_at(p, thread) : none;
+  Borders borders = {0, 0, 0, 0, false, 0.f};
+  Request own = thread < p.batches ? request_at(p, thread) : none;
   auto of_round = [&](int round) {
     const int b = round * kRound + thread;
     return round == 0 ? own : b < p.batches ? request_at(p, b) : none;
   };
-  Borders borders = {0, 0, 0, 0, false};
   int64_t cost = 0;
   int most_tiles = 0, least_tiles = INT32_MAX, most_cost = 0, least_cost = INT32_MAX;
   for (int round = 0; round < rounds; ++round) {
@@ -261,13 +293,50 @@ __device__ __forceinline__ Borders plan_block(const Params& p, int64_t* scratch,
   const int grid = int(gridDim.x), most = most_cost + kFixed;
   int blocks = int(min(max(borders.total / (kLeastChunks * kChunk), int64_t(1)), int64_t(grid)));
   // The longest stretch if no tile is shared: whole rounds where all cost the same, otherwise half a tile more than the mean, and a tile at least.
-  const int64_t tiles = borders.total / most;  // (where all cost the same)
-  const int64_t longest = most_cost == least_cost ? (tiles + grid - 1) / grid * most : max(int64_t(most), borders.total / grid + most / 2);
-  borders.whole = longest <= borders.total / blocks + kSharing + kSharingMany * min(tiles, int64_t(grid)) / grid;
-  if (most_tiles == least_tiles && blocks % most_tiles <= blocks / 16) blocks -= blocks % most_tiles;
+  const bool alike = most_cost == least_cost;
+  const int64_t tiles = quotient(borders.total, most), mean = quotient(borders.total, blocks);  // (tiles: where all cost the same)
+  const int64_t longest = alike ? quotient(tiles + grid - 1, grid) * most : max(int64_t(most), (blocks == grid ? mean : quotient(borders.total, grid)) + most / 2);
+  borders.whole = longest <= mean + kSharing + kSharingMany * int(min(tiles, int64_t(grid))) / grid;
+  static_assert(kWarps == 1 || kRound > 255, "a thread for each of as many requests as blocks");
+  if (!borders.whole && tiles <= grid && p.batches <= grid && mean < (1 << 30)) {  // blocks of their own for every tile?
+    const int rows = min(kRows, int(uint32_t(p.tokens * p.heads) / uint32_t(p.batches)));
+    const int more = kTwoTiles * rows / kRows;  // (what a second tile costs is its rows' sums)
+    if (alike) {
+      const int each = min(int(uint32_t(grid) / uint32_t(tiles)), (most_cost + kLeastChunks * kChunk - 1) / (kLeastChunks * kChunk));
+      if ((mean + more) * each * tiles >= borders.total) blocks = each * int(tiles);
+    } else {
+      // The shortest stretch that will do, nearly.
+      int needed = 0, stretch = 0;
+#pragma unroll 1
+      for (int candidate = int(mean), step = more;;) {
+        const float tried = 1.f / float(candidate);
+        // (a request's tiles have to cost the same; each thread has a request at most)
+        const int wanted = own.near == own.far && own.tiles <= grid ? own.tiles * min(own.blocks(tried), grid + 1) : grid + 1;
+        const int sum = plan_count<kWarps>(own.tiles == 0 ? 0 : wanted, scratch);
+        if (sum <= grid) {
+          stretch = candidate;
+          borders.density = tried;
+          needed = sum;
+        }
+        if (candidate == int(mean)) {
+          if (stretch > 0 || more == 0) break;
+          candidate += more;
+        } else {
+          step >>= 1;
+          if (stretch == 0 || step < kChunk / 3) break;
+          candidate = stretch - step;
+        }
+      }
+      if (stretch > 0) {
+        borders.total = blocks = needed;
+        if (thread < p.batches) own.dealt(borders.density);
+      }
+    }
+  }
+  if (borders.density == 0.f && most_tiles == least_tiles && uint32_t(blocks) % uint32_t(most_tiles) <= uint32_t(blocks) / 16) blocks -= uint32_t(blocks) % uint32_t(most_tiles);
   if (int(blockIdx.x) >= blocks) return borders;
   borders.blocks = uint32_t(blocks);
-  borders.each = borders.total / blocks;
+  borders.each = borders.density > 0.f ? 1 : quotient(borders.total, blocks);
   borders.rest = uint32_t(borders.total - borders.each * blocks);
   const int64_t mine = borders.at(blockIdx.x);
   // The tile: the last whose predecessors cost no more.
@@ -351,7 +420,7 @@ __device__ void plan_role(const Params& p, const Shared& sm, const Borders& bord
     int request = place.request, tile = place.tile;
     int64_t start = place.start;
     while (at < end) {
-      const Request r = request_at(p, request);
+      const Request r = request_at(p, request, borders.density);
       const int64_t cost = r.cost(tile + 1) - r.cost(tile), past = start + cost;
       const int chunks = chunks_of(p, r, tile);
       Piece piece;

@@ -68,6 +68,7 @@ inline unsigned __ballot_sync(unsigned, bool v) {
 }
 inline int __reduce_max_sync(unsigned, int v) { const int64_t* all = meet(v); return int(*std::max_element(all, all + 32)); }
 inline int __reduce_min_sync(unsigned, int v) { const int64_t* all = meet(v); return int(*std::min_element(all, all + 32)); }
+inline int __reduce_add_sync(unsigned, int v) { const int64_t* all = meet(v); int sum = 0; for (int i = 0; i < 32; ++i) sum += int(all[i]); return sum; }
 inline bool run_block() {
   running = kBlockThreads;
   block_arrived = 0;

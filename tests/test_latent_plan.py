@@ -125,3 +125,27 @@ def test_stretches_are_even_and_tiles_side_by_side(plan):
     # one tile for each of 100 blocks: none is shared
     pieces, _ = plan(148, 64, [1] * 100, [400] * 100, 1 << 20, 64)
     assert sorted(len(own) for own in pieces) == [0] * 48 + [1] * 100
+
+
+@pytest.mark.parametrize("heads,count,requests,length,stretch", [(64, 1, 8, 8192, 18), (64, 1, 3, 8192, 49), (64, 1, 32, 2048, 4), (16, 2, 16, 8192, 9), (64, 6, 4, 8192, 6), (64, 1, 1, 8192, 64)])
+def test_tiles_alike_have_blocks_of_their_own(plan, heads, count, requests, length, stretch):
+    loads = check(plan, 148, heads, [count] * requests, [length] * requests)
+    pieces, _ = plan(148, heads, [count] * requests, [length] * requests, 1 << 20, 64)
+    tiles = requests * -(-heads * count // ROWS)
+    assert [len(own) for own in pieces] == [1] * (tiles * stretch) + [0] * (148 - tiles * stretch)
+    assert max(loads) == -(-(-(-length // CHUNK)) // stretch)
+
+
+@pytest.mark.parametrize("requests,seed", [(2, 0), (12, 2), (33, 4), (60, 5), (148, 7)])
+def test_ragged_tiles_have_blocks_of_their_own(plan, requests, seed):
+    rng = np.random.default_rng(seed)
+    lengths = rng.integers(1000, 9000, requests).tolist()
+    loads = check(plan, 148, 64, [1] * requests, lengths)
+    pieces, _ = plan(148, 64, [1] * requests, lengths, 1 << 20, 64)
+    if requests <= 60:  # (with more of them a block of their own for each would be too long a stretch)
+        assert max(len(own) for own in pieces) == 1
+    # no stretch is longer than the mean by more than ten chunks, rounding, or a whole tile that is not worth sharing
+    assert max(loads) <= sum(loads) / 148 + 10 + 2 or max(len(own) for own in pieces) <= 2
+    check(plan, 148, 64, [1] * requests, [0] * (requests - 1) + [9000])
+    check(plan, 148, 16, [1] * requests, lengths)
+    check(plan, 148, 16, [1] * (requests - 1) + [400], lengths)  # (a request's tiles differ)
