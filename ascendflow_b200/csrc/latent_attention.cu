@@ -955,18 +955,19 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
   if (warp == kScoreWarp) tmem_dealloc(tmem, 512);
 }
 
-// Tiles that several blocks worked on. Every block makes the list of them, with what there is to do for each: half a row by one warp where
-// the parts are few, by the eight warps of a block together where they are many. Sums are added in the order of the parts (of the
-// warps' shares), whatever block does it. Bound by latency: the list, statistics, and eight parts' sums at a time.
-constexpr int kCombineThreads = 256, kCombineWarps = kCombineThreads / 32, kMostBlocks = 256, kFewParts = 16, kPartsInFlight = 8;
+// Tiles that several blocks worked on. Every block makes the list of them, with what there is to do for each: half a row by one to eight
+// warps of a block, as many as bring all parts with one round of loads if there are blocks enough for that. Sums are added in the order of
+// the parts (of the warps' shares), whatever block does it. Bound by latency: the list; statistics and the first round of sums together; the others.
+// (8 requests of 8192 keys, one token, 64 heads, 18 parts each: 4.0 us, and 8.7 with eight warps for every half row and statistics in front of the sums.)
+constexpr int kCombineThreads = 256, kCombineWarps = kCombineThreads / 32, kMostBlocks = 256, kPartsInFlight = 6;
 
 template <int kFormat>
 __global__ void __launch_bounds__(kCombineThreads, 2) combine_kernel(const __grid_constant__ Params p, int blocks) {
   struct Tile {
     int64_t row;
-    int rows, head, block, parts, items;  // `items`: with those in front of it
+    int rows, head, block, parts, warps, items;  // `items` for a block: with those in front of it
   };
-  __shared__ int ends[kCombineWarps];
+  __shared__ int wishes[kCombineWarps], ends[kCombineWarps];
   __shared__ Tile list[kMostBlocks];
   __shared__ float factors[kCombineWarps][kMostBlocks], shares[kCombineWarps][LATENT_VALUES / 2];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -977,7 +978,15 @@ __global__ void __launch_bounds__(kCombineThreads, 2) combine_kernel(const __gri
     Record record = {0, 0, 0, -1, {0, 0, 0}};
     if (own < blocks) record = p.records[own];
     const int parts = record.last >= 0 ? record.last - own + 1 : 0;
-    const int items = parts == 0 ? 0 : parts <= kFewParts ? (2 * record.rows + kCombineWarps - 1) / kCombineWarps : 2 * record.rows;
+    int warps = parts <= kPartsInFlight ? 1 : parts <= 2 * kPartsInFlight ? 2 : parts <= 4 * kPartsInFlight ? 4 : kCombineWarps;
+    const int wish = __reduce_add_sync(0xffffffffu, parts == 0 ? 0 : 2 * record.rows * warps);
+    if (lane == 0) wishes[warp] = wish;
+    __syncthreads();
+    int wanted = 0;
+#pragma unroll
+    for (int w = 0; w < kCombineWarps; ++w) wanted += wishes[w];
+    for (; wanted > int(gridDim.x) * kCombineWarps; wanted >>= 1) warps = max(1, warps >> 1);
+    const int items = parts == 0 ? 0 : (2 * record.rows * warps + kCombineWarps - 1) / kCombineWarps;
     int packed = items << 8 | (parts > 0);  // both sums at once: items below 2^16, tiles below 2^8
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -989,7 +998,7 @@ __global__ void __launch_bounds__(kCombineThreads, 2) combine_kernel(const __gri
 #pragma unroll
     for (int w = 0; w < kCombineWarps; ++w)
       if (w < warp) packed += ends[w];
-    if (parts > 0) list[(packed & 255) - 1] = {record.row, record.rows, record.head, own, parts, packed >> 8};
+    if (parts > 0) list[(packed & 255) - 1] = {record.row, record.rows, record.head, own, parts, warps, packed >> 8};
     __syncthreads();
   }
   int items = 0;
@@ -999,61 +1008,66 @@ __global__ void __launch_bounds__(kCombineThreads, 2) combine_kernel(const __gri
   for (int item = blockIdx.x; item < items; item += gridDim.x) {
     while (list[index].items <= item) ++index;
     const Tile tile = list[index];
-    const int place = item - (index > 0 ? list[index - 1].items : 0);
-    const bool few = tile.parts <= kFewParts;
-    const int unit = few ? place * kCombineWarps + warp : place, row = unit >> 1, half = unit & 1;
-    if (few && row >= tile.rows) continue;  // (no barrier in this branch)
+    const int place = item - (index > 0 ? list[index - 1].items : 0), warps = tile.warps;
+    const int unit = (place * kCombineWarps + warp) / warps, first = warp & (warps - 1), row = unit >> 1, half = unit & 1;
+    const bool live = row < tile.rows;
     auto slot_of = [&](int part) { return size_t(part == 0 ? 2 * tile.block + 1 : 2 * (tile.block + part)); };
-    // Factors of the parts (a block that had none of the tile's chunks has said so: reference -infinity).
-    float reference = -INFINITY, sum = 0.f;
-    for (int part = lane; part < tile.parts; part += 32) {
-      const float own = __ldg(&p.statistics[slot_of(part) * kRows + row].x);
-      factors[warp][part] = own;
-      reference = fmaxf(reference, own);
-    }
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) reference = fmaxf(reference, __shfl_xor_sync(0xffffffffu, reference, d));
-    for (int part = lane; part < tile.parts; part += 32) {
-      const float own = factors[warp][part], factor = own == -INFINITY ? 0.f : exp2f(own - reference);
-      factors[warp][part] = factor;
-      sum += factor * __ldg(&p.statistics[slot_of(part) * kRows + row].y);
-    }
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    __syncwarp();
-    // This warp's parts: lane l adds up features 4 l .. + 3 and 128 + 4 l .. + 3 of the half.
-    float4 total[2] = {};
-    const int step = few ? 1 : kCombineWarps, first = few ? 0 : warp;
-    const float* sums = p.sums + size_t(row) * LATENT_VALUES + half * 256 + lane * 4;
-    for (int part = first; part < tile.parts; part += step * kPartsInFlight) {
-      float4 v[kPartsInFlight][2];
-      float factor[kPartsInFlight];
+    // This warp's parts: every `warps`-th, lane l adds up features 4 l .. + 3 and 128 + 4 l .. + 3 of the half.
+    const float* sums = p.sums + size_t(min(row, kRows - 1)) * LATENT_VALUES + half * 256 + lane * 4;
+    float4 v[kPartsInFlight][2], total[2] = {};
+    auto load = [&](int part) {
 #pragma unroll
       for (int n = 0; n < kPartsInFlight; ++n) {
-        const int at = part + n * step, here = min(at, tile.parts - 1);
-        const float4* values = reinterpret_cast<const float4*>(sums + slot_of(here) * kSlotFloats);
+        if (part + n * warps >= tile.parts) break;
+        const float4* values = reinterpret_cast<const float4*>(sums + slot_of(part + n * warps) * kSlotFloats);
         v[n][0] = __ldg(values);
         v[n][1] = __ldg(values + 32);
-        factor[n] = factors[warp][here];
-        if (at >= tile.parts) factor[n] = 0.f;
+      }
+    };
+    if (live) load(first);
+    // Factors of the parts (a block that had none of the tile's chunks has said so: reference -infinity).
+    float reference = -INFINITY, sum = 0.f;
+    if (live) {
+      for (int part = lane; part < tile.parts; part += 32) {
+        const float own = __ldg(&p.statistics[slot_of(part) * kRows + row].x);
+        factors[warp][part] = own;
+        reference = fmaxf(reference, own);
       }
 #pragma unroll
-      for (int n = 0; n < kPartsInFlight; ++n) {
-        if (factor[n] == 0.f) continue;  // (what a block without chunks of the tile has there may be anything)
+      for (int d = 16; d > 0; d >>= 1) reference = fmaxf(reference, __shfl_xor_sync(0xffffffffu, reference, d));
+      for (int part = lane; part < tile.parts; part += 32) {
+        const float own = factors[warp][part], factor = own == -INFINITY ? 0.f : exp2f(own - reference);
+        factors[warp][part] = factor;
+        sum += factor * __ldg(&p.statistics[slot_of(part) * kRows + row].y);
+      }
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          total[i].x += v[n][i].x * factor[n]; total[i].y += v[n][i].y * factor[n];
-          total[i].z += v[n][i].z * factor[n]; total[i].w += v[n][i].w * factor[n];
+      for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      __syncwarp();
+      for (int part = first; part < tile.parts;) {
+#pragma unroll
+        for (int n = 0; n < kPartsInFlight; ++n) {
+          const int at = part + n * warps;
+          if (at >= tile.parts) break;
+          const float factor = factors[warp][at];
+          if (factor == 0.f) continue;  // (what a block without chunks of the tile has there may be anything)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            total[i].x += v[n][i].x * factor; total[i].y += v[n][i].y * factor;
+            total[i].z += v[n][i].z * factor; total[i].w += v[n][i].w * factor;
+          }
         }
+        part += kPartsInFlight * warps;
+        if (part < tile.parts) load(part);
       }
+      __syncwarp();  // the factors may be overwritten
     }
-    __syncwarp();  // the factors may be overwritten
     float log_sum;
     const float sink = p.sinks != nullptr ? __ldg(p.sinks + (tile.head + row) % p.heads) * kLog2E : -INFINITY;
     const float inverse = inverse_of(reference, sum, sink, &log_sum);
-    if (p.lse != nullptr && half == 0 && lane == 0 && (few || warp == 0)) p.lse[tile.row + row] = log_sum * kLn2;
+    if (live && p.lse != nullptr && half == 0 && lane == 0 && first == 0) p.lse[tile.row + row] = log_sum * kLn2;
     char* out = p.out + ((tile.row + row) * LATENT_VALUES + half * 256) * 2;
-    if (few) {
+    if (warps == 1) {
+      if (!live) continue;  // (no barrier in this branch)
 #pragma unroll
       for (int i = 0; i < 2; ++i)
         reinterpret_cast<uint2*>(out)[i * 32 + lane] = inverse == 0.f ? make_uint2(0, 0)
@@ -1063,15 +1077,14 @@ __global__ void __launch_bounds__(kCombineThreads, 2) combine_kernel(const __gri
 #pragma unroll
     for (int i = 0; i < 2; ++i) reinterpret_cast<float4*>(shares[warp])[i * 32 + lane] = total[i];
     __syncthreads();
-    if (threadIdx.x < 128) {
-      float2 v = make_float2(0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < kCombineWarps; ++w) {
-        const float2 share = reinterpret_cast<const float2*>(shares[w])[threadIdx.x];
-        v.x += share.x;
-        v.y += share.y;
+    for (int pair = first * 32 + lane; live && pair < 128; pair += warps * 32) {
+      float2 value = make_float2(0.f, 0.f);
+      for (int w = 0; w < warps; ++w) {
+        const float2 share = reinterpret_cast<const float2*>(shares[warp - first + w])[pair];
+        value.x += share.x;
+        value.y += share.y;
       }
-      reinterpret_cast<uint32_t*>(out)[threadIdx.x] = inverse == 0.f ? 0u : pack2<kFormat>(v.x * inverse, v.y * inverse);
+      reinterpret_cast<uint32_t*>(out)[pair] = inverse == 0.f ? 0u : pack2<kFormat>(value.x * inverse, value.y * inverse);
     }
     __syncthreads();  // the shares may be overwritten
   }
