@@ -96,6 +96,19 @@ inline size_t statistics_offset(int blocks) { return size_t(blocks) * sizeof(Rec
 inline size_t sums_offset(int blocks) { return (statistics_offset(blocks) + size_t(blocks) * 2 * kRows * sizeof(float2) + 511) / 512 * 512; }
 inline size_t workspace_bytes(int blocks) { return sums_offset(blocks) + size_t(blocks) * 2 * kSlotFloats * sizeof(float); }
 
+// x / divisor for x from 0 to 2^31 - 1 (exact: 2^shift / divisor is rounded up by less than 2^-31 of it). A division by a number that is not known takes
+// 130 cycles, in a chain that the whole call waits for.
+struct Divisor {
+  uint32_t factor;
+  int32_t shift;
+};
+inline Divisor divisor_of(int divisor) {
+  int bits = 0;
+  while ((int64_t(1) << bits) < divisor) ++bits;
+  return {uint32_t((uint64_t(1) << (31 + bits)) / uint32_t(divisor) + 1), 31 + bits};
+}
+__device__ __forceinline__ int over(int x, const Divisor& by) { return int(uint64_t(uint32_t(x)) * by.factor >> by.shift); }
+
 struct Params {
   CUtensorMap cache;
   const char* q;
@@ -108,6 +121,8 @@ struct Params {
   float* sums;
   int32_t* status;
   int32_t batches, tokens, heads, pages, blocks, page_rows;
+  Divisor by_heads, by_page;  // a page's chunks
+  int32_t tile_tokens;        // that a tile's rows belong to, at most
   float scale_log2;
 };
 
@@ -129,8 +144,9 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
 
 // ---- the plan -----------------------------------------------------------------------------------------------------
 
-// A request's tiles and what they cost, in cached rows: the tiles' rows see from `near` keys on up to `far`, a tile costs kFixed more.
+// A request's tiles and what they cost, in cached rows: kFixed for a tile, and the keys that its rows see, from `near` on up to `far`.
 constexpr int kFixed = 128;
+
 struct Request {
   int begin, count;  // tokens
   int length;        // keys
@@ -161,7 +177,7 @@ __device__ __forceinline__ Request request_at(const Params& p, int b, float dens
   r.tiles = (r.rows + kRows - 1) / kRows;
   // (one key behind the table is enough to report a length that does not fit)
   r.seen = r.far = int(min(int64_t(r.length), int64_t(p.pages) * p.page_rows + 1));
-  r.near = int(min(int64_t(r.far), max(int64_t(r.length) - r.count, int64_t(0)) + kRows / p.heads + 1));
+  r.near = int(min(int64_t(r.far), max(int64_t(r.length) - r.count, int64_t(0)) + p.tile_tokens));
   // Nearly alike (as where tokens are decoded), or too many for the product in `cost`: taken to be alike, which spares a division.
   if (r.far - r.near <= kChunk) r.near = r.far;
   else if (r.tiles > 65536) r.near = r.far = (r.near >> 1) + (r.far >> 1);
@@ -172,7 +188,7 @@ __device__ __forceinline__ Request request_at(const Params& p, int b, float dens
 
 // Chunks that tile t's rows see.
 __device__ __forceinline__ int chunks_of(const Params& p, const Request& r, int t) {
-  const int last_token = (min((t + 1) * kRows, r.rows) - 1) / p.heads;
+  const int last_token = over(min((t + 1) * kRows, r.rows) - 1, p.by_heads);
   const int64_t seen = int64_t(r.length) - r.count + last_token + 1;
   return int((min(max(seen, int64_t(0)), int64_t(r.seen)) + kChunk - 1) / kChunk);
 }
@@ -183,16 +199,17 @@ struct Borders {
   uint32_t rest, blocks;  // that get a stretch (at most 255)
   bool whole;             // stretches end between tiles
   float density;          // > 0: every tile has blocks of its own, so many per row; costs are numbers of blocks
-  __device__ __forceinline__ int64_t at(uint32_t i) const { return each * i + rest * i / blocks; }
+  float inverse;          // 1 / blocks
+  __device__ __forceinline__ int64_t at(uint32_t i) const { return each * i + int(float(rest * i) * inverse + 0.001f); }  // (the quotient rounded down: both are at most 255)
 };
 // Quotients of numbers that are not negative (a 64-bit division takes several times as long as one of 32 bits).
 __device__ __forceinline__ int64_t quotient(int64_t value, int64_t divisor) {
   if ((uint64_t(value) | uint64_t(divisor)) >> 32 == 0) return uint32_t(value) / uint32_t(divisor);
   return value / divisor;
 }
-// value * factor / divisor, rounded down: everybody who asks gets the same.
+// value * factor / divisor, rounded down or nearly so, for value <= divisor: everybody who asks gets the same, and more for a larger value.
 __device__ __forceinline__ int share_of(int64_t value, int factor, int64_t divisor) {
-  return int(quotient(value * factor, divisor));
+  return min(int(float(value) * (float(factor) / float(divisor)) + 0.001f), factor);
 }
 // What sharing tiles costs a call, in cached rows: the parts' way through memory and `combine_kernel`, the more of both the more tiles there are to share.
 // Where giving every tile to one block makes no block's stretch longer than that, none is shared: the borders move to the nearest tile's. (64 heads, one
@@ -216,16 +233,19 @@ struct Place {
 // Sum over the threads that plan, for all of them: a block's, or a warp's.
 template <int kWarps>
 __device__ __forceinline__ int64_t plan_sum(int64_t value, int64_t* scratch) {
+  if constexpr (kWarps == 1)  // up to 32 requests: below 2^56
+    return (int64_t(__reduce_add_sync(0xffffffffu, uint32_t(value >> 27))) << 27) + __reduce_add_sync(0xffffffffu, uint32_t(value) & ((1u << 27) - 1));
+  else {
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) value += __shfl_xor_sync(0xffffffffu, value, d);
-  if constexpr (kWarps == 1) return value;
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = value;
-  __syncthreads();
-  int64_t sum = 0;
+    for (int d = 16; d > 0; d >>= 1) value += __shfl_xor_sync(0xffffffffu, value, d);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = value;
+    __syncthreads();
+    int64_t sum = 0;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) sum += scratch[w];
-  return sum;
+    for (int w = 0; w < kWarps; ++w) sum += scratch[w];
+    return sum;
+  }
 }
 
 // The same for numbers whose sum fits.
@@ -255,7 +275,7 @@ __device__ __forceinline__ Borders plan_block(const Params& p, int64_t* scratch,
   const int warp = kWarps == 1 ? 0 : int(threadIdx.x >> 5), lane = threadIdx.x & 31, thread = warp * 32 + lane;
   const int rounds = (p.batches + kRound - 1) / kRound;
   Request none = {};
-  Borders borders = {0, 0, 0, 0, false, 0.f};
+  Borders borders = {0, 0, 0, 0, false, 0.f, 0.f};
   Request own = thread < p.batches ? request_at(p, thread) : none;
   auto of_round = [&](int round) {
     const int b = round * kRound + thread;
@@ -292,18 +312,18 @@ __device__ __forceinline__ Borders plan_block(const Params& p, int64_t* scratch,
   if (borders.total == 0) return borders;
   const int grid = int(gridDim.x), most = most_cost + kFixed;
   int blocks = int(min(max(borders.total / (kLeastChunks * kChunk), int64_t(1)), int64_t(grid)));
-  // The longest stretch if no tile is shared: whole rounds where all cost the same, otherwise half a tile more than the mean, and a tile at least.
   const bool alike = most_cost == least_cost;
-  const int64_t tiles = quotient(borders.total, most), mean = quotient(borders.total, blocks);  // (tiles: where all cost the same)
-  const int64_t longest = alike ? quotient(tiles + grid - 1, grid) * most : max(int64_t(most), (blocks == grid ? mean : quotient(borders.total, grid)) + most / 2);
-  borders.whole = longest <= mean + kSharing + kSharingMany * int(min(tiles, int64_t(grid))) / grid;
+  const float total = float(borders.total), part = 1.f / float(grid), mean = total / float(blocks), tiles = total / float(most);  // (tiles: where all cost the same)
+  // The longest stretch if no tile is shared: whole rounds where all cost the same, otherwise half a tile more than the mean, and a tile at least.
+  const float longest = alike ? ceilf(tiles * part - 0.003f) * float(most) : fmaxf(float(most), total * part + 0.5f * float(most));
+  borders.whole = longest <= mean + float(kSharing) + float(kSharingMany) * fminf(tiles * part, 1.f);
   static_assert(kWarps == 1 || kRound > 255, "a thread for each of as many requests as blocks");
-  if (!borders.whole && tiles <= grid && p.batches <= grid && mean < (1 << 30)) {  // blocks of their own for every tile?
-    const int rows = min(kRows, int(uint32_t(p.tokens * p.heads) / uint32_t(p.batches)));
-    const int more = kTwoTiles * rows / kRows;  // (what a second tile costs is its rows' sums)
+  if (!borders.whole && tiles < float(grid) + 0.5f && p.batches <= grid && mean < float(1 << 30)) {  // blocks of their own for every tile?
+    const float rows = fminf(float(kRows), float(p.tokens * p.heads) / float(p.batches));
+    const int more = int(float(kTwoTiles / kRows) * rows);  // (what a second tile costs is its rows' sums)
     if (alike) {
-      const int each = min(int(uint32_t(grid) / uint32_t(tiles)), (most_cost + kLeastChunks * kChunk - 1) / (kLeastChunks * kChunk));
-      if ((mean + more) * each * tiles >= borders.total) blocks = each * int(tiles);
+      const int each = min(int(float(grid) / tiles + 0.001f), int(uint32_t(most_cost + kLeastChunks * kChunk - 1) / (kLeastChunks * kChunk)));
+      if ((mean + float(more)) * float(each) * tiles >= total) blocks = each * int(tiles + 0.5f);
     } else {
       // The shortest stretch that will do, nearly.
       int needed = 0, stretch = 0;
@@ -333,9 +353,10 @@ __device__ __forceinline__ Borders plan_block(const Params& p, int64_t* scratch,
       }
     }
   }
-  if (borders.density == 0.f && most_tiles == least_tiles && uint32_t(blocks) % uint32_t(most_tiles) <= uint32_t(blocks) / 16) blocks -= uint32_t(blocks) % uint32_t(most_tiles);
+  if (borders.density == 0.f && most_tiles == least_tiles && most_tiles > 1 && uint32_t(blocks) % uint32_t(most_tiles) <= uint32_t(blocks) / 16) blocks -= uint32_t(blocks) % uint32_t(most_tiles);
   if (int(blockIdx.x) >= blocks) return borders;
   borders.blocks = uint32_t(blocks);
+  borders.inverse = 1.f / float(blocks);
   borders.each = borders.density > 0.f ? 1 : quotient(borders.total, blocks);
   borders.rest = uint32_t(borders.total - borders.each * blocks);
   const int64_t mine = borders.at(blockIdx.x);
@@ -362,10 +383,20 @@ __device__ __forceinline__ Borders plan_block(const Params& p, int64_t* scratch,
     const Request r = of_round(round);
     const int64_t value = r.tiles > tile ? r.cost(tile + 1) - r.cost(tile) : 0;
     int64_t inclusive = value;
+    if (borders.total <= INT32_MAX) {
+      int few = int(value);
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int64_t other = __shfl_up_sync(0xffffffffu, inclusive, d);
-      if (lane >= d) inclusive += other;
+      for (int d = 1; d < 32; d <<= 1) {
+        const int other = __shfl_up_sync(0xffffffffu, few, d);
+        if (lane >= d) few += other;
+      }
+      inclusive = few;
+    } else {
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int64_t other = __shfl_up_sync(0xffffffffu, inclusive, d);
+        if (lane >= d) inclusive += other;
+      }
     }
     int64_t sum = 0, in_front = 0;
     if constexpr (kWarps > 1) {
@@ -439,8 +470,8 @@ __device__ void plan_role(const Params& p, const Shared& sm, const Borders& bord
         piece.row = int64_t(r.begin) * p.heads + row;
         piece.rows = min(kRows, r.rows - row);
         piece.request = request;
-        piece.token = row / p.heads;
-        piece.head = row % p.heads;
+        piece.token = over(row, p.by_heads);
+        piece.head = row - piece.token * p.heads;
         piece.base = r.length - r.count + 1;
         piece.length = r.seen;
         const bool whole = piece.first == 0 && piece.last == chunks;
@@ -518,7 +549,7 @@ __device__ void copy_role(const Params& p, const Shared& sm) {
     if (piece.first == piece.last) continue;  // sees nothing
     const int32_t* table = p.table + size_t(piece.request) * p.pages;
     auto page_of = [&](int chunk) {  // lane l: the page of chunk `chunk + l`, or -1
-      const int column = min(chunk + lane, piece.last - 1) * kChunk / p.page_rows;
+      const int column = over(min(chunk + lane, piece.last - 1), p.by_page);
       return column < p.pages ? __ldg(table + column) : -1;
     };
     int pages = 0, next_pages = page_of(piece.first);  // of 32 chunks; of the next 32
@@ -539,7 +570,7 @@ __device__ void copy_role(const Params& p, const Shared& sm) {
         *sm.live(stage) = valid;
         if (legal) {
           mbar_arrive_expect(bar, L::kTileBytes);
-          const int row = page * p.page_rows + chunk * kChunk % p.page_rows;
+          const int row = page * p.page_rows + chunk * kChunk - over(chunk, p.by_page) * p.page_rows;
 #pragma unroll
           for (int box = 0; box < L::kBoxes; ++box) copy_box(target + box * kBoxBytes, &p.cache, box * 64, row, bar);
         } else {
@@ -730,7 +761,7 @@ __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
   for (; walk.next_of_warp(); walk.done_of_warp()) {
     const Piece& piece = walk.piece;
     const int chunks = piece.last - piece.first;
-    const int end = row < piece.rows ? piece.base + (piece.head + row) / p.heads + piece.token : INT32_MAX;  // this row sees keys below
+    const int end = row < piece.rows ? piece.base + over(piece.head + row, p.by_heads) + piece.token : INT32_MAX;  // this row sees keys below
     const int warp_end = __reduce_min_sync(0xffffffffu, end);
     float reference = -INFINITY, sum = 0.f;
     for (int i = 0; i < chunks; ++i, ++count) {
@@ -1158,9 +1189,12 @@ int launch_latent_attention(void* stream, const latent_attention_call* call) {
   p.batches = int32_t(c.batches);
   p.tokens = int32_t(c.tokens);
   p.heads = int32_t(c.heads);
+  p.by_heads = absorbed::divisor_of(p.heads);
+  p.tile_tokens = absorbed::kRows / p.heads + 1;
   p.pages = int32_t(c.pages);
   p.blocks = int32_t(c.blocks);
   p.page_rows = int32_t(c.page_rows);
+  p.by_page = absorbed::divisor_of(p.page_rows / absorbed::kChunk);
   p.scale_log2 = float(c.scale * 1.4426950408889634);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (c.type == LATENT_BF16) return c.width == 576 ? absorbed::launch<1, 576>(p, blocks, s) : absorbed::launch<1, 512>(p, blocks, s);

@@ -68,7 +68,7 @@ inline unsigned __ballot_sync(unsigned, bool v) {
 }
 inline int __reduce_max_sync(unsigned, int v) { const int64_t* all = meet(v); return int(*std::max_element(all, all + 32)); }
 inline int __reduce_min_sync(unsigned, int v) { const int64_t* all = meet(v); return int(*std::min_element(all, all + 32)); }
-inline int __reduce_add_sync(unsigned, int v) { const int64_t* all = meet(v); int sum = 0; for (int i = 0; i < 32; ++i) sum += int(all[i]); return sum; }
+template <typename T> inline T __reduce_add_sync(unsigned, T v) { const int64_t* all = meet(v); T sum = 0; for (int i = 0; i < 32; ++i) sum += T(all[i]); return sum; }
 inline bool run_block() {
   running = kBlockThreads;
   block_arrived = 0;
@@ -111,6 +111,8 @@ int main() {
   if (int(fread(cu.data(), 4, batches + 1, stdin)) != batches + 1 || int(fread(lengths.data(), 4, batches, stdin)) != batches) return 1;
   Params p = {};
   p.heads = head[1];
+  p.by_heads = divisor_of(p.heads);
+  p.tile_tokens = kRows / p.heads + 1;
   p.batches = batches;
   p.pages = head[3];
   p.page_rows = head[4];
