@@ -92,6 +92,11 @@ struct Record {
   int pad[3];
 };
 constexpr int kSlotFloats = kRows * LATENT_VALUES;
+// Sums of eight features of 32 rows lie next to each other, as warps write them: 32 bytes to a row, 1 KiB to an instruction (in rows, a write
+// touched 32 lines, and 128 KiB took 3.6 us instead of 2.4). First feature of eight.
+__host__ __device__ constexpr int sums_place(int row, int feature) {
+  return ((((feature >> 7 & 1) * 2 + (row >> 5)) * 32 + (feature >> 8) * 16 + (feature & 127) / 8) * 32 + (row & 31)) * 8;
+}
 inline size_t statistics_offset(int blocks) { return size_t(blocks) * sizeof(Record); }
 inline size_t sums_offset(int blocks) { return (statistics_offset(blocks) + size_t(blocks) * 2 * kRows * sizeof(float2) + 511) / 512 * 512; }
 inline size_t workspace_bytes(int blocks) { return sums_offset(blocks) + size_t(blocks) * 2 * kSlotFloats * sizeof(float); }
@@ -870,7 +875,7 @@ __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
     }
     if (piece.slot >= 0) {  // a part of a tile: sums as they are
       if (half == 0 && row < piece.rows) p.statistics[size_t(piece.slot) * kRows + row] = make_float2(reference, sum);
-      float* sums = p.sums + size_t(piece.slot) * kSlotFloats + o_row * LATENT_VALUES + o_feature;
+      float* sums = p.sums + size_t(piece.slot) * kSlotFloats + sums_place(o_row, o_feature);
 #pragma unroll 1
       for (int c = 0; c < 256; c += 64) {
         uint32_t o[64];
@@ -879,7 +884,7 @@ __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
         tmem_wait_ld();
         if (o_row < piece.rows) {
 #pragma unroll
-          for (int e = 0; e < 64; e += 8) store_sector(sums + (c >> 7) * 256 + (c & 127) + e, o + e);
+          for (int e = 0; e < 64; e += 8) store_sector(sums + (c + e) * 32, o + e);
         }
       }
       continue;
@@ -986,11 +991,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
   if (warp == kScoreWarp) tmem_dealloc(tmem, 512);
 }
 
-// Tiles that several blocks worked on. Every block makes the list of them, with what there is to do for each: half a row by one to eight
-// warps of a block, as many as bring all parts with one round of loads if there are blocks enough for that. Sums are added in the order of
+// Tiles that several blocks worked on. Every block makes the list of them, with what there is to do for each: 32 features of eight rows by one to
+// eight warps of a block, as many as bring all parts with one round of loads if there are blocks enough for that. Sums are added in the order of
 // the parts (of the warps' shares), whatever block does it. Bound by latency: the list; statistics and the first round of sums together; the others.
 // (8 requests of 8192 keys, one token, 64 heads, 18 parts each: 4.0 us, and 8.7 with eight warps for every half row and statistics in front of the sums.)
-constexpr int kCombineThreads = 256, kCombineWarps = kCombineThreads / 32, kMostBlocks = 256, kPartsInFlight = 6;
+constexpr int kCombineThreads = 256, kCombineWarps = kCombineThreads / 32, kMostBlocks = 256, kPartsInFlight = 4;
+constexpr int kUnitRows = 8, kUnitFeatures = 32, kUnits = LATENT_VALUES / kUnitFeatures;
 
 template <int kFormat>
 __global__ void __launch_bounds__(kCombineThreads, 2) combine_kernel(const __grid_constant__ Params p, int blocks) {
@@ -1000,7 +1006,8 @@ __global__ void __launch_bounds__(kCombineThreads, 2) combine_kernel(const __gri
   };
   __shared__ int wishes[kCombineWarps], ends[kCombineWarps];
   __shared__ Tile list[kMostBlocks];
-  __shared__ float factors[kCombineWarps][kMostBlocks], shares[kCombineWarps][LATENT_VALUES / 2];
+  __shared__ float shares[kCombineWarps][kUnitRows * kUnitFeatures];
+  __shared__ float2 shares_of[kCombineWarps][kUnitRows];  // reference and sum
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   wait_for_predecessor();
   let_successor_start();
@@ -1010,14 +1017,14 @@ __global__ void __launch_bounds__(kCombineThreads, 2) combine_kernel(const __gri
     if (own < blocks) record = p.records[own];
     const int parts = record.last >= 0 ? record.last - own + 1 : 0;
     int warps = parts <= kPartsInFlight ? 1 : parts <= 2 * kPartsInFlight ? 2 : parts <= 4 * kPartsInFlight ? 4 : kCombineWarps;
-    const int wish = __reduce_add_sync(0xffffffffu, parts == 0 ? 0 : 2 * record.rows * warps);
+    const int wish = __reduce_add_sync(0xffffffffu, parts == 0 ? 0 : (record.rows + kUnitRows - 1) / kUnitRows * kUnits * warps);
     if (lane == 0) wishes[warp] = wish;
     __syncthreads();
     int wanted = 0;
 #pragma unroll
     for (int w = 0; w < kCombineWarps; ++w) wanted += wishes[w];
     for (; wanted > int(gridDim.x) * kCombineWarps; wanted >>= 1) warps = max(1, warps >> 1);
-    const int items = parts == 0 ? 0 : (2 * record.rows * warps + kCombineWarps - 1) / kCombineWarps;
+    const int items = parts == 0 ? 0 : (record.rows + kUnitRows - 1) / kUnitRows * kUnits * warps / kCombineWarps;
     int packed = items << 8 | (parts > 0);  // both sums at once: items below 2^16, tiles below 2^8
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -1040,82 +1047,82 @@ __global__ void __launch_bounds__(kCombineThreads, 2) combine_kernel(const __gri
     while (list[index].items <= item) ++index;
     const Tile tile = list[index];
     const int place = item - (index > 0 ? list[index - 1].items : 0), warps = tile.warps;
-    const int unit = (place * kCombineWarps + warp) / warps, first = warp & (warps - 1), row = unit >> 1, half = unit & 1;
-    const bool live = row < tile.rows;
+    const int unit = (place * kCombineWarps + warp) / warps, first = warp & (warps - 1);
+    const int rows = unit / kUnits * kUnitRows, segment = unit % kUnits;
+    auto feature_of = [&](int lane) { return (segment >> 3) * 256 + (segment & 1) * 128 + (segment >> 1 & 3) * 32 + (lane >> 3) * 8; };
     auto slot_of = [&](int part) { return size_t(part == 0 ? 2 * tile.block + 1 : 2 * (tile.block + part)); };
-    // This warp's parts: every `warps`-th, lane l adds up features 4 l .. + 3 and 128 + 4 l .. + 3 of the half.
-    const float* sums = p.sums + size_t(min(row, kRows - 1)) * LATENT_VALUES + half * 256 + lane * 4;
-    float4 v[kPartsInFlight][2], total[2] = {};
-    auto load = [&](int part) {
+    // This warp's parts: every `warps`-th. Lane l adds up eight features of row l % 8.
+    const int row = rows + (lane & 7), count = (tile.parts - first + warps - 1) / warps;
+    const float* sums = p.sums + sums_place(row, feature_of(lane));
+    float total[8] = {}, reference = -INFINITY, sum = 0.f;
+    for (int round = 0; round < count; round += kPartsInFlight) {
+      uint32_t v[kPartsInFlight][8];
+#pragma unroll
+      for (int n = 0; n < kPartsInFlight; ++n)
+        if (round + n < count) load_sector(sums + slot_of(first + (round + n) * warps) * kSlotFloats, v[n]);
+      // Statistics: lane l has part l / 8 of the round. (A block that had none of the tile's chunks has said so: reference -infinity.)
+      static_assert(kPartsInFlight == 4, "a part for every eight lanes");
+      const int mine = round + (lane >> 3);
+      const float2 own = mine < count ? __ldg(p.statistics + slot_of(first + mine * warps) * kRows + row) : make_float2(-INFINITY, 0.f);
+      float next = fmaxf(reference, own.x);
+      next = fmaxf(next, __shfl_xor_sync(0xffffffffu, next, 8));
+      next = fmaxf(next, __shfl_xor_sync(0xffffffffu, next, 16));
+      const float factor = own.x == -INFINITY ? 0.f : exp2f(own.x - next);
+      float more = factor * own.y;
+      more += __shfl_xor_sync(0xffffffffu, more, 8);
+      more += __shfl_xor_sync(0xffffffffu, more, 16);
+      const float alpha = reference == -INFINITY ? 0.f : exp2f(reference - next);
+      sum = sum * alpha + more;
+      reference = next;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) total[e] *= alpha;
 #pragma unroll
       for (int n = 0; n < kPartsInFlight; ++n) {
-        if (part + n * warps >= tile.parts) break;
-        const float4* values = reinterpret_cast<const float4*>(sums + slot_of(part + n * warps) * kSlotFloats);
-        v[n][0] = __ldg(values);
-        v[n][1] = __ldg(values + 32);
-      }
-    };
-    if (live) load(first);
-    // Factors of the parts (a block that had none of the tile's chunks has said so: reference -infinity).
-    float reference = -INFINITY, sum = 0.f;
-    if (live) {
-      for (int part = lane; part < tile.parts; part += 32) {
-        const float own = __ldg(&p.statistics[slot_of(part) * kRows + row].x);
-        factors[warp][part] = own;
-        reference = fmaxf(reference, own);
-      }
+        if (round + n >= count) break;
+        const float by = __shfl_sync(0xffffffffu, factor, n * 8 + (lane & 7));
+        if (by != 0.f) {  // (what a block without chunks of the tile has there may be anything)
 #pragma unroll
-      for (int d = 16; d > 0; d >>= 1) reference = fmaxf(reference, __shfl_xor_sync(0xffffffffu, reference, d));
-      for (int part = lane; part < tile.parts; part += 32) {
-        const float own = factors[warp][part], factor = own == -INFINITY ? 0.f : exp2f(own - reference);
-        factors[warp][part] = factor;
-        sum += factor * __ldg(&p.statistics[slot_of(part) * kRows + row].y);
-      }
-#pragma unroll
-      for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-      __syncwarp();
-      for (int part = first; part < tile.parts;) {
-#pragma unroll
-        for (int n = 0; n < kPartsInFlight; ++n) {
-          const int at = part + n * warps;
-          if (at >= tile.parts) break;
-          const float factor = factors[warp][at];
-          if (factor == 0.f) continue;  // (what a block without chunks of the tile has there may be anything)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            total[i].x += v[n][i].x * factor; total[i].y += v[n][i].y * factor;
-            total[i].z += v[n][i].z * factor; total[i].w += v[n][i].w * factor;
-          }
+          for (int e = 0; e < 8; ++e) total[e] += __uint_as_float(v[n][e]) * by;
         }
-        part += kPartsInFlight * warps;
-        if (part < tile.parts) load(part);
       }
-      __syncwarp();  // the factors may be overwritten
     }
-    float log_sum;
-    const float sink = p.sinks != nullptr ? __ldg(p.sinks + (tile.head + row) % p.heads) * kLog2E : -INFINITY;
-    const float inverse = inverse_of(reference, sum, sink, &log_sum);
-    if (live && p.lse != nullptr && half == 0 && lane == 0 && first == 0) p.lse[tile.row + row] = log_sum * kLn2;
-    char* out = p.out + ((tile.row + row) * LATENT_VALUES + half * 256) * 2;
-    if (warps == 1) {
-      if (!live) continue;  // (no barrier in this branch)
+    auto finish = [&](int row, float reference, float sum, bool first_of_row) {  // what the row's sums are multiplied with
+      float log_sum;
+      const float sink = p.sinks != nullptr ? __ldg(p.sinks + (tile.head + row) % p.heads) * kLog2E : -INFINITY;
+      const float inverse = inverse_of(reference, sum, sink, &log_sum);
+      if (p.lse != nullptr && first_of_row && segment == 0) p.lse[tile.row + row] = log_sum * kLn2;
+      return inverse;
+    };
+    if (warps == 1) {  // (no barrier in this branch)
+      if (row < tile.rows) {
+        const float inverse = finish(row, reference, sum, lane < 8);
+        uint32_t words[4];
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        reinterpret_cast<uint2*>(out)[i * 32 + lane] = inverse == 0.f ? make_uint2(0, 0)
-            : make_uint2(pack2<kFormat>(total[i].x * inverse, total[i].y * inverse), pack2<kFormat>(total[i].z * inverse, total[i].w * inverse));
+        for (int e = 0; e < 4; ++e) words[e] = inverse == 0.f ? 0u : pack2<kFormat>(total[2 * e] * inverse, total[2 * e + 1] * inverse);
+        *reinterpret_cast<uint4*>(p.out + ((tile.row + row) * LATENT_VALUES + feature_of(lane)) * 2) = make_uint4(words[0], words[1], words[2], words[3]);
+      }
       continue;
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i) reinterpret_cast<float4*>(shares[warp])[i * 32 + lane] = total[i];
+    for (int e = 0; e < 8; e += 4) *reinterpret_cast<float4*>(&shares[warp][lane * 8 + e]) = make_float4(total[e], total[e + 1], total[e + 2], total[e + 3]);
+    if (lane < 8) shares_of[warp][lane] = make_float2(reference, sum);
     __syncthreads();
-    for (int pair = first * 32 + lane; live && pair < 128; pair += warps * 32) {
+    for (int pair = first * 32 + lane; pair < kUnitRows * kUnitFeatures / 2; pair += warps * 32) {
+      const int owner = pair >> 2, row = rows + (owner & 7);  // the lane that had it
+      if (row >= tile.rows) continue;
+      float reference = -INFINITY, sum = 0.f;
+      for (int w = 0; w < warps; ++w) reference = fmaxf(reference, shares_of[warp - first + w][owner & 7].x);
       float2 value = make_float2(0.f, 0.f);
       for (int w = 0; w < warps; ++w) {
-        const float2 share = reinterpret_cast<const float2*>(shares[warp - first + w])[pair];
-        value.x += share.x;
-        value.y += share.y;
+        const float2 share = *reinterpret_cast<const float2*>(&shares[warp - first + w][pair * 2]), own = shares_of[warp - first + w][owner & 7];
+        const float by = own.x == -INFINITY ? 0.f : exp2f(own.x - reference);
+        value.x += share.x * by;
+        value.y += share.y * by;
+        sum += own.y * by;
       }
-      reinterpret_cast<uint32_t*>(out)[pair] = inverse == 0.f ? 0u : pack2<kFormat>(value.x * inverse, value.y * inverse);
+      const float inverse = finish(row, reference, sum, pair < 32 && (pair & 3) == 0);
+      *reinterpret_cast<uint32_t*>(p.out + ((tile.row + row) * LATENT_VALUES + feature_of(owner) + (pair & 3) * 2) * 2) =
+          inverse == 0.f ? 0u : pack2<kFormat>(value.x * inverse, value.y * inverse);
     }
     __syncthreads();  // the shares may be overwritten
   }

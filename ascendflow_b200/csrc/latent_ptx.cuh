@@ -105,6 +105,11 @@ __device__ __forceinline__ void store_sector(void* at, const uint32_t* v) {
                ::"l"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
 }
 
+__device__ __forceinline__ void load_sector(const void* at, uint32_t* v) {
+  asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "l"(at) : "memory");
+}
+
 // ---- arithmetic on pairs -------------------------------------------------------------------------------------------
 
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
