@@ -26,8 +26,8 @@
 // requests share their pages). A chunk takes 2.0 k cycles, 1.43 k of them the two products' own; shared memory's ports are busy for
 // two thirds of it. Two tiles of weights (room for them by a ring of its own for the last 64 features), weights without looking for the
 // maximum, and fewer barriers per chunk were each built and slower by 2 to 12 per cent in loops.
-// A call of few chunks is a chain of 21 us: plan 2.5, pieces and page 2.4, copy 1.6, chunks 0.8 each, sums to memory 3.6 (128 KiB
-// per block at the SM's 32 bytes per cycle), the next kernel's start 1.0, their sum 3 to 4.
+// A call of few chunks is a chain of 16 us: plan 2.5, pieces and page 0.8, copy 2.2, chunks 0.8 each, last products 0.5, sums to memory 1.8 (128 KiB
+// per block), the next kernel's start 2.3, their sum 3.3.
 //
 // Rows of a chunk behind the request's length are cleared in the tile's value part (a zero weight times infinity is a
 // NaN) and their scores replaced; so are whole chunks whose page is not in the cache, which are reported.
@@ -93,8 +93,8 @@ struct Record {
 };
 constexpr int kSlotFloats = kRows * LATENT_VALUES;
 // Sums of eight features of 32 rows lie next to each other, as warps write them: 32 bytes to a row, 1 KiB to an instruction (in rows, a write
-// touched 32 lines, and 128 KiB took 3.6 us instead of 2.4). First feature of eight.
-__host__ __device__ constexpr int sums_place(int row, int feature) {
+// touched 32 lines, and 128 KiB took 3.6 us instead of 1.8). First feature of eight.
+__device__ __forceinline__ int sums_place(int row, int feature) {
   return ((((feature >> 7 & 1) * 2 + (row >> 5)) * 32 + (feature >> 8) * 16 + (feature & 127) / 8) * 32 + (row & 31)) * 8;
 }
 inline size_t statistics_offset(int blocks) { return size_t(blocks) * sizeof(Record); }
@@ -218,15 +218,15 @@ __device__ __forceinline__ int share_of(int64_t value, int factor, int64_t divis
 }
 // What sharing tiles costs a call, in cached rows: the parts' way through memory and `combine_kernel`, the more of both the more tiles there are to share.
 // Where giving every tile to one block makes no block's stretch longer than that, none is shared: the borders move to the nearest tile's. (64 heads, one
-// token; whole / shared: 512 keys 16.7 / 16.1 us, 32 requests of 1024 25.4 / 23.9, 64 of 1024 28.1 / 30, 64 of 2048 49.7 / 52.5.)
-constexpr int kSharing = 6 * kChunk, kSharingMany = 32 * kChunk;
+// token, whole / shared: 512 keys 16.0 / 13.3 us, 16 requests of 512 16.9 / 15.9, 32 of 768 20.4 / 19.6, 64 of 1024 27.5 / 32.9, of 1500 41.3 / 42.5,
+// of 2048 48.9 / 48.6.)
+constexpr int kSharing = 4 * kChunk, kSharingMany = 28 * kChunk;
 // A block that ends one tile and begins another writes sums twice, and all wait for it. Where every tile can have blocks of its own without making the
-// stretches longer than by this (for 64 rows), it has: 64 heads, one token, 3, 8, 16, 32 requests of 8192 keys 27.1, 36.6, 48.2, 76.5 us with borders anywhere,
-// 24.3, 33.4, 45.9, 73.4 so; 32 requests of 512 to 4096 keys 38.0 and 34.1.
+// stretches longer than by this (for 64 rows), it has: 64 heads, one token, 3, 8, 16, 32 requests of 8192 keys 21.7, 29.5, 45.8, 74.4 us with borders anywhere,
+// 19.8, 27.4, 44.5, 71.8 so; 4, 16, 64 requests of 1024 to 8192 keys 22.2, 32.2, 89.3 and 19.5, 29.7, 85.3.
 constexpr int kTwoTiles = 10 * kChunk;
 // A block with fewer chunks than these loses more with its start and with its part of the sums than it takes off the others (64 heads, one
-// token; 1, 2, 3, 4 chunks: 2048 keys 18.6, 18.3, 18.8, 22.8 us, 8192 26.2, 22.1, 21.4, 21.2, four requests of 8192 24.1, 24.0, 24.0, 26.2,
-// four of 1024 with six tokens 26.4, 26.2, 31.2, 30.8).
+// token; 1, 2, 3 chunks: 512 keys 13.8, 13.4, 13.8 us, 2048 14.1, 14.4, 14.7, 8192 18.1, 16.1, 16.3, four requests of 8192 20.6 each).
 constexpr int kLeastChunks = 2;
 
 // Where a stretch begins: a request's tile and the cost in front of that.
