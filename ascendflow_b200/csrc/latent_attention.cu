@@ -205,7 +205,7 @@ struct Borders {
   bool whole;             // stretches end between tiles
   float density;          // > 0: every tile has blocks of its own, so many per row; costs are numbers of blocks
   float inverse;          // 1 / blocks
-  __device__ __forceinline__ int64_t at(uint32_t i) const { return each * i + int(float(rest * i) * inverse + 0.001f); }  // (the quotient rounded down: both are at most 255)
+  __device__ __forceinline__ int64_t at(uint32_t i) const { return each * i + int(fmaf(float(rest * i), inverse, 0.001f)); }  // (the quotient rounded down: both are at most 255)
 };
 // Quotients of numbers that are not negative (a 64-bit division takes several times as long as one of 32 bits).
 __device__ __forceinline__ int64_t quotient(int64_t value, int64_t divisor) {
@@ -214,7 +214,7 @@ __device__ __forceinline__ int64_t quotient(int64_t value, int64_t divisor) {
 }
 // value * factor / divisor, rounded down or nearly so, for value <= divisor: everybody who asks gets the same, and more for a larger value.
 __device__ __forceinline__ int share_of(int64_t value, int factor, int64_t divisor) {
-  return min(int(float(value) * (float(factor) / float(divisor)) + 0.001f), factor);
+  return min(int(fmaf(float(value), float(factor) / float(divisor), 0.001f)), factor);
 }
 // What sharing tiles costs a call, in cached rows: the parts' way through memory and `combine_kernel`, the more of both the more tiles there are to share.
 // Where giving every tile to one block makes no block's stretch longer than that, none is shared: the borders move to the nearest tile's. (64 heads, one

@@ -315,6 +315,24 @@ def test_attention_batches_between_sharing_and_not(heads, queries, lengths):
     check_attention(normal(2, queries * len(lengths), heads, 576), cache, table, [queries] * len(lengths), lengths, 192 ** -0.5)
 
 
+@pytest.mark.parametrize("heads", [1, 9, 23, 64])
+@pytest.mark.parametrize("requests,length,ragged", [(1, 20000, 0), (3, 12000, 0), (7, 7000, 500), (16, 5000, 0), (40, 3500, 61)])
+def test_attention_sums_of_shared_tiles(heads, requests, length, ragged):
+    """Tiles of few to many parts, rows that are no multiple of eight; scores that rise along the keys, so that each part's reference is another, sinks, and
+    parts none of whose pages is in the cache."""
+    lengths = [length - ragged * b for b in range(requests)]
+    cache, table = paged(requests, lengths, 576, 64, BF16)
+    for b, n in enumerate(lengths):
+        pages = table[b, : -(-n // 64)].long()
+        cache[pages] *= torch.linspace(0.2, 1.5, len(pages), device="cuda").to(BF16).view(-1, 1, 1, 1)
+    q = normal(2, requests, heads, 576, spread=2.0)
+    check_attention(q, cache, table, [1] * requests, lengths, 0.06, normal(3, heads, dtype=F32, spread=4.0))
+    bad = [(0, column) for column in range(20, min(lengths[0] // 64, 60))]
+    for _, column in bad:
+        table[0, column] = -1
+    check_attention(q, cache, table, [1] * requests, lengths, 0.06, bad=bad)
+
+
 def test_attention_offsets_beyond_32_bits():
     """A cache of more than 2^32 bytes and 2^31 features, its last pages in use."""
     blocks = 4_000_000 // 64
