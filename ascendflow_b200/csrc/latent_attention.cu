@@ -32,6 +32,7 @@
 // Rows of a chunk behind the request's length are cleared in the tile's value part (a zero weight times infinity is a
 // NaN) and their scores replaced; so are whole chunks whose page is not in the cache, which are reported.
 #include "latent_common.cuh"
+#include "latent_parts.cuh"
 #include "latent_ptx.cuh"
 
 namespace latent {
@@ -874,7 +875,7 @@ __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
       tc_fence_after_sync();
     }
     if (piece.slot >= 0) {  // a part of a tile: sums as they are
-      if (half == 0 && row < piece.rows) p.statistics[size_t(piece.slot) * kRows + row] = make_float2(reference, sum);
+      if (half == 0 && row < piece.rows) p.statistics[size_t(piece.slot) * kRows + row] = part_statistics(reference, sum);
       float* sums = p.sums + size_t(piece.slot) * kSlotFloats + sums_place(o_row, o_feature);
 #pragma unroll 1
       for (int c = 0; c < 256; c += 64) {
@@ -995,8 +996,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
 // eight warps of a block, as many as bring all parts with one round of loads if there are blocks enough for that. Sums are added in the order of
 // the parts (of the warps' shares), whatever block does it. Bound by latency: the list; statistics and the first round of sums together; the others.
 // (8 requests of 8192 keys, one token, 64 heads, 18 parts each: 4.0 us, and 8.7 with eight warps for every half row and statistics in front of the sums.)
-constexpr int kCombineThreads = 256, kCombineWarps = kCombineThreads / 32, kMostBlocks = 256, kPartsInFlight = 4;
-constexpr int kUnitRows = 8, kUnitFeatures = 32, kUnits = LATENT_VALUES / kUnitFeatures;
+constexpr int kMostBlocks = 256, kUnits = LATENT_VALUES / kUnitFeatures;
 
 template <int kFormat>
 __global__ void __launch_bounds__(kCombineThreads, 2) combine_kernel(const __grid_constant__ Params p, int blocks) {
@@ -1006,8 +1006,7 @@ __global__ void __launch_bounds__(kCombineThreads, 2) combine_kernel(const __gri
   };
   __shared__ int wishes[kCombineWarps], ends[kCombineWarps];
   __shared__ Tile list[kMostBlocks];
-  __shared__ float shares[kCombineWarps][kUnitRows * kUnitFeatures];
-  __shared__ float2 shares_of[kCombineWarps][kUnitRows];  // reference and sum
+  __shared__ Shares shared;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   wait_for_predecessor();
   let_successor_start();
@@ -1016,7 +1015,7 @@ __global__ void __launch_bounds__(kCombineThreads, 2) combine_kernel(const __gri
     Record record = {0, 0, 0, -1, {0, 0, 0}};
     if (own < blocks) record = p.records[own];
     const int parts = record.last >= 0 ? record.last - own + 1 : 0;
-    int warps = parts <= kPartsInFlight ? 1 : parts <= 2 * kPartsInFlight ? 2 : parts <= 4 * kPartsInFlight ? 4 : kCombineWarps;
+    int warps = warps_for(parts);
     const int wish = __reduce_add_sync(0xffffffffu, parts == 0 ? 0 : (record.rows + kUnitRows - 1) / kUnitRows * kUnits * warps);
     if (lane == 0) wishes[warp] = wish;
     __syncthreads();
@@ -1047,84 +1046,22 @@ __global__ void __launch_bounds__(kCombineThreads, 2) combine_kernel(const __gri
     while (list[index].items <= item) ++index;
     const Tile tile = list[index];
     const int place = item - (index > 0 ? list[index - 1].items : 0), warps = tile.warps;
-    const int unit = (place * kCombineWarps + warp) / warps, first = warp & (warps - 1);
+    const int unit = (place * kCombineWarps + warp) / warps;
     const int rows = unit / kUnits * kUnitRows, segment = unit % kUnits;
     auto feature_of = [&](int lane) { return (segment >> 3) * 256 + (segment & 1) * 128 + (segment >> 1 & 3) * 32 + (lane >> 3) * 8; };
     auto slot_of = [&](int part) { return size_t(part == 0 ? 2 * tile.block + 1 : 2 * (tile.block + part)); };
-    // This warp's parts: every `warps`-th. Lane l adds up eight features of row l % 8.
-    const int row = rows + (lane & 7), count = (tile.parts - first + warps - 1) / warps;
-    const float* sums = p.sums + sums_place(row, feature_of(lane));
-    float total[8] = {}, reference = -INFINITY, sum = 0.f;
-    for (int round = 0; round < count; round += kPartsInFlight) {
-      uint32_t v[kPartsInFlight][8];
-#pragma unroll
-      for (int n = 0; n < kPartsInFlight; ++n)
-        if (round + n < count) load_sector(sums + slot_of(first + (round + n) * warps) * kSlotFloats, v[n]);
-      // Statistics: lane l has part l / 8 of the round. (A block that had none of the tile's chunks has said so: reference -infinity.)
-      static_assert(kPartsInFlight == 4, "a part for every eight lanes");
-      const int mine = round + (lane >> 3);
-      const float2 own = mine < count ? __ldg(p.statistics + slot_of(first + mine * warps) * kRows + row) : make_float2(-INFINITY, 0.f);
-      float next = fmaxf(reference, own.x);
-      next = fmaxf(next, __shfl_xor_sync(0xffffffffu, next, 8));
-      next = fmaxf(next, __shfl_xor_sync(0xffffffffu, next, 16));
-      const float factor = own.x == -INFINITY ? 0.f : exp2f(own.x - next);
-      float more = factor * own.y;
-      more += __shfl_xor_sync(0xffffffffu, more, 8);
-      more += __shfl_xor_sync(0xffffffffu, more, 16);
-      const float alpha = reference == -INFINITY ? 0.f : exp2f(reference - next);
-      sum = sum * alpha + more;
-      reference = next;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) total[e] *= alpha;
-#pragma unroll
-      for (int n = 0; n < kPartsInFlight; ++n) {
-        if (round + n >= count) break;
-        const float by = __shfl_sync(0xffffffffu, factor, n * 8 + (lane & 7));
-        if (by != 0.f) {  // (what a block without chunks of the tile has there may be anything)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) total[e] += __uint_as_float(v[n][e]) * by;
-        }
-      }
-    }
-    auto finish = [&](int row, float reference, float sum, bool first_of_row) {  // what the row's sums are multiplied with
-      float log_sum;
-      const float sink = p.sinks != nullptr ? __ldg(p.sinks + (tile.head + row) % p.heads) * kLog2E : -INFINITY;
-      const float inverse = inverse_of(reference, sum, sink, &log_sum);
-      if (p.lse != nullptr && first_of_row && segment == 0) p.lse[tile.row + row] = log_sum * kLn2;
-      return inverse;
-    };
-    if (warps == 1) {  // (no barrier in this branch)
-      if (row < tile.rows) {
-        const float inverse = finish(row, reference, sum, lane < 8);
-        uint32_t words[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) words[e] = inverse == 0.f ? 0u : pack2<kFormat>(total[2 * e] * inverse, total[2 * e + 1] * inverse);
-        *reinterpret_cast<uint4*>(p.out + ((tile.row + row) * LATENT_VALUES + feature_of(lane)) * 2) = make_uint4(words[0], words[1], words[2], words[3]);
-      }
-      continue;
-    }
-#pragma unroll
-    for (int e = 0; e < 8; e += 4) *reinterpret_cast<float4*>(&shares[warp][lane * 8 + e]) = make_float4(total[e], total[e + 1], total[e + 2], total[e + 3]);
-    if (lane < 8) shares_of[warp][lane] = make_float2(reference, sum);
-    __syncthreads();
-    for (int pair = first * 32 + lane; pair < kUnitRows * kUnitFeatures / 2; pair += warps * 32) {
-      const int owner = pair >> 2, row = rows + (owner & 7);  // the lane that had it
-      if (row >= tile.rows) continue;
-      float reference = -INFINITY, sum = 0.f;
-      for (int w = 0; w < warps; ++w) reference = fmaxf(reference, shares_of[warp - first + w][owner & 7].x);
-      float2 value = make_float2(0.f, 0.f);
-      for (int w = 0; w < warps; ++w) {
-        const float2 share = *reinterpret_cast<const float2*>(&shares[warp - first + w][pair * 2]), own = shares_of[warp - first + w][owner & 7];
-        const float by = own.x == -INFINITY ? 0.f : exp2f(own.x - reference);
-        value.x += share.x * by;
-        value.y += share.y * by;
-        sum += own.y * by;
-      }
-      const float inverse = finish(row, reference, sum, pair < 32 && (pair & 3) == 0);
-      *reinterpret_cast<uint32_t*>(p.out + ((tile.row + row) * LATENT_VALUES + feature_of(owner) + (pair & 3) * 2) * 2) =
-          inverse == 0.f ? 0u : pack2<kFormat>(value.x * inverse, value.y * inverse);
-    }
-    __syncthreads();  // the shares may be overwritten
+    join_parts<kFormat>(
+        shared, warps, tile.parts, rows, tile.rows,
+        [&](int part, int row) { return p.sums + slot_of(part) * kSlotFloats + sums_place(row, feature_of(lane)); },
+        [&](int part, int row) { return p.statistics + slot_of(part) * kRows + row; },
+        [&](int row, int owner) { return p.out + ((tile.row + row) * LATENT_VALUES + feature_of(owner)) * 2; },
+        [&](int row, float reference, float sum, bool first_of_row) {  // what the row's sums are multiplied with
+          float log_sum;
+          const float sink = p.sinks != nullptr ? __ldg(p.sinks + (tile.head + row) % p.heads) * kLog2E : -INFINITY;
+          const float inverse = inverse_of(reference, sum, sink, &log_sum);
+          if (p.lse != nullptr && first_of_row && segment == 0) p.lse[tile.row + row] = log_sum * kLn2;
+          return inverse;
+        });
   }
 }
 

@@ -25,6 +25,7 @@ decltype(&launch_latent_append) launch_append = nullptr;
 decltype(&launch_latent_attention) launch_attention = nullptr;
 decltype(&launch_latent_prefill) launch_prefill = nullptr;
 decltype(&workspace_size_latent_attention) workspace_size = nullptr;
+decltype(&workspace_size_latent_prefill) prefill_workspace_size = nullptr;
 
 constexpr double kLeastScale = 1e-30, kMostScale = 1e30;  // what FP32 holds with room to spare
 constexpr int64_t kMostRows = int64_t(1) << 30;  // tokens x heads
@@ -343,9 +344,15 @@ PyObject* call_prefill(PyObject*, PyObject* const* arguments, Py_ssize_t count) 
     pybind11::gil_scoped_release no_gil;
     const c10::cuda::CUDAStream stream = c10::cuda::getCurrentCUDAStream(device);
     used_on(stream, {t[0], t[1], t[2], t[3], t[4], t[5], out, lse});
-    Tensor kept;
+    uint64_t bytes = 0;
+    status = prefill_workspace_size(&bytes, &c);
+    Tensor kept, scratch;  // (scratch: of this call alone, as above)
     void* block = nullptr;
-    status = int(ascendflow_host::status_block(stream, &kept, &block));
+    if (status == 0 && bytes > 0) {
+      scratch = at::empty({int64_t(bytes)}, at::TensorOptions(at::kByte).device(at::kCUDA, device));
+      c.workspace = scratch.mutable_data_ptr();
+    }
+    if (status == 0) status = int(ascendflow_host::status_block(stream, &kept, &block));
     c.status = static_cast<int32_t*>(block);
     if (status == 0) status = launch_prefill(stream.stream(), &c);
   }
@@ -355,13 +362,14 @@ PyObject* call_prefill(PyObject*, PyObject* const* arguments, Py_ssize_t count) 
 
 // Addresses of the C ABI's functions, in the order in which they are declared.
 PyObject* configure(PyObject*, PyObject* arguments) {
-  unsigned long long rotary, append, attention, prefill, workspace;
-  if (!PyArg_ParseTuple(arguments, "KKKKK", &rotary, &append, &attention, &prefill, &workspace)) return nullptr;
+  unsigned long long rotary, append, attention, prefill, workspace, prefill_workspace;
+  if (!PyArg_ParseTuple(arguments, "KKKKKK", &rotary, &append, &attention, &prefill, &workspace, &prefill_workspace)) return nullptr;
   launch_rotary = reinterpret_cast<decltype(launch_rotary)>(rotary);
   launch_append = reinterpret_cast<decltype(launch_append)>(append);
   launch_attention = reinterpret_cast<decltype(launch_attention)>(attention);
   launch_prefill = reinterpret_cast<decltype(launch_prefill)>(prefill);
   workspace_size = reinterpret_cast<decltype(workspace_size)>(workspace);
+  prefill_workspace_size = reinterpret_cast<decltype(prefill_workspace_size)>(prefill_workspace);
   Py_RETURN_NONE;
 }
 

@@ -26,6 +26,7 @@
 // Rows of a value box behind the request's last key are cleared before they are multiplied: their weights are zero, but they
 // belong to other requests (or to nobody) and 0 x infinity would be a NaN. Scores of such keys are replaced, whatever they are.
 #include "latent_common.cuh"
+#include "latent_parts.cuh"
 #include "latent_ptx.cuh"
 
 namespace latent {
@@ -40,6 +41,13 @@ constexpr int kSoftmaxWarps = 8, kProductWarp = 8, kCopyWarp = 9, kPlanWarp = 10
 constexpr int kBoxBytes = kTile * 128;        // 64 features of 128 rows
 constexpr int kQBoxes = kFeatures / 64, kKeyBoxes = 3, kValueBoxes = 2, kRing = 8;
 constexpr int kItems = 2;                     // announced ahead
+
+// A call of few items leaves SMs without work, so items of many steps are cut into pieces there (for all SMs, no piece shorter than kLeastSteps), and
+// `join_kernel` adds up what they leave. The sums' way through memory and the second launch take 13 us, a step 2: not where the longest item is
+// not shortened by kSavedSteps. (16 heads, whole / cut: 512 queries at 2048 keys 39 / 27 us, at 16384 255 / 85-95, 1024 at 8192 134 / 88-94, one at
+// 131072 1890 / 241-264; five steps saved, 256 at 1025, 26 / 30. A call of few items whose requests turn out too short pays 3 us for the launch.)
+constexpr int kItemRows = 2 * kTile, kLeastSteps = 4, kSavedSteps = 8;
+constexpr int kSlotFloats = kItemRows * LATENT_NOPE;
 
 constexpr int kSmemQ = 0;                                       // two tiles of three boxes
 constexpr int kSmemRing = kSmemQ + 2 * kQBoxes * kBoxBytes;
@@ -64,8 +72,13 @@ struct Params {
   int32_t* status;
   int32_t batches, tokens, keys, heads, q_head, k_head, v_head;  // *_head: 0 where all heads share memory
   int32_t causal;
+  int32_t slots;      // of the workspace, one for every piece; 0: items are whole
+  float2* statistics; // [slots, 256]
+  float* sums;        // [slots], see sums_place
   float scale_log2;
 };
+// Sums of eight features of 32 rows lie next to each other, as warps write them. First feature of eight.
+__device__ __forceinline__ int sums_place(int row, int feature) { return (((row >> 5) * (LATENT_NOPE / 8) + feature / 8) * 32 + (row & 31)) * 8; }
 
 struct Shared {
   uint32_t base;
@@ -85,7 +98,9 @@ struct Item {
   int first;  // first key of the request
   int keys;   // keys that the request has
   int offset; // row i sees keys below offset + i + 1 (causal)
+  int slot;   // -1: the item is whole; >= 0: a piece, whose sums go there; kNoPiece: there is nothing to do
 };
+constexpr int kNoPiece = -2;
 static_assert(sizeof(Item) <= 32, "the item ring holds 32-byte entries");
 __device__ __forceinline__ Item* Shared::item(uint32_t index) const { return reinterpret_cast<Item*>(ptr + kSmemMisc + 64 + index % kItems * 32); }
 
@@ -97,15 +112,38 @@ __device__ __forceinline__ int reach(const Params& p, const Item& item, int rows
 
 __device__ __forceinline__ int bounded(int value, int most) { return min(max(value, 0), most); }
 
-// Item number `index`, by whole warps; false when there are fewer. Items: heads, of each all requests, of each request blocks of
-// 256 rows from its end (where causal rows see most keys) to its beginning.
-__device__ __forceinline__ bool find_item(const Params& p, int index, Item& item) {
+// Key steps of tile t.
+__device__ __forceinline__ int steps_of(const Params& p, const Item& item, int t) {
+  return item.rows <= t * kTile ? 0 : (reach(p, item, min(item.rows, (t + 1) * kTile)) + kTile - 1) / kTile;
+}
+
+// How a call's items are cut: up to `pieces` of each, of `steps` key steps; pieces == 1: not at all.
+struct Cut {
+  int pieces, steps;
+  __device__ __forceinline__ int of(const Params& p, const Item& item) const { return max((max(steps_of(p, item, 0), steps_of(p, item, 1)) + steps - 1) / steps, 1); }
+};
+
+// Item number `index` (whole), by whole warps; false when there are fewer. Items: heads, of each all requests, of each request blocks of
+// 256 rows from its end (where causal rows see most keys) to its beginning. With kPieces, `index` counts pieces,
+// as many for each item as the call's longest may be cut into.
+template <bool kPieces>
+__device__ __forceinline__ bool find_whole(const Params& p, int index, Item& item, Cut* cut) {
   const int lane = threadIdx.x & 31;
-  int per_head = 0;
-  for (int b = lane; b < p.batches; b += 32)
-    per_head += (max(bounded(__ldg(p.cu_q + b + 1), p.tokens) - bounded(__ldg(p.cu_q + b), p.tokens), 0) + 255) >> 8;
+  int per_head = 0, most_keys = 0;
+  for (int b = lane; b < p.batches; b += 32) {
+    const int blocks = (max(bounded(__ldg(p.cu_q + b + 1), p.tokens) - bounded(__ldg(p.cu_q + b), p.tokens), 0) + 255) >> 8;
+    per_head += blocks;
+    if (kPieces && blocks > 0) most_keys = max(most_keys, bounded(__ldg(p.cu_k + b + 1), p.keys) - bounded(__ldg(p.cu_k + b), p.keys));
+  }
   per_head = __reduce_add_sync(0xffffffffu, per_head);
-  if (per_head == 0 || index / per_head >= p.heads) return false;
+  if (per_head == 0) return false;
+  if (kPieces) {
+    const int most = (__reduce_max_sync(0xffffffffu, most_keys) + kTile - 1) / kTile, pieces = max(p.slots / p.heads / per_head, 1);
+    cut->steps = max((most + pieces - 1) / pieces, kLeastSteps);
+    cut->pieces = most - cut->steps >= kSavedSteps ? pieces : 1;
+    index /= cut->pieces;
+  }
+  if (index / per_head >= p.heads) return false;
   item.head = index / per_head;
   int left = index - item.head * per_head;
   for (int first = 0;; first += 32) {  // (ends: left < per_head)
@@ -134,13 +172,29 @@ __device__ __forceinline__ bool find_item(const Params& p, int index, Item& item
     item.first = __shfl_sync(0xffffffffu, k_begin, owner);
     item.keys = __shfl_sync(0xffffffffu, k_count, owner);
     item.offset = item.keys - request_count + start;
+    item.slot = -1;
     return true;
   }
 }
 
-// Key steps of tile t.
-__device__ __forceinline__ int steps_of(const Params& p, const Item& item, int t) {
-  return item.rows <= t * kTile ? 0 : (reach(p, item, min(item.rows, (t + 1) * kTile)) + kTile - 1) / kTile;
+// What block `index` does: an item, or a piece of one, which is the item as it would be if its keys began and ended with the piece's.
+template <bool kPieces>
+__device__ __forceinline__ bool find_item(const Params& p, int index, Item& item) {
+  Cut cut;
+  if (!find_whole<kPieces>(p, index, item, &cut)) return false;
+  if (kPieces && cut.pieces > 1) {
+    const int count = cut.of(p, item), piece = index % cut.pieces, keys = cut.steps * kTile;  // (of a piece)
+    if (piece >= count) {
+      item.slot = kNoPiece;
+      item.keys = 0;
+    } else if (count > 1) {
+      item.slot = index;
+      item.first += piece * keys;
+      item.offset -= piece * keys;
+      item.keys = min(item.keys - piece * keys, keys);
+    }
+  }
+  return true;
 }
 
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, long long limit = 1ll << 31) {
@@ -172,6 +226,7 @@ __device__ __forceinline__ int block_given(uint32_t answer) {
 }
 
 // By a whole warp. `item` is the first.
+template <bool kPieces>
 __device__ void plan_role(const Params& p, const Shared& sm, Item item) {
   const int lane = threadIdx.x & 31;
   volatile int* abort_flag = sm.abort_flag();
@@ -200,7 +255,7 @@ __device__ void plan_role(const Params& p, const Shared& sm, Item item) {
     if (*abort_flag != 0) return;
     int index = block_given(sm.answer());
     __syncwarp();
-    has = index >= 0 && find_item(p, index, item);
+    has = index >= 0 && find_item<kPieces>(p, index, item);
     if (!has) {
       // Numbers grow: the blocks behind this one have nothing to do either. They are taken over so that they need not start.
       while (index >= 0) {
@@ -224,6 +279,7 @@ struct Walk {
   Item item;
   __device__ __forceinline__ explicit Walk(const Shared& shared) : sm(shared) {}
   __device__ __forceinline__ bool read() { item = *sm.item(index); return item.rows > 0; }
+  __device__ __forceinline__ int slot() const { return *static_cast<volatile int*>(&sm.item(index)->slot); }  // (read where it is wanted: registers are scarce)
   __device__ __forceinline__ bool next_of_warp() { return warp_wait(sm.bar(kItemReady0 + index % kItems), (index / kItems) & 1, sm.abort_flag(), kLongWait) && read(); }
   __device__ __forceinline__ bool next_of_thread() { return mbar_wait(sm.bar(kItemReady0 + index % kItems), (index / kItems) & 1, sm.abort_flag(), kLongWait) && read(); }
   __device__ __forceinline__ void done() { mbar_arrive(sm.bar(kItemDone0 + index % kItems)); ++index; }
@@ -391,7 +447,7 @@ __device__ void product_role(const Params& p, const Shared& sm, uint32_t tmem) {
 constexpr float kStep = 8.f, kMostWeight = 32768.f;
 static_assert(kTile * 256 <= kMostWeight, "the smallest sum that is looked into");
 
-template <int kFormat>
+template <int kFormat, bool kPieces>
 __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, t = warp >> 2;
   volatile int* abort_flag = sm.abort_flag();
@@ -490,7 +546,8 @@ __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
       if (lane == 0) mbar_arrive(sm.bar(kWeights0 + t));
     }
     // Output: a row's 256 bytes by its own thread, in whole sectors.
-    const bool live = row < item.rows;
+    const int slot = kPieces ? walk.slot() : -1;
+    const bool live = row < item.rows && slot == -1;
     if (p.lse != nullptr && live)
       p.lse[size_t(item.row + row) * p.heads + item.head] = sum > 0.f ? (reference + log2f(sum)) * 0.6931471805599453f : (sum == 0.f ? -INFINITY : sum);
     const float inverse = sum == 0.f ? 0.f : 1.f / sum;
@@ -498,6 +555,21 @@ __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
     if (steps > 0) {
       if (!warp_wait(sm.bar(kOut0 + t), outputs++ & 1, abort_flag)) return;
       tc_fence_after_sync();
+    }
+    if (kPieces && slot != -1) {
+      if (slot == kNoPiece) continue;
+      if (row < item.rows) p.statistics[size_t(slot) * kItemRows + row] = part_statistics(reference, sum);
+      float* sums = p.sums + size_t(slot) * kSlotFloats + sums_place(row, 0);
+#pragma unroll 1
+      for (int c = 0; c < (steps > 0 ? kTile : 0); c += 32) {
+        uint32_t o[32];
+        tmem_ld32(o_tmem + c, o);
+        tmem_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 32; e += 8) store_sector(sums + (c + e) * 32, o + e);
+      }
+      tc_fence_before_sync();
+      continue;
     }
 #pragma unroll 1
     for (int c = 0; c < kTile; c += 32) {
@@ -519,7 +591,7 @@ __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
   }
 }
 
-template <int kFormat>
+template <int kFormat, bool kPieces>
 __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_constant__ Params p) {
   extern __shared__ unsigned char smem_raw[];
   Shared sm;
@@ -530,7 +602,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
   wait_for_predecessor();
   let_successor_start();
   Item item;
-  if (!find_item(p, blockIdx.x, item)) return;  // the whole block
+  if (!find_item<kPieces>(p, blockIdx.x, item)) return;  // the whole block
   if (threadIdx.x == 0) {
     for (int i = 0; i < kBarCount; ++i)
       mbar_init(sm.bar(i), i >= kWeights0 && i < kWeights0 + 2 ? 4 : i >= kItemDone0 ? kSoftmaxWarps + 2 : 1);
@@ -545,7 +617,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
   // A softmax thread holds a row's 128 scores: the third warpgroup's registers go to the first two (200 + 200 + 104 of 3 x 168).
   if (warp < kSoftmaxWarps) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 200;\n");
-    softmax_role<kFormat>(p, sm, tmem);
+    softmax_role<kFormat, kPieces>(p, sm, tmem);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 104;\n");
     if (warp == kProductWarp) {
@@ -557,13 +629,45 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
     } else if (warp == kCopyWarp) {
       copy_role(p, sm);
     } else if (warp == kPlanWarp) {
-      plan_role(p, sm, item);
+      plan_role<kPieces>(p, sm, item);
     }
   }
   tc_fence_before_sync();
   __syncthreads();
   if (threadIdx.x == 0 && *sm.abort_flag() != 0) report(p.status, SPARSE_MLA_STATUS_WAIT_EXPIRED, item.row, item.head);
   if (warp == kProductWarp) tmem_dealloc(tmem, 512);
+}
+
+// Items that were cut. Every block finds out what there is; 32 features of eight rows to one to eight of its warps. Bound by latency.
+template <int kFormat>
+__global__ void __launch_bounds__(kCombineThreads, 2) join_kernel(const __grid_constant__ Params p) {
+  __shared__ Shares shared;
+  wait_for_predecessor();
+  let_successor_start();
+  constexpr int kSegments = LATENT_NOPE / kUnitFeatures, kUnits = kItemRows / kUnitRows * kSegments;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  Item item;
+  Cut cut;
+  if (!find_whole<true>(p, 0, item, &cut) || cut.pieces == 1) return;
+  const int warps = warps_for(cut.pieces), turns = kUnits * warps / kCombineWarps;  // of a block for an item
+  for (int turn = blockIdx.x;; turn += gridDim.x) {
+    const int number = turn / turns;
+    if (!find_whole<true>(p, number * cut.pieces, item, &cut)) return;  // the whole block
+    const int count = cut.of(p, item);
+    if (count == 1) continue;
+    const int unit = ((turn - number * turns) * kCombineWarps + warp) / warps, segment = unit % kSegments;
+    auto feature_of = [&](int lane) { return segment * kUnitFeatures + (lane >> 3) * 8; };
+    join_parts<kFormat>(
+        shared, warps, count, unit / kSegments * kUnitRows, item.rows,
+        [&](int part, int row) { return p.sums + size_t(number * cut.pieces + part) * kSlotFloats + sums_place(row, feature_of(lane)); },
+        [&](int part, int row) { return p.statistics + size_t(number * cut.pieces + part) * kItemRows + row; },
+        [&](int row, int owner) { return static_cast<char*>(p.out) + ((size_t(item.row + row) * p.heads + item.head) * LATENT_NOPE + feature_of(owner)) * 2; },
+        [&](int row, float reference, float sum, bool first_of_row) {
+          if (p.lse != nullptr && first_of_row && segment == 0)
+            p.lse[size_t(item.row + row) * p.heads + item.head] = sum > 0.f ? (reference + log2f(sum)) * 0.6931471805599453f : (sum == 0.f ? -INFINITY : sum);
+          return sum == 0.f ? 0.f : 1.f / sum;
+        });
+  }
 }
 
 // The map of [rows, heads, features] with boxes of 128 rows of a head; *step: what a head adds to its coordinate (0: all share memory).
@@ -574,21 +678,41 @@ int map_heads(CUtensorMap* map, int format, const void* base, int64_t rows, int6
   return encode_map(map, format, 3, base, sizes, strides, 2, kTile);
 }
 
-template <int kFormat>
+template <int kFormat, bool kPieces>
 int launch(const Params& p, int blocks, cudaStream_t stream) {
   static bool configured[64] = {false};  // a per-device setting: plain words written with the same value by whoever gets there first
   int device = 0;
   if (const cudaError_t error = cudaGetDevice(&device)) return int(error);
   if (device < 0 || device >= 64) return -1;
   if (!configured[device]) {
-    if (const cudaError_t error = cudaFuncSetAttribute(prefill_kernel<kFormat>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes)) return int(error);
+    if (const cudaError_t error = cudaFuncSetAttribute(prefill_kernel<kFormat, kPieces>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes)) return int(error);
     configured[device] = true;
   }
-  return int(launch_overlapped(prefill_kernel<kFormat>, blocks, kThreads, kSmemBytes, stream, p));
+  if (const cudaError_t error = launch_overlapped(prefill_kernel<kFormat, kPieces>, blocks, kThreads, kSmemBytes, stream, p)) return int(error);
+  if constexpr (kPieces) return int(launch_overlapped(join_kernel<kFormat>, 2 * p.slots, kCombineThreads, 0, stream, p));
+  return 0;
 }
+
+// Pieces that a call may be cut into: a block for every SM where even the most items that it may have take half of them, and requests may be long enough.
+int slots_of(const latent_prefill_call& c) {
+  const int64_t requests = c.tokens < c.batches ? c.tokens : c.batches;
+  if (requests == 0 || c.keys <= (kLeastSteps + kSavedSteps - 1) * kTile) return 0;
+  const int64_t items = requests + (c.tokens - requests) / kItemRows;  // of a head
+  const int count = multiprocessors();
+  return items * c.heads <= count / 2 ? count : 0;
+}
+inline size_t sums_offset(int slots) { return size_t(slots) * kItemRows * sizeof(float2); }
 
 }  // namespace prefill
 }  // namespace latent
+
+extern "C" int workspace_size_latent_prefill(uint64_t* bytes, const latent_prefill_call* call) {
+  using namespace latent;
+  if (bytes == nullptr || call == nullptr || call->tokens < 0 || call->batches < 0 || call->keys < 0 || call->heads < 0 || call->heads > 65535) return -1;
+  const int slots = prefill::slots_of(*call);
+  *bytes = prefill::sums_offset(slots) + size_t(slots) * prefill::kSlotFloats * sizeof(float);
+  return 0;
+}
 
 extern "C" int launch_latent_prefill(void* stream, const latent_prefill_call* call) {
   using namespace latent;
@@ -596,10 +720,17 @@ extern "C" int launch_latent_prefill(void* stream, const latent_prefill_call* ca
   const latent_prefill_call& c = *call;
   if ((c.type != LATENT_F16 && c.type != LATENT_BF16) || !(c.scale > 0) || c.status == nullptr) return -1;
   if (c.batches < 0 || c.batches >= INT32_MAX || c.tokens < 0 || c.tokens > INT32_MAX - 256 || c.keys < 0 || c.keys > INT32_MAX - 256 || c.heads < 1 || c.heads > 65535) return -1;
-  const int64_t blocks = (c.tokens / 256 + c.batches) * c.heads;  // at least as many as there are items
+  int64_t blocks = (c.tokens / 256 + c.batches) * c.heads;  // at least as many as there are items
   if (blocks > INT32_MAX) return -1;
   if (c.tokens == 0 || c.batches == 0) return 0;
   prefill::Params p = {};
+  p.slots = prefill::slots_of(c);
+  if (p.slots > 0) {
+    if (c.workspace == nullptr || reinterpret_cast<uintptr_t>(c.workspace) % 32 != 0) return -1;
+    p.statistics = static_cast<float2*>(c.workspace);
+    p.sums = reinterpret_cast<float*>(static_cast<char*>(c.workspace) + prefill::sums_offset(p.slots));
+    if (blocks < p.slots) blocks = p.slots;
+  }
   const int64_t keys = c.keys > 0 ? c.keys : 1;  // (without keys nothing is copied)
   const void* any = c.q;
   if (const int e = prefill::map_heads(&p.q, c.type, c.q, c.tokens, c.heads, prefill::kFeatures, c.q_token, c.q_head, &p.q_head)) return e;
@@ -619,5 +750,6 @@ extern "C" int launch_latent_prefill(void* stream, const latent_prefill_call* ca
   p.causal = c.causal;
   p.scale_log2 = float(c.scale * 1.4426950408889634);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return c.type == LATENT_BF16 ? prefill::launch<1>(p, int(blocks), s) : prefill::launch<0>(p, int(blocks), s);
+  if (p.slots > 0) return c.type == LATENT_BF16 ? prefill::launch<1, true>(p, int(blocks), s) : prefill::launch<0, true>(p, int(blocks), s);
+  return c.type == LATENT_BF16 ? prefill::launch<1, false>(p, int(blocks), s) : prefill::launch<0, false>(p, int(blocks), s);
 }

@@ -114,6 +114,7 @@ def connect_latent():
 
     library = _library(library_path())
     calls.configure_latent(*(ct.cast(getattr(library, name), ct.c_void_p).value for name in (
-        "launch_latent_rotary", "launch_latent_append", "launch_latent_attention", "launch_latent_prefill", "workspace_size_latent_attention")))
+        "launch_latent_rotary", "launch_latent_append", "launch_latent_attention", "launch_latent_prefill", "workspace_size_latent_attention",
+        "workspace_size_latent_prefill")))
     _latent_connected = True
     return True

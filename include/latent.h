@@ -98,11 +98,14 @@ typedef struct {
   const int32_t *cu_seqlens_q, *cu_seqlens_k;
   void* out;  /* [T, heads, 128], contiguous */
   float* lse; /* [T, heads] or NULL */
+  void* workspace;
   int32_t* status;
   int64_t q_token, q_head, k_token, k_head, v_token, v_head, rope_token; /* strides */
   int64_t batches, tokens, keys, heads;
   double scale;
 } latent_prefill_call;
+/* Bytes of `workspace` (32-byte aligned; none: NULL will do) for a call of these batches, tokens, keys and heads on the current device; as above. */
+int workspace_size_latent_prefill(uint64_t* bytes, const latent_prefill_call* call);
 int launch_latent_prefill(void* stream, const latent_prefill_call* call);
 
 #ifdef __cplusplus

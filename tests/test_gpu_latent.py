@@ -1,5 +1,6 @@
 """Operators around dense latent attention on a GPU, against their definitions in 64 bits."""
 
+import functools
 import itertools
 
 import pytest
@@ -497,6 +498,67 @@ def test_prefill_ragged_batches(heads):
     counts[33], lengths[33] = 700, 900
     counts[64:100] = [0] * 36
     check_prefill(normal(1, sum(counts), heads, 192), normal(2, sum(lengths), heads, 256), normal(3, sum(lengths), 64), counts, lengths, 192 ** -0.5)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("heads,counts,lengths", [
+    (1, [1], [1537]), (1, [1], [20000]), (16, [3], [5000]), (5, [300], [4001]), (4, [1000], [3333]), (2, [257, 0, 1, 130], [2000, 5000, 1, 7001]), (1, [40] * 9, [128 * b for b in range(9)] ),
+    (24, [129], [9000]), (2, [2000], [1700]), (37, [1, 1], [3000, 6000]), (74, [2], [1664]), (75, [2], [1664]),
+])
+def test_prefill_of_few_queries_and_many_keys(dtype, causal, heads, counts, lengths):
+    """Calls whose items are cut into pieces, and those next to them: pieces that rows do not reach, pieces that end inside a tile of keys, requests too
+    short to be cut beside long ones, tokens that see nothing, as many items as are still cut, and one more."""
+    q, kv, rope = normal(1, sum(counts), heads, 192, dtype=dtype), normal(2, sum(lengths), heads, 256, dtype=dtype), normal(3, sum(lengths), 64, dtype=dtype)
+    check_prefill(q, kv, rope, counts, lengths, 192 ** -0.5, causal=causal)
+
+
+@pytest.mark.parametrize("spread", [0.01, 12.0])
+def test_prefill_pieces_of_flat_and_steep_scores(spread):
+    """Every piece with another reference, the last keys with nearly all of the weight."""
+    kv, rope = normal(2, 6000, 4, 256), normal(3, 6000, 64)
+    kv[..., :128] *= torch.linspace(0.1, 2.0, 6000, device="cuda").to(BF16).view(-1, 1, 1)
+    check_prefill(normal(1, 70, 4, 192, spread=spread), kv, rope, [70], [6000], 0.07)
+
+
+def test_prefill_pieces_leave_padding_alone_and_do_not_see_others():
+    counts, lengths = [3, 5], [2500, 3100]
+    kv, rope = normal(2, 6000, 2, 256), normal(3, 6000, 64)
+    kv[:100], kv[5700:], rope[:100], rope[5700:] = (torch.nan,) * 4
+    check_prefill(normal(1, 20, 2, 192), kv, rope, counts, lengths, 0.07, first=4, first_key=100)
+
+
+def test_prefill_in_pieces_in_graphs_and_on_two_streams():
+    """Sums between the two kernels are a call's own: two captured graphs and calls of another stream, in turn and at once."""
+    calls = []
+    for seed, (heads, count, length) in enumerate([(16, 200, 5000), (3, 1, 9000), (16, 200, 5000)]):
+        q, kv, rope = normal(seed, count, heads, 192), normal(seed + 10, length, heads, 256), normal(seed + 20, length, 64)
+        cu_q, cu_k, out = i32([0, count]), i32([0, length]), torch.empty((count, heads, 128), dtype=BF16, device="cuda")
+        calls.append((functools.partial(latent.latent_prefill, q, kv[..., :128], kv[..., 128:], rope, cu_q, cu_k, scale=0.07, out=out), out))
+    expected = []
+    for call, out in calls:
+        call()
+        torch.cuda.synchronize()
+        expected.append(out.clone())
+    graphs = []
+    for call, _ in calls[:2]:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            call()
+        graphs.append(graph)
+    side, other = torch.cuda.Stream(), torch.cuda.Stream()
+    for _, out in calls:
+        out.zero_()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        graphs[0].replay()
+        with torch.cuda.stream(side):
+            graphs[1].replay()
+        with torch.cuda.stream(other):
+            calls[2][0]()
+    torch.cuda.synchronize()
+    for (_, out), right in zip(calls, expected):
+        assert torch.equal(out, right)
 
 
 @pytest.mark.parametrize("causal", [True, False])
