@@ -1,11 +1,13 @@
 """Operators around dense latent attention where there is no device: their refusals, and the frequencies."""
 
+import ctypes
 import math
 
 import pytest
 import torch
 
 from ascendflow_b200 import latent
+from ascendflow_b200.build import library_path
 from ascendflow_b200.diagnostics import CompileError
 
 
@@ -67,3 +69,33 @@ def test_frequencies():
                   dict(dims=64, scaling="yarn", beta_slow=0.0)):
         with pytest.raises(CompileError):
             latent.rotary_frequencies(**wrong, device="cpu")
+
+
+class PrefillCall(ctypes.Structure):
+    _fields_ = [("type", ctypes.c_int32), ("causal", ctypes.c_int32), *((name, ctypes.c_void_p) for name in (
+        "q", "k", "v", "k_rope", "cu_seqlens_q", "cu_seqlens_k", "out", "lse", "workspace", "status")), *((name, ctypes.c_int64) for name in (
+            "q_token", "q_head", "k_token", "k_head", "v_token", "v_head", "rope_token", "batches", "tokens", "keys", "heads")), ("scale", ctypes.c_double)]
+
+
+def test_workspace_of_the_expanded_call():
+    """Calls of few items and many keys want one, others do not; a call without the one that it wants is refused before anything is launched."""
+    library = ctypes.CDLL(str(library_path()))
+    size = ctypes.c_uint64()
+
+    def wanted(batches, tokens, keys, heads):
+        call = PrefillCall(batches=batches, tokens=tokens, keys=keys, heads=heads)
+        assert library.workspace_size_latent_prefill(ctypes.byref(size), ctypes.byref(call)) == 0
+        return size.value
+
+    slot = 256 * 128 * 4 + 256 * 8
+    for few in ((1, 1, 1537, 1), (1, 512, 16384, 16), (3, 3, 9000, 16), (1, 256, 5000, 66), (2, 257, 5000, 22)):
+        assert wanted(*few) > 0 and wanted(*few) % slot == 0
+    for other in ((1, 1, 1408, 1), (1, 0, 16384, 1), (0, 0, 16384, 1), (1, 2048, 16384, 16), (1, 1, 5000, 1000), (400, 400, 10 ** 6, 1), (1, 8192, 8192, 64)):
+        assert wanted(*other) == 0
+    assert library.workspace_size_latent_prefill(None, ctypes.byref(PrefillCall())) == -1 and library.workspace_size_latent_prefill(ctypes.byref(size), None) == -1
+    for wrong in (dict(heads=-1), dict(heads=65536), dict(tokens=-1), dict(keys=-1), dict(batches=-1)):
+        assert library.workspace_size_latent_prefill(ctypes.byref(size), ctypes.byref(PrefillCall(**wrong))) == -1
+    call = PrefillCall(type=1, batches=1, tokens=2, keys=5000, heads=2, scale=1.0, status=64)
+    for workspace in (None, 16):
+        call.workspace = workspace
+        assert library.launch_latent_prefill(None, ctypes.byref(call)) == -1
