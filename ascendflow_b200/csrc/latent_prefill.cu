@@ -72,6 +72,7 @@ struct Params {
   int32_t* status;
   int32_t batches, tokens, keys, heads, q_head, k_head, v_head;  // *_head: 0 where all heads share memory
   int32_t causal;
+  int32_t sectors;    // rows of `out` begin on 32-byte boundaries (otherwise on 16-byte ones)
   int32_t slots;      // of the workspace, one for every piece; 0: items are whole
   float2* statistics; // [slots, 256]
   float* sums;        // [slots], see sums_place
@@ -545,7 +546,7 @@ __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
       __syncwarp();
       if (lane == 0) mbar_arrive(sm.bar(kWeights0 + t));
     }
-    // Output: a row's 256 bytes by its own thread, in whole sectors.
+    // Output: a row's 256 bytes by its own thread, in whole sectors where rows begin with one.
     const int slot = kPieces ? walk.slot() : -1;
     const bool live = row < item.rows && slot == -1;
     if (p.lse != nullptr && live)
@@ -582,9 +583,12 @@ __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         words[i] = sum == 0.f ? 0u : pack2<kFormat>(__uint_as_float(o[2 * i]) * inverse, __uint_as_float(o[2 * i + 1]) * inverse);
-      if (live) {
+      if (live && p.sectors) {
         store_sector(out + c * 2, words);
         store_sector(out + c * 2 + 32, words + 8);
+      } else if (live) {
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) *reinterpret_cast<uint4*>(out + c * 2 + i * 4) = make_uint4(words[i], words[i + 1], words[i + 2], words[i + 3]);
       }
     }
     tc_fence_before_sync();  // (the accumulator may be overwritten when this warp's next weights are there)
@@ -748,6 +752,7 @@ extern "C" int launch_latent_prefill(void* stream, const latent_prefill_call* ca
   p.keys = int32_t(c.keys);
   p.heads = int32_t(c.heads);
   p.causal = c.causal;
+  p.sectors = reinterpret_cast<uintptr_t>(c.out) % 32 == 0;
   p.scale_log2 = float(c.scale * 1.4426950408889634);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (p.slots > 0) return c.type == LATENT_BF16 ? prefill::launch<1, true>(p, int(blocks), s) : prefill::launch<0, true>(p, int(blocks), s);
