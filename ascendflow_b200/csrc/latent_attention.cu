@@ -1111,6 +1111,7 @@ int launch_latent_attention(void* stream, const latent_attention_call* call) {
   if ((c.type != LATENT_F16 && c.type != LATENT_BF16) || (c.width != 512 && c.width != 576) || !(c.scale > 0)) return -1;
   if (c.batches < 0 || c.batches > INT32_MAX / 2 || c.tokens < 0 || c.heads < 1 || c.tokens > (int64_t(1) << 30) / c.heads) return -1;
   if (c.pages < 0 || c.blocks < 0 || c.page_rows < 64 || c.page_rows % 64 != 0 || c.pages > (INT32_MAX - 128) / c.page_rows || c.blocks > INT32_MAX / c.page_rows) return -1;
+  if (!aligned(c.q) || !aligned(c.cache) || !aligned(c.out)) return -1;
   if (c.tokens == 0 || c.batches == 0) return 0;
   if (c.workspace == nullptr || reinterpret_cast<uintptr_t>(c.workspace) % 32 != 0 || c.status == nullptr) return -1;
   const int blocks = absorbed::grid();

@@ -53,6 +53,8 @@ __device__ __forceinline__ int request_of(const int32_t* cu, int batches, int to
   return lo;
 }
 
+inline bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
 inline int multiprocessors() {
   static int cached[64] = {0};  // plain words written with the same value by whoever gets there first
   int device = 0;

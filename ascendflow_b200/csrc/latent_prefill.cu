@@ -726,6 +726,9 @@ extern "C" int launch_latent_prefill(void* stream, const latent_prefill_call* ca
   if (c.batches < 0 || c.batches >= INT32_MAX || c.tokens < 0 || c.tokens > INT32_MAX - 256 || c.keys < 0 || c.keys > INT32_MAX - 256 || c.heads < 1 || c.heads > 65535) return -1;
   int64_t blocks = (c.tokens / 256 + c.batches) * c.heads;  // at least as many as there are items
   if (blocks > INT32_MAX) return -1;
+  // (what has no entries has no alignment)
+  if (c.tokens > 0 && (!aligned(c.q) || !aligned(c.out) || (c.q_token | c.q_head) % 8 != 0)) return -1;
+  if (c.keys > 0 && (!aligned(c.k) || !aligned(c.v) || !aligned(c.k_rope) || (c.k_token | c.k_head | c.v_token | c.v_head | c.rope_token) % 8 != 0)) return -1;
   if (c.tokens == 0 || c.batches == 0) return 0;
   prefill::Params p = {};
   p.slots = prefill::slots_of(c);

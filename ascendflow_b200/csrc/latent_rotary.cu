@@ -150,7 +150,6 @@ int launch_append(const latent_append_call& c, cudaStream_t stream) {
 }
 
 bool pairs_fit(int64_t pairs) { return pairs >= 8 && pairs <= LATENT_MOST_PAIRS && pairs % 8 == 0; }
-bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 }  // namespace
 }  // namespace latent

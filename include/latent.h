@@ -52,7 +52,7 @@ int launch_latent_rotary(void* stream, const latent_rotary_call* call);
 
 /* Row j of the n of request b goes to logical position p = seqused_kv[b] - n + j of the paged cache (seqused_kv counts
  * the new rows): `latent`, then `rope` turned by p * inv_freq[i] as above. width = latent's features (a
- * multiple of 8) + 2 pairs. */
+ * multiple of 8) + 2 pairs. latent_token is a multiple of 8, addresses of latent and cache of 16 bytes. */
 typedef struct {
   int32_t type, layout;
   const void* latent; /* [T, width - 2 pairs] */
@@ -71,7 +71,8 @@ int launch_latent_append(void* stream, const latent_append_call* call);
  * seen if k < seqused_kv[b] - n + j + 1; scores scale * q . row over all `width` (512 or 576) features, values are the
  * row's first 512. sinks (or NULL): a logit per head in the denominator. lse (or NULL): the natural
  * logarithm of the denominator. A token that sees no key gets zeros. page_rows: a multiple of 64.
- * Rows behind a request's length are never multiplied; rows within it have to be finite. */
+ * Rows behind a request's length are never multiplied; rows within it have to be finite. Addresses of q, cache and out are
+ * multiples of 16 bytes. */
 typedef struct {
   int32_t type, reserved;
   const void* q;     /* [T, heads, width] */
@@ -91,7 +92,7 @@ int launch_latent_attention(void* stream, const latent_attention_call* call);
 
 /* Attention in expanded form: keys are [k | k_rope], 128 features per head and 64 shared by all heads; values 128
  * per head. Request b owns keys cu_seqlens_k[b] .. ; causal: token j of n sees the first K - n + j + 1 of its K keys,
- * otherwise all. Strides are multiples of 8, addresses of 16 bytes. */
+ * otherwise all. Strides are multiples of 8, addresses of q, k, v, k_rope and out of 16 bytes. */
 typedef struct {
   int32_t type, causal;
   const void *q, *k, *v, *k_rope; /* [T, heads, 192], [S, heads, 128], [S, heads, 128], [S, 64] */
