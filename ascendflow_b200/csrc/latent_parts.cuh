@@ -13,7 +13,7 @@ using namespace sm100;
 constexpr int kUnitRows = 8, kUnitFeatures = 32, kPartsInFlight = 4;
 constexpr int kCombineThreads = 256, kCombineWarps = kCombineThreads / 32;
 
-struct Shares {  // what the warps of a block have
+struct alignas(16) Shares {  // what the warps of a block have; read and written 16 bytes at a time
   float sums[kCombineWarps][kUnitRows * kUnitFeatures];
   float2 statistics[kCombineWarps][kUnitRows];
 };
