@@ -54,7 +54,8 @@ def rotary_frequencies(dims, *, base=10000.0, scaling="none", factor=1.0, origin
     def pair_of(turns):  # the pair that turns so many times within the original length
         return half * math.log(original_length / (turns * 2 * math.pi)) / math.log(base)
 
-    low, high = max(math.floor(pair_of(beta_fast)), 0), min(math.ceil(pair_of(beta_slow)), half - 1)
+    # (the ramp may end behind the last pair, which then is on it; it is bounded by the number of features, as published)
+    low, high = max(math.floor(pair_of(beta_fast)), 0), min(math.ceil(pair_of(beta_slow)), dims - 1)
     ramp = ((torch.arange(half, dtype=torch.float64) - low) / max(high - low, 1e-3)).clamp(0, 1)
     return (plain * (1 - ramp) + plain / factor * ramp).to(device)
 
