@@ -720,8 +720,10 @@ __device__ void value_role(const Shared& sm, uint32_t tmem) {
 
 // ---- softmax ----------------------------------------------------------------------------------------------------------
 
-// A row's reference (log2) starts at the maximum of its first scores and moves when others exceed it by more than kRoom, to kStep below
-// them: weights of up to 2^15 fit IEEE half, and the accumulator is rarely rescaled.
+// A row's reference (log2) starts kStep below the maximum of its first scores and moves when others exceed it by more than kRoom, to kStep below
+// them. Weights are rounded to the storage type for the second product. In IEEE half they fit up to 2^15, so that the accumulator is rarely
+// rescaled; what counts below the greatest is off by at most 2^-25 of the unit, which is 2^-33 of the greatest: 128 K of those are 2^-16 (with the
+// reference at the maximum itself they were 2^-8, and keys 25 binades below a dominant first one were lost altogether).
 constexpr float kRoom = 15.f, kStep = 8.f;
 constexpr float kLog2E = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -817,7 +819,7 @@ __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
       if (look) {
         const float top = fmaxf(own, __shfl_xor_sync(0xffffffffu, own, 16));
         if (top > reference + kRoom) {
-          const float next = reference == -INFINITY ? top : top - kStep;
+          const float next = top - kStep;
           alpha = exp2f(reference - next);
           reference = next;
         }

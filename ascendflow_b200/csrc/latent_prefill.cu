@@ -442,11 +442,12 @@ __device__ void product_role(const Params& p, const Shared& sm, uint32_t tmem) {
 
 // ---- softmax ----------------------------------------------------------------------------------------------------------
 
-// A row's reference (log2) starts at the maximum of its first scores. It moves, to kStep below the maximum of a step, where the step's weights
-// sum up to more than kMostWeight: weights fit IEEE half, and the accumulator is rarely rescaled. (A sum that large has a weight of
-// more than 2^kStep in it, so that it does move.)
-constexpr float kStep = 8.f, kMostWeight = 32768.f;
-static_assert(kTile * 256 <= kMostWeight, "the smallest sum that is looked into");
+// A row's reference (log2) starts kStep below the maximum of its first scores. It moves, to kStep below the maximum of a step, where the step's weights
+// sum up to more than kMostWeight. Weights are rounded to the storage type for the second product: up to that sum they fit IEEE half, so that the
+// accumulator is rarely rescaled, and below the greatest they are off by at most 2^-33 of it (latent_attention.cu). (A sum that large has
+// a weight of more than 2^kStep in it, so that the reference does move.)
+constexpr float kStep = 8.f, kMostWeight = 61440.f;
+static_assert(kTile * 256 <= kMostWeight && kMostWeight < 65504.f, "the smallest sum that is looked into, and the largest weight");
 
 template <int kFormat, bool kPieces>
 __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
@@ -471,8 +472,8 @@ __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
       uint32_t words[kTile / 2];
       float own;
       // Weights are worked out with the reference as it is, without looking for the maximum: as long as their sum stays below kMostWeight so does
-      // each of them. Where it does not (for some row of the warp) the reference may move, and they are worked out again. A row's first reference is
-      // the maximum of its first 32 scores.
+      // each of them. Where it does not (for some row of the warp) the reference may move, and they are worked out again. A row's first reference comes
+      // from the maximum of its first 32 scores.
       for (int look = step == 0 ? 1 : 0;; look = 4) {  // parts of 32 scores to look at
         float2 s[2][16];  // 32 scores, and the next 32 on their way
         auto load = [&](int part) { tmem_ld32(s_tmem + part * 32, reinterpret_cast<uint32_t*>(&s[part & 1][0])); };
@@ -499,7 +500,7 @@ __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
           const bool moves = top > reference + kStep;
           float alpha = 1.f;
           if (moves) {
-            const float next = reference == -INFINITY ? top : top - kStep;
+            const float next = top - kStep;
             alpha = exp2f(reference - next);
             reference = next;
           }
