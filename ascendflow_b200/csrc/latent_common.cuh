@@ -42,6 +42,8 @@ __device__ __forceinline__ float2 turn_of(int64_t position, uint64_t turns, floa
   return make_float2(cosine * amplitude, sine * amplitude);
 }
 
+__device__ __forceinline__ int bounded(int value, int most) { return min(max(value, 0), most); }
+
 // The request that owns `token` (binary search; empty requests are skipped), or -1 in front of the first and behind the last.
 __device__ __forceinline__ int request_of(const int32_t* cu, int batches, int token) {
   if (token < __ldg(cu) || token >= __ldg(cu + batches)) return -1;

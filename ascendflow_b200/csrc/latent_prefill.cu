@@ -111,8 +111,6 @@ __device__ __forceinline__ int reach(const Params& p, const Item& item, int rows
   return p.causal ? min(item.keys, max(0, item.offset + rows)) : item.keys;
 }
 
-__device__ __forceinline__ int bounded(int value, int most) { return min(max(value, 0), most); }
-
 // Key steps of tile t.
 __device__ __forceinline__ int steps_of(const Params& p, const Item& item, int t) {
   return item.rows <= t * kTile ? 0 : (reach(p, item, min(item.rows, (t + 1) * kTile)) + kTile - 1) / kTile;

@@ -112,7 +112,8 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const latent_append_ca
   if (token >= c.tokens) return;
   const int request = request_of(c.cu_seqlens_q, int(c.batches), int(token));
   if (request < 0) return;
-  const int begin = __ldg(c.cu_seqlens_q + request), count = __ldg(c.cu_seqlens_q + request + 1) - begin;
+  // (the request's tokens as the attention calls see them: offsets outside of the call's tokens are clamped)
+  const int begin = bounded(__ldg(c.cu_seqlens_q + request), int(c.tokens)), count = bounded(__ldg(c.cu_seqlens_q + request + 1), int(c.tokens)) - begin;
   const int64_t position = int64_t(__ldg(c.seqused_kv + request)) - count + (token - begin);
   const int64_t column = position / c.page_rows;
   int64_t page = -1;
