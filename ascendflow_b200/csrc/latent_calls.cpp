@@ -86,7 +86,15 @@ bool disjoint(const Tensor& a, const Tensor& b) {
   return x.first == x.second || y.first == y.second || x.second <= y.first || y.second <= x.first;
 }
 
+PyObject* real_numbers = nullptr;  // numbers.Real
+
+// A real number of any kind, but no tensor: that would have to be waited for.
 bool number_of(PyObject* object, double* value) {
+  if (!PyFloat_Check(object) && !PyLong_Check(object)) {
+    const int real = real_numbers == nullptr ? 0 : PyObject_IsInstance(object, real_numbers);
+    if (real < 0) PyErr_Clear();
+    if (real != 1) return false;
+  }
   *value = PyFloat_AsDouble(object);
   if (*value == -1.0 && PyErr_Occurred()) {
     PyErr_Clear();
@@ -360,10 +368,12 @@ PyObject* call_prefill(PyObject*, PyObject* const* arguments, Py_ssize_t count) 
   END_HANDLE_TH_ERRORS
 }
 
-// Addresses of the C ABI's functions, in the order in which they are declared.
+// Addresses of the C ABI's functions, in the order in which they are declared; the class of real numbers.
 PyObject* configure(PyObject*, PyObject* arguments) {
   unsigned long long rotary, append, attention, prefill, workspace, prefill_workspace;
-  if (!PyArg_ParseTuple(arguments, "KKKKKK", &rotary, &append, &attention, &prefill, &workspace, &prefill_workspace)) return nullptr;
+  PyObject* real;
+  if (!PyArg_ParseTuple(arguments, "KKKKKKO", &rotary, &append, &attention, &prefill, &workspace, &prefill_workspace, &real)) return nullptr;
+  Py_XSETREF(real_numbers, Py_NewRef(real));
   launch_rotary = reinterpret_cast<decltype(launch_rotary)>(rotary);
   launch_append = reinterpret_cast<decltype(launch_append)>(append);
   launch_attention = reinterpret_cast<decltype(launch_attention)>(attention);

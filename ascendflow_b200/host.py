@@ -15,6 +15,7 @@ from __future__ import annotations
 import ctypes as ct
 import importlib.machinery
 import importlib.util
+import numbers
 
 import torch  # noqa: F401  (its libraries are what the module links against)
 
@@ -115,6 +116,6 @@ def connect_latent():
     library = _library(library_path())
     calls.configure_latent(*(ct.cast(getattr(library, name), ct.c_void_p).value for name in (
         "launch_latent_rotary", "launch_latent_append", "launch_latent_attention", "launch_latent_prefill", "workspace_size_latent_attention",
-        "workspace_size_latent_prefill")))
+        "workspace_size_latent_prefill")), numbers.Real)
     _latent_connected = True
     return True

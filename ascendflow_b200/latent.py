@@ -15,6 +15,8 @@ back here, where the violated rule is put into words. Nothing is ever cast, copi
 from __future__ import annotations
 
 import math
+import numbers
+import sys
 
 import torch
 
@@ -178,8 +180,8 @@ def _disjoint(written, others):
             require(begin == end or first == last or end <= first or last <= begin, "tensors that are written must not overlap others")
 
 
-def _number(value, name):
-    require(isinstance(value, (int, float)) and math.isfinite(value), f"{name}: expected a finite number")
+def _number(value, name, least=-sys.float_info.max, most=sys.float_info.max):
+    require(isinstance(value, numbers.Real) and least <= value <= most, f"{name}: expected a finite number from {least:g} to {most:g}")
 
 
 def _check_frequencies(inv_freq):
@@ -243,8 +245,7 @@ def _check_written(out, lse, inputs):
 
 
 def _check_attention(q, cache, block_table, cu_seqlens_q, seqused_kv, scale, sinks, out, lse):
-    _number(scale, "scale")
-    require(1e-30 <= scale <= 1e30, "scale must be a positive float32 number")
+    _number(scale, "scale", 1e-30, 1e30)
     _tensor(q, "q", _STORED)
     require(q.dim() == 3 and q.shape[2] in (512, 576) and q.shape[1] >= 1 and q.is_contiguous(), "q: expected contiguous [T, H, 512] or [T, H, 576]")
     require(q.shape[:2].numel() <= MOST_ROWS, "q: too many rows")
@@ -261,8 +262,7 @@ def _check_attention(q, cache, block_table, cu_seqlens_q, seqused_kv, scale, sin
 
 
 def _check_prefill(q, k, v, k_rope, cu_seqlens_q, cu_seqlens_k, scale, causal, out, lse):
-    _number(scale, "scale")
-    require(1e-30 <= scale <= 1e30, "scale must be a positive float32 number")
+    _number(scale, "scale", 1e-30, 1e30)
     require(isinstance(causal, bool), "causal: expected True or False")
     _tensor(q, "q", _STORED)
     require(q.dim() == 3 and q.shape[2] == NOPE + ROPE and 1 <= q.shape[1] <= 65535, "q: expected [T, H, 192]")

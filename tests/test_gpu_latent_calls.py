@@ -36,3 +36,45 @@ def test_append_puts_rows_where_attention_reads_them(starts, counts):
     R.within(cache, expected, R.HALF_STEP[BF16] * expected.abs() + 16 * 2.0 ** -24 * 8, "cache")
     latent.rotary_append(rows, rope, clamped, table, i32([min(max(s, 0), 3) for s in starts]), i32(lengths), inv_freq)
     assert torch.equal(cache, clamped)
+
+
+def test_numbers_are_taken_or_refused_alike_by_all_calls():
+    """Real numbers of any kind are taken, whether or not the call stays in native code; tensors and texts are not."""
+    q, kv, rope, cu = normal(1, 4, 2, 192), normal(2, 4, 2, 256), normal(3, 4, 64), i32([0, 4])
+    cache, table, seq, inv_freq = normal(4, 1, 64, 1, 576), i32([[0]]), i32([20]), latent.rotary_frequencies(64)
+    absorbed, rows = normal(5, 4, 2, 576), normal(6, 4, 512)
+    calls = {
+        "scale": (lambda n: latent.latent_prefill(q, kv[..., :128], kv[..., 128:], rope, cu, cu, scale=n), lambda n: latent.latent_attention(absorbed, cache, table, cu, seq, scale=n)),
+        "amplitude": (lambda n: latent.rotary(q, i32([1, 2, 3, 4]), inv_freq, amplitude=n), lambda n: latent.rotary_append(rows, rope, cache, table, cu, seq, inv_freq, amplitude=n)),
+    }
+    for name, group in calls.items():
+        for call in group:
+            expected = call(0.5).clone()
+            for number in (np.float32(0.5), np.float64(0.5), np.float16(0.5)):
+                assert torch.equal(call(number), expected)
+            assert torch.equal(call(1), call(np.int64(1)))
+            for wrong in (torch.tensor(0.5), torch.tensor(0.5, device="cuda"), np.array(0.5), "0.5", None, 10 ** 400, float("nan"), float("inf")):
+                with pytest.raises(CompileError, match=name):
+                    call(wrong)
+
+
+@pytest.mark.parametrize("name", ["np.float32(0.5)", "torch.tensor(0.5)"])
+def test_the_first_call_of_a_process_takes_what_others_take(name):
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    program = """
+import numpy as np, torch
+from ascendflow_b200 import latent
+q, kv, cu = torch.randn((4, 2, 192), device="cuda").half(), torch.randn((4, 2, 256), device="cuda").half(), torch.tensor([0, 4], dtype=torch.int32, device="cuda")
+for _ in range(2):
+    try:
+        latent.latent_prefill(q, kv[..., :128], kv[..., 128:], q[:, 0, 128:], cu, cu, scale=NUMBER)
+        print("taken")
+    except Exception as error:
+        print(type(error).__name__)
+    latent.latent_prefill(q, kv[..., :128], kv[..., 128:], q[:, 0, 128:], cu, cu, scale=0.5)
+""".replace("NUMBER", name)
+    result = subprocess.run([sys.executable, "-c", program], cwd=Path(__file__).resolve().parents[1], capture_output=True, text=True, timeout=120)
+    assert result.stdout.split() == ["taken" if "np" in name else "CompileError"] * 2, result.stderr[-2000:]
