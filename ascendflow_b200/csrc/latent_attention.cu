@@ -1110,7 +1110,7 @@ int launch_latent_attention(void* stream, const latent_attention_call* call) {
   using namespace latent;
   if (call == nullptr) return -1;
   const latent_attention_call& c = *call;
-  if ((c.type != LATENT_F16 && c.type != LATENT_BF16) || (c.width != 512 && c.width != 576) || !(c.scale > 0)) return -1;
+  if ((c.type != LATENT_F16 && c.type != LATENT_BF16) || (c.width != 512 && c.width != 576) || !scale_fits(c.scale)) return -1;
   if (c.batches < 0 || c.batches > INT32_MAX / 2 || c.tokens < 0 || c.heads < 1 || c.tokens > (int64_t(1) << 30) / c.heads) return -1;
   if (c.pages < 0 || c.blocks < 0 || c.page_rows < 64 || c.page_rows % 64 != 0 || c.pages > (INT32_MAX - 128) / c.page_rows || c.blocks > INT32_MAX / c.page_rows) return -1;
   if (!aligned(c.q) || !aligned(c.cache) || !aligned(c.out)) return -1;

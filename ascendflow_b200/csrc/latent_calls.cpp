@@ -13,6 +13,7 @@
 #include <algorithm>
 #include <array>
 #include <cmath>
+#include <limits>
 
 #include "../../include/latent.h"
 
@@ -102,6 +103,8 @@ bool number_of(PyObject* object, double* value) {
   }
   return std::isfinite(*value);
 }
+// What cosines and sines are multiplied by, in FP32.
+bool amplitude_of(PyObject* object, double* value) { return number_of(object, value) && std::abs(*value) <= std::numeric_limits<float>::max(); }
 bool flag_of(PyObject* object, int32_t* value) {
   if (!PyBool_Check(object)) return false;
   *value = object == Py_True;
@@ -133,7 +136,7 @@ PyObject* call_rotary(PyObject*, PyObject* const* arguments, Py_ssize_t count) {
   const Tensor *x = tensor_of(arguments[0]), *positions = tensor_of(arguments[1]), *inv_freq = tensor_of(arguments[2]), *out = tensor_of(arguments[6]);
   latent_rotary_call c = {};
   if (x == nullptr || positions == nullptr || inv_freq == nullptr || out == nullptr || !x->is_cuda()) Py_RETURN_FALSE;
-  if (!flag_of(arguments[3], &c.layout) || !flag_of(arguments[4], &c.inverse) || !number_of(arguments[5], &c.amplitude)) Py_RETURN_FALSE;
+  if (!flag_of(arguments[3], &c.layout) || !flag_of(arguments[4], &c.inverse) || !amplitude_of(arguments[5], &c.amplitude)) Py_RETURN_FALSE;
   const c10::DeviceIndex device = c10::cuda::current_device();
   c.type = type_of(*x);
   if (c.type < 0 || (x->dim() != 2 && x->dim() != 3) || !on_device(*x, device, x->scalar_type()) || !on_device(*out, device, x->scalar_type())) Py_RETURN_FALSE;
@@ -190,7 +193,7 @@ PyObject* call_append(PyObject*, PyObject* const* arguments, Py_ssize_t count) {
   for (int i = 0; i < 7; ++i)
     if ((t[i] = tensor_of(arguments[i])) == nullptr) Py_RETURN_FALSE;
   latent_append_call c = {};
-  if (!flag_of(arguments[7], &c.layout) || !number_of(arguments[8], &c.amplitude) || !t[0]->is_cuda()) Py_RETURN_FALSE;
+  if (!flag_of(arguments[7], &c.layout) || !amplitude_of(arguments[8], &c.amplitude) || !t[0]->is_cuda()) Py_RETURN_FALSE;
   const Tensor &latent = *t[0], &rope = *t[1], &cache = *t[2], &inv_freq = *t[6];
   const c10::DeviceIndex device = c10::cuda::current_device();
   const at::ScalarType type = latent.scalar_type();

@@ -4,6 +4,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <float.h>
 #include <stdint.h>
 
 #include "../../include/latent.h"
@@ -55,6 +56,9 @@ __device__ __forceinline__ int request_of(const int32_t* cu, int batches, int to
   return lo;
 }
 
+// Finite in FP32, which the kernels work in.
+inline bool fits_float(double value) { return value >= -FLT_MAX && value <= FLT_MAX; }
+inline bool scale_fits(double value) { return value >= 1e-30 && value <= 1e30; }
 inline bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 inline int multiprocessors() {

@@ -721,7 +721,7 @@ extern "C" int launch_latent_prefill(void* stream, const latent_prefill_call* ca
   using namespace latent;
   if (call == nullptr) return -1;
   const latent_prefill_call& c = *call;
-  if ((c.type != LATENT_F16 && c.type != LATENT_BF16) || !(c.scale > 0) || c.status == nullptr) return -1;
+  if ((c.type != LATENT_F16 && c.type != LATENT_BF16) || !scale_fits(c.scale) || c.status == nullptr) return -1;
   if (c.batches < 0 || c.batches >= INT32_MAX || c.tokens < 0 || c.tokens > INT32_MAX - 256 || c.keys < 0 || c.keys > INT32_MAX - 256 || c.heads < 1 || c.heads > 65535) return -1;
   int64_t blocks = (c.tokens / 256 + c.batches) * c.heads;  // at least as many as there are items
   if (blocks > INT32_MAX) return -1;

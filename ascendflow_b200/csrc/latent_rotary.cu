@@ -166,7 +166,7 @@ int launch_latent_rotary(void* stream, const latent_rotary_call* call) {
   if (c.tokens < 0 || c.tokens > INT32_MAX || c.heads < 0 || c.heads > 65536 || c.features > 65536) return -1;
   for (const int64_t stride : {c.x_token, c.x_head, c.out_token, c.out_head})
     if (stride * size % 16 != 0) return -1;
-  if (!aligned(c.x) || !aligned(c.out)) return -1;
+  if (!aligned(c.x) || !aligned(c.out) || !fits_float(c.amplitude)) return -1;
   if (c.tokens == 0 || c.heads == 0) return 0;
   RotaryParams p = {c, 1, int(c.layout ? c.pairs / 8 : c.pairs / 4), 0};
   p.units = p.rotated_units + (c.x == c.out ? 0 : int(c.features - 2 * c.pairs) / 8);
@@ -185,7 +185,7 @@ int launch_latent_append(void* stream, const latent_append_call* call) {
   const latent_append_call& c = *call;
   if ((c.type != LATENT_F16 && c.type != LATENT_BF16) || !pairs_fit(c.pairs) || c.width < 2 * c.pairs || c.width % 8 != 0 || c.width > 65536) return -1;
   if (c.batches < 0 || c.batches >= INT32_MAX || c.tokens < 0 || c.tokens > INT32_MAX || c.pages < 0 || c.blocks < 0 || c.page_rows < 1) return -1;
-  if (!aligned(c.latent) || c.latent_token % 8 != 0 || !aligned(c.cache) || c.status == nullptr) return -1;
+  if (!aligned(c.latent) || c.latent_token % 8 != 0 || !aligned(c.cache) || !fits_float(c.amplitude) || c.status == nullptr) return -1;
   if (c.tokens == 0 || c.batches == 0) return 0;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   return c.type == LATENT_BF16 ? launch_append<__nv_bfloat16>(c, s) : launch_append<__half>(c, s);

@@ -16,7 +16,6 @@ from __future__ import annotations
 
 import math
 import numbers
-import sys
 
 import torch
 
@@ -24,6 +23,7 @@ from . import host
 from .diagnostics import ErrorKind, require
 
 VALUES, NOPE, ROPE, MOST_PAIRS, MOST_ROWS = 512, 128, 64, 128, 1 << 30
+MOST_FLOAT = torch.finfo(torch.float32).max
 _HALVES = {"interleaved": False, "half": True}
 _STORED = (torch.bfloat16, torch.float16)
 
@@ -180,7 +180,7 @@ def _disjoint(written, others):
             require(begin == end or first == last or end <= first or last <= begin, "tensors that are written must not overlap others")
 
 
-def _number(value, name, least=-sys.float_info.max, most=sys.float_info.max):
+def _number(value, name, least, most):
     require(isinstance(value, numbers.Real) and least <= value <= most, f"{name}: expected a finite number from {least:g} to {most:g}")
 
 
@@ -191,7 +191,7 @@ def _check_frequencies(inv_freq):
 
 
 def _check_rotary(x, positions, inv_freq, halves, inverse, amplitude, out):
-    _number(amplitude, "amplitude")
+    _number(amplitude, "amplitude", -MOST_FLOAT, MOST_FLOAT)
     require(isinstance(inverse, bool), "inverse: expected True or False")
     for tensor, name in ((x, "x"), (out, "out")):
         _tensor(tensor, name, (*_STORED, torch.float32))
@@ -224,7 +224,7 @@ def _check_paged(cache, block_table, cu_seqlens_q, seqused_kv, dtype):
 
 
 def _check_append(latent, rope, cache, block_table, cu_seqlens_q, seqused_kv, inv_freq, halves, amplitude):
-    _number(amplitude, "amplitude")
+    _number(amplitude, "amplitude", -MOST_FLOAT, MOST_FLOAT)
     for tensor, name in ((latent, "latent"), (rope, "rope")):
         _tensor(tensor, name, _STORED)
         require(tensor.dim() == 2, f"{name}: expected [T, features]")

@@ -34,7 +34,7 @@ extern "C" {
 #define LATENT_MOST_PAIRS 128
 
 /* out[t, h] = x[t, h] with its last 2 `pairs` features turned by positions[t] * inv_freq[i] radians and
- * multiplied by `amplitude`. layout 0: pair i is features (2 i, 2 i + 1) of the turned part; 1: (i, i + pairs).
+ * multiplied by `amplitude` (finite in FP32). layout 0: pair i is features (2 i, 2 i + 1) of the turned part; 1: (i, i + pairs).
  * inverse: turned back. The features in front are copied, unless out is x. x and out are the same memory with the same
  * strides, or disjoint. Base addresses and strides are multiples of 16 bytes, `features` a multiple of 8,
  * `pairs` a multiple of 8 up to LATENT_MOST_PAIRS. positions: int32, or int64 with `positions64`; any value. */
@@ -68,7 +68,7 @@ typedef struct {
 int launch_latent_append(void* stream, const latent_append_call* call);
 
 /* Causal attention of every request's tokens over its cached rows, keys and values in one: key k of token j of n is
- * seen if k < seqused_kv[b] - n + j + 1; scores scale * q . row over all `width` (512 or 576) features, values are the
+ * seen if k < seqused_kv[b] - n + j + 1; scores scale (1e-30 to 1e30) * q . row over all `width` (512 or 576) features, values are the
  * row's first 512. sinks (or NULL): a logit per head in the denominator. lse (or NULL): the natural
  * logarithm of the denominator. A token that sees no key gets zeros. page_rows: a multiple of 64.
  * Rows behind a request's length are never multiplied; rows within it have to be finite. Addresses of q, cache and out are
@@ -92,7 +92,7 @@ int launch_latent_attention(void* stream, const latent_attention_call* call);
 
 /* Attention in expanded form: keys are [k | k_rope], 128 features per head and 64 shared by all heads; values 128
  * per head. Request b owns keys cu_seqlens_k[b] .. ; causal: token j of n sees the first K - n + j + 1 of its K keys,
- * otherwise all. Strides are multiples of 8, addresses of q, k, v, k_rope and out of 16 bytes. */
+ * otherwise all. scale: as above. Strides are multiples of 8, addresses of q, k, v, k_rope and out of 16 bytes. */
 typedef struct {
   int32_t type, causal;
   const void *q, *k, *v, *k_rope; /* [T, heads, 192], [S, heads, 128], [S, heads, 128], [S, 64] */

@@ -53,7 +53,7 @@ def test_numbers_are_taken_or_refused_alike_by_all_calls():
             for number in (np.float32(0.5), np.float64(0.5), np.float16(0.5)):
                 assert torch.equal(call(number), expected)
             assert torch.equal(call(1), call(np.int64(1)))
-            for wrong in (torch.tensor(0.5), torch.tensor(0.5, device="cuda"), np.array(0.5), "0.5", None, 10 ** 400, float("nan"), float("inf")):
+            for wrong in (torch.tensor(0.5), torch.tensor(0.5, device="cuda"), np.array(0.5), "0.5", None, 10 ** 400, float("nan"), float("inf"), 1e39):
                 with pytest.raises(CompileError, match=name):
                     call(wrong)
 

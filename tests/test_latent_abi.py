@@ -41,3 +41,26 @@ def test_addresses_and_strides(name, pointers, strides):
         assert launch(None, ctypes.byref(call)) == -1, field
         setattr(call, field, right)
     assert launch(None, ctypes.byref(call)) == 0
+
+
+Rotary = structure(["type", "layout", "inverse", "positions64"], ["x", "out", "positions", "inv_freq"], ["x_token", "x_head", "out_token", "out_head", "tokens", "heads", "features", "pairs"])
+
+
+def test_amplitudes():
+    """Finite in FP32 (the field behind the whole numbers)."""
+    library, append = ctypes.CDLL(str(library_path())), CALLS["launch_latent_append"]
+    rotary = Rotary(type=1, x=64, out=64, x_token=64, x_head=64, out_token=64, out_head=64, tokens=0, heads=1, features=64, pairs=32)
+    for amplitude, expected in ((1.0, 0), (-3.4e38, 0), (0.0, 0), (3.5e38, -1), (-1e39, -1), (float("inf"), -1), (float("nan"), -1)):
+        rotary.scale = append.scale = amplitude
+        assert library.launch_latent_rotary(None, ctypes.byref(rotary)) == expected, amplitude
+        assert library.launch_latent_append(None, ctypes.byref(append)) == expected, amplitude
+    append.scale = 1.0
+
+
+@pytest.mark.parametrize("name", ["launch_latent_attention", "launch_latent_prefill"])
+def test_scales(name):
+    launch, call = getattr(ctypes.CDLL(str(library_path())), name), CALLS[name]
+    for scale, expected in ((1.0, 0), (1e-30, 0), (1e30, 0), (0.0, -1), (-1.0, -1), (1e-40, -1), (1e39, -1), (float("inf"), -1), (float("nan"), -1)):
+        call.scale = scale
+        assert launch(None, ctypes.byref(call)) == expected, scale
+    call.scale = 1.0
