@@ -8,6 +8,7 @@
 #include <ATen/ops/empty.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/VariableTypeUtils.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
@@ -123,8 +124,13 @@ void used_on(const c10::cuda::CUDAStream& stream, std::initializer_list<const Te
     if (t != nullptr) c10::cuda::CUDACachingAllocator::recordStream(t->storage().data_ptr(), stream);
 }
 
-PyObject* finished(int status) {
-  if (status == 0) Py_RETURN_TRUE;
+// Behind the launch. What was written in place counts its version up, as for any in-place operation (a tensor made in inference mode has none).
+PyObject* finished(int status, std::initializer_list<const Tensor*> written) {
+  if (status == 0) {
+    for (const Tensor* t : written)
+      if (t != nullptr && !t->is_inference()) torch::autograd::increment_version(*t);
+    Py_RETURN_TRUE;
+  }
   PyErr_Format(PyExc_RuntimeError, "kernel launch failed with status %d; device retries are disabled", status);
   return nullptr;
 }
@@ -169,7 +175,7 @@ PyObject* call_rotary(PyObject*, PyObject* const* arguments, Py_ssize_t count) {
     used_on(stream, {x, positions, inv_freq, out});
     status = launch_rotary(stream.stream(), &c);
   }
-  return finished(status);
+  return finished(status, {out});
   END_HANDLE_TH_ERRORS
 }
 
@@ -234,7 +240,7 @@ PyObject* call_append(PyObject*, PyObject* const* arguments, Py_ssize_t count) {
     c.status = static_cast<int32_t*>(block);
     if (status == 0) status = launch_append(stream.stream(), &c);
   }
-  return finished(status);
+  return finished(status, {&cache});
   END_HANDLE_TH_ERRORS
 }
 
@@ -296,7 +302,7 @@ PyObject* call_attention(PyObject*, PyObject* const* arguments, Py_ssize_t count
     c.status = static_cast<int32_t*>(block);
     if (status == 0) status = launch_attention(stream.stream(), &c);
   }
-  return finished(status);
+  return finished(status, {out, lse});
   END_HANDLE_TH_ERRORS
 }
 
@@ -367,7 +373,7 @@ PyObject* call_prefill(PyObject*, PyObject* const* arguments, Py_ssize_t count) 
     c.status = static_cast<int32_t*>(block);
     if (status == 0) status = launch_prefill(stream.stream(), &c);
   }
-  return finished(status);
+  return finished(status, {out, lse});
   END_HANDLE_TH_ERRORS
 }
 

@@ -78,3 +78,40 @@ for _ in range(2):
 """.replace("NUMBER", name)
     result = subprocess.run([sys.executable, "-c", program], cwd=Path(__file__).resolve().parents[1], capture_output=True, text=True, timeout=120)
     assert result.stdout.split() == ["taken" if "np" in name else "CompileError"] * 2, result.stderr[-2000:]
+
+
+def written_by(name, target):
+    """A call that writes `target`."""
+    if name == "rotary":
+        return lambda: latent.rotary(target, i32([1, 2, 3, 4]), latent.rotary_frequencies(64), out=target)
+    cache, table, cu, seq = normal(4, 1, 64, 1, 576), i32([[0]]), i32([0, 4]), i32([20])
+    if name == "append":
+        return lambda: latent.rotary_append(normal(1, 4, 512), normal(2, 4, 64), target, table, cu, seq, latent.rotary_frequencies(64))
+    if name.startswith("attention"):
+        q = normal(3, 4, 2, 576)
+        return lambda: latent.latent_attention(q, cache, table, cu, seq, scale=0.1, **{name.split()[1]: target})
+    q, kv = normal(3, 4, 2, 192), normal(5, 4, 2, 256)
+    return lambda: latent.latent_prefill(q, kv[..., :128], kv[..., 128:], q[:, 0, 128:], cu, cu, scale=0.1, **{name.split()[1]: target})
+
+
+TARGETS = [("rotary", (4, 2, 64), BF16), ("append", (1, 64, 1, 576), BF16), ("attention out", (4, 2, 512), BF16), ("attention lse", (4, 2), torch.float32),
+           ("prefill out", (4, 2, 128), BF16), ("prefill lse", (4, 2), torch.float32)]
+
+
+@pytest.mark.parametrize("name,shape,dtype", TARGETS)
+def test_writes_count_the_version_up(name, shape, dtype):
+    """So that autograd sees that a tensor which it keeps has changed; tensors made in inference mode have no version."""
+    target = normal(7, *shape, dtype=dtype)
+    call = written_by(name, target)
+    call()
+    before = target._version
+    call()
+    assert target._version == before + 1
+    leaf = normal(8, *shape, dtype=dtype).requires_grad_()
+    product = leaf * target  # keeps target
+    with torch.no_grad():
+        call()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        product.sum().backward()
+    with torch.inference_mode():
+        written_by(name, normal(7, *shape, dtype=dtype))()
