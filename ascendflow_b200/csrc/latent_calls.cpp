@@ -43,7 +43,7 @@ bool optional_of(PyObject* object, const Tensor** tensor) {
 
 bool on_device(const Tensor& t, int device, at::ScalarType type) {
   return t.defined() && t.layout() == at::kStrided && t.is_cuda() && t.device().index() == device && t.scalar_type() == type &&
-         !t.is_conj() && !t.is_neg() && !(t.requires_grad() && at::GradMode::is_enabled());
+         !t.is_conj() && !t.is_neg() && !(t.requires_grad() && at::GradMode::is_enabled()) && !t._fw_grad(0).defined();
 }
 bool shaped(const Tensor& t, std::initializer_list<int64_t> sizes) {
   return t.dim() == int64_t(sizes.size()) && std::equal(sizes.begin(), sizes.end(), t.sizes().begin());

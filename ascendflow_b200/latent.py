@@ -18,6 +18,7 @@ import math
 import numbers
 
 import torch
+from torch.autograd import forward_ad
 
 from . import host
 from .diagnostics import ErrorKind, require
@@ -148,7 +149,8 @@ def _tensor(tensor, name, dtypes, shape=None):
     require(tensor.is_cuda and tensor.layout == torch.strided, f"{name}: expected a CUDA tensor")
     require(tensor.dtype in dtypes, f"{name}: expected {' or '.join(map(str, dtypes))}")
     require(not tensor.is_conj() and not tensor.is_neg(), f"{name}: lazily negated tensors are not supported")
-    require(not (tensor.requires_grad and torch.is_grad_enabled()), f"{name}: the operator has no gradient", kind=ErrorKind.UNSUPPORTED)
+    wanted = tensor.requires_grad and torch.is_grad_enabled() or forward_ad.unpack_dual(tensor).tangent is not None
+    require(not wanted, f"{name}: the operator has no gradient", kind=ErrorKind.UNSUPPORTED)
     require(tensor.device.index == torch.cuda.current_device(), f"{name}: expected a tensor on the current CUDA device")
     if shape is not None:
         require(tuple(tensor.shape) == tuple(shape), f"{name}: expected shape {list(shape)}")

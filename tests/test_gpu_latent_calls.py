@@ -115,3 +115,14 @@ def test_writes_count_the_version_up(name, shape, dtype):
         product.sum().backward()
     with torch.inference_mode():
         written_by(name, normal(7, *shape, dtype=dtype))()
+
+
+@pytest.mark.parametrize("name,shape,dtype", TARGETS)
+def test_tensors_with_a_tangent_are_refused(name, shape, dtype):
+    import torch.autograd.forward_ad as forward
+
+    with forward.dual_level():
+        target = forward.make_dual(normal(7, *shape, dtype=dtype), normal(8, *shape, dtype=dtype))
+        with pytest.raises(CompileError, match="gradient"):
+            written_by(name, target)()
+    written_by(name, normal(7, *shape, dtype=dtype))()
