@@ -166,6 +166,7 @@ PyObject* call_rotary(PyObject*, PyObject* const* arguments, Py_ssize_t count) {
   c.out = memory(*out);
   const bool in_place = c.x == c.out && c.x_token == c.out_token && c.x_head == c.out_head;
   if ((!in_place && !disjoint(*x, *out)) || !disjoint(*positions, *out) || !disjoint(*inv_freq, *out)) Py_RETURN_FALSE;
+  if (x->numel() == 0) Py_RETURN_TRUE;  // (the strides of what has no entries count for nothing)
   c.positions = memory(*positions);
   c.inv_freq = memory_as<double>(*inv_freq);
   int status;
@@ -222,7 +223,7 @@ PyObject* call_append(PyObject*, PyObject* const* arguments, Py_ssize_t count) {
   c.cu_seqlens_q = memory_as<int32_t>(*t[4]);
   c.seqused_kv = memory_as<int32_t>(*t[5]);
   c.inv_freq = memory_as<double>(inv_freq);
-  c.latent_token = stride_of(latent, 0);
+  c.latent_token = latent.size(1) > 0 ? stride_of(latent, 0) : 0;
   c.rope_token = stride_of(rope, 0);
   c.batches = p.batches;
   c.pages = p.pages;

@@ -126,3 +126,17 @@ def test_tensors_with_a_tangent_are_refused(name, shape, dtype):
         with pytest.raises(CompileError, match="gradient"):
             written_by(name, target)()
     written_by(name, normal(7, *shape, dtype=dtype))()
+
+
+def test_calls_of_nothing_with_odd_strides():
+    """What has no entries has no alignment: empty batches out of odd projections, rows that are rope alone."""
+    inv_freq = latent.rotary_frequencies(64)
+    assert latent.rotary(normal(1, 3, 2, 100)[:0, :, 1:65], i32([]), inv_freq).shape == (0, 2, 64)
+    assert latent.rotary(normal(1, 3, 2, 100)[:, :0, 1:65], i32([1, 2, 3]), inv_freq).shape == (3, 0, 64)
+    cache, rope = normal(2, 2, 64, 1, 64), normal(3, 3, 64)
+    for latents in (normal(4, 3, 0), normal(4, 3, 7)[:, 3:3], normal(4, 3, 64)[:, :0]):
+        own = cache.clone()
+        latent.rotary_append(latents, rope, own, i32([[1, 0]]), i32([0, 3]), i32([70]), inv_freq)
+        expected = R.append(latents, rope, cache, i32([[1, 0]]), [3], [70], inv_freq, "interleaved")
+        R.within(own, expected, R.HALF_STEP[BF16] * expected.abs() + 16 * 2.0 ** -24 * 8)
+    latent.rotary_append(normal(4, 3, 519)[:0, 1:513], rope[:0], normal(2, 2, 64, 1, 576), i32([[1, 0]]), i32([0, 0]), i32([70]), inv_freq)
