@@ -170,8 +170,7 @@ int launch_latent_rotary(void* stream, const latent_rotary_call* call) {
   if (c.tokens == 0 || c.heads == 0) return 0;
   RotaryParams p = {c, 1, int(c.layout ? c.pairs / 8 : c.pairs / 4), 0};
   p.units = p.rotated_units + (c.x == c.out ? 0 : int(c.features - 2 * c.pairs) / 8);
-  const int64_t per_token = c.heads * p.units;
-  if (per_token * 32 > INT32_MAX) return -1;
+  const int64_t per_token = c.heads * p.units;  // 2^29 at most
   // All blocks run at once where there are enough tokens; tokens with few units share a block. Angles take 32 KiB at most.
   const int64_t together = kThreads / per_token, resident = int64_t(multiprocessors()) * kBlocks;
   p.tokens_per_block = int(std::min<int64_t>(std::max<int64_t>({1, together, (c.tokens + resident - 1) / resident}), 4096 / c.pairs));

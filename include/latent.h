@@ -36,8 +36,8 @@ extern "C" {
 /* out[t, h] = x[t, h] with its last 2 `pairs` features turned by positions[t] * inv_freq[i] radians and
  * multiplied by `amplitude` (finite in FP32). layout 0: pair i is features (2 i, 2 i + 1) of the turned part; 1: (i, i + pairs).
  * inverse: turned back. The features in front are copied, unless out is x. x and out are the same memory with the same
- * strides, or disjoint. Base addresses and strides are multiples of 16 bytes, `features` a multiple of 8,
- * `pairs` a multiple of 8 up to LATENT_MOST_PAIRS. positions: int32, or int64 with `positions64`; any value. */
+ * strides, or disjoint. Base addresses and strides are multiples of 16 bytes, `features` a multiple of 8 up to 65536,
+ * `heads` up to 65536, `pairs` a multiple of 8 up to LATENT_MOST_PAIRS. positions: int32, or int64 with `positions64`; any value. */
 typedef struct {
   int32_t type, layout, inverse, positions64;
   const void* x;

@@ -140,3 +140,14 @@ def test_calls_of_nothing_with_odd_strides():
         expected = R.append(latents, rope, cache, i32([[1, 0]]), [3], [70], inv_freq, "interleaved")
         R.within(own, expected, R.HALF_STEP[BF16] * expected.abs() + 16 * 2.0 ** -24 * 8)
     latent.rotary_append(normal(4, 3, 519)[:0, 1:513], rope[:0], normal(2, 2, 64, 1, 576), i32([[1, 0]]), i32([0, 0]), i32([70]), inv_freq)
+
+
+def test_rotary_of_the_widest_tokens():
+    """As many heads and features as the call takes: 2^29 features of one token."""
+    x = torch.zeros((1, 65536, 8192), dtype=BF16, device="cuda")
+    x[0, ::4099] = normal(1, 16, 8192)
+    out = latent.rotary(x, i32([12345]), latent.rotary_frequencies(64))
+    some = latent.rotary(x[:, ::4099].contiguous(), i32([12345]), latent.rotary_frequencies(64))
+    assert torch.equal(out[:, ::4099], some)
+    out[0, ::4099] = 0
+    assert not out.any()
