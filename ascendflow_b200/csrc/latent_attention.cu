@@ -176,9 +176,9 @@ struct Request {
 
 __device__ __forceinline__ Request request_at(const Params& p, int b, float density = 0.f) {
   Request r;
-  r.begin = min(max(__ldg(p.cu + b), 0), p.tokens);
-  r.count = max(min(max(__ldg(p.cu + b + 1), 0), p.tokens) - r.begin, 0);
-  r.length = max(__ldg(p.lengths + b), 0);
+  r.begin = min(max(p.cu[b], 0), p.tokens);
+  r.count = max(min(max(p.cu[b + 1], 0), p.tokens) - r.begin, 0);
+  r.length = max(p.lengths[b], 0);
   r.rows = r.count * p.heads;
   r.tiles = (r.rows + kRows - 1) / kRows;
   // (one key behind the table is enough to report a length that does not fit)
@@ -556,7 +556,7 @@ __device__ void copy_role(const Params& p, const Shared& sm) {
     const int32_t* table = p.table + size_t(piece.request) * p.pages;
     auto page_of = [&](int chunk) {  // lane l: the page of chunk `chunk + l`, or -1
       const int column = over(min(chunk + lane, piece.last - 1), p.by_page);
-      return column < p.pages ? __ldg(table + column) : -1;
+      return column < p.pages ? table[column] : -1;
     };
     int pages = 0, next_pages = page_of(piece.first);  // of 32 chunks; of the next 32
     for (int chunk = piece.first; chunk < piece.last; ++chunk, ++count) {
@@ -631,7 +631,7 @@ __device__ void query_role(const Params& p, const Shared& sm, uint32_t tmem) {
       for (int k = 0; k < 2; ++k) {
         const int row = subpartition * 16 + (lane >> 2) + 8 * k;
         words[2 * s + k] = make_uint4(0, 0, 0, 0);
-        if (row < piece.rows) words[2 * s + k] = __ldg(reinterpret_cast<const uint4*>(p.q + (piece.row + row) * (kWidth * 2) + segment * 64 + (lane & 3) * 16));
+        if (row < piece.rows) words[2 * s + k] = *reinterpret_cast<const uint4*>(p.q + (piece.row + row) * (kWidth * 2) + segment * 64 + (lane & 3) * 16);
       }
     }
     if (loads > 0 && !warp_wait(sm.bar(kQFree), (loads - 1) & 1, abort_flag, kLongWait)) return;
@@ -893,7 +893,7 @@ __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
       continue;
     }
     float log_sum;
-    const float sink = p.sinks != nullptr && row < piece.rows ? __ldg(p.sinks + (piece.head + row) % p.heads) * kLog2E : -INFINITY;
+    const float sink = p.sinks != nullptr && row < piece.rows ? p.sinks[(piece.head + row) % p.heads] * kLog2E : -INFINITY;
     const float inverse = inverse_of(reference, sum, sink, &log_sum);
     if (half == 0) {
       inverses[row] = inverse;
@@ -1059,7 +1059,7 @@ __global__ void __launch_bounds__(kCombineThreads, 2) combine_kernel(const __gri
         [&](int row, int owner) { return p.out + ((tile.row + row) * LATENT_VALUES + feature_of(owner)) * 2; },
         [&](int row, float reference, float sum, bool first_of_row) {  // what the row's sums are multiplied with
           float log_sum;
-          const float sink = p.sinks != nullptr ? __ldg(p.sinks + (tile.head + row) % p.heads) * kLog2E : -INFINITY;
+          const float sink = p.sinks != nullptr ? p.sinks[(tile.head + row) % p.heads] * kLog2E : -INFINITY;
           const float inverse = inverse_of(reference, sum, sink, &log_sum);
           if (p.lse != nullptr && first_of_row && segment == 0) p.lse[tile.row + row] = log_sum * kLn2;
           return inverse;

@@ -47,11 +47,11 @@ __device__ __forceinline__ int bounded(int value, int most) { return min(max(val
 
 // The request that owns `token` (binary search; empty requests are skipped), or -1 in front of the first and behind the last.
 __device__ __forceinline__ int request_of(const int32_t* cu, int batches, int token) {
-  if (token < __ldg(cu) || token >= __ldg(cu + batches)) return -1;
+  if (token < *cu || token >= cu[batches]) return -1;
   int lo = 0, hi = batches;  // cu[lo] <= token < cu[hi]
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (__ldg(cu + mid) <= token) lo = mid; else hi = mid;
+    if (cu[mid] <= token) lo = mid; else hi = mid;
   }
   return lo;
 }

@@ -41,7 +41,7 @@ __device__ __forceinline__ void join_parts(Shares& shares, int warps, int parts,
     for (int n = 0; n < kPartsInFlight; ++n)
       if (round + n < count) load_sector(sums_of(first + (round + n) * warps, row), v[n]);
     const int mine = round + (lane >> 3);  // lane l has the statistics of part l / 8 of the round
-    const float2 own = mine < count ? __ldg(statistics_of(first + mine * warps, row)) : make_float2(-INFINITY, 0.f);
+    const float2 own = mine < count ? *statistics_of(first + mine * warps, row) : make_float2(-INFINITY, 0.f);
     float next = fmaxf(reference, own.x);
     next = fmaxf(next, __shfl_xor_sync(0xffffffffu, next, 8));
     next = fmaxf(next, __shfl_xor_sync(0xffffffffu, next, 16));

@@ -48,7 +48,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) rotary_kernel(const RotaryP
   for (int i = threadIdx.x; i < tokens * pairs; i += kThreads) {
     const int64_t token = first + i / pairs;
     const int64_t position = c.positions64 ? static_cast<const int64_t*>(c.positions)[token] : static_cast<const int32_t*>(c.positions)[token];
-    const uint64_t turns = turns_of(__ldg(c.inv_freq + i % pairs));
+    const uint64_t turns = turns_of(c.inv_freq[i % pairs]);
     turn[i] = turn_of(c.inverse ? -position : position, turns, float(c.amplitude));
   }
   __syncthreads();
@@ -113,11 +113,11 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const latent_append_ca
   const int request = request_of(c.cu_seqlens_q, int(c.batches), int(token));
   if (request < 0) return;
   // (the request's tokens as the attention calls see them: offsets outside of the call's tokens are clamped)
-  const int begin = bounded(__ldg(c.cu_seqlens_q + request), int(c.tokens)), count = bounded(__ldg(c.cu_seqlens_q + request + 1), int(c.tokens)) - begin;
-  const int64_t position = int64_t(__ldg(c.seqused_kv + request)) - count + (token - begin);
+  const int begin = bounded(c.cu_seqlens_q[request], int(c.tokens)), count = bounded(c.cu_seqlens_q[request + 1], int(c.tokens)) - begin;
+  const int64_t position = int64_t(c.seqused_kv[request]) - count + (token - begin);
   const int64_t column = position / c.page_rows;
   int64_t page = -1;
-  if (position >= 0 && column < c.pages) page = __ldg(c.block_table + request * c.pages + column);
+  if (position >= 0 && column < c.pages) page = c.block_table[request * c.pages + column];
   if (page < 0 || page >= c.blocks) {  // nowhere to put it: reported, not written
     if (lane == 0) report(c.status, SPARSE_MLA_STATUS_BAD_PAGE, int(token), int(position));
     return;
@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const latent_append_ca
   for (int at = lane * 8; at < front; at += 256) *reinterpret_cast<uint4*>(target + at) = *reinterpret_cast<const uint4*>(latent + at);
   const T* rope = static_cast<const T*>(c.rope) + token * c.rope_token;
   for (int i = lane; i < pairs; i += 32) {
-    const float2 t = turn_of(position, turns_of(__ldg(c.inv_freq + i)), float(c.amplitude));
+    const float2 t = turn_of(position, turns_of(c.inv_freq[i]), float(c.amplitude));
     const int low = kHalves ? i : 2 * i, high = kHalves ? i + pairs : 2 * i + 1;
     const float u = to_float(rope[low]), v = to_float(rope[high]);
     target[front + low] = from_float<T>(u * t.x - v * t.y);
