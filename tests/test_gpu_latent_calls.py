@@ -151,3 +151,40 @@ def test_rotary_of_the_widest_tokens():
     assert torch.equal(out[:, ::4099], some)
     out[0, ::4099] = 0
     assert not out.any()
+
+
+def test_calls_of_several_threads_at_once():
+    """Each on a stream of its own; scratch memory and reports are a call's own."""
+    lengths = [3000, 50, 700]
+    cache, table, cu, seq = normal(1, 70, 64, 1, 576), torch.arange(63 * 3, dtype=torch.int32, device="cuda").view(3, 63) % 70, i32([0, 2, 3, 6]), i32(lengths)
+    kv, rope, cu_k = normal(2, 9000, 2, 256), normal(3, 9000, 64), i32([0, 3000, 4000, 9000])
+    queries = [normal(10 + i, 6, 64, 576) for i in range(4)]
+
+    def both(q):
+        out = latent.latent_attention(q, cache, table, cu, seq, scale=0.07)
+        prompt = latent.rotary(q[:, :2, :192], i32([1, 2, 3, 4, 5, 6]), frequencies)
+        return out, latent.latent_prefill(prompt, kv[..., :128], kv[..., 128:], rope, cu, cu_k, scale=0.07)
+
+    frequencies = latent.rotary_frequencies(64)
+    expected = [both(q) for q in queries]
+    torch.cuda.synchronize()
+    found, failed = [[] for _ in queries], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(25):
+                    found[i].append(both(queries[i]))
+                torch.cuda.current_stream().synchronize()
+                assert ops.status()[0] == 0
+        except BaseException as error:  # noqa: BLE001
+            failed.append(error)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(queries))]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    assert not failed, failed
+    for own, (out, prompt) in zip(found, expected):
+        assert len(own) == 25 and all(torch.equal(a, out) and torch.equal(b, prompt) for a, b in own)
