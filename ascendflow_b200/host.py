@@ -13,6 +13,7 @@ a stand-in refuses everything, and `connect()`, on the way of every call with CU
 from __future__ import annotations
 
 import ctypes as ct
+import functools
 import importlib.machinery
 import importlib.util
 import numbers
@@ -57,6 +58,13 @@ class _Unavailable:
 
     latent_append = latent_attention = latent_prefill = rotary
 
+    def set_latent_fallback(self, fallback):
+        self.latent_registration = torch.library.Library("ascendflow_b200", "FRAGMENT")
+        for schema in LATENT_SCHEMAS:
+            name = schema[: schema.index("(")]
+            self.latent_registration.define(schema, tags=(torch.Tag.pt2_compliant_tag,))
+            self.latent_registration.impl(name, functools.partial(fallback, name), "CUDA")
+
     def read_status(self):
         raise RuntimeError("the native host side is not available") from self.error
 
@@ -67,6 +75,15 @@ class _Unavailable:
 SCHEMA = ("sparse_mla(Tensor q, Tensor ori_kv, Tensor cmp_kv, Tensor cmp_sparse_indices, Tensor ori_block_table, "
           "Tensor cmp_block_table, Tensor cu_seqlens_q, Tensor seqused_ori_kv, Tensor seqused_cmp_kv, "
           "Tensor cmp_residual_kv, Tensor ori_topk_length, Tensor sinks, Tensor(a12!) attention_out) -> ()")
+LATENT_SCHEMAS = (
+    "rotary(Tensor x, Tensor positions, Tensor inv_freq, bool halves, bool inverse, float amplitude, Tensor(a!) out) -> ()",
+    "latent_append(Tensor latent, Tensor rope, Tensor(a!) cache, Tensor block_table, Tensor cu_seqlens_q, Tensor seqused_kv, Tensor inv_freq, bool halves, "
+    "float amplitude) -> ()",
+    "latent_attention(Tensor q, Tensor cache, Tensor block_table, Tensor cu_seqlens_q, Tensor seqused_kv, float scale, Tensor? sinks, Tensor(a!) out, "
+    "Tensor(b!)? lse) -> ()",
+    "latent_prefill(Tensor q, Tensor k, Tensor v, Tensor k_rope, Tensor cu_seqlens_q, Tensor cu_seqlens_k, float scale, bool causal, Tensor(a!) out, "
+    "Tensor(b!)? lse) -> ()",
+)
 
 try:
     calls = _load()

@@ -10,6 +10,9 @@ All launch on torch's current stream and never wait. They have no gradient and r
 launch has to report (a block-table entry outside of the cache) is read with `ops.status()`, as for `ops.sparse_mla`.
 A call normally stays in native code (`csrc/latent_calls.cpp`); what that refuses, and the first call of a process, comes
 back here, where the violated rule is put into words. Nothing is ever cast, copied or padded implicitly.
+
+While a graph is traced (`torch.compile`, `torch.export`, fake tensors) the functions call the registered ops of the same work,
+`torch.ops.ascendflow_b200.rotary` and so on, which write outputs that are given.
 """
 
 from __future__ import annotations
@@ -82,8 +85,8 @@ def rotary(x, positions, inv_freq, *, layout="interleaved", inverse=False, ampli
         require(isinstance(x, torch.Tensor), "x: expected a Torch tensor")
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     arguments = (x, positions, inv_freq, halves, inverse, amplitude, out)
-    if not host.calls.rotary(*arguments):
-        _again(host.calls.rotary, arguments, _check_rotary)
+    if torch.compiler.is_compiling() or not _rotary(*arguments):
+        _otherwise("rotary", arguments)
     return out
 
 
@@ -98,8 +101,8 @@ def rotary_append(latent, rope, cache, block_table, cu_seqlens_q, seqused_kv, in
     halves = _HALVES.get(layout)
     require(halves is not None, "rotary layout is interleaved or half", kind=ErrorKind.UNSUPPORTED)
     arguments = (latent, rope, cache, block_table, cu_seqlens_q, seqused_kv, inv_freq, halves, amplitude)
-    if not host.calls.latent_append(*arguments):
-        _again(host.calls.latent_append, arguments, _check_append)
+    if torch.compiler.is_compiling() or not _latent_append(*arguments):
+        _otherwise("latent_append", arguments)
     return cache
 
 
@@ -116,8 +119,8 @@ def latent_attention(q, cache, block_table, cu_seqlens_q, seqused_kv, *, scale, 
         require(isinstance(q, torch.Tensor) and q.dim() == 3, "q: expected a [T, H, W] Torch tensor")
         out = torch.empty((*q.shape[:2], VALUES), dtype=q.dtype, device=q.device)
     arguments = (q, cache, block_table, cu_seqlens_q, seqused_kv, scale, sinks, out, lse)
-    if not host.calls.latent_attention(*arguments):
-        _again(host.calls.latent_attention, arguments, _check_attention)
+    if torch.compiler.is_compiling() or not _latent_attention(*arguments):
+        _otherwise("latent_attention", arguments)
     return out
 
 
@@ -132,16 +135,29 @@ def latent_prefill(q, k, v, k_rope, cu_seqlens_q, cu_seqlens_k, *, scale, causal
         require(isinstance(q, torch.Tensor) and q.dim() == 3, "q: expected a [T, H, 192] Torch tensor")
         out = torch.empty((*q.shape[:2], NOPE), dtype=q.dtype, device=q.device)
     arguments = (q, k, v, k_rope, cu_seqlens_q, cu_seqlens_k, scale, causal, out, lse)
-    if not host.calls.latent_prefill(*arguments):
-        _again(host.calls.latent_prefill, arguments, _check_prefill)
+    if torch.compiler.is_compiling() or not _latent_prefill(*arguments):
+        _otherwise("latent_prefill", arguments)
     return out
 
 
-def _again(call, arguments, check):
+def _otherwise(name, arguments):
+    """A call while a graph is traced, which is the registered op's, or one that the native side refused."""
+    if torch.compiler.is_compiling() or any(_traced(argument) for argument in arguments):
+        getattr(torch.ops.ascendflow_b200, name)(*arguments)
+    else:
+        _checked(name, *arguments)
+
+
+def _traced(argument):
+    """A tensor that stands for another or for none, as in tracing."""
+    return isinstance(argument, torch.Tensor) and type(argument).__torch_dispatch__ is not torch.Tensor.__torch_dispatch__
+
+
+def _checked(name, *arguments):
     """A refused call: the rule that it violates, or (the first call of a process) a second attempt with the entry points at hand."""
-    check(*arguments)
+    _CHECKS[name](*arguments)
     host.connect_latent()
-    require(call(*arguments), "call refused by the native host side")
+    require(getattr(host.calls, name)(*arguments), "call refused by the native host side")
 
 
 def _tensor(tensor, name, dtypes, shape=None):
@@ -285,3 +301,12 @@ def _check_prefill(q, k, v, k_rope, cu_seqlens_q, cu_seqlens_k, scale, causal, o
     if lse is not None:
         _tensor(lse, "lse", (torch.float32,), q.shape[:2])
     _check_written(out, lse, (q, k, v, k_rope, cu_seqlens_q, cu_seqlens_k))
+
+
+# `torch.ops.ascendflow_b200.rotary`, `.latent_append`, `.latent_attention` and `.latent_prefill` are registered by the native module when it is loaded: no result,
+# outputs mutated, CUDA only, no gradient. Tracing needs nothing computed.
+_CHECKS = {"rotary": _check_rotary, "latent_append": _check_append, "latent_attention": _check_attention, "latent_prefill": _check_prefill}
+_rotary, _latent_append, _latent_attention, _latent_prefill = (getattr(host.calls, name) for name in _CHECKS)
+host.calls.set_latent_fallback(_checked)
+for _name in _CHECKS:
+    torch.library.register_fake(f"ascendflow_b200::{_name}", lambda *arguments: None)
