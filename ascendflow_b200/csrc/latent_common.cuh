@@ -43,6 +43,12 @@ __device__ __forceinline__ float2 turn_of(int64_t position, uint64_t turns, floa
   return make_float2(cosine * amplitude, sine * amplitude);
 }
 
+// A plain load, spelled out. (As `*at` it let the compiler arrange the expanded call's loop otherwise: 2K queries at 16K keys 314.0 us so, 316.1 with `*at`.)
+__device__ __forceinline__ int fetch(const int32_t* at) {
+  int value;
+  asm volatile("ld.global.s32 %0, [%1];\n" : "=r"(value) : "l"(at));
+  return value;
+}
 __device__ __forceinline__ int bounded(int value, int most) { return min(max(value, 0), most); }
 
 // The request that owns `token` (binary search; empty requests are skipped), or -1 in front of the first and behind the last.

@@ -130,9 +130,9 @@ __device__ __forceinline__ bool find_whole(const Params& p, int index, Item& ite
   const int lane = threadIdx.x & 31;
   int per_head = 0, most_keys = 0;
   for (int b = lane; b < p.batches; b += 32) {
-    const int blocks = (max(bounded(p.cu_q[b + 1], p.tokens) - bounded(p.cu_q[b], p.tokens), 0) + 255) >> 8;
+    const int blocks = (max(bounded(fetch(p.cu_q + b + 1), p.tokens) - bounded(fetch(p.cu_q + b), p.tokens), 0) + 255) >> 8;
     per_head += blocks;
-    if (kPieces && blocks > 0) most_keys = max(most_keys, bounded(p.cu_k[b + 1], p.keys) - bounded(p.cu_k[b], p.keys));
+    if (kPieces && blocks > 0) most_keys = max(most_keys, bounded(fetch(p.cu_k + b + 1), p.keys) - bounded(fetch(p.cu_k + b), p.keys));
   }
   per_head = __reduce_add_sync(0xffffffffu, per_head);
   if (per_head == 0) return false;
@@ -147,8 +147,8 @@ __device__ __forceinline__ bool find_whole(const Params& p, int index, Item& ite
   int left = index - item.head * per_head;
   for (int first = 0;; first += 32) {  // (ends: left < per_head)
     const int b = first + lane;
-    const int begin = b < p.batches ? bounded(p.cu_q[b], p.tokens) : 0;
-    const int count = b < p.batches ? max(bounded(p.cu_q[b + 1], p.tokens) - begin, 0) : 0;
+    const int begin = b < p.batches ? bounded(fetch(p.cu_q + b), p.tokens) : 0;
+    const int count = b < p.batches ? max(bounded(fetch(p.cu_q + b + 1), p.tokens) - begin, 0) : 0;
     const int blocks = (count + 255) >> 8;
     int before = blocks;  // inclusive prefix sum
 #pragma unroll
@@ -162,8 +162,8 @@ __device__ __forceinline__ bool find_whole(const Params& p, int index, Item& ite
       continue;
     }
     const int owner = __ffs(hit) - 1;
-    const int k_begin = b < p.batches ? bounded(p.cu_k[b], p.keys) : 0;
-    const int k_count = b < p.batches ? max(bounded(p.cu_k[b + 1], p.keys) - k_begin, 0) : 0;
+    const int k_begin = b < p.batches ? bounded(fetch(p.cu_k + b), p.keys) : 0;
+    const int k_count = b < p.batches ? max(bounded(fetch(p.cu_k + b + 1), p.keys) - k_begin, 0) : 0;
     const int block = __shfl_sync(0xffffffffu, before - 1 - left, owner);  // from the request's end
     const int request_count = __shfl_sync(0xffffffffu, count, owner), start = block << 8;
     item.row = __shfl_sync(0xffffffffu, begin, owner) + start;
