@@ -39,7 +39,7 @@ def rotary_frequencies(dims, *, base=10000.0, scaling="none", factor=1.0, origin
     "linear"  divided by the factor (positions are interpolated);
     "ntk"     with the base grown so that the slowest pair is divided by the factor and the fastest is left;
     "yarn"    pairs that turn less than `beta_slow` times within `original_length` positions divided by the factor, those that turn
-              more than `beta_fast` times left, a ramp between; `rotary_amplitude(factor)` goes with it.
+              more than `beta_fast` times left, a ramp between; `rotary_amplitude(factor)` goes with it, see there.
 
     What a program keeps: computed once, on the host.
     """
@@ -67,7 +67,11 @@ def rotary_frequencies(dims, *, base=10000.0, scaling="none", factor=1.0, origin
 
 
 def rotary_amplitude(factor, mscale=1.0):
-    """What cosines and sines are multiplied by when "yarn" stretches a context `factor` times."""
+    """The amplitude that goes with "yarn" stretching a context `factor` times: scores are to grow by its square.
+
+    Where a head is turned as a whole, it is the `amplitude` of queries and keys. Where only a part is (64 of 192 or 576 features here) that would leave the
+    other features' scores as they were: the turn's amplitude stays 1, and its square goes into the attention call's `scale`.
+    """
     return 1.0 if factor <= 1 else 0.1 * mscale * math.log(factor) + 1.0
 
 
