@@ -440,11 +440,14 @@ __device__ void product_role(const Params& p, const Shared& sm, uint32_t tmem) {
 
 // ---- softmax ----------------------------------------------------------------------------------------------------------
 
-// A row's reference (log2) starts kStep below the maximum of its first scores. It moves, to kStep below the maximum of a step, where the step's weights
-// sum up to more than kMostWeight. Weights are rounded to the storage type for the second product: up to that sum they fit IEEE half, so that the
-// accumulator is rarely rescaled, and below the greatest they are off by at most 2^-33 of it (latent_attention.cu). (A sum that large has
-// a weight of more than 2^kStep in it, so that the reference does move.)
+// A row's reference (log2) starts kFirst below the maximum of its first scores (latent_attention.cu has the reason). It moves, to kStep below the maximum of a
+// step, where the step's weights sum up to more than kMostWeight: up to that sum weights fit IEEE half, and the accumulator is rarely rescaled. (A sum that
+// large has a weight of more than 2^kStep in it, so that it does move.) The lower the first reference, the sooner it moves, so that with IEEE
+// half all scores of the first step are looked at: 4096 x 4096 tokens of 32 heads, scores of a deviation of 1, 2, 3, 8: 190, 201, 210, 287 us, with the
+// reference at the maximum of the first 32 scores 190, 201, 207, 294, with that less 8 190, 220, 237, 295.
 constexpr float kStep = 8.f, kMostWeight = 61440.f;
+template <int kFormat> constexpr float kFirst = kFormat == 1 ? 0.f : 6.f;
+template <int kFormat> constexpr int kFirstLook = kFormat == 1 ? 1 : 4;  // parts of 32 scores
 static_assert(kTile * 256 <= kMostWeight && kMostWeight < 65504.f, "the smallest sum that is looked into, and the largest weight");
 
 template <int kFormat, bool kPieces>
@@ -471,8 +474,8 @@ __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
       float own;
       // Weights are worked out with the reference as it is, without looking for the maximum: as long as their sum stays below kMostWeight so does
       // each of them. Where it does not (for some row of the warp) the reference may move, and they are worked out again. A row's first reference comes
-      // from the maximum of its first 32 scores.
-      for (int look = step == 0 ? 1 : 0;; look = 4) {  // parts of 32 scores to look at
+      // from the maximum of its first 32 or 128 scores.
+      for (int look = step == 0 ? kFirstLook<kFormat> : 0;; look = 4) {  // parts of 32 scores to look at
         float2 s[2][16];  // 32 scores, and the next 32 on their way
         auto load = [&](int part) { tmem_ld32(s_tmem + part * 32, reinterpret_cast<uint32_t*>(&s[part & 1][0])); };
         auto mask = [&](int part) {
@@ -498,7 +501,7 @@ __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
           const bool moves = top > reference + kStep;
           float alpha = 1.f;
           if (moves) {
-            const float next = top - kStep;
+            const float next = top - (reference == -INFINITY ? kFirst<kFormat> : kStep);
             alpha = exp2f(reference - next);
             reference = next;
           }

@@ -30,14 +30,14 @@ def peaked(dtype, keys, features, gap, seed):
 def check(out, dtype, decides, values, q):
     """Scores are single products, exact in FP32, and one product by the scale's (2^-24 of up to 64 binades; twice, since the reference has one too). Weights
     are rounded to the storage type by half a step or, where they are small, by 2^-25 (half) or 2^-134 (bfloat16) of a unit that
-    is at most 2^-8 of the row's greatest weight; exponentials to 2^-18; FP32 sums are of terms of one sign, 16 keys at a time at least, each addition off by 2^-23
+    is at most 2^-6 of the row's greatest weight (what a first reference leaves); exponentials to 2^-18; FP32 sums are of terms of one sign, 16 keys at a time at least, each addition off by 2^-23
     of the sum, once for the values and once for the denominator; the output by half a step."""
     score = SCALE * q.double() * decides.double()
     weights = torch.exp(score - score.amax())
     total, values = weights.sum(), values.double()
     step, least = R.HALF_STEP[dtype], 2.0 ** -25 if dtype == F16 else 2.0 ** -134
     expected = (weights @ values) / total
-    error = (step + 2.0 ** -16 + 2.0 ** -18 + 2 * len(decides) / 16 * 2.0 ** -23) * (weights @ values.abs()) / total + least * 2.0 ** -8 * values.abs().sum(0) / total
+    error = (step + 2.0 ** -16 + 2.0 ** -18 + 2 * len(decides) / 16 * 2.0 ** -23) * (weights @ values.abs()) / total + least * 2.0 ** -6 * values.abs().sum(0) / total
     error = error + step * (expected.abs() + error) + least
     R.within(out, expected.expand(out.shape), error, "values")
     # What is tested for can be seen: small weights off by a thirtieth, all the same way, lie outside.
