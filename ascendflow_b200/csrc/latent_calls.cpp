@@ -6,6 +6,7 @@
 
 #include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/VariableTypeUtils.h>
@@ -348,9 +349,10 @@ PyObject* finished(int status, std::initializer_list<const Tensor*> written) {
   Py_RETURN_TRUE;
 }
 
-// Plain tensors in the first arguments.
+// Plain tensors in the first arguments, and nobody who wants to see what is called (a dispatch mode, as in tracing; the front end then calls the registered op).
 template <size_t N>
 bool tensors_of(PyObject* const* arguments, std::array<const Tensor*, N>* tensors) {
+  if (c10::impl::TorchDispatchModeTLS::any_modes_set()) return false;
   for (size_t i = 0; i < N; ++i)
     if (((*tensors)[i] = tensor_of(arguments[i])) == nullptr) return false;
   return true;

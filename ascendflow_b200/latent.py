@@ -11,7 +11,7 @@ launch has to report (a block-table entry outside of the cache) is read with `op
 A call normally stays in native code (`csrc/latent_calls.cpp`); what that refuses, and the first call of a process, comes
 back here, where the violated rule is put into words. Nothing is ever cast, copied or padded implicitly.
 
-While a graph is traced (`torch.compile`, `torch.export`, fake tensors) the functions call the registered ops of the same work,
+While a graph is traced (`torch.compile`, `torch.export`, fake tensors, any dispatch mode) the functions call the registered ops of the same work,
 `torch.ops.ascendflow_b200.rotary` and so on, which write outputs that are given.
 """
 
@@ -22,6 +22,7 @@ import numbers
 
 import torch
 from torch.autograd import forward_ad
+from torch.utils._python_dispatch import _get_current_dispatch_mode
 
 from . import host
 from .diagnostics import ErrorKind, require
@@ -145,8 +146,8 @@ def latent_prefill(q, k, v, k_rope, cu_seqlens_q, cu_seqlens_k, *, scale, causal
 
 
 def _otherwise(name, arguments):
-    """A call while a graph is traced, which is the registered op's, or one that the native side refused."""
-    if torch.compiler.is_compiling() or any(_traced(argument) for argument in arguments):
+    """A call while a graph is traced (or a dispatch mode looks on), which is the registered op's, or one that the native side refused."""
+    if torch.compiler.is_compiling() or _get_current_dispatch_mode() is not None or any(_traced(argument) for argument in arguments):
         getattr(torch.ops.ascendflow_b200, name)(*arguments)
     else:
         _checked(name, *arguments)

@@ -53,6 +53,21 @@ def test_a_compiled_step_is_the_eager_one(layer, sinks, backend):
     assert ops.status()[0] == 0
 
 
+def test_dispatch_modes_see_calls_with_tensors_of_memory(layer):
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    layer["sinks"] = None
+    before = layer["cache"].clone()
+    expected = [t.clone() for t in step(layer)]
+    layer["cache"].copy_(before)
+    names = list(layer)
+    graph = make_fx(lambda *values: step(dict(zip(names, values))))(*layer.values())
+    assert sum("ascendflow" in str(node.target) for node in graph.graph.nodes) == 5
+    for _ in range(2):  # what was traced does it again
+        layer["cache"].copy_(before)
+        assert all(torch.equal(a, b) for a, b in zip(graph(*layer.values()), expected))
+
+
 def test_ops_do_what_the_functions_do(layer):
     s, call = layer, torch.ops.ascendflow_b200
     out, lse = torch.empty((5, 16, 512), dtype=BF16, device="cuda"), torch.empty((5, 16), device="cuda")

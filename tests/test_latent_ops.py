@@ -107,6 +107,26 @@ def test_fake_tensors(call):
         assert out.shape == SHAPES[call] and out.dtype == torch.bfloat16
 
 
+@pytest.mark.parametrize("call", CALLS)
+def test_dispatch_modes_see_the_call(call):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    arguments = make(call.split()[0], "meta")[0]
+    graph = make_fx(lambda *tensors: CALLS[call](list(tensors)))(*arguments)
+    assert op(call.split()[0]).default in [node.target for node in graph.graph.nodes]
+    seen = []
+
+    class Look(TorchDispatchMode):
+        def __torch_dispatch__(self, function, types, args=(), kwargs=None):
+            seen.append(function)
+            return function(*args, **(kwargs or {}))
+
+    with Look():
+        CALLS[call](arguments)
+    assert op(call.split()[0]).default in seen
+
+
 @pytest.mark.parametrize("name", NAMES)
 def test_the_stand_in_registers_the_same_schemas(name):
     """What the package defines where the native module cannot be had."""
