@@ -22,10 +22,11 @@ import numbers
 
 import torch
 from torch.autograd import forward_ad
+from torch.compiler import is_compiling
 from torch.utils._python_dispatch import _get_current_dispatch_mode
 
 from . import host
-from .diagnostics import ErrorKind, require
+from .diagnostics import CompileError, ErrorKind, require
 
 VALUES, NOPE, ROPE, MOST_PAIRS, MOST_ROWS = 512, 128, 64, 128, 1 << 30
 MOST_FLOAT = torch.finfo(torch.float32).max
@@ -85,12 +86,13 @@ def rotary(x, positions, inv_freq, *, layout="interleaved", inverse=False, ampli
     positions: int32 or int64, any value; inv_freq: float64, see `rotary_frequencies`.
     """
     halves = _HALVES.get(layout)
-    require(halves is not None, "rotary layout is interleaved or half", kind=ErrorKind.UNSUPPORTED)
+    if halves is None:
+        raise CompileError("rotary layout is interleaved or half", kind=ErrorKind.UNSUPPORTED)
     if out is None:
         require(isinstance(x, torch.Tensor), "x: expected a Torch tensor")
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     arguments = (x, positions, inv_freq, halves, inverse, amplitude, out)
-    if torch.compiler.is_compiling() or not _rotary(*arguments):
+    if is_compiling() or not _rotary(*arguments):
         _otherwise("rotary", arguments)
     return out
 
@@ -104,9 +106,10 @@ def rotary_append(latent, rope, cache, block_table, cu_seqlens_q, seqused_kv, in
     is not written and reported in `ops.status()`. Rows behind the last request are left out.
     """
     halves = _HALVES.get(layout)
-    require(halves is not None, "rotary layout is interleaved or half", kind=ErrorKind.UNSUPPORTED)
+    if halves is None:
+        raise CompileError("rotary layout is interleaved or half", kind=ErrorKind.UNSUPPORTED)
     arguments = (latent, rope, cache, block_table, cu_seqlens_q, seqused_kv, inv_freq, halves, amplitude)
-    if torch.compiler.is_compiling() or not _latent_append(*arguments):
+    if is_compiling() or not _latent_append(*arguments):
         _otherwise("latent_append", arguments)
     return cache
 
@@ -124,7 +127,7 @@ def latent_attention(q, cache, block_table, cu_seqlens_q, seqused_kv, *, scale, 
         require(isinstance(q, torch.Tensor) and q.dim() == 3, "q: expected a [T, H, W] Torch tensor")
         out = torch.empty((*q.shape[:2], VALUES), dtype=q.dtype, device=q.device)
     arguments = (q, cache, block_table, cu_seqlens_q, seqused_kv, scale, sinks, out, lse)
-    if torch.compiler.is_compiling() or not _latent_attention(*arguments):
+    if is_compiling() or not _latent_attention(*arguments):
         _otherwise("latent_attention", arguments)
     return out
 
@@ -140,14 +143,14 @@ def latent_prefill(q, k, v, k_rope, cu_seqlens_q, cu_seqlens_k, *, scale, causal
         require(isinstance(q, torch.Tensor) and q.dim() == 3, "q: expected a [T, H, 192] Torch tensor")
         out = torch.empty((*q.shape[:2], NOPE), dtype=q.dtype, device=q.device)
     arguments = (q, k, v, k_rope, cu_seqlens_q, cu_seqlens_k, scale, causal, out, lse)
-    if torch.compiler.is_compiling() or not _latent_prefill(*arguments):
+    if is_compiling() or not _latent_prefill(*arguments):
         _otherwise("latent_prefill", arguments)
     return out
 
 
 def _otherwise(name, arguments):
     """A call while a graph is traced (or a dispatch mode looks on), which is the registered op's, or one that the native side refused."""
-    if torch.compiler.is_compiling() or _get_current_dispatch_mode() is not None or any(_traced(argument) for argument in arguments):
+    if is_compiling() or _get_current_dispatch_mode() is not None or any(_traced(argument) for argument in arguments):
         getattr(torch.ops.ascendflow_b200, name)(*arguments)
     else:
         _checked(name, *arguments)
