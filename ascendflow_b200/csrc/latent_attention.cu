@@ -22,7 +22,7 @@
 //
 // What bounds it: memory where a request brings one token (64 requests of 64 heads at 32K: 2.42 GB in 380 us in a few calls after a pause, 6.4 TB/s;
 // in a long loop 410-465 us at 1.0 GHz, since reading random data at that rate takes the board's 1000 W by itself: a plain reduction of as
-// many bytes takes 393 us there), products where it brings several (32 requests of six tokens at 16K: 475-490 us, 0.9 PFLOP/s, 1.0 where all
+// many bytes takes 393 us there), products where it brings several (32 requests of six tokens at 16K: 455-490 us, 0.9 PFLOP/s, 1.0 where all
 // requests share their pages). A chunk takes 2.0 k cycles, 1.43 k of them the two products' own; shared memory's ports are busy for
 // two thirds of it. Two tiles of weights (room for them by a ring of its own for the last 64 features), weights without looking for the
 // maximum, and fewer barriers per chunk were each built and slower by 2 to 12 per cent in loops.

@@ -18,7 +18,7 @@
 // What paces it: a tile's chain of scores to weights (about 1.9 k cycles: 128 exponentials per thread at 8 cycles a warp are 1.0 k of them) and products
 // (1.6 k, of which 1.3 k are the tensor core's), 3.8 k per step of both tiles against 2.6 k of products. In a loop of large calls the
 // board's power limit, not the chain, decides: 8192 x 8192 tokens of 64 heads, causal, take 1.13 ms in a few calls after a pause (1.22 PFLOP/s) and
-// 1.20 ms in a long loop (1.14 PFLOP/s, 1.6 GHz), and what shortens the chain gives a third of that there. Before: one block per 256 rows and
+// 1.20 to 1.25 ms in a long loop (1.10 to 1.14 PFLOP/s, 1.6 GHz), and what shortens the chain gives a third of that there. Before: one block per 256 rows and
 // a maximum for every step 1.29 ms; a quarter of the exponentials by a polynomial, weights handed over in halves, and the rows of two heads
 // in a block where a request has no more than 128 were no faster or slowed the large calls down. Registers decide: 160 bytes of spills in the softmax
 // loop make 1.39 ms of it.

@@ -33,7 +33,8 @@ struct RotaryParams {
 // A block takes a few whole tokens: their angles are worked out once for all heads. A thread turns 16 bytes of a head and, where pairs are of
 // halves, the 16 bytes that go with them (or copies eight features of its part in front), of several tokens with their loads in flight
 // together. Bound by memory: 8192 tokens of 64 heads and 64 features (134 MB) take 25.7 us from and to contiguous memory (5.2 TB/s), 30.7 out of
-// a projection of 192 features per head into queries of 576, where every 128 bytes lie apart. (32 bytes per thread and more blocks than run at
+// a projection of 192 features per head into queries of 576, where every 128 bytes lie apart (no sector is read or written twice in either; cold
+// launches of half as many tokens take 14.2 and 15.0). (32 bytes per thread and more blocks than run at
 // once: 27.4 and 31.4.)
 constexpr int kBlocks = 4;  // per SM
 template <typename T, bool kHalves>
