@@ -137,7 +137,8 @@ def latent_prefill(q, k, v, k_rope, cu_seqlens_q, cu_seqlens_k, *, scale, causal
 
     A head's key is `[k | k_rope]`. Request b owns queries `cu_seqlens_q[b]..` and keys `cu_seqlens_k[b]..`; causal: token j of n sees the
     first K - n + j + 1 of its K keys (a chunk behind a context has more keys than queries), otherwise all K. q, k, v and k_rope
-    may be strided (k and v halves of one projection). lse, rows that see nothing and rows behind the last request: as in `latent_attention`.
+    may be strided (k and v halves of one projection). lse, rows that see nothing and rows behind the last request: as in `latent_attention`. Values of a request
+    have to be finite, those of keys that a token does not see yet too (their weights of zero are multiplied); what lies outside of the requests may be anything.
     """
     if out is None:
         require(isinstance(q, torch.Tensor) and q.dim() == 3, "q: expected a [T, H, 192] Torch tensor")

@@ -92,7 +92,8 @@ int launch_latent_attention(void* stream, const latent_attention_call* call);
 
 /* Attention in expanded form: keys are [k | k_rope], 128 features per head and 64 shared by all heads; values 128
  * per head. Request b owns keys cu_seqlens_k[b] .. ; causal: token j of n sees the first K - n + j + 1 of its K keys,
- * otherwise all. scale: as above. Strides are multiples of 8, addresses of q, k, v, k_rope and out of 16 bytes. */
+ * otherwise all. A request's values have to be finite (those of keys that a token does not see are multiplied by zero);
+ * others are never multiplied. scale: as above. Strides are multiples of 8, addresses of q, k, v, k_rope and out of 16 bytes. */
 typedef struct {
   int32_t type, causal;
   const void *q, *k, *v, *k_rope; /* [T, heads, 192], [S, heads, 128], [S, heads, 128], [S, 64] */

@@ -82,6 +82,22 @@ def test_ops_do_what_the_functions_do(layer):
     assert turned._version == version + 1
 
 
+def test_registrations_hold_together(layer):
+    """Schemas (what is mutated and what is not), fake kernels and autograd, as torch checks them."""
+    s, call, f32 = layer, torch.ops.ascendflow_b200, dict(dtype=torch.float32, device="cuda")
+    out = torch.zeros((5, 16, 512), dtype=BF16, device="cuda")
+    prompt = s["projected"], s["kv"][..., :128], s["kv"][..., 128:], s["k_rope"], s["cu"], s["cu_k"], 0.07, True, torch.zeros((5, 16, 128), dtype=BF16, device="cuda")
+    for op, arguments in (
+        (call.rotary, (s["projected"], s["positions"], s["inv_freq"], False, True, 1.0, torch.zeros_like(s["projected"]))),
+        (call.latent_append, (s["rows"], s["rope"], s["cache"], s["table"], s["cu"], s["lengths"], s["inv_freq"], True, 1.0)),
+        (call.latent_attention, (s["absorbed"], s["cache"], s["table"], s["cu"], s["lengths"], 0.07, None, out, None)),
+        (call.latent_attention, (s["absorbed"], s["cache"], s["table"], s["cu"], s["lengths"], 0.07, torch.zeros(16, **f32), out, torch.zeros((5, 16), **f32))),
+        (call.latent_prefill, (*prompt, None)),
+        (call.latent_prefill, (*prompt, torch.zeros((5, 16), **f32))),
+    ):
+        torch.library.opcheck(op.default, arguments, test_utils=("test_schema", "test_autograd_registration", "test_faketensor"))
+
+
 def test_refused_calls_raise_the_front_ends_error(layer):
     s, call = layer, torch.ops.ascendflow_b200
     out = torch.empty((5, 16, 512), dtype=BF16, device="cuda")
