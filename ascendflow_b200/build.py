@@ -18,8 +18,9 @@ from .diagnostics import ErrorKind, require
 PACKAGE = Path(__file__).resolve().parent
 ROOT = PACKAGE.parent
 SOURCES = tuple(PACKAGE / "csrc" / name for name in (
-    "sparse_mla_abi.cu", "sparse_mla_neighbours.cu", "latent_rotary.cu", "latent_attention.cu", "latent_prefill.cu"))
-HEADERS = (ROOT / "include" / "sparse_mla.h", ROOT / "include" / "latent.h")
+    "sparse_mla_abi.cu", "sparse_mla_neighbours.cu", "latent_rotary.cu", "latent_attention.cu", "latent_prefill.cu",
+    "latent_append8.cu", "pages.cu"))
+HEADERS = (ROOT / "include" / "sparse_mla.h", ROOT / "include" / "latent.h", ROOT / "include" / "pages.h")
 LIBRARY = PACKAGE / "lib" / "libsparse_mla_sm100a.so"
 STAMP = LIBRARY.with_suffix(".stamp")
 FLAGS = (
@@ -65,7 +66,7 @@ def build_library(force=False, verbose=False):
     return LIBRARY
 
 
-HOST_SOURCES = (PACKAGE / "csrc" / "host_calls.cpp", PACKAGE / "csrc" / "latent_calls.cpp")
+HOST_SOURCES = tuple(PACKAGE / "csrc" / name for name in ("host_calls.cpp", "latent_calls.cpp", "pages_calls.cpp"))
 HOST_LIBRARY = PACKAGE / "lib" / "_host_calls.so"
 HOST_STAMP = HOST_LIBRARY.with_suffix(".stamp")
 
@@ -95,7 +96,7 @@ def _host_identity():
 
     parts = (torch.__version__, torch.__file__, sys.version, *HOST_FLAGS, *HOST_LINKED)
     digest = hashlib.sha256("\n".join(parts).encode())
-    for path in (*HOST_SOURCES, PACKAGE / "csrc" / "host_calls.h", *HEADERS):
+    for path in (*HOST_SOURCES, PACKAGE / "csrc" / "host_calls.h", PACKAGE / "csrc" / "call_checks.h", *HEADERS):
         digest.update(path.read_bytes())
     return digest.hexdigest()
 

@@ -500,6 +500,7 @@ cudaError_t ascendflow_host::status_block(const c10::cuda::CUDAStream& stream, a
 
 PyMODINIT_FUNC PyInit__host_calls() {
   PyObject* created = PyModule_Create(&module);
-  if (created != nullptr && PyModule_AddFunctions(created, ascendflow_host::latent_methods) != 0) Py_CLEAR(created);
+  for (PyMethodDef* methods : {ascendflow_host::latent_methods, ascendflow_host::pages_methods})
+    if (created != nullptr && PyModule_AddFunctions(created, methods) != 0) Py_CLEAR(created);
   return created;
 }

@@ -14,5 +14,7 @@ cudaError_t status_block(const c10::cuda::CUDAStream& stream, at::Tensor* kept, 
 
 // The functions of the operators around dense latent attention (latent_calls.cpp).
 extern PyMethodDef latent_methods[];
+// ... and of those on the pages of a cache (pages_calls.cpp).
+extern PyMethodDef pages_methods[];
 
 }  // namespace ascendflow_host

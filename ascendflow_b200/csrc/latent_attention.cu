@@ -130,6 +130,9 @@ struct Params {
   Divisor by_heads, by_page;  // a page's chunks
   int32_t tile_tokens;        // that a tile's rows belong to, at most
   float scale_log2;
+  const char* held;           // rows in 8 bits, and their scales
+  const uint8_t* scales;
+  int32_t block_shift;        // 2^this rows share a scale
 };
 
 struct Shared {
@@ -937,11 +940,21 @@ __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
   meet(false);  // with a warp that has given up since the last time
 }
 
+}  // namespace absorbed
+}  // namespace latent
+
+#include "latent_held8.cuh"
+
+namespace latent {
+namespace absorbed {
+
 // ---- kernels and launch ------------------------------------------------------------------------------------------------
 
-template <int kFormat, int kWidth>
-__global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_constant__ Params p) {
+// kHeld8: rows in 8 bits; the warps from number 6 on have other roles then, see latent_held8.cuh.
+template <int kFormat, int kWidth, bool kHeld8>
+__global__ void __launch_bounds__(kHeld8 ? kThreads8 : kThreads, 1) attention_kernel(const __grid_constant__ Params p) {
   using L = Layout<kWidth>;
+  constexpr int kOwnThreads = kHeld8 ? kThreads8 : kThreads, kOwnQueryWarps = kHeld8 ? kQueryWarps8 : kQueryWarps;
   extern __shared__ unsigned char smem_raw[];
   Shared sm;
   const uint32_t raw = smem_u32(smem_raw), pad = (1024u - (raw & 1023u)) & 1023u;
@@ -954,8 +967,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
   if (threadIdx.x == 0) {
     for (int i = 0; i < kBarCount; ++i) {
       int arrivals = 1;
-      if (i >= kPieceDone0 && i < kPieceDone0 + kPieces) arrivals = kSoftmaxWarps + 3 + kQueryWarps;
-      else if (i == kQFull) arrivals = kQueryWarps;
+      if (i >= kPieceDone0 && i < kPieceDone0 + kPieces) arrivals = kSoftmaxWarps + 2 + (kHeld8 ? kConvertWarps : 1) + kOwnQueryWarps;
+      else if (i == kQFull) arrivals = kOwnQueryWarps;
+      else if (kHeld8 && i < kFull0 + kStages) arrivals = kConvertWarps;
       else if (i == kScoresFree || i == kWeightsFull || i == kPlaces) arrivals = kSoftmaxWarps;
       mbar_init(sm.bar(i), arrivals);
     }
@@ -972,10 +986,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
   Place place = {};
   Borders borders = {};
   if (p.batches > 32) {
-    borders = plan_block<kThreads / 32>(p, sm.scan(), &place);
+    borders = plan_block<kOwnThreads / 32>(p, sm.scan(), &place);
     fence_proxy_async();  // the plan's scratch is the first tile's memory
     __syncthreads();
   }
+  if constexpr (kHeld8) share_registers(warp);
   if (warp < kSoftmaxWarps) softmax_role<kFormat, kWidth>(p, sm, tmem);
   else if (warp == kScoreWarp || warp == kValueWarp) {
     if (elect_one()) {
@@ -985,11 +1000,15 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     }
     __syncwarp();
   }
-  else if (warp == kCopyWarp) copy_role<kWidth>(p, sm);
   else if (warp == kPlanWarp) {
     if (p.batches <= 32) borders = plan_block<1>(p, nullptr, &place);
     plan_role(p, sm, borders, place);
   }
+  else if constexpr (kHeld8) {
+    if (warp >= kConvertWarp0) convert_role<kFormat, kWidth>(p, sm);
+    else if (warp >= kQueryWarp0) query_role8<kWidth>(p, sm, tmem);
+  }
+  else if (warp == kCopyWarp) copy_role<kWidth>(p, sm);
   else query_role<kWidth>(p, sm, tmem);
   tc_fence_before_sync();
   __syncthreads();
@@ -1073,7 +1092,7 @@ __global__ void __launch_bounds__(kCombineThreads, 2) combine_kernel(const __gri
 // One block per SM; no more than `combine_kernel` has room for.
 int grid() { const int count = multiprocessors(); return count < kMostBlocks ? count : kMostBlocks - 1; }
 
-template <int kFormat, int kWidth>
+template <int kFormat, int kWidth, bool kHeld8>
 int launch(const Params& p, int blocks, cudaStream_t stream) {
   using L = Layout<kWidth>;
   static bool configured[64] = {false};  // a per-device setting: plain words written with the same value by whoever gets there first
@@ -1081,10 +1100,10 @@ int launch(const Params& p, int blocks, cudaStream_t stream) {
   if (const cudaError_t error = cudaGetDevice(&device)) return int(error);
   if (device < 0 || device >= 64) return -1;
   if (!configured[device]) {
-    if (const cudaError_t error = cudaFuncSetAttribute(attention_kernel<kFormat, kWidth>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmemBytes)) return int(error);
+    if (const cudaError_t error = cudaFuncSetAttribute(attention_kernel<kFormat, kWidth, kHeld8>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmemBytes)) return int(error);
     configured[device] = true;
   }
-  if (const cudaError_t error = launch_overlapped(attention_kernel<kFormat, kWidth>, blocks, kThreads, L::kSmemBytes, stream, p)) return int(error);
+  if (const cudaError_t error = launch_overlapped(attention_kernel<kFormat, kWidth, kHeld8>, blocks, kHeld8 ? kThreads8 : kThreads, L::kSmemBytes, stream, p)) return int(error);
   cudaLaunchAttribute overlap = {};
   overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   overlap.val.programmaticStreamSerializationAllowed = 1;
@@ -1109,21 +1128,32 @@ int workspace_size_latent_attention(uint64_t* bytes) {
   return 0;
 }
 
-int launch_latent_attention(void* stream, const latent_attention_call* call) {
-  using namespace latent;
-  if (call == nullptr) return -1;
-  const latent_attention_call& c = *call;
+}  // extern "C"
+
+namespace latent {
+namespace absorbed {
+namespace {
+
+template <bool kHeld8>
+int launch_call(void* stream, const latent_attention_call& c, const uint8_t* scales, int64_t block_rows) {
   if ((c.type != LATENT_F16 && c.type != LATENT_BF16) || (c.width != 512 && c.width != 576) || !scale_fits(c.scale)) return -1;
   if (c.batches < 0 || c.batches > INT32_MAX / 2 || c.tokens < 0 || c.heads < 1 || c.tokens > (int64_t(1) << 30) / c.heads) return -1;
   if (c.pages < 0 || c.blocks < 0 || c.page_rows < 64 || c.page_rows % 64 != 0 || c.pages > (INT32_MAX - 128) / c.page_rows || c.blocks > INT32_MAX / c.page_rows) return -1;
   if (!aligned(c.q) || !aligned(c.cache) || !aligned(c.out)) return -1;
+  if (kHeld8 && (block_rows < 1 || block_rows > 64 || (block_rows & (block_rows - 1)) != 0)) return -1;
   if (c.tokens == 0 || c.batches == 0) return 0;
   if (c.workspace == nullptr || reinterpret_cast<uintptr_t>(c.workspace) % 32 != 0 || c.status == nullptr) return -1;
-  const int blocks = absorbed::grid();
-  absorbed::Params p = {};
-  // (without pages nothing is copied)
-  const int64_t sizes[2] = {c.width, c.blocks > 0 ? c.blocks * c.page_rows : 1}, strides[1] = {c.width};
-  if (const int e = sm100::encode_map(&p.cache, c.type, 2, c.blocks > 0 ? c.cache : c.q, sizes, strides, 1, absorbed::kChunk)) return e;
+  const int blocks = grid();
+  Params p = {};
+  if constexpr (kHeld8) {
+    p.held = static_cast<const char*>(c.cache);
+    p.scales = scales;
+    while ((int64_t(1) << p.block_shift) < block_rows) ++p.block_shift;
+  } else {
+    // (without pages nothing is copied)
+    const int64_t sizes[2] = {c.width, c.blocks > 0 ? c.blocks * c.page_rows : 1}, strides[1] = {c.width};
+    if (const int e = sm100::encode_map(&p.cache, c.type, 2, c.blocks > 0 ? c.cache : c.q, sizes, strides, 1, kChunk)) return e;
+  }
   char* workspace = static_cast<char*>(c.workspace);
   p.q = static_cast<const char*>(c.q);
   p.table = c.block_table;
@@ -1132,23 +1162,35 @@ int launch_latent_attention(void* stream, const latent_attention_call* call) {
   p.sinks = c.sinks;
   p.out = static_cast<char*>(c.out);
   p.lse = c.lse;
-  p.records = reinterpret_cast<absorbed::Record*>(workspace);
-  p.statistics = reinterpret_cast<float2*>(workspace + absorbed::statistics_offset(blocks));
-  p.sums = reinterpret_cast<float*>(workspace + absorbed::sums_offset(blocks));
+  p.records = reinterpret_cast<Record*>(workspace);
+  p.statistics = reinterpret_cast<float2*>(workspace + statistics_offset(blocks));
+  p.sums = reinterpret_cast<float*>(workspace + sums_offset(blocks));
   p.status = c.status;
   p.batches = int32_t(c.batches);
   p.tokens = int32_t(c.tokens);
   p.heads = int32_t(c.heads);
-  p.by_heads = absorbed::divisor_of(p.heads);
-  p.tile_tokens = absorbed::kRows / p.heads + 1;
+  p.by_heads = divisor_of(p.heads);
+  p.tile_tokens = kRows / p.heads + 1;
   p.pages = int32_t(c.pages);
   p.blocks = int32_t(c.blocks);
   p.page_rows = int32_t(c.page_rows);
-  p.by_page = absorbed::divisor_of(p.page_rows / absorbed::kChunk);
+  p.by_page = divisor_of(p.page_rows / kChunk);
   p.scale_log2 = float(c.scale * 1.4426950408889634);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (c.type == LATENT_BF16) return c.width == 576 ? absorbed::launch<1, 576>(p, blocks, s) : absorbed::launch<1, 512>(p, blocks, s);
-  return c.width == 576 ? absorbed::launch<0, 576>(p, blocks, s) : absorbed::launch<0, 512>(p, blocks, s);
+  if (c.type == LATENT_BF16) return c.width == 576 ? launch<1, 576, kHeld8>(p, blocks, s) : launch<1, 512, kHeld8>(p, blocks, s);
+  return c.width == 576 ? launch<0, 576, kHeld8>(p, blocks, s) : launch<0, 512, kHeld8>(p, blocks, s);
+}
+
+}  // namespace
+}  // namespace absorbed
+}  // namespace latent
+
+extern "C" {
+
+int launch_latent_attention(void* stream, const latent_attention_call* call) { return call == nullptr ? -1 : latent::absorbed::launch_call<false>(stream, *call, nullptr, 0); }
+
+int launch_latent_attention8(void* stream, const latent_attention8_call* call) {
+  return call == nullptr ? -1 : latent::absorbed::launch_call<true>(stream, call->attention, call->scales, call->block_rows);
 }
 
 }  // extern "C"

@@ -1,0 +1,603 @@
+// The pages of a cache: who has which, on the device and without waiting (a step that grows requests may be captured in a graph).
+//
+// All three operators rank things in a fixed order: free pages by number, wishes by request and entry. One cluster of eight blocks does that: a
+// block marks the pages of its eighth as bits in shared memory, the blocks exchange their sums, and each knows what is in front of it; the cluster's barrier costs a
+// fraction of a microsecond where another launch costs two. Pages are copied by a second kernel on all SMs.
+//
+// Bound by latency (chains of loads and four to six barriers) for tables up to a megabyte, by what eight SMs read above that.
+#include <cuda_runtime.h>
+#include <limits.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "../../include/pages.h"
+#include "../../include/sparse_mla.h"
+#include "latent_common.cuh"
+
+namespace pages {
+namespace {
+
+using namespace sm100;
+using latent::report;
+
+constexpr int kCluster = 8, kThreads = 1024, kWarps = kThreads / 32;
+
+struct Plan {
+  pages_call c;
+  const int32_t* parents;
+  int32_t* places;
+  int32_t children;
+  int32_t *numbers;            // free pages in order; compact: the pages that are moved
+  int32_t *first, *heirs;      // resize: wishes of a request, first entry that wishes; fork: a request's first child, its number of children
+  int4* copies;                // source, target, rows
+  int32_t* copy_count;
+  int32_t words;               // of 32 pages, per block
+};
+
+struct Shared {
+  int32_t totals[4][kCluster];  // what the blocks tell each other
+  int32_t sums[kWarps];
+  uint32_t marks[1];            // [words]
+};
+
+__device__ __forceinline__ void cluster_barrier() {
+  cluster_arrive();
+  cluster_wait();
+}
+// Tells all blocks of the cluster this block's `value`; read behind the next cluster barrier. One thread for each of them.
+__device__ __forceinline__ void tell(Shared& sm, int which, int rank, int value) {
+  if (threadIdx.x < kCluster) {
+    const uint32_t at = cluster_address(smem_u32(&sm.totals[which][rank]), threadIdx.x);
+    asm volatile("st.shared::cluster.u32 [%0], %1;\n" ::"r"(at), "r"(value) : "memory");
+  }
+}
+__device__ __forceinline__ int in_front(const Shared& sm, int which, int rank) {
+  int sum = 0;
+#pragma unroll
+  for (int r = 0; r < kCluster; ++r) sum += r < rank ? sm.totals[which][r] : 0;
+  return sum;
+}
+__device__ __forceinline__ int in_all(const Shared& sm, int which) { return in_front(sm, which, kCluster); }
+
+// Sum over the block, for all threads.
+__device__ __forceinline__ int block_sum(Shared& sm, int value) {
+  value = __reduce_add_sync(0xffffffffu, value);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) sm.sums[threadIdx.x >> 5] = value;
+  __syncthreads();
+  return __reduce_add_sync(0xffffffffu, sm.sums[threadIdx.x & 31]);
+}
+// Sum over the threads in front; *total over all.
+__device__ __forceinline__ int block_rank(Shared& sm, int value, int* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int inclusive = value;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int other = __shfl_up_sync(0xffffffffu, inclusive, d);
+    if (lane >= d) inclusive += other;
+  }
+  __syncthreads();
+  if (lane == 31) sm.sums[warp] = inclusive;
+  __syncthreads();
+  const int sum = sm.sums[lane];
+  *total = __reduce_add_sync(0xffffffffu, sum);
+  return inclusive - value + __reduce_add_sync(0xffffffffu, lane < warp ? sum : 0);
+}
+
+// Marks of this block's pages: bit i of word w for page 32 (rank * words + w) + i. Free pages (kUsed: those in use); their number. Copies the counts where there are two.
+template <bool kUsed>
+__device__ __forceinline__ int mark_pages(const Plan& p, Shared& sm, int rank, const int32_t* counts, int32_t* copy) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, blocks = int(p.c.blocks);
+  constexpr int kInFlight = 8;
+  int found = 0;
+  for (int word = warp; word < p.words; word += kWarps * kInFlight) {
+    int count[kInFlight];
+#pragma unroll
+    for (int n = 0; n < kInFlight; ++n) {
+      const int64_t page = int64_t(rank * p.words + word + n * kWarps) * 32 + lane;
+      count[n] = word + n * kWarps < p.words && page < blocks ? __ldcg(counts + page) : INT_MIN;
+    }
+#pragma unroll
+    for (int n = 0; n < kInFlight; ++n) {
+      const uint32_t marks = __ballot_sync(0xffffffffu, kUsed ? count[n] != INT_MIN && count[n] != 0 : count[n] == 0);
+      if (word + n * kWarps < p.words) {
+        if (lane == 0) sm.marks[word + n * kWarps] = marks;
+        const int64_t page = int64_t(rank * p.words + word + n * kWarps) * 32 + lane;
+        if (copy != nullptr && page < blocks) copy[page] = count[n];
+        found += __popc(marks);
+      }
+    }
+  }
+  return block_sum(sm, lane == 0 ? found : 0);
+}
+
+// Calls list(rank, page) for the marked pages of this block (behind a filter of words), ranks from `rank` on; stops at `most`.
+template <class Filter, class List>
+__device__ __forceinline__ void list_marked(const Plan& p, Shared& sm, int block_rank_, int rank, int most, Filter filter, List list) {
+  for (int word0 = 0; word0 < p.words && rank < most; word0 += kThreads) {
+    const int word = word0 + int(threadIdx.x);
+    const int page0 = (block_rank_ * p.words + word) * 32;
+    uint32_t marks = word < p.words ? filter(sm.marks[word], page0) : 0u;
+    int total, own = rank + block_rank(sm, __popc(marks), &total);
+    for (; marks != 0 && own < most; marks &= marks - 1, ++own) list(own, page0 + __ffs(marks) - 1);
+    rank += total;
+  }
+}
+
+// Bits of pages below `border` in the word that begins with `page0`.
+__device__ __forceinline__ uint32_t below(int page0, int border) {
+  const int n = min(max(border - page0, 0), 32);
+  return n == 32 ? 0xffffffffu : (1u << n) - 1u;
+}
+
+// What a length counts: rows (within the table) and entries.
+struct Extent {
+  int64_t rows;
+  int entries;
+};
+__device__ __forceinline__ Extent extent_of(const Plan& p, int request, int length, bool reports) {
+  const int64_t room = p.c.entries * p.c.page_rows;
+  if (reports && length > room) report(p.c.status, SPARSE_MLA_STATUS_BAD_PAGE, request, length);
+  const int64_t rows = min(int64_t(max(length, 0)), room);
+  return {rows, int((rows + p.c.page_rows - 1) / p.c.page_rows)};
+}
+__device__ __forceinline__ bool names_page(const Plan& p, int entry) { return unsigned(entry) < unsigned(p.c.blocks); }
+
+// Calls each(i, entry) for a warp's share of `entries` entries, several loads at a time.
+template <class Each>
+__device__ __forceinline__ void each_entry(const int32_t* row, int entries, Each each) {
+  constexpr int kInFlight = 8;
+  for (int at = threadIdx.x & 31; at < entries; at += 32 * kInFlight) {
+    int entry[kInFlight];
+#pragma unroll
+    for (int n = 0; n < kInFlight; ++n) entry[n] = at + 32 * n < entries ? row[at + 32 * n] : -1;
+#pragma unroll
+    for (int n = 0; n < kInFlight; ++n)
+      if (at + 32 * n < entries) each(at + 32 * n, entry[n]);
+  }
+}
+
+// ---- resize ---------------------------------------------------------------------------------------------------------
+
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 1) resize_kernel(const __grid_constant__ Plan p) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  Shared& sm = *reinterpret_cast<Shared*>(smem);
+  const int rank = int(cluster_rank()), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int requests = int(p.c.requests), entries = int(p.c.entries);
+  const int share = (requests + kCluster - 1) / kCluster, begin = min(rank * share, requests), end = min(begin + share, requests);
+  wait_for_predecessor();
+  let_successor_start();
+  if (p.c.counts_in != p.c.counts_out) {
+    for (int64_t page = rank * kThreads + threadIdx.x; page < p.c.blocks; page += kCluster * kThreads) p.c.counts_out[page] = p.c.counts_in[page];
+  }
+  cluster_barrier();
+  // What is given back; wishes of every request.
+  int wishes = 0;
+  for (int request = begin + warp; request < end; request += kWarps) {
+    const Extent extent = extent_of(p, request, p.c.lengths[request], lane == 0);
+    const int32_t* in = p.c.table_in + int64_t(request) * entries;
+    int32_t* out = p.c.table_out + int64_t(request) * entries;
+    int own = 0, first = INT_MAX;
+    each_entry(in, entries, [&](int i, int entry) {
+      const bool has = names_page(p, entry), counts = i < extent.entries;
+      if (has && !counts) atomicSub(p.c.counts_out + entry, 1);
+      if (!has && counts) {
+        ++own;
+        first = min(first, i);
+      }
+      const int next = has && counts ? entry : -1;
+      if (in != out || next != entry) out[i] = next;
+    });
+    own = __reduce_add_sync(0xffffffffu, own);
+    first = __reduce_min_sync(0xffffffffu, first);
+    if (lane == 0) {
+      p.first[request] = first;
+      p.heirs[request] = own;
+    }
+    wishes += own;
+  }
+  wishes = block_sum(sm, lane == 0 ? wishes : 0);
+  tell(sm, 0, rank, wishes);
+  cluster_barrier();
+  const int free_here = mark_pages<false>(p, sm, rank, p.c.counts_out, nullptr);
+  tell(sm, 1, rank, free_here);
+  cluster_barrier();
+  const int all = in_all(sm, 0), free = in_all(sm, 1);
+  list_marked(p, sm, rank, in_front(sm, 1, rank), all, [](uint32_t marks, int) { return marks; }, [&](int at, int page) { p.numbers[at] = page; });
+  cluster_barrier();  // (the last: nobody is told anything behind it)
+  // Every wish gets the free page of its rank.
+  int rank_of_tile = in_front(sm, 0, rank);
+  for (int tile = begin; tile < end; tile += kThreads) {
+    const int own = tile + int(threadIdx.x) < end ? p.heirs[tile + threadIdx.x] : 0;
+    int total;
+    const int start = rank_of_tile + block_rank(sm, own, &total);
+    rank_of_tile += total;
+    // a warp per request that wishes
+    const int warp_first = tile + warp * 32;
+    for (unsigned wishing = __ballot_sync(0xffffffffu, own > 0); wishing != 0; wishing &= wishing - 1) {
+      const int source = __ffs(wishing) - 1, request = warp_first + source;
+      int at = __shfl_sync(0xffffffffu, start, source), left = __shfl_sync(0xffffffffu, own, source);
+      const int counted = extent_of(p, request, p.c.lengths[request], false).entries;
+      int32_t* out = p.c.table_out + int64_t(request) * entries;
+      for (int i0 = p.first[request]; left > 0 && i0 < counted; i0 += 32) {
+        const int i = i0 + lane;
+        const bool wants = i < counted && out[i] < 0;
+        const unsigned wanting = __ballot_sync(0xffffffffu, wants);
+        if (wants) {
+          const int place = at + __popc(wanting & ((1u << lane) - 1u));
+          if (place < free) {
+            const int page = __ldcg(p.numbers + place);
+            out[i] = page;
+            p.c.counts_out[page] = 1;
+          } else {
+            report(p.c.status, SPARSE_MLA_STATUS_NO_PAGE, request, i);
+          }
+        }
+        at += __popc(wanting);
+        left -= __popc(wanting);
+      }
+    }
+  }
+}
+
+// ---- fork -----------------------------------------------------------------------------------------------------------
+
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 1) fork_kernel(const __grid_constant__ Plan p) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  Shared& sm = *reinterpret_cast<Shared*>(smem);
+  const int rank = int(cluster_rank()), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int requests = int(p.c.requests), entries = int(p.c.entries), children = p.children;
+  const int share = (children + kCluster - 1) / kCluster, begin = min(rank * share, children), end = min(begin + share, children);
+  wait_for_predecessor();
+  let_successor_start();
+  for (int request = rank * kThreads + threadIdx.x; request < requests; request += kCluster * kThreads) {
+    p.first[request] = INT_MAX;
+    p.heirs[request] = 0;
+  }
+  const int free_here = mark_pages<false>(p, sm, rank, p.c.counts_in, p.c.counts_in != p.c.counts_out ? p.c.counts_out : nullptr);
+  cluster_barrier();
+  tell(sm, 0, rank, free_here);
+  for (int child = begin + int(threadIdx.x); child < end; child += kThreads) {
+    const int parent = p.parents[child];
+    if (unsigned(parent) < unsigned(requests)) {
+      atomicMin(p.first + parent, child);
+      atomicAdd(p.heirs + parent, 1);
+    }
+  }
+  cluster_barrier();
+  // Who wants a page: all but the first to continue a request whose last page is partly filled.
+  auto wants_page = [&](int child, int* source, int* rows) {
+    const int parent = p.parents[child];
+    if (unsigned(parent) >= unsigned(requests) || __ldcg(p.first + parent) == child) return false;
+    const Extent extent = extent_of(p, parent, p.c.lengths[parent], false);
+    *rows = int(extent.rows % p.c.page_rows);
+    if (*rows == 0) return false;
+    *source = p.c.table_in[int64_t(parent) * entries + extent.entries - 1];
+    return names_page(p, *source);
+  };
+  int wishes = 0, source, rows;
+  for (int child = begin + int(threadIdx.x); child < end; child += kThreads) wishes += wants_page(child, &source, &rows);
+  wishes = block_sum(sm, wishes);
+  tell(sm, 1, rank, wishes);
+  const int free = in_all(sm, 0);
+  list_marked(p, sm, rank, in_front(sm, 0, rank), children, [](uint32_t marks, int) { return marks; }, [&](int at, int page) { p.numbers[at] = page; });
+  cluster_barrier();  // (the last: nobody is told anything behind it)
+  if (rank == 0 && threadIdx.x == 0) *p.copy_count = min(in_all(sm, 1), free);
+  // Entries of the table as it was: one reference less, and one more for each row that has them. (Other pages than those that are given out.)
+  for (int request = rank * kWarps + warp; request < requests; request += kCluster * kWarps) {
+    const Extent extent = extent_of(p, request, p.c.lengths[request], lane == 0);
+    const int heirs = __ldcg(p.heirs + request), filled = int(extent.rows % p.c.page_rows);
+    each_entry(p.c.table_in + int64_t(request) * entries, entries, [&](int i, int page) {
+      const int more = (i >= extent.entries ? 0 : i == extent.entries - 1 && filled != 0 ? min(heirs, 1) : heirs) - 1;
+      if (more != 0 && names_page(p, page)) atomicAdd(p.c.counts_out + page, more);
+    });
+  }
+  int rank_of_tile = in_front(sm, 1, rank);
+  for (int tile = begin; tile < end; tile += kThreads) {
+    const int child = tile + int(threadIdx.x);
+    const bool wants = child < end && wants_page(child, &source, &rows);
+    int total, page = -2;  // -2: as the parent has it
+    const int place = rank_of_tile + block_rank(sm, wants, &total);
+    rank_of_tile += total;
+    if (wants && place < free) {
+      page = __ldcg(p.numbers + place);
+      p.c.counts_out[page] = 1;
+      p.copies[place] = make_int4(source, page, rows, 0);
+    } else if (wants) {
+      page = -1;
+      report(p.c.status, SPARSE_MLA_STATUS_NO_PAGE, child, extent_of(p, p.parents[child], p.c.lengths[p.parents[child]], false).entries - 1);
+    }
+    // rows of the new table, 32 of them by each warp
+    for (int k = 0; k < 32 && tile + warp * 32 + k < end; ++k) {
+      const int own = tile + warp * 32 + k, parent = p.parents[own], last_page = __shfl_sync(0xffffffffu, page, k);
+      const int counted = unsigned(parent) < unsigned(requests) ? extent_of(p, parent, p.c.lengths[parent], false).entries : 0;
+      int32_t* out = p.c.table_out + int64_t(own) * entries;
+      if (counted > 0)
+        each_entry(p.c.table_in + int64_t(parent) * entries, counted, [&](int i, int entry) {
+          if (i == counted - 1 && last_page != -2) entry = last_page;
+          out[i] = names_page(p, entry) ? entry : -1;
+        });
+      for (int i = counted + lane; i < entries; i += 32) out[i] = -1;
+    }
+  }
+}
+
+// ---- compact --------------------------------------------------------------------------------------------------------
+
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 1) compact_kernel(const __grid_constant__ Plan p) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  Shared& sm = *reinterpret_cast<Shared*>(smem);
+  const int rank = int(cluster_rank()), blocks = int(p.c.blocks);
+  wait_for_predecessor();
+  let_successor_start();
+  const int used_here = mark_pages<true>(p, sm, rank, p.c.counts_in, p.c.counts_in != p.c.counts_out ? p.c.counts_out : nullptr);
+  cluster_barrier();
+  tell(sm, 0, rank, used_here);
+  cluster_barrier();
+  const int border = in_all(sm, 0);  // pages in use
+  auto movers = [&](uint32_t marks, int page0) { return marks & ~below(page0, border); };
+  auto holes = [&](uint32_t marks, int page0) { return ~marks & below(page0, border); };  // (border <= blocks)
+  int moving = 0, free = 0;
+  for (int word = threadIdx.x; word < p.words; word += kThreads) {
+    const uint32_t marks = sm.marks[word];
+    const int page0 = (rank * p.words + word) * 32;
+    moving += __popc(movers(marks, page0));
+    free += __popc(holes(marks, page0));
+    for (int i = 0; i < 32 && page0 + i < blocks; ++i) {
+      const bool used = marks >> i & 1;
+      if (!used || page0 + i < border) p.places[page0 + i] = used ? page0 + i : -1;
+    }
+  }
+  moving = block_sum(sm, moving);
+  free = block_sum(sm, free);
+  tell(sm, 1, rank, moving);
+  tell(sm, 2, rank, free);
+  cluster_barrier();
+  int* const lists = reinterpret_cast<int*>(p.copies);
+  list_marked(p, sm, rank, in_front(sm, 1, rank), INT_MAX, movers, [&](int at, int page) { lists[4 * at] = page; });
+  list_marked(p, sm, rank, in_front(sm, 2, rank), INT_MAX, holes, [&](int at, int page) { lists[4 * at + 1] = page; });
+  cluster_barrier();  // (the last: nobody is told anything behind it)
+  const int moves = in_all(sm, 1);
+  if (rank == 0 && threadIdx.x == 0) *p.copy_count = moves;
+  for (int move = rank * kThreads + threadIdx.x; move < moves; move += kCluster * kThreads) {
+    const int source = __ldcg(lists + 4 * move), target = __ldcg(lists + 4 * move + 1);
+    lists[4 * move + 2] = int(p.c.page_rows);
+    p.places[source] = target;
+    p.c.counts_out[target] = p.c.counts_in[source];
+    p.c.counts_out[source] = 0;
+  }
+}
+
+// ---- copies ---------------------------------------------------------------------------------------------------------
+
+constexpr int kCopyThreads = 256, kUnitBytes = 16384, kCopyBlocks = 6;  // per SM
+
+struct Copies {
+  const int4* copies;
+  const int32_t* count;
+  const int32_t *table_in, *places;  // a table whose entries get their new numbers, or NULL
+  int32_t* table_out;
+  int64_t entries, page_rows;
+  int32_t blocks, tensors, units;  // units of all tensors, for one copy
+  struct {
+    char* memory;
+    int64_t page_bytes;
+    int32_t rows, first_unit;
+  } tensor[PAGES_MOST_TENSORS];
+};
+
+__device__ __forceinline__ uint4 load_once(const uint4* at) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(at) : "memory");
+  return v;
+}
+
+// A block copies 16 KiB of a page at a time, 64 bytes by a thread with all loads in flight. Pages that are not 16-byte aligned go byte by byte (scales of a few bytes).
+__global__ void __launch_bounds__(kCopyThreads, kCopyBlocks) copy_kernel(const __grid_constant__ Copies p) {
+  wait_for_predecessor();
+  let_successor_start();
+  if (p.table_out != nullptr) {
+    for (int64_t i = int64_t(blockIdx.x) * kCopyThreads + threadIdx.x; i < p.entries; i += int64_t(gridDim.x) * kCopyThreads) {
+      const int page = p.table_in[i];
+      p.table_out[i] = unsigned(page) < unsigned(p.blocks) ? p.places[page] : page;
+    }
+  }
+  const int64_t items = int64_t(*p.count) * p.units;
+  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const int which = int(item / p.units), unit = int(item - int64_t(which) * p.units);
+    int tensor = 0;
+    for (int high = p.tensors; high - tensor > 1;) {
+      const int middle = (tensor + high) >> 1;
+      if (p.tensor[middle].first_unit <= unit) tensor = middle; else high = middle;
+    }
+    const int4 copy = p.copies[which];
+    const int64_t page_bytes = p.tensor[tensor].page_bytes, rows = p.tensor[tensor].rows;
+    const int64_t first = int64_t(unit - p.tensor[tensor].first_unit) * kUnitBytes;
+    const int64_t filled = (copy.z * rows + p.page_rows - 1) / p.page_rows * (page_bytes / rows);  // bytes of the page to copy
+    const int bytes = int(min(filled - first, int64_t(kUnitBytes)));
+    if (bytes <= 0) continue;
+    const char* source = p.tensor[tensor].memory + copy.x * page_bytes + first;
+    char* target = p.tensor[tensor].memory + copy.y * page_bytes + first;
+    int done = 0;
+    if (((reinterpret_cast<uintptr_t>(source) | reinterpret_cast<uintptr_t>(target)) & 15) == 0) {
+      const int words = bytes / 16;
+      uint4 v[kUnitBytes / 16 / kCopyThreads];
+#pragma unroll
+      for (int n = 0; n < kUnitBytes / 16 / kCopyThreads; ++n) {
+        const int at = n * kCopyThreads + int(threadIdx.x);
+        if (at < words) v[n] = load_once(reinterpret_cast<const uint4*>(source) + at);
+      }
+#pragma unroll
+      for (int n = 0; n < kUnitBytes / 16 / kCopyThreads; ++n) {
+        const int at = n * kCopyThreads + int(threadIdx.x);
+        if (at < words) reinterpret_cast<uint4*>(target)[at] = v[n];
+      }
+      done = words * 16;
+    }
+    for (int at = done + int(threadIdx.x); at < bytes; at += kCopyThreads) target[at] = source[at];
+  }
+}
+
+// ---- launch ---------------------------------------------------------------------------------------------------------
+
+bool fits(const pages_call& c) {
+  return c.requests >= 0 && c.requests < INT_MAX && c.entries >= 0 && c.entries < INT_MAX && (c.entries == 0 || c.requests <= INT_MAX / c.entries) && c.blocks >= 0 &&
+         c.blocks <= PAGES_MOST_BLOCKS && c.page_rows >= 1 && c.page_rows <= INT_MAX;
+}
+
+// Where things lie in the workspace.
+struct Layout {
+  size_t bytes = 16;  // the number of copies
+  size_t take(int64_t size) {
+    const size_t at = bytes;
+    bytes += (size_t(size) + 15) / 16 * 16;
+    return at;
+  }
+};
+
+int words_of(const pages_call& c) { return int((c.blocks + 32 * kCluster - 1) / (32 * kCluster)); }
+
+int launch_plan(void (*kernel)(const Plan), const Plan& p, cudaStream_t stream) {
+  const size_t shared = sizeof(Shared) + size_t(p.words) * sizeof(uint32_t);
+  if (shared > 48 * 1024)  // (a per-device setting; always the same value)
+    if (const cudaError_t error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(Shared) + PAGES_MOST_BLOCKS / 8 / kCluster))) return int(error);
+  return int(launch_overlapped(kernel, kCluster, kThreads, shared, stream, p));
+}
+
+int fill_tensors(Copies* copies, const pages_call& c, const pages_tensor* tensors, int64_t count) {
+  if (count < 0 || count > PAGES_MOST_TENSORS || (count > 0 && tensors == nullptr)) return -1;
+  int64_t units = 0;
+  for (int64_t t = 0; t < count; ++t) {
+    const pages_tensor& own = tensors[t];
+    if (own.page_bytes < 0 || own.rows < 1 || own.rows > c.page_rows || c.page_rows % own.rows != 0 || own.page_bytes % own.rows != 0) return -1;
+    copies->tensor[t] = {static_cast<char*>(own.memory), own.page_bytes, int32_t(own.rows), int32_t(units)};
+    units += std::max<int64_t>((own.page_bytes + kUnitBytes - 1) / kUnitBytes, 1);
+    if (units > INT_MAX) return -1;
+  }
+  copies->tensors = int32_t(count);
+  copies->units = int32_t(units);
+  copies->page_rows = c.page_rows;
+  copies->blocks = int32_t(c.blocks);
+  return 0;
+}
+
+int launch_copies(const Copies& copies, int64_t most, cudaStream_t stream) {
+  const int64_t items = std::max(most * copies.units, copies.table_out != nullptr ? (copies.entries + kCopyThreads - 1) / kCopyThreads : 0);
+  if (items == 0) return 0;
+  const int grid = int(std::min<int64_t>(items, int64_t(latent::multiprocessors()) * kCopyBlocks));
+  return int(launch_overlapped(copy_kernel, grid, kCopyThreads, 0, stream, copies));
+}
+
+bool usable(const pages_call& c) { return c.workspace != nullptr && latent::aligned(c.workspace) && c.status != nullptr; }
+
+}  // namespace
+}  // namespace pages
+
+extern "C" {
+
+int workspace_size_pages_resize(uint64_t* bytes, const pages_call* call) {
+  using namespace pages;
+  if (bytes == nullptr || call == nullptr || !fits(*call)) return -1;
+  Layout layout;
+  layout.take(4 * call->blocks);
+  layout.take(4 * call->requests);
+  layout.take(4 * call->requests);
+  *bytes = layout.bytes;
+  return 0;
+}
+
+int launch_pages_resize(void* stream, const pages_call* call) {
+  using namespace pages;
+  if (call == nullptr || !fits(*call)) return -1;
+  if ((call->requests == 0 || call->entries == 0) && (call->blocks == 0 || call->counts_in == call->counts_out)) return 0;
+  if (!usable(*call)) return -1;
+  char* workspace = static_cast<char*>(call->workspace);
+  Plan p = {};
+  Layout layout;
+  p.c = *call;
+  p.numbers = reinterpret_cast<int32_t*>(workspace + layout.take(4 * call->blocks));
+  p.first = reinterpret_cast<int32_t*>(workspace + layout.take(4 * call->requests));
+  p.heirs = reinterpret_cast<int32_t*>(workspace + layout.take(4 * call->requests));
+  p.words = words_of(*call);
+  return launch_plan(resize_kernel, p, static_cast<cudaStream_t>(stream));
+}
+
+int workspace_size_pages_fork(uint64_t* bytes, const pages_fork_call* call) {
+  using namespace pages;
+  if (bytes == nullptr || call == nullptr || !fits(call->pages) || call->children < 0 || call->children >= INT_MAX) return -1;
+  Layout layout;
+  layout.take(4 * call->children);
+  layout.take(4 * call->pages.requests);
+  layout.take(4 * call->pages.requests);
+  layout.take(16 * call->children);
+  *bytes = layout.bytes;
+  return 0;
+}
+
+int launch_pages_fork(void* stream, const pages_fork_call* call) {
+  using namespace pages;
+  if (call == nullptr || !fits(call->pages) || call->children < 0 || call->children >= INT_MAX) return -1;
+  const pages_call& c = call->pages;
+  if (c.entries > 0 && call->children > INT_MAX / c.entries) return -1;
+  Copies copies = {};
+  if (const int status = fill_tensors(&copies, c, call->tensors, call->tensor_count)) return status;
+  if ((c.requests == 0 || c.entries == 0) && (call->children == 0 || c.entries == 0) && (c.blocks == 0 || c.counts_in == c.counts_out)) return 0;
+  if (!usable(c)) return -1;
+  char* workspace = static_cast<char*>(c.workspace);
+  Plan p = {};
+  Layout layout;
+  p.c = c;
+  p.parents = call->parents;
+  p.children = int32_t(call->children);
+  p.numbers = reinterpret_cast<int32_t*>(workspace + layout.take(4 * call->children));
+  p.first = reinterpret_cast<int32_t*>(workspace + layout.take(4 * c.requests));
+  p.heirs = reinterpret_cast<int32_t*>(workspace + layout.take(4 * c.requests));
+  p.copies = reinterpret_cast<int4*>(workspace + layout.take(16 * call->children));
+  p.copy_count = reinterpret_cast<int32_t*>(workspace);
+  p.words = words_of(c);
+  copies.copies = p.copies;
+  copies.count = p.copy_count;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (const int status = launch_plan(fork_kernel, p, s)) return status;
+  return launch_copies(copies, call->children > 0 ? call->children - 1 : 0, s);
+}
+
+int workspace_size_pages_compact(uint64_t* bytes, const pages_compact_call* call) {
+  using namespace pages;
+  if (bytes == nullptr || call == nullptr || !fits(call->pages)) return -1;
+  Layout layout;
+  layout.take(16 * (call->pages.blocks / 2 + 1));
+  *bytes = layout.bytes;
+  return 0;
+}
+
+int launch_pages_compact(void* stream, const pages_compact_call* call) {
+  using namespace pages;
+  if (call == nullptr || !fits(call->pages)) return -1;
+  const pages_call& c = call->pages;
+  Copies copies = {};
+  if (const int status = fill_tensors(&copies, c, call->tensors, call->tensor_count)) return status;
+  const bool table = c.requests > 0 && c.entries > 0;
+  if (c.blocks == 0 && (!table || c.table_in == c.table_out)) return 0;
+  if (!usable(c)) return -1;
+  char* workspace = static_cast<char*>(c.workspace);
+  Plan p = {};
+  Layout layout;
+  p.c = c;
+  p.places = call->places;
+  p.copies = reinterpret_cast<int4*>(workspace + layout.take(16 * (c.blocks / 2 + 1)));  // (no more moves than free pages, or than pages in use)
+  p.copy_count = reinterpret_cast<int32_t*>(workspace);
+  p.words = words_of(c);
+  copies.copies = p.copies;
+  copies.count = p.copy_count;
+  copies.places = call->places;
+  copies.table_in = c.table_in;
+  copies.table_out = table ? c.table_out : nullptr;
+  copies.entries = c.requests * c.entries;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (const int status = launch_plan(compact_kernel, p, s)) return status;
+  return launch_copies(copies, c.blocks / 2, s);
+}
+
+}  // extern "C"

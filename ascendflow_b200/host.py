@@ -57,10 +57,11 @@ class _Unavailable:
         return False
 
     latent_append = latent_attention = latent_prefill = rotary
+    latent_append8 = latent_attention8 = pages_resize = pages_fork = pages_compact = rotary
 
     def set_latent_fallback(self, fallback):
         self.latent_registration = torch.library.Library("ascendflow_b200", "FRAGMENT")
-        for schema in LATENT_SCHEMAS:
+        for schema in (*LATENT_SCHEMAS, *PAGES_SCHEMAS):
             name = schema[: schema.index("(")]
             self.latent_registration.define(schema, tags=(torch.Tag.pt2_compliant_tag,))
             self.latent_registration.impl(name, functools.partial(fallback, name), "CUDA")
@@ -83,6 +84,15 @@ LATENT_SCHEMAS = (
     "Tensor(b!)? lse) -> ()",
     "latent_prefill(Tensor q, Tensor k, Tensor v, Tensor k_rope, Tensor cu_seqlens_q, Tensor cu_seqlens_k, float scale, bool causal, Tensor(a!) out, "
     "Tensor(b!)? lse) -> ()",
+    "latent_append8(Tensor latent, Tensor rope, Tensor(a!) cache, Tensor(b!) scales, Tensor block_table, Tensor cu_seqlens_q, Tensor seqused_kv, Tensor inv_freq, "
+    "bool halves, float amplitude) -> ()",
+    "latent_attention8(Tensor q, Tensor cache, Tensor scales, Tensor block_table, Tensor cu_seqlens_q, Tensor seqused_kv, float scale, Tensor? sinks, Tensor(a!) out, "
+    "Tensor(b!)? lse) -> ()",
+)
+PAGES_SCHEMAS = (
+    "pages_resize(Tensor block_table, Tensor counts, Tensor lengths, int page_rows, Tensor(a!) table_out, Tensor(b!) counts_out) -> ()",
+    "pages_fork(Tensor(a!)[] caches, Tensor block_table, Tensor counts, Tensor parents, Tensor lengths, int page_rows, Tensor(b!) table_out, Tensor(c!) counts_out) -> ()",
+    "pages_compact(Tensor(a!)[] caches, Tensor block_table, Tensor counts, Tensor(b!) table_out, Tensor(c!) counts_out, Tensor(d!) places) -> ()",
 )
 
 try:
@@ -121,7 +131,7 @@ def connect():
 
 
 def connect_latent():
-    """The same for the operators around dense latent attention."""
+    """The same for the operators around dense latent attention and on the pages of a cache."""
     global _latent_connected
     if _latent_connected:
         return False
@@ -133,6 +143,9 @@ def connect_latent():
     library = _library(library_path())
     calls.configure_latent(*(ct.cast(getattr(library, name), ct.c_void_p).value for name in (
         "launch_latent_rotary", "launch_latent_append", "launch_latent_attention", "launch_latent_prefill", "workspace_size_latent_attention",
-        "workspace_size_latent_prefill")), numbers.Real)
+        "workspace_size_latent_prefill", "launch_latent_append8", "launch_latent_attention8")), numbers.Real)
+    calls.configure_pages(*(ct.cast(getattr(library, name), ct.c_void_p).value for name in (
+        "launch_pages_resize", "launch_pages_fork", "launch_pages_compact", "workspace_size_pages_resize", "workspace_size_pages_fork",
+        "workspace_size_pages_compact")))
     _latent_connected = True
     return True

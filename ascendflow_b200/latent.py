@@ -250,14 +250,14 @@ def _check_paged(cache, block_table, cu_seqlens_q, seqused_kv, dtype):
     _tensor(seqused_kv, "seqused_kv", (torch.int32,), (batches,))
 
 
-def _check_append(latent, rope, cache, block_table, cu_seqlens_q, seqused_kv, inv_freq, halves, amplitude):
+def _check_append(latent, rope, cache, block_table, cu_seqlens_q, seqused_kv, inv_freq, halves, amplitude, held=None):
     _number(amplitude, "amplitude", -MOST_FLOAT, MOST_FLOAT)
     for tensor, name in ((latent, "latent"), (rope, "rope")):
         _tensor(tensor, name, _STORED)
         require(tensor.dim() == 2, f"{name}: expected [T, features]")
     _rows(latent, "latent")
     require(rope.dtype == latent.dtype and (rope.numel() == 0 or rope.stride(1) == 1), "rope: expected the type of latent and contiguous features")
-    _check_paged(cache, block_table, cu_seqlens_q, seqused_kv, latent.dtype)
+    _check_paged(cache, block_table, cu_seqlens_q, seqused_kv, held or latent.dtype)
     _check_frequencies(inv_freq)
     turned = 2 * inv_freq.shape[0]
     require(tuple(rope.shape) == (latent.shape[0], turned) and latent.shape[1] + turned == cache.shape[3], "expected latent [T, W - R], rope [T, R] and cache rows of W")
@@ -271,13 +271,13 @@ def _check_written(out, lse, inputs):
         _disjoint(lse, inputs)
 
 
-def _check_attention(q, cache, block_table, cu_seqlens_q, seqused_kv, scale, sinks, out, lse):
+def _check_attention(q, cache, block_table, cu_seqlens_q, seqused_kv, scale, sinks, out, lse, held=None):
     _number(scale, "scale", 1e-30, 1e30)
     _tensor(q, "q", _STORED)
     require(q.dim() == 3 and q.shape[2] in (512, 576) and q.shape[1] >= 1 and q.is_contiguous(), "q: expected contiguous [T, H, 512] or [T, H, 576]")
     require(q.shape[:2].numel() <= MOST_ROWS, "q: too many rows")
     _rows(q, "q")
-    _check_paged(cache, block_table, cu_seqlens_q, seqused_kv, q.dtype)
+    _check_paged(cache, block_table, cu_seqlens_q, seqused_kv, held or q.dtype)
     require(cache.shape[3] == q.shape[2], "cache: rows must be as wide as q")
     _tensor(out, "out", (q.dtype,), (*q.shape[:2], VALUES))
     _rows(out, "out")

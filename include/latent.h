@@ -90,6 +90,32 @@ typedef struct {
 int workspace_size_latent_attention(uint64_t* bytes);
 int launch_latent_attention(void* stream, const latent_attention_call* call);
 
+/* ---- rows held in 8 bits ------------------------------------------------------------------------------------------------
+ *
+ * A cache of e4m3 numbers [blocks, page_rows, 1, width] with a scale for every `block_rows` rows of a page, [blocks, page_rows / block_rows]: a byte e stands for
+ * 2^(e - 127), 255 for NaN (the e8m0 format). block_rows: a power of two up to 64. A held value is its number times its row's scale. */
+
+/* The append of rotated rows: as launch_latent_append, with page_rows a multiple of 64, `width` one of 16 and `cache` of 8 bits. What is held is worked out in FP32 and
+ * rounded once: numbers to the nearest e4m3 number after the division by the scale. A block's scale is the least power of two s with |v| <= 448 s for
+ * all its new rows v, and, unless the first of these begins the block, not below the scale that the block has: where that grows, the numbers of the rows in front of the
+ * new ones are divided by the growth and rounded to nearest. From half rows, values beyond 61440 (the greatest whose number times its scale half holds) are taken
+ * as that. A row that is not finite makes its block's scale NaN. Values below 2^-126 count as zero. */
+typedef struct {
+  latent_append_call append; /* cache: e4m3 */
+  uint8_t* scales;
+  int64_t block_rows;
+} latent_append8_call;
+int launch_latent_append8(void* stream, const latent_append8_call* call);
+
+/* Attention as launch_latent_attention over such a cache; its workspace is as large as that one's. Held values are taken as they are (in the type of q, which holds them exactly
+ * where they are finite and normal numbers there; for half: scales up to 2^22). NaN among the numbers of rows that are seen is not looked for; scales that are NaN make what sees them NaN. */
+typedef struct {
+  latent_attention_call attention; /* cache: e4m3 */
+  const uint8_t* scales;
+  int64_t block_rows;
+} latent_attention8_call;
+int launch_latent_attention8(void* stream, const latent_attention8_call* call);
+
 /* Attention in expanded form: keys are [k | k_rope], 128 features per head and 64 shared by all heads; values 128
  * per head. Request b owns keys cu_seqlens_k[b] .. ; causal: token j of n sees the first K - n + j + 1 of its K keys,
  * otherwise all. A request's values have to be finite (those of keys that a token does not see are multiplied by zero);

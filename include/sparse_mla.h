@@ -54,6 +54,7 @@ extern "C" {
 #define SPARSE_MLA_STATUS_OK 0
 #define SPARSE_MLA_STATUS_BAD_PAGE 1    /* block-table entry outside [0, blocks): slot masked   */
 #define SPARSE_MLA_STATUS_WAIT_EXPIRED 2 /* a bounded on-chip wait gave up: output is not valid  */
+#define SPARSE_MLA_STATUS_NO_PAGE 3      /* pages.h: no free page was left (request, entry)       */
 
 /* ---- BF16 kernel "sparse_mla" ------------------------------------------------------------- */
 
