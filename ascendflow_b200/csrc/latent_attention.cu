@@ -74,13 +74,14 @@ struct Layout {
   static constexpr int kSmemAlpha = kSmemBars + 256;             // float[2][64]
   static constexpr int kSmemInverse = kSmemAlpha + 2 * kRows * 4;  // float[64]
   static constexpr int kSmemMisc = kSmemInverse + kRows * 4;
-  static constexpr int kSmemBytes = kSmemMisc + 128 + 1024;      // the tiles are aligned to 1024 bytes
+  static constexpr int kSmemScales = kSmemMisc + 64;             // bytes[3][64], of rows in 8 bits
+  static constexpr int kSmemBytes = kSmemScales + kStages * kChunk + 1024;  // the tiles are aligned to 1024 bytes
 };
 static_assert(Layout<576>::kSmemBytes <= 232448, "one block per SM");
 
 enum Bar {
   kFull0 = 0, kFree0 = kFull0 + kStages, kPieceReady0 = kFree0 + kStages, kPieceDone0 = kPieceReady0 + kPieces, kQFull = kPieceDone0 + kPieces,
-  kQFree, kPlaces, kScoresFull, kScoresFree, kWeightsFull, kWeightsFree, kMended, kGivenUp0, kGivenUp1, kBarCount
+  kQFree, kPlaces, kScoresFull, kScoresFree, kWeightsFull, kWeightsFree, kMended, kGivenUp0, kGivenUp1, kLanded0, kBarCount = kLanded0 + kStages
 };
 static_assert(kBarCount <= 32, "the barrier area");
 
@@ -659,26 +660,27 @@ __device__ void query_role(const Params& p, const Shared& sm, uint32_t tmem) {
 template <int kFormat> constexpr uint32_t kIdescScores = idesc_f16(128, kChunk, kFormat, 0, 0) | kSparseA;
 template <int kFormat> constexpr uint32_t kIdescValues = idesc_f16(64, 256, kFormat, 0, 1);  // issued as .ws
 
-template <int kFormat, int kSteps, int K = 0>
+// A tile's boxes of 64 features are kBox bytes apart, its groups of eight rows kGroup.
+template <int kFormat, int kSteps, int kBox, int K = 0>
 __device__ __forceinline__ void issue_scores(uint32_t tmem, uint64_t x_desc) {
   if constexpr (K < kSteps) {
-    constexpr uint32_t offset = (K >> 1) * kBoxBytes + (K & 1) * 64;
+    constexpr uint32_t offset = (K >> 1) * kBox + (K & 1) * 64;
     constexpr uint32_t q = K < 16 ? kColumnsQ + K * 8 : kColumnsQRest + (K - 16) * 8;
     mma_sparse_ts_c<K != 0>(tmem + kColumnsScores, tmem + q, x_desc + (offset >> 4), tmem + kColumnsPlaces, kIdescScores<kFormat>);
-    issue_scores<kFormat, kSteps, K + 1>(tmem, x_desc);
+    issue_scores<kFormat, kSteps, kBox, K + 1>(tmem, x_desc);
   }
 }
-template <int kFormat, bool kFirst, int I = 0>
+template <int kFormat, int kBox, int kGroup, bool kFirst, int I = 0>
 __device__ __forceinline__ void issue_values(uint32_t tmem, uint64_t p_desc, uint64_t x_desc) {
   if constexpr (I < 2 * (kChunk / 16)) {
     constexpr int half = I % 2, k = I / 2;
-    constexpr uint32_t offset = half * 4 * kBoxBytes + k * 2048;
+    constexpr uint32_t offset = half * 4 * kBox + k * 2 * kGroup;
     mma_ws_ss_c<!(kFirst && k == 0)>(tmem + half * 128, p_desc + ((k * 32) >> 4), x_desc + (offset >> 4), kIdescValues<kFormat>);
-    issue_values<kFormat, kFirst, I + 1>(tmem, p_desc, x_desc);
+    issue_values<kFormat, kBox, kGroup, kFirst, I + 1>(tmem, p_desc, x_desc);
   }
 }
 
-template <int kFormat, int kWidth>
+template <int kFormat, int kWidth, int kBox, int kGroup>
 __device__ void score_role(const Shared& sm, uint32_t tmem) {
   volatile int* abort_flag = sm.abort_flag();
   uint32_t count = 0, loads = 0;
@@ -693,14 +695,14 @@ __device__ void score_role(const Shared& sm, uint32_t tmem) {
       if (!mbar_wait(sm.bar(kFull0 + stage), (count / kStages) & 1, abort_flag)) return;
       if (!mbar_wait(sm.bar(kScoresFree), (count & 1) ^ 1, abort_flag)) return;
       tc_fence_after_sync();
-      issue_scores<kFormat, kWidth / 32>(tmem, smem_desc_sw128(sm.base + stage * Layout<kWidth>::kTileBytes, 16, 1024));
+      issue_scores<kFormat, kWidth / 32, kBox>(tmem, smem_desc_sw128(sm.base + stage * Layout<kWidth>::kTileBytes, 16, kGroup));
       mma_commit(sm.bar(kScoresFull));
     }
     mma_commit(sm.bar(kQFree));
   }
 }
 
-template <int kFormat, int kWidth>
+template <int kFormat, int kWidth, int kBox, int kGroup>
 __device__ void value_role(const Shared& sm, uint32_t tmem) {
   volatile int* abort_flag = sm.abort_flag();
   uint32_t count = 0;
@@ -712,9 +714,9 @@ __device__ void value_role(const Shared& sm, uint32_t tmem) {
       const uint32_t stage = count % kStages;
       if (!mbar_wait(sm.bar(kWeightsFull), count & 1, abort_flag)) return;
       tc_fence_after_sync();
-      const uint64_t x_desc = smem_desc_sw128(sm.base + stage * Layout<kWidth>::kTileBytes, kBoxBytes, 1024);
-      if (i == 0) issue_values<kFormat, true>(tmem, p_desc, x_desc);
-      else issue_values<kFormat, false>(tmem, p_desc, x_desc);
+      const uint64_t x_desc = smem_desc_sw128(sm.base + stage * Layout<kWidth>::kTileBytes, kBox, kGroup);
+      if (i == 0) issue_values<kFormat, kBox, kGroup, true>(tmem, p_desc, x_desc);
+      else issue_values<kFormat, kBox, kGroup, false>(tmem, p_desc, x_desc);
       mma_commit(sm.bar(kWeightsFree));
       mma_commit(sm.bar(kFree0 + stage));
     }
@@ -967,7 +969,7 @@ __global__ void __launch_bounds__(kHeld8 ? kThreads8 : kThreads, 1) attention_ke
   if (threadIdx.x == 0) {
     for (int i = 0; i < kBarCount; ++i) {
       int arrivals = 1;
-      if (i >= kPieceDone0 && i < kPieceDone0 + kPieces) arrivals = kSoftmaxWarps + 2 + (kHeld8 ? kConvertWarps : 1) + kOwnQueryWarps;
+      if (i >= kPieceDone0 && i < kPieceDone0 + kPieces) arrivals = kSoftmaxWarps + 3 + (kHeld8 ? kConvertWarps : 0) + kOwnQueryWarps;
       else if (i == kQFull) arrivals = kOwnQueryWarps;
       else if (kHeld8 && i < kFull0 + kStages) arrivals = kConvertWarps;
       else if (i == kScoresFree || i == kWeightsFull || i == kPlaces) arrivals = kSoftmaxWarps;
@@ -990,26 +992,40 @@ __global__ void __launch_bounds__(kHeld8 ? kThreads8 : kThreads, 1) attention_ke
     fence_proxy_async();  // the plan's scratch is the first tile's memory
     __syncthreads();
   }
-  if constexpr (kHeld8) share_registers(warp);
-  if (warp < kSoftmaxWarps) softmax_role<kFormat, kWidth>(p, sm, tmem);
-  else if (warp == kScoreWarp || warp == kValueWarp) {
+  auto issue = [&]() {
     if (elect_one()) {
-      if (warp == kScoreWarp) score_role<kFormat, kWidth>(sm, tmem);
-      else value_role<kFormat, kWidth>(sm, tmem);
+      constexpr int kBox = kHeld8 ? 1024 : kBoxBytes, kGroup = kHeld8 ? kGroupBytes<kWidth> : 1024;
+      if (warp == kScoreWarp) score_role<kFormat, kWidth, kBox, kGroup>(sm, tmem);
+      else value_role<kFormat, kWidth, kBox, kGroup>(sm, tmem);
       if (*sm.abort_flag() != 0) wait_for_products(sm.bar(warp == kScoreWarp ? kGivenUp0 : kGivenUp1));
     }
     __syncwarp();
-  }
-  else if (warp == kPlanWarp) {
+  };
+  auto plan = [&]() {
     if (p.batches <= 32) borders = plan_block<1>(p, nullptr, &place);
     plan_role(p, sm, borders, place);
+  };
+  if constexpr (kHeld8) {
+    if (warp < kSoftmaxWarps) {
+      take_128_registers();
+      softmax_role<kFormat, kWidth>(p, sm, tmem);
+    } else if (warp < kConvertWarp0) {
+      keep_64_registers();
+      if (warp == kScoreWarp || warp == kValueWarp) issue();
+      else if (warp == kCopyWarp) copy_role8<kWidth>(p, sm);
+      else if (warp == kPlanWarp) plan();
+      else if (warp >= kQueryWarp0) query_role8<kWidth>(p, sm, tmem);
+    } else {
+      take_112_registers();
+      convert_role<kFormat, kWidth>(p, sm);
+    }
+  } else {
+    if (warp < kSoftmaxWarps) softmax_role<kFormat, kWidth>(p, sm, tmem);
+    else if (warp == kScoreWarp || warp == kValueWarp) issue();
+    else if (warp == kCopyWarp) copy_role<kWidth>(p, sm);
+    else if (warp == kPlanWarp) plan();
+    else query_role<kWidth>(p, sm, tmem);
   }
-  else if constexpr (kHeld8) {
-    if (warp >= kConvertWarp0) convert_role<kFormat, kWidth>(p, sm);
-    else if (warp >= kQueryWarp0) query_role8<kWidth>(p, sm, tmem);
-  }
-  else if (warp == kCopyWarp) copy_role<kWidth>(p, sm);
-  else query_role<kWidth>(p, sm, tmem);
   tc_fence_before_sync();
   __syncthreads();
   if (threadIdx.x == 0 && *sm.abort_flag() != 0) report(p.status, SPARSE_MLA_STATUS_WAIT_EXPIRED, blockIdx.x, 0);

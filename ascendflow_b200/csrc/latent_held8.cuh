@@ -6,8 +6,8 @@
 // rest: a permutation, a shift, a mask and a product for two values.
 //
 //   warps 8-11   Q of the next piece from global to tensor memory (a subpartition each)
-//   warps 12-19  chunks: 64 rows of W bytes, nine (eight) loads of 16 bytes per thread, sixteen values to 32 bytes of the tile each. What is loaded
-//                for the next chunk takes the place of what has been stored, so that loads are always on their way.
+//   warp 6       brings chunks (64 rows of W bytes, contiguous) by bulk copies, and asks for the rows behind them in L2
+//   warps 12-19  a group of eight of the chunk's rows each: e4m3 numbers out of shared memory, values over them
 #pragma once
 
 namespace latent {
@@ -54,28 +54,34 @@ __device__ __forceinline__ uint32_t widened(uint32_t word, uint32_t factor) {
   return multiply_pair<kFormat>(kFormat == 1 ? spread << 4 & 0x87f087f0u : spread << 7 & 0xbf80bf80u, factor);
 }
 
-__device__ __forceinline__ uint4 load_held(const char* at) {
+__device__ __forceinline__ void store_shared(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ uint4 load_shared(uint32_t at) {
   uint4 v;
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(at) : "memory");
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
   return v;
 }
+// Global to shared memory (16-byte aligned, a multiple of 16 bytes); counts its bytes on `bar`.
+__device__ __forceinline__ void bulk_copy(uint32_t target, const char* source, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(target), "l"(source), "r"(bytes), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void bulk_prefetch(const char* source, uint32_t bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;\n" ::"l"(source), "r"(bytes) : "memory");
+}
 
-template <int kFormat, int kWidth>
-__device__ void convert_role(const Params& p, const Shared& sm) {
+// Eight rows of a tile (a group) lie together: their boxes of 64 features one after the other, each 1024 bytes as the products want them. Before that the rows' 8-bit
+// numbers lie in the upper half of the same memory.
+template <int kWidth> constexpr int kGroupBytes = kWidth / 64 * 1024;
+template <int kWidth> constexpr int kHeldBytes = kWidth * 8;
+static_assert(kGroupBytes<576> == 2 * kHeldBytes<576> && kGroupBytes<512> == 2 * kHeldBytes<512>, "the numbers fill half of what their values do");
+constexpr int kAhead = 4;  // chunks whose rows are on their way to L2
+
+template <int kWidth>
+__device__ void copy_role8(const Params& p, const Shared& sm) {
   using L = Layout<kWidth>;
-  constexpr int kLoads = kWidth == 576 ? 9 : 8;
-  const int warp = (threadIdx.x >> 5) - kConvertWarp0, lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31;
   volatile int* abort_flag = sm.abort_flag();
-  // Load k < 8: row `row` + 8 k, sixteen of the first 512 features; two warps share a pair of rows. Eight neighbouring lanes have rows of either parity, so that their
-  // stores go to different banks (the swizzle exchanges a row's units of 16 bytes by its number). Load 8: the other 64 features of eight rows.
-  const int row = 2 * (warp & 3) + (lane >> 2 & 1), box = 4 * (warp >> 2) + (lane >> 3), unit = 2 * (lane & 3);
-  const int rest_row = 8 * warp + (lane >> 2);
-  const int source = row * kWidth + box * 64 + unit * 8, rest_source = rest_row * kWidth + LATENT_VALUES + unit * 8;
-  const uint32_t target = box * kBoxBytes + row * 128 + ((unit ^ row) << 4);
-  const uint32_t rest_target = (LATENT_VALUES / 64) * kBoxBytes + rest_row * 128 + ((unit ^ (rest_row & 7)) << 4);
-  uint4 raw[kLoads];
-#pragma unroll
-  for (int k = 0; k < kLoads; ++k) raw[k] = make_uint4(0, 0, 0, 0);
   uint32_t count = 0;
   bool given_up = false;
   Walk walk(sm);
@@ -83,68 +89,95 @@ __device__ void convert_role(const Params& p, const Shared& sm) {
     const Piece& piece = walk.piece;
     if (piece.first == piece.last) continue;  // sees nothing
     const int32_t* table = p.table + size_t(piece.request) * p.pages;
-    auto page_of = [&](int chunk) {  // lane l: the page of chunk `chunk + l`, or -1
-      const int column = over(min(chunk + lane, piece.last - 1), p.by_page);
-      return column < p.pages ? table[column] : -1;
+    // Lane l: the first row of chunk `chunk + l` in the cache, or -1.
+    auto rows_of = [&](int chunk) {
+      const int own = min(chunk + lane, piece.last - 1), column = over(own, p.by_page);
+      const int page = column < p.pages ? table[column] : -1;
+      return unsigned(page) < unsigned(p.blocks) ? int64_t(page) * p.page_rows + (own * kChunk - column * p.page_rows) : int64_t(-1);
     };
-    int pages = page_of(piece.first);  // of 32 chunks
-    // Where the chunk lies; its rows' scales, of rows `lane` and `lane` + 32; how many rows may be read.
-    struct Place {
-      const char* at;
-      int scale_low, scale_high, valid;
-    };
-    auto place_of = [&](int chunk) {
-      const int page = __shfl_sync(0xffffffffu, pages, (chunk - piece.first) & 31);
-      Place place = {p.held, 0, 0, 0};
-      if (unsigned(page) < unsigned(p.blocks)) {
-        const int64_t first = int64_t(page) * p.page_rows + (chunk * kChunk - over(chunk, p.by_page) * p.page_rows);
-        place.at = p.held + first * kWidth;
-        place.valid = min(kChunk, piece.length - chunk * kChunk);
-        place.scale_low = p.scales[(first + lane) >> p.block_shift];
-        place.scale_high = p.scales[(first + lane + 32) >> p.block_shift];
-      } else if (warp == 0 && lane == 0) {
-        report(p.status, SPARSE_MLA_STATUS_BAD_PAGE, int(piece.row / p.heads), chunk * kChunk);
-      }
-      return place;
-    };
-    auto load = [&](const Place& place, int k) { raw[k] = load_held(place.at + (k < 8 ? source + k * 8 * kWidth : rest_source)); };
-    Place next = place_of(piece.first);
-    if (next.valid > 0) {
-#pragma unroll
-      for (int k = 0; k < kLoads; ++k) load(next, k);
-    }
+    auto valid_of = [&](int chunk) { return min(kChunk, piece.length - chunk * kChunk); };
+    int64_t rows = 0, next_rows = rows_of(piece.first);  // of 32 chunks; of the next 32
     for (int chunk = piece.first; chunk < piece.last; ++chunk, ++count) {
-      const Place own = next;
-      next.valid = 0;
-      if (chunk + 1 < piece.last) {
-        if (((chunk + 1 - piece.first) & 31) == 0) pages = page_of(chunk + 1);
-        next = place_of(chunk + 1);
+      const int place = (chunk - piece.first) & 31;
+      if (place == 0) {
+        rows = next_rows;
+        if (chunk + 32 < piece.last) next_rows = rows_of(chunk + 32);
+        if (lane < kAhead && chunk + lane < piece.last && rows >= 0) bulk_prefetch(p.held + rows * kWidth, valid_of(chunk + lane) * kWidth);
       }
-      // (what is behind the request's length, or in no page, becomes zeros: as bits any byte is a finite number)
-      const uint32_t low = lane < own.valid ? multiplier_of<kFormat>(own.scale_low) : 0u, high = lane + 32 < own.valid ? multiplier_of<kFormat>(own.scale_high) : 0u;
-      const bool twice = __any_sync(0xffffffffu, max(own.scale_low == 255 ? 0 : own.scale_low, own.scale_high == 255 ? 0 : own.scale_high) > kMostInOne);
-      const uint32_t stage = count % kStages, use = count / kStages;
+      // (the first chunks of a window are asked for above)
+      if (place + kAhead < 32 && lane == place + kAhead && chunk + kAhead < piece.last && rows >= 0) bulk_prefetch(p.held + rows * kWidth, valid_of(chunk + kAhead) * kWidth);
+      const int64_t first = __shfl_sync(0xffffffffu, rows, place);
+      const int valid = first >= 0 ? valid_of(chunk) : 0;
+      int low = 0, high = 0;
+      if (first >= 0) {
+        low = p.scales[(first + lane) >> p.block_shift];
+        high = p.scales[(first + lane + 32) >> p.block_shift];
+      }
+      const uint32_t stage = count % kStages, use = count / kStages, target = sm.base + stage * L::kTileBytes, bar = sm.bar(kLanded0 + stage);
       if (use > 0 && !warp_wait(sm.bar(kFree0 + stage), (use - 1) & 1, abort_flag)) { given_up = true; break; }
-      unsigned char* tile = sm.ptr + stage * L::kTileBytes;
-      if (warp == 0 && lane == 0) *sm.live(stage) = own.valid;
+      if (lane == 0) {
+        *sm.live(stage) = valid;
+        if (first < 0) report(p.status, SPARSE_MLA_STATUS_BAD_PAGE, int(piece.row / p.heads), chunk * kChunk);
+      }
+      unsigned char* scales = sm.ptr + L::kSmemScales + stage * kChunk;
+      scales[lane] = static_cast<unsigned char>(low);
+      scales[lane + 32] = static_cast<unsigned char>(high);
+      __syncwarp();
+      if (lane == 0) mbar_arrive_expect(bar, valid * kWidth);
+      __syncwarp();
+      const int own = min(valid - lane * 8, 8);  // rows of group `lane`
+      if (lane < 8 && own > 0) bulk_copy(target + lane * kGroupBytes<kWidth> + kHeldBytes<kWidth>, p.held + (first + lane * 8) * kWidth, own * kWidth, bar);
+    }
+  }
+  if (*abort_flag != 0) {  // nothing of this block may be written behind its end
+    int never = 0;
+    for (uint32_t i = count > kStages ? count - kStages : 0; i < count; ++i) mbar_wait(sm.bar(kLanded0 + i % kStages), (i / kStages) & 1, &never);
+  }
+}
+
+// A warp to each group: its numbers to registers, and as values over the memory that they lay in.
+template <int kFormat, int kWidth>
+__device__ void convert_role(const Params& p, const Shared& sm) {
+  using L = Layout<kWidth>;
+  constexpr int kLoads = kWidth == 576 ? 9 : 8;
+  const int group = (threadIdx.x >> 5) - kConvertWarp0, lane = threadIdx.x & 31;
+  volatile int* abort_flag = sm.abort_flag();
+  // Load k < 8: of row 2 (k / 2) + `odd` sixteen features of its half number k % 2. Eight neighbouring lanes have rows of either parity, so that their stores go to
+  // different banks (the swizzle exchanges a row's units of 16 bytes by its number), and 64 bytes in different halves of 128 for the loads. Load 8: the other
+  // 64 features of all rows.
+  const int odd = lane >> 2 & 1, unit = 2 * (lane & 3), box = lane >> 3 ^ (kWidth == 512 ? odd : 0), rest_row = lane >> 2;
+  const uint32_t base = sm.base + group * kGroupBytes<kWidth>;
+  const uint32_t source = base + kHeldBytes<kWidth> + odd * kWidth + box * 64 + unit * 8, rest_source = base + kHeldBytes<kWidth> + rest_row * kWidth + LATENT_VALUES + unit * 8;
+  const uint32_t target = base + box * 1024 + odd * 128 + ((unit ^ odd) << 4), rest_target = base + LATENT_VALUES / 64 * 1024 + rest_row * 128 + ((unit ^ rest_row) << 4);
+  uint32_t count = 0;
+  Walk walk(sm);
+  for (; walk.next_of_warp(); walk.done_of_warp()) {
+    for (int left = walk.piece.last - walk.piece.first; left > 0; --left, ++count) {
+      const uint32_t stage = count % kStages, tile = stage * L::kTileBytes;
+      if (!warp_wait(sm.bar(kLanded0 + stage), (count / kStages) & 1, abort_flag)) return;
+      const int byte = sm.ptr[L::kSmemScales + stage * kChunk + group * 8 + (lane & 7)], live = *sm.live(stage);
+      uint4 raw[kLoads];
+#pragma unroll
+      for (int k = 0; k < kLoads; ++k) raw[k] = load_shared(tile + (k < 8 ? source + (k >> 1) * 2 * kWidth + (k & 1) * 256 : rest_source));
+      // What is behind the request's length, or in no page, becomes zeros: as bits any byte is a finite number.
+      const uint32_t own = group * 8 + (lane & 7) < live ? multiplier_of<kFormat>(byte) : 0u;
+      const bool twice = __any_sync(0xffffffffu, byte != 255 && byte > kMostInOne);  // (scales above 2^7)
+      const uint32_t more = twice ? second_multiplier_of<kFormat>(byte) : 0u;
+      __syncwarp();  // all of the group's numbers are in registers
 #pragma unroll
       for (int k = 0; k < kLoads; ++k) {
-        const int from = k < 8 ? (row + 8 * k) & 31 : rest_row & 31;
-        const bool upper = k < 8 ? k >= 4 : warp >= 4;
-        const uint32_t factor = __shfl_sync(0xffffffffu, upper ? high : low, from);
-        const uint4 v = raw[k];
-        uint32_t words[8] = {widened<kFormat, 0>(v.x, factor), widened<kFormat, 1>(v.x, factor), widened<kFormat, 0>(v.y, factor), widened<kFormat, 1>(v.y, factor),
-                             widened<kFormat, 0>(v.z, factor), widened<kFormat, 1>(v.z, factor), widened<kFormat, 0>(v.w, factor), widened<kFormat, 1>(v.w, factor)};
+        const int row = k < 8 ? 2 * (k >> 1) + odd : rest_row;
+        const uint32_t factor = __shfl_sync(0xffffffffu, own, row);
+        const uint32_t to = tile + (k < 8 ? (target ^ (k >> 1) << 5) + (k >> 1) * 256 + (k & 1) * 4096 : rest_target);
+        uint32_t words[8] = {widened<kFormat, 0>(raw[k].x, factor), widened<kFormat, 1>(raw[k].x, factor), widened<kFormat, 0>(raw[k].y, factor), widened<kFormat, 1>(raw[k].y, factor),
+                             widened<kFormat, 0>(raw[k].z, factor), widened<kFormat, 1>(raw[k].z, factor), widened<kFormat, 0>(raw[k].w, factor), widened<kFormat, 1>(raw[k].w, factor)};
         if (twice) {
-          const int byte = __shfl_sync(0xffffffffu, upper ? own.scale_high : own.scale_low, from);
-          const uint32_t more = second_multiplier_of<kFormat>(byte);
+          const uint32_t again = __shfl_sync(0xffffffffu, more, row);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) words[e] = multiply_pair<kFormat>(words[e], more);
+          for (int e = 0; e < 8; ++e) words[e] = multiply_pair<kFormat>(words[e], again);
         }
-        const uint32_t at = k < 8 ? target + k * 1024 : rest_target;
-        *reinterpret_cast<uint4*>(tile + at) = make_uint4(words[0], words[1], words[2], words[3]);
-        *reinterpret_cast<uint4*>(tile + (at ^ 16)) = make_uint4(words[4], words[5], words[6], words[7]);
-        if (next.valid > 0) load(next, k);
+        store_shared(to, words[0], words[1], words[2], words[3]);
+        store_shared(to ^ 16, words[4], words[5], words[6], words[7]);
       }
       fence_proxy_async();  // products read the tile through the async proxy
       __syncwarp();
@@ -153,20 +186,19 @@ __device__ void convert_role(const Params& p, const Shared& sm) {
   }
 }
 
-// A softmax thread holds a row's 32 scores twice: 144 + 72 + 72 + 96 + 96 of the warpgroups' 5 x 96 registers.
-__device__ __forceinline__ void share_registers(int warp) {
-  if (warp < kSoftmaxWarps) asm volatile("setmaxnreg.inc.sync.aligned.u32 144;\n");
-  else if (warp < kConvertWarp0) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n");
-}
+// Of the warpgroups' 5 x 96 registers a softmax thread has 128, one that brings chunks 112, the others 64. (Each at the head of its role's branch.)
+__device__ __forceinline__ void take_128_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 128;\n"); }
+__device__ __forceinline__ void take_112_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 112;\n"); }
+__device__ __forceinline__ void keep_64_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 64;\n"); }
 
-// As `query_role`, with a subpartition's rows all one warp's: in three parts, so that few registers do.
+// As `query_role`, with a subpartition's rows all one warp's: in four parts, so that few registers do.
 template <int kWidth>
 __device__ void query_role8(const Params& p, const Shared& sm, uint32_t tmem) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int* abort_flag = sm.abort_flag();
   const int subpartition = warp & 3;
   const uint32_t lanes = uint32_t(subpartition * 32) << 16;
-  constexpr int kSegments = kWidth / 32, kParts = 3, kOwn = (kSegments + kParts - 1) / kParts;
+  constexpr int kSegments = kWidth / 32, kParts = 4, kOwn = (kSegments + kParts - 1) / kParts;
   uint32_t loads = 0;
   Walk walk(sm);
   for (; walk.next_of_warp(); walk.done_of_warp()) {
