@@ -71,7 +71,7 @@ struct Layout {
   static constexpr int kSmemP = kStages * kTileBytes;            // 64 rows x 64 weights; the output on its way out
   static constexpr int kSmemPieces = kSmemP + kRows * 128;
   static constexpr int kSmemBars = kSmemPieces + kPieces * 64;
-  static constexpr int kSmemAlpha = kSmemBars + 256;             // float[2][64]
+  static constexpr int kSmemAlpha = kSmemBars + 320;             // float[2][64]
   static constexpr int kSmemInverse = kSmemAlpha + 2 * kRows * 4;  // float[64]
   static constexpr int kSmemMisc = kSmemInverse + kRows * 4;
   static constexpr int kSmemScales = kSmemMisc + 64;             // bytes[3][64], of rows in 8 bits
@@ -81,9 +81,10 @@ static_assert(Layout<576>::kSmemBytes <= 232448, "one block per SM");
 
 enum Bar {
   kFull0 = 0, kFree0 = kFull0 + kStages, kPieceReady0 = kFree0 + kStages, kPieceDone0 = kPieceReady0 + kPieces, kQFull = kPieceDone0 + kPieces,
-  kQFree, kPlaces, kScoresFull, kScoresFree, kWeightsFull, kWeightsFree, kMended, kGivenUp0, kGivenUp1, kLanded0, kBarCount = kLanded0 + kStages
+  kQFree, kPlaces, kScoresFull, kScoresFree, kWeightsFull, kWeightsFree, kMended, kGivenUp0, kGivenUp1, kLanded0, kFreeHalf0 = kLanded0 + 2 * kStages,
+  kBarCount = kFreeHalf0 + kStages
 };
-static_assert(kBarCount <= 32, "the barrier area");
+static_assert(kBarCount <= 40, "the barrier area");
 
 // Workspace: per block a record, statistics and sums of two slots (2 i: a tile that begins in an earlier block; 2 i + 1: one that begins here and
 // ends in a later one).
@@ -670,13 +671,14 @@ __device__ __forceinline__ void issue_scores(uint32_t tmem, uint64_t x_desc) {
     issue_scores<kFormat, kSteps, kBox, K + 1>(tmem, x_desc);
   }
 }
-template <int kFormat, int kBox, int kGroup, bool kFirst, int I = 0>
+// Steps I to kEnd - 1 of the chunk's, two for every 16 rows.
+template <int kFormat, int kBox, int kGroup, bool kFirst, int kEnd, int I>
 __device__ __forceinline__ void issue_values(uint32_t tmem, uint64_t p_desc, uint64_t x_desc) {
-  if constexpr (I < 2 * (kChunk / 16)) {
+  if constexpr (I < kEnd) {
     constexpr int half = I % 2, k = I / 2;
     constexpr uint32_t offset = half * 4 * kBox + k * 2 * kGroup;
     mma_ws_ss_c<!(kFirst && k == 0)>(tmem + half * 128, p_desc + ((k * 32) >> 4), x_desc + (offset >> 4), kIdescValues<kFormat>);
-    issue_values<kFormat, kBox, kGroup, kFirst, I + 1>(tmem, p_desc, x_desc);
+    issue_values<kFormat, kBox, kGroup, kFirst, kEnd, I + 1>(tmem, p_desc, x_desc);
   }
 }
 
@@ -702,7 +704,8 @@ __device__ void score_role(const Shared& sm, uint32_t tmem) {
   }
 }
 
-template <int kFormat, int kWidth, int kBox, int kGroup>
+// kHalves: says so when the first half of the chunk's rows have been used.
+template <int kFormat, int kWidth, int kBox, int kGroup, bool kHalves>
 __device__ void value_role(const Shared& sm, uint32_t tmem) {
   volatile int* abort_flag = sm.abort_flag();
   uint32_t count = 0;
@@ -715,8 +718,16 @@ __device__ void value_role(const Shared& sm, uint32_t tmem) {
       if (!mbar_wait(sm.bar(kWeightsFull), count & 1, abort_flag)) return;
       tc_fence_after_sync();
       const uint64_t x_desc = smem_desc_sw128(sm.base + stage * Layout<kWidth>::kTileBytes, kBox, kGroup);
-      if (i == 0) issue_values<kFormat, kBox, kGroup, true>(tmem, p_desc, x_desc);
-      else issue_values<kFormat, kBox, kGroup, false>(tmem, p_desc, x_desc);
+      constexpr int kSteps = 2 * (kChunk / 16);
+      if constexpr (kHalves) {
+        if (i == 0) issue_values<kFormat, kBox, kGroup, true, kSteps / 2, 0>(tmem, p_desc, x_desc);
+        else issue_values<kFormat, kBox, kGroup, false, kSteps / 2, 0>(tmem, p_desc, x_desc);
+        mma_commit(sm.bar(kFreeHalf0 + stage));
+        issue_values<kFormat, kBox, kGroup, false, kSteps, kSteps / 2>(tmem, p_desc, x_desc);
+      } else {
+        if (i == 0) issue_values<kFormat, kBox, kGroup, true, kSteps, 0>(tmem, p_desc, x_desc);
+        else issue_values<kFormat, kBox, kGroup, false, kSteps, 0>(tmem, p_desc, x_desc);
+      }
       mma_commit(sm.bar(kWeightsFree));
       mma_commit(sm.bar(kFree0 + stage));
     }
@@ -996,7 +1007,7 @@ __global__ void __launch_bounds__(kHeld8 ? kThreads8 : kThreads, 1) attention_ke
     if (elect_one()) {
       constexpr int kBox = kHeld8 ? 1024 : kBoxBytes, kGroup = kHeld8 ? kGroupBytes<kWidth> : 1024;
       if (warp == kScoreWarp) score_role<kFormat, kWidth, kBox, kGroup>(sm, tmem);
-      else value_role<kFormat, kWidth, kBox, kGroup>(sm, tmem);
+      else value_role<kFormat, kWidth, kBox, kGroup, kHeld8>(sm, tmem);
       if (*sm.abort_flag() != 0) wait_for_products(sm.bar(warp == kScoreWarp ? kGivenUp0 : kGivenUp1));
     }
     __syncwarp();

@@ -83,7 +83,7 @@ __device__ void copy_role8(const Params& p, const Shared& sm) {
   const int lane = threadIdx.x & 31;
   volatile int* abort_flag = sm.abort_flag();
   uint32_t count = 0;
-  bool given_up = false;
+  bool given_up = false, half_given = false;
   Walk walk(sm);
   for (; !given_up && walk.next_of_warp(); walk.done_of_warp()) {
     const Piece& piece = walk.piece;
@@ -113,25 +113,40 @@ __device__ void copy_role8(const Params& p, const Shared& sm) {
         low = p.scales[(first + lane) >> p.block_shift];
         high = p.scales[(first + lane + 32) >> p.block_shift];
       }
-      const uint32_t stage = count % kStages, use = count / kStages, target = sm.base + stage * L::kTileBytes, bar = sm.bar(kLanded0 + stage);
-      if (use > 0 && !warp_wait(sm.bar(kFree0 + stage), (use - 1) & 1, abort_flag)) { given_up = true; break; }
-      if (lane == 0) {
-        *sm.live(stage) = valid;
-        if (first < 0) report(p.status, SPARSE_MLA_STATUS_BAD_PAGE, int(piece.row / p.heads), chunk * kChunk);
+      const uint32_t stage = count % kStages, use = count / kStages, target = sm.base + stage * L::kTileBytes + lane * kGroupBytes<kWidth> + kHeldBytes<kWidth>;
+      const char* source = p.held + (first + lane * 8) * kWidth;
+      const int own = min(max(valid - lane * 8, 0), 8);  // rows of group `lane`
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {  // (the first four groups' memory is free earlier)
+        const uint32_t bar = sm.bar(kLanded0 + 2 * stage + half);
+        if (use > 0 && !warp_wait(sm.bar((half ? kFree0 : kFreeHalf0) + stage), (use - 1) & 1, abort_flag)) {
+          given_up = true;
+          half_given = half == 1;
+          break;
+        }
+        if (half == 0) {
+          // (what the chunk before says has been read: its second product has begun)
+          if (lane == 0) {
+            *sm.live(stage) = valid;
+            if (first < 0) report(p.status, SPARSE_MLA_STATUS_BAD_PAGE, int(piece.row / p.heads), chunk * kChunk);
+          }
+          unsigned char* scales = sm.ptr + L::kSmemScales + stage * kChunk;
+          scales[lane] = static_cast<unsigned char>(low);
+          scales[lane + 32] = static_cast<unsigned char>(high);
+          __syncwarp();
+        }
+        if (lane == 0) mbar_arrive_expect(bar, min(max(valid - half * 32, 0), 32) * kWidth);
+        __syncwarp();
+        if (lane >> 2 == half && own > 0) bulk_copy(target, source, own * kWidth, bar);
       }
-      unsigned char* scales = sm.ptr + L::kSmemScales + stage * kChunk;
-      scales[lane] = static_cast<unsigned char>(low);
-      scales[lane + 32] = static_cast<unsigned char>(high);
-      __syncwarp();
-      if (lane == 0) mbar_arrive_expect(bar, valid * kWidth);
-      __syncwarp();
-      const int own = min(valid - lane * 8, 8);  // rows of group `lane`
-      if (lane < 8 && own > 0) bulk_copy(target + lane * kGroupBytes<kWidth> + kHeldBytes<kWidth>, p.held + (first + lane * 8) * kWidth, own * kWidth, bar);
+      if (given_up) break;
     }
   }
   if (*abort_flag != 0) {  // nothing of this block may be written behind its end
     int never = 0;
-    for (uint32_t i = count > kStages ? count - kStages : 0; i < count; ++i) mbar_wait(sm.bar(kLanded0 + i % kStages), (i / kStages) & 1, &never);
+    for (uint32_t i = count > kStages ? count - kStages : 0; i < count; ++i)
+      for (int half = 0; half < 2; ++half) mbar_wait(sm.bar(kLanded0 + 2 * (i % kStages) + half), (i / kStages) & 1, &never);
+    if (half_given) mbar_wait(sm.bar(kLanded0 + 2 * (count % kStages)), (count / kStages) & 1, &never);
   }
 }
 
@@ -154,7 +169,7 @@ __device__ void convert_role(const Params& p, const Shared& sm) {
   for (; walk.next_of_warp(); walk.done_of_warp()) {
     for (int left = walk.piece.last - walk.piece.first; left > 0; --left, ++count) {
       const uint32_t stage = count % kStages, tile = stage * L::kTileBytes;
-      if (!warp_wait(sm.bar(kLanded0 + stage), (count / kStages) & 1, abort_flag)) return;
+      if (!warp_wait(sm.bar(kLanded0 + 2 * stage + (group >> 2)), (count / kStages) & 1, abort_flag)) return;
       const int byte = sm.ptr[L::kSmemScales + stage * kChunk + group * 8 + (lane & 7)], live = *sm.live(stage);
       uint4 raw[kLoads];
 #pragma unroll
@@ -163,9 +178,7 @@ __device__ void convert_role(const Params& p, const Shared& sm) {
       const uint32_t own = group * 8 + (lane & 7) < live ? multiplier_of<kFormat>(byte) : 0u;
       const bool twice = __any_sync(0xffffffffu, byte != 255 && byte > kMostInOne);  // (scales above 2^7)
       const uint32_t more = twice ? second_multiplier_of<kFormat>(byte) : 0u;
-      __syncwarp();  // all of the group's numbers are in registers
-#pragma unroll
-      for (int k = 0; k < kLoads; ++k) {
+      auto widen = [&](int k) {
         const int row = k < 8 ? 2 * (k >> 1) + odd : rest_row;
         const uint32_t factor = __shfl_sync(0xffffffffu, own, row);
         const uint32_t to = tile + (k < 8 ? (target ^ (k >> 1) << 5) + (k >> 1) * 256 + (k & 1) * 4096 : rest_target);
@@ -178,7 +191,13 @@ __device__ void convert_role(const Params& p, const Shared& sm) {
         }
         store_shared(to, words[0], words[1], words[2], words[3]);
         store_shared(to ^ 16, words[4], words[5], words[6], words[7]);
-      }
+      };
+#pragma unroll
+      for (int k = 0; k < 8; k += 2) widen(k);  // to the lower half of the group's memory
+      __syncwarp();  // all of its numbers are in registers
+#pragma unroll
+      for (int k = 1; k < 8; k += 2) widen(k);
+      if constexpr (kLoads > 8) widen(8);
       fence_proxy_async();  // products read the tile through the async proxy
       __syncwarp();
       if (lane == 0) mbar_arrive(sm.bar(kFull0 + stage));
