@@ -2,15 +2,19 @@
 //
 // k = least whole number with max|v| <= 448 2^k over the block's new rows, and not below the block's own where older rows precede them; c = v 2^-k rounded
 // to e4m3. As scales are powers of two, a division by one is exact: a number is rounded once (and once more where its block's scale grows and it becomes a
-// subnormal one). Rows are read twice, for the maximum and for the numbers, the second time from L1 or L2.
+// subnormal one). Bound by latency: four rows to a warp, all of whose loads are on their way together, and which stay in registers between the maximum and the
+// numbers (rows of more than 512 features in front or 32 pairs are read twice). A block's warps meet once. 8192 rows in blocks of 64 (14 MB): 14.6 us with eight rows to a warp that
+// were read twice.
 #include "latent_common.cuh"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace latent {
 namespace {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kThreads = 512, kWarps = kThreads / 32, kRowsPerWarp = 4;
+constexpr int kMostFront = 512, kMostPairs = 32;  // of rows that registers hold
 constexpr uint32_t kInfinity = 0x7f800000u, kMostHalf = 0x47700000u;  // bits of FP32 numbers: infinity, 61440
 
 struct Append8Params {
@@ -52,80 +56,113 @@ __device__ __forceinline__ float cut(float v) {
   return std::is_same<T, __half>::value ? fminf(fmaxf(v, -61440.f), 61440.f) : v;
 }
 
-// A block of rows by one warp (kTogether 1) or by the eight of a block of threads.
-template <typename T, bool kHalves, int kTogether>
+// A block of rows by `together` neighbouring warps of a block of threads, every together-th row by one of them.
+template <typename T, bool kHalves, bool kKept>
 __global__ void __launch_bounds__(kThreads) append8_kernel(const Append8Params p) {
   __shared__ uint32_t maxima[kWarps];
   const latent_append_call& c = p.c;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, member = kTogether == 1 ? 0 : warp;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, block = 1 << p.shift, together = max(block / kRowsPerWarp, 1), member = warp & (together - 1);
   sm100::wait_for_predecessor();
   sm100::let_successor_start();
-  const int64_t item = kTogether == 1 ? int64_t(blockIdx.x) * kWarps + warp : blockIdx.x;
-  const int batches = int(c.batches), block = 1 << p.shift;
-  if (item >= items_before(p, batches)) return;
-  int request = 0;
-  for (int high = batches; high - request > 1;) {
-    const int middle = (request + high) >> 1;
-    if (items_before(p, middle) <= item) request = middle; else high = middle;
+  const int64_t item = (int64_t(blockIdx.x) * kWarps + warp) / together;
+  const int batches = int(c.batches), pairs = int(c.pairs), front = int(c.width) - 2 * pairs;
+  // Rows `older` .. rows - 1 of a block are the call's; its first row lies at `row0` of the cache and has position `base`. None: older = rows.
+  int older = 0, rows = 0, begin = 0;
+  int64_t base = 0, row0 = 0, start = 0;
+  if (item < items_before(p, batches)) {
+    int request = 0;
+    for (int high = batches; high - request > 1;) {
+      const int middle = (request + high) >> 1;
+      if (items_before(p, middle) <= item) request = middle; else high = middle;
+    }
+    const int64_t which = item - items_before(p, request);
+    // (the request's tokens as the attention calls see them: offsets outside of the call's tokens are clamped)
+    begin = bounded(c.cu_seqlens_q[request], int(c.tokens));
+    const int count = bounded(c.cu_seqlens_q[request + 1], int(c.tokens)) - begin;
+    const int64_t end = c.seqused_kv[request];
+    start = end - count;  // position of the request's first new row
+    if (which >= 0 && count > 0) {
+      if (which == 0 && start < 0 && member == 0 && lane == 0) report(c.status, SPARSE_MLA_STATUS_BAD_PAGE, begin, int(start));
+      base = ((max(start, int64_t(0)) >> p.shift) + which) << p.shift;
+      const int64_t first = max(max(start, int64_t(0)), base), last = min(end, base + block);
+      if (first < last) {
+        const int64_t column = base / c.page_rows;
+        int64_t page = -1;
+        if (column < c.pages) page = c.block_table[request * c.pages + column];
+        if (page >= 0 && page < c.blocks) {
+          row0 = page * c.page_rows + (base - column * c.page_rows);
+          older = int(first - base);
+          rows = int(last - base);
+        } else if (member == 0 && lane == 0) {  // nowhere to put them: reported, not written
+          report(c.status, SPARSE_MLA_STATUS_BAD_PAGE, int(begin + (first - start)), int(first));
+        }
+      }
+    }
   }
-  const int64_t which = item - items_before(p, request);
-  // (the request's tokens as the attention calls see them: offsets outside of the call's tokens are clamped)
-  const int begin = bounded(c.cu_seqlens_q[request], int(c.tokens)), count = bounded(c.cu_seqlens_q[request + 1], int(c.tokens)) - begin;
-  const int64_t end = c.seqused_kv[request], start = end - count;  // positions of the new rows
-  if (which < 0 || count <= 0) return;
-  if (which == 0 && start < 0 && member == 0 && lane == 0) report(c.status, SPARSE_MLA_STATUS_BAD_PAGE, begin, int(start));
-  const int64_t base = ((max(start, int64_t(0)) >> p.shift) + which) << p.shift;  // of the block
-  const int64_t first = max(max(start, int64_t(0)), base), last = min(end, base + block);
-  if (first >= last) return;
-  const int64_t column = base / c.page_rows;
-  int64_t page = -1;
-  if (column < c.pages) page = c.block_table[request * c.pages + column];
-  if (page < 0 || page >= c.blocks) {  // nowhere to put them: reported, not written
-    if (member == 0 && lane == 0) report(c.status, SPARSE_MLA_STATUS_BAD_PAGE, int(begin + (first - start)), int(first));
-    return;
-  }
-  const int64_t row0 = page * c.page_rows + (base - column * c.page_rows);  // the block's first row in the cache
-  const int older = int(first - base), rows = int(last - base), pairs = int(c.pairs), front = int(c.width) - 2 * pairs;
   const T* latent = static_cast<const T*>(c.latent) + (begin + (base - start)) * c.latent_token;  // of the block's row 0, which may be none of the call's
   const T* rope = static_cast<const T*>(c.rope) + (begin + (base - start)) * c.rope_token;
   uint8_t* held = static_cast<uint8_t*>(c.cache) + row0 * c.width;
-  auto turned = [&](int row, int i) {
+  auto mine = [&](int n) { return member + n * together; };
+  auto is_new = [&](int n) { return mine(n) >= older && mine(n) < rows; };
+  auto turned = [&](int row, int i, float u, float v) {
     const float2 t = turn_of(base + row, turns_of(c.inv_freq[i]), float(c.amplitude));
-    const T* own = rope + row * c.rope_token;
-    const float u = to_float(own[kHalves ? i : 2 * i]), v = to_float(own[kHalves ? i + pairs : 2 * i + 1]);
     return make_float2(u * t.x - v * t.y, u * t.y + v * t.x);
   };
+  auto rope_of = [&](int row, int i) {
+    const T* own = rope + row * c.rope_token;
+    return make_float2(to_float(own[kHalves ? i : 2 * i]), to_float(own[kHalves ? i + pairs : 2 * i + 1]));
+  };
 
+  uint4 kept[kRowsPerWarp][2];
+  float2 kept_pair[kRowsPerWarp];
   uint32_t most = 0;
-#pragma unroll 2
-  for (int row = older + member; row < rows; row += kTogether) {
-    for (int at = lane * 8; at < front; at += 256) {
-      const uint4 words = *reinterpret_cast<const uint4*>(latent + row * c.latent_token + at);
-      const T* v = reinterpret_cast<const T*>(&words);
+  auto see = [&](const uint4& words) {
+    const T* v = reinterpret_cast<const T*>(&words);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) most = max(most, magnitude<T>(to_float(v[e])));
+    for (int e = 0; e < 8; ++e) most = max(most, magnitude<T>(to_float(v[e])));
+  };
+  if constexpr (kKept) {
+#pragma unroll
+    for (int n = 0; n < kRowsPerWarp; ++n) {
+      kept[n][0] = kept[n][1] = make_uint4(0, 0, 0, 0);
+      kept_pair[n] = make_float2(0.f, 0.f);
+      if (!is_new(n)) continue;
+      const T* row = latent + mine(n) * c.latent_token;
+      if (lane * 8 < front) kept[n][0] = *reinterpret_cast<const uint4*>(row + lane * 8);
+      if (lane * 8 + 256 < front) kept[n][1] = *reinterpret_cast<const uint4*>(row + lane * 8 + 256);
+      if (lane < pairs) kept_pair[n] = rope_of(mine(n), lane);
     }
-    for (int i = lane; i < pairs; i += 32) {
-      const float2 v = turned(row, i);
-      most = max(most, max(magnitude<T>(v.x), magnitude<T>(v.y)));
+#pragma unroll
+    for (int n = 0; n < kRowsPerWarp; ++n) {
+      if (!is_new(n)) continue;
+      see(kept[n][0]);
+      see(kept[n][1]);
+      if (lane < pairs) kept_pair[n] = turned(mine(n), lane, kept_pair[n].x, kept_pair[n].y);
+      most = max(most, max(magnitude<T>(kept_pair[n].x), magnitude<T>(kept_pair[n].y)));
+    }
+  } else {
+    for (int n = 0; n < kRowsPerWarp; ++n) {
+      if (!is_new(n)) continue;
+      for (int at = lane * 8; at < front; at += 256) see(*reinterpret_cast<const uint4*>(latent + mine(n) * c.latent_token + at));
+      for (int i = lane; i < pairs; i += 32) {
+        const float2 v = rope_of(mine(n), i), w = turned(mine(n), i, v.x, v.y);
+        most = max(most, max(magnitude<T>(w.x), magnitude<T>(w.y)));
+      }
     }
   }
   most = __reduce_max_sync(0xffffffffu, most);
-  if constexpr (kTogether > 1) {
-    if (lane == 0) maxima[warp] = most;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kTogether; ++w) most = max(most, maxima[w]);
-  }
   uint8_t* own_scale = p.scales + (row0 >> p.shift);
-  const int had = older > 0 ? *own_scale : 0, scale = max(scale_for(most), had);
-  if constexpr (kTogether > 1) __syncthreads();  // everybody has read the scale
-  else __syncwarp();
+  const int had = older > 0 ? *own_scale : 0;
+  if (lane == 0) maxima[warp] = most;
+  __syncthreads();  // (everybody has read the scale, too)
+  for (int w = warp - member; w < warp - member + together; ++w) most = max(most, maxima[w]);
+  if (older >= rows) return;
+  const int scale = max(scale_for(most), had);
   if (member == 0 && lane == 0) *own_scale = uint8_t(scale);
 
   if (scale > had && scale != 255) {  // the rows in front, in terms of the new scale
     const __half2 factor = __float2half2_rn(had - scale < -24 ? 0.f : __uint_as_float(uint32_t(127 + had - scale) << 23));
-    for (int row = member; row < older; row += kTogether) {
+    for (int row = member; row < older; row += together) {
       for (int at = lane * 8; at < int(c.width); at += 256) {
         uint2* place = reinterpret_cast<uint2*>(held + row * c.width + at);
         uint2 v = *place;
@@ -138,36 +175,47 @@ __global__ void __launch_bounds__(kThreads) append8_kernel(const Append8Params p
   // 1 / scale in two factors: either is a normal number
   const int half = (127 - scale) / 2, rest = 127 - scale - half;
   const float by = scale == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float(uint32_t(127 + half) << 23), and_by = __uint_as_float(uint32_t(127 + rest) << 23);
-#pragma unroll 2
-  for (int row = older + member; row < rows; row += kTogether) {
-    uint8_t* target = held + row * c.width;
-    for (int at = lane * 8; at < front; at += 256) {
-      const uint4 words = *reinterpret_cast<const uint4*>(latent + row * c.latent_token + at);
-      const T* v = reinterpret_cast<const T*>(&words);
-      uint32_t pair[4];
+  auto number = [&](float low, float high) { return numbers_of(cut<T>(low) * by * and_by, cut<T>(high) * by * and_by); };
+  auto store_latent = [&](uint8_t* target, const uint4& words) {
+    const T* v = reinterpret_cast<const T*>(&words);
+    uint32_t pair[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) pair[e] = numbers_of(cut<T>(to_float(v[2 * e])) * by * and_by, cut<T>(to_float(v[2 * e + 1])) * by * and_by);
-      *reinterpret_cast<uint2*>(target + at) = make_uint2(pair[0] | pair[1] << 16, pair[2] | pair[3] << 16);
+    for (int e = 0; e < 4; ++e) pair[e] = number(to_float(v[2 * e]), to_float(v[2 * e + 1]));
+    *reinterpret_cast<uint2*>(target) = make_uint2(pair[0] | pair[1] << 16, pair[2] | pair[3] << 16);
+  };
+  auto store_pair = [&](uint8_t* target, int i, float2 v) {
+    const uint32_t pair = number(v.x, v.y);
+    if constexpr (kHalves) {
+      target[front + i] = uint8_t(pair);
+      target[front + i + pairs] = uint8_t(pair >> 8);
+    } else {
+      *reinterpret_cast<uint16_t*>(target + front + 2 * i) = uint16_t(pair);
     }
-    for (int i = lane; i < pairs; i += 32) {
-      const float2 v = turned(row, i);
-      const uint32_t pair = numbers_of(cut<T>(v.x) * by * and_by, cut<T>(v.y) * by * and_by);
-      if constexpr (kHalves) {
-        target[front + i] = uint8_t(pair);
-        target[front + i + pairs] = uint8_t(pair >> 8);
-      } else {
-        *reinterpret_cast<uint16_t*>(target + front + 2 * i) = uint16_t(pair);
+  };
+#pragma unroll
+  for (int n = 0; n < kRowsPerWarp; ++n) {
+    if (!is_new(n)) continue;
+    uint8_t* target = held + mine(n) * c.width;
+    if constexpr (kKept) {
+      if (lane * 8 < front) store_latent(target + lane * 8, kept[n][0]);
+      if (lane * 8 + 256 < front) store_latent(target + lane * 8 + 256, kept[n][1]);
+      if (lane < pairs) store_pair(target, lane, kept_pair[n]);
+    } else {
+      for (int at = lane * 8; at < front; at += 256) store_latent(target + at, *reinterpret_cast<const uint4*>(latent + mine(n) * c.latent_token + at));
+      for (int i = lane; i < pairs; i += 32) {
+        const float2 v = rope_of(mine(n), i);
+        store_pair(target, i, turned(mine(n), i, v.x, v.y));
       }
     }
   }
 }
 
-// A warp to blocks of up to eight rows, a block of threads to larger ones.
 template <typename T, bool kHalves>
 int launch_append8(const Append8Params& p, cudaStream_t stream) {
-  const int64_t items = (p.c.tokens >> p.shift) + 2 * p.c.batches;
-  if (p.shift <= 3) return int(sm100::launch_overlapped(append8_kernel<T, kHalves, 1>, int((items + kWarps - 1) / kWarps), kThreads, 0, stream, p));
-  return int(sm100::launch_overlapped(append8_kernel<T, kHalves, kWarps>, int(items), kThreads, 0, stream, p));
+  const int64_t items = (p.c.tokens >> p.shift) + 2 * p.c.batches, together = std::max((1 << p.shift) / kRowsPerWarp, 1);
+  const bool kept = p.c.pairs <= kMostPairs && p.c.width - 2 * p.c.pairs <= kMostFront;
+  auto* kernel = kept ? append8_kernel<T, kHalves, true> : append8_kernel<T, kHalves, false>;
+  return int(sm100::launch_overlapped(kernel, int((items * together + kWarps - 1) / kWarps), kThreads, 0, stream, p));
 }
 
 }  // namespace
@@ -179,7 +227,7 @@ extern "C" int launch_latent_append8(void* stream, const latent_append8_call* ca
   const latent_append_call& c = call->append;
   if ((c.type != LATENT_F16 && c.type != LATENT_BF16) || c.pairs < 8 || c.pairs > LATENT_MOST_PAIRS || c.pairs % 8 != 0) return -1;
   if (c.width < 2 * c.pairs || c.width % 16 != 0 || c.width > 65536) return -1;
-  if (c.batches < 0 || c.batches > INT32_MAX / 4 || c.tokens < 0 || c.tokens > (int64_t(1) << 30) || c.pages < 0 || c.blocks < 0) return -1;
+  if (c.batches < 0 || c.batches > (1 << 26) || c.tokens < 0 || c.tokens > (int64_t(1) << 30) || c.pages < 0 || c.blocks < 0) return -1;
   if (c.page_rows < 64 || c.page_rows % 64 != 0 || c.pages > (INT32_MAX - 128) / c.page_rows || c.blocks > INT32_MAX / c.page_rows) return -1;
   if (call->block_rows < 1 || call->block_rows > 64 || (call->block_rows & (call->block_rows - 1)) != 0) return -1;
   if (!aligned(c.latent) || c.latent_token % 8 != 0 || !aligned(c.cache) || !fits_float(c.amplitude) || c.status == nullptr) return -1;

@@ -98,7 +98,7 @@ int append(const Tensor& latent, const Tensor& rope, const Tensor& cache, const 
   if (!on_device(latent, device, type) || !on_device(rope, device, type) || !paged(cache, table, cu, lengths, device, scales != nullptr ? at::kFloat8_e4m3fn : type, &p))
     return kRefused;
   int64_t block_rows = 0;
-  if (scales != nullptr && (!scaled(*scales, p, device, &block_rows) || p.width % 16 != 0)) return kRefused;
+  if (scales != nullptr && (!scaled(*scales, p, device, &block_rows) || p.width % 16 != 0 || p.batches > (1 << 26))) return kRefused;
   c.tokens = latent.size(0);
   c.pairs = inv_freq.size(0);
   if (c.pairs < 8 || c.pairs > LATENT_MOST_PAIRS || c.pairs % 8 != 0 || !plain(inv_freq, device, at::kDouble, {c.pairs})) return kRefused;

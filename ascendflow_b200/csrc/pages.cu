@@ -2,9 +2,10 @@
 //
 // All three operators rank things in a fixed order: free pages by number, wishes by request and entry. One cluster of eight blocks does that: a
 // block marks the pages of its eighth as bits in shared memory, the blocks exchange their sums, and each knows what is in front of it; the cluster's barrier costs a
-// fraction of a microsecond where another launch costs two. Pages are copied by a second kernel on all SMs.
+// fraction of a microsecond where another launch costs two. Pages are copied by a second kernel on all SMs, which also writes what is long and needs no order (a fork's
+// table, a compacted one). Resizing a large table is shared out in the same way: what eight SMs read of it would take longer than two more launches.
 //
-// Bound by latency (chains of loads and four to six barriers) for tables up to a megabyte, by what eight SMs read above that.
+// Bound by latency (chains of loads, and four cluster barriers) for small tables, by memory for copies.
 #include <cuda_runtime.h>
 #include <limits.h>
 #include <stdint.h>
@@ -29,11 +30,15 @@ struct Plan {
   int32_t* places;
   int32_t children;
   int32_t *numbers;            // free pages in order; compact: the pages that are moved
-  int32_t *first, *heirs;      // resize: wishes of a request, first entry that wishes; fork: a request's first child, its number of children
+  int32_t *first, *heirs;      // resize: a request's first entry that wishes, its number of wishes; fork: its first child, its number of children
+  int32_t *ranks;              // resize: wishes in front of a request's; fork: the page that a child has of its own, -1: none was left, kShared
+  int32_t *free;               // pages in `numbers`
   int4* copies;                // source, target, rows
   int32_t* copy_count;
   int32_t words;               // of 32 pages, per block
 };
+
+constexpr int kShared = -2;
 
 struct Shared {
   int32_t totals[4][kCluster];  // what the blocks tell each other
@@ -144,51 +149,111 @@ __device__ __forceinline__ Extent extent_of(const Plan& p, int request, int leng
 }
 __device__ __forceinline__ bool names_page(const Plan& p, int entry) { return unsigned(entry) < unsigned(p.c.blocks); }
 
-// Calls each(i, entry) for a warp's share of `entries` entries, several loads at a time.
+// Calls each(i, entry) for a thread's share of `entries` entries, several loads at a time.
 template <class Each>
-__device__ __forceinline__ void each_entry(const int32_t* row, int entries, Each each) {
+__device__ __forceinline__ void each_entry(const int32_t* row, int entries, int thread, int threads, Each each) {
   constexpr int kInFlight = 8;
-  for (int at = threadIdx.x & 31; at < entries; at += 32 * kInFlight) {
+  for (int at = thread; at < entries; at += threads * kInFlight) {
     int entry[kInFlight];
 #pragma unroll
-    for (int n = 0; n < kInFlight; ++n) entry[n] = at + 32 * n < entries ? row[at + 32 * n] : -1;
+    for (int n = 0; n < kInFlight; ++n) entry[n] = at + threads * n < entries ? row[at + threads * n] : -1;
 #pragma unroll
     for (int n = 0; n < kInFlight; ++n)
-      if (at + 32 * n < entries) each(at + 32 * n, entry[n]);
+      if (at + threads * n < entries) each(at + threads * n, entry[n]);
   }
 }
 
 // ---- resize ---------------------------------------------------------------------------------------------------------
 
+// Counts to another tensor, several at a time.
+__device__ __forceinline__ void copy_counts(const Plan& p, int64_t thread, int64_t threads) {
+  constexpr int kInFlight = 8;
+  for (int64_t at = thread; at < p.c.blocks; at += threads * kInFlight) {
+    int count[kInFlight];
+#pragma unroll
+    for (int n = 0; n < kInFlight; ++n) count[n] = at + n * threads < p.c.blocks ? p.c.counts_in[at + n * threads] : 0;
+#pragma unroll
+    for (int n = 0; n < kInFlight; ++n)
+      if (at + n * threads < p.c.blocks) p.c.counts_out[at + n * threads] = count[n];
+  }
+}
+
+// What a request gives back, and what it keeps; entry by entry, by `threads` threads. Wishes of this thread's entries, the first of them.
+__device__ __forceinline__ int release(const Plan& p, int request, int thread, int threads, int* first) {
+  const Extent extent = extent_of(p, request, p.c.lengths[request], thread == 0);
+  const int entries = int(p.c.entries);
+  const int32_t* in = p.c.table_in + int64_t(request) * entries;
+  int32_t* out = p.c.table_out + int64_t(request) * entries;
+  int own = 0;
+  *first = INT_MAX;
+  each_entry(in, entries, thread, threads, [&](int i, int entry) {
+    const bool has = names_page(p, entry), counts = i < extent.entries;
+    if (has && !counts) atomicSub(p.c.counts_out + entry, 1);
+    if (!has && counts) {
+      ++own;
+      *first = min(*first, i);
+    }
+    const int next = has && counts ? entry : -1;
+    if (in != out || next != entry) out[i] = next;
+  });
+  return own;
+}
+
+// A request's wishes, `wishes` from entry `first` on, get the free pages from rank `rank` on.
+__device__ __forceinline__ void give(const Plan& p, int request, int thread, int threads, int rank, int wishes, int first, int free) {
+  int32_t* out = p.c.table_out + int64_t(request) * p.c.entries;
+  auto take = [&](int i, int place) {
+    if (place < free) {
+      const int page = __ldcg(p.numbers + place);
+      out[i] = page;
+      p.c.counts_out[page] = 1;
+    } else {
+      report(p.c.status, SPARSE_MLA_STATUS_NO_PAGE, request, i);
+    }
+  };
+  const int counted = extent_of(p, request, p.c.lengths[request], false).entries;
+  if (counted - first == wishes) {  // one after the other, as where a request has grown
+    for (int i = thread; i < wishes; i += threads) take(first + i, rank + i);
+  } else if (thread < 32) {
+    for (int i0 = first; i0 < counted; i0 += 32) {
+      const int i = i0 + thread;
+      const bool wants = i < counted && out[i] < 0;
+      const unsigned wanting = __ballot_sync(0xffffffffu, wants);
+      if (wants) take(i, rank + __popc(wanting & ((1u << thread) - 1u)));
+      rank += __popc(wanting);
+    }
+  }
+}
+
+// Marks of the free pages and their list; the requests' ranks. By the cluster, behind everybody's releases; The blocks' wishes are in totals[0] behind the next cluster barrier.
+__device__ __forceinline__ void rank_wishes(const Plan& p, Shared& sm, int rank, int begin, int end) {
+  const int free_here = mark_pages<false>(p, sm, rank, p.c.counts_out, nullptr);
+  tell(sm, 1, rank, free_here);
+  cluster_barrier();
+  list_marked(p, sm, rank, in_front(sm, 1, rank), in_all(sm, 0), [](uint32_t marks, int) { return marks; }, [&](int at, int page) { p.numbers[at] = page; });
+  int rank_of_tile = in_front(sm, 0, rank);
+  for (int tile = begin; tile < end; tile += kThreads) {
+    const int request = tile + int(threadIdx.x), own = request < end ? p.heirs[request] : 0;
+    int total;
+    const int start = rank_of_tile + block_rank(sm, own, &total);
+    if (request < end) p.ranks[request] = start;
+    rank_of_tile += total;
+  }
+}
+
+// The whole of it, for a small table.
 __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 1) resize_kernel(const __grid_constant__ Plan p) {
   extern __shared__ __align__(16) unsigned char smem[];
   Shared& sm = *reinterpret_cast<Shared*>(smem);
-  const int rank = int(cluster_rank()), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int requests = int(p.c.requests), entries = int(p.c.entries);
+  const int rank = int(cluster_rank()), lane = threadIdx.x & 31, warp = threadIdx.x >> 5, requests = int(p.c.requests);
   const int share = (requests + kCluster - 1) / kCluster, begin = min(rank * share, requests), end = min(begin + share, requests);
   wait_for_predecessor();
   let_successor_start();
-  if (p.c.counts_in != p.c.counts_out) {
-    for (int64_t page = rank * kThreads + threadIdx.x; page < p.c.blocks; page += kCluster * kThreads) p.c.counts_out[page] = p.c.counts_in[page];
-  }
+  if (p.c.counts_in != p.c.counts_out) copy_counts(p, rank * kThreads + threadIdx.x, kCluster * kThreads);
   cluster_barrier();
-  // What is given back; wishes of every request.
   int wishes = 0;
   for (int request = begin + warp; request < end; request += kWarps) {
-    const Extent extent = extent_of(p, request, p.c.lengths[request], lane == 0);
-    const int32_t* in = p.c.table_in + int64_t(request) * entries;
-    int32_t* out = p.c.table_out + int64_t(request) * entries;
-    int own = 0, first = INT_MAX;
-    each_entry(in, entries, [&](int i, int entry) {
-      const bool has = names_page(p, entry), counts = i < extent.entries;
-      if (has && !counts) atomicSub(p.c.counts_out + entry, 1);
-      if (!has && counts) {
-        ++own;
-        first = min(first, i);
-      }
-      const int next = has && counts ? entry : -1;
-      if (in != out || next != entry) out[i] = next;
-    });
+    int first, own = release(p, request, lane, 32, &first);
     own = __reduce_add_sync(0xffffffffu, own);
     first = __reduce_min_sync(0xffffffffu, first);
     if (lane == 0) {
@@ -200,45 +265,70 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 1) 
   wishes = block_sum(sm, lane == 0 ? wishes : 0);
   tell(sm, 0, rank, wishes);
   cluster_barrier();
-  const int free_here = mark_pages<false>(p, sm, rank, p.c.counts_out, nullptr);
-  tell(sm, 1, rank, free_here);
-  cluster_barrier();
-  const int all = in_all(sm, 0), free = in_all(sm, 1);
-  list_marked(p, sm, rank, in_front(sm, 1, rank), all, [](uint32_t marks, int) { return marks; }, [&](int at, int page) { p.numbers[at] = page; });
+  rank_wishes(p, sm, rank, begin, end);
   cluster_barrier();  // (the last: nobody is told anything behind it)
-  // Every wish gets the free page of its rank.
-  int rank_of_tile = in_front(sm, 0, rank);
-  for (int tile = begin; tile < end; tile += kThreads) {
-    const int own = tile + int(threadIdx.x) < end ? p.heirs[tile + threadIdx.x] : 0;
-    int total;
-    const int start = rank_of_tile + block_rank(sm, own, &total);
-    rank_of_tile += total;
-    // a warp per request that wishes
-    const int warp_first = tile + warp * 32;
-    for (unsigned wishing = __ballot_sync(0xffffffffu, own > 0); wishing != 0; wishing &= wishing - 1) {
-      const int source = __ffs(wishing) - 1, request = warp_first + source;
-      int at = __shfl_sync(0xffffffffu, start, source), left = __shfl_sync(0xffffffffu, own, source);
-      const int counted = extent_of(p, request, p.c.lengths[request], false).entries;
-      int32_t* out = p.c.table_out + int64_t(request) * entries;
-      for (int i0 = p.first[request]; left > 0 && i0 < counted; i0 += 32) {
-        const int i = i0 + lane;
-        const bool wants = i < counted && out[i] < 0;
-        const unsigned wanting = __ballot_sync(0xffffffffu, wants);
-        if (wants) {
-          const int place = at + __popc(wanting & ((1u << lane) - 1u));
-          if (place < free) {
-            const int page = __ldcg(p.numbers + place);
-            out[i] = page;
-            p.c.counts_out[page] = 1;
-          } else {
-            report(p.c.status, SPARSE_MLA_STATUS_NO_PAGE, request, i);
-          }
-        }
-        at += __popc(wanting);
-        left -= __popc(wanting);
-      }
-    }
+  const int free = in_all(sm, 1);
+  for (int request = begin + warp; request < end; request += kWarps) {
+    const int own = p.heirs[request];
+    if (own > 0) give(p, request, lane, 32, p.ranks[request], own, p.first[request], free);
   }
+}
+
+// A large table: a block to each request in front and behind, the cluster between. (1024 requests of 2049 entries, 700 K pages: 192 us by the cluster alone.)
+constexpr int kRowThreads = 256;
+constexpr int64_t kSmallTable = 1 << 16;
+
+__global__ void __launch_bounds__(kRowThreads) copy_counts_kernel(const __grid_constant__ Plan p) {
+  wait_for_predecessor();
+  let_successor_start();
+  copy_counts(p, int64_t(blockIdx.x) * kRowThreads + threadIdx.x, int64_t(gridDim.x) * kRowThreads);
+}
+
+__global__ void __launch_bounds__(kRowThreads) release_kernel(const __grid_constant__ Plan p) {
+  __shared__ int counts[kRowThreads / 32], firsts[kRowThreads / 32];
+  wait_for_predecessor();
+  let_successor_start();
+  const int request = blockIdx.x;
+  int first, own = release(p, request, threadIdx.x, kRowThreads, &first);
+  own = __reduce_add_sync(0xffffffffu, own);
+  first = __reduce_min_sync(0xffffffffu, first);
+  if ((threadIdx.x & 31) == 0) {
+    counts[threadIdx.x >> 5] = own;
+    firsts[threadIdx.x >> 5] = first;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < kRowThreads / 32; ++w) {
+      own += counts[w];
+      first = min(first, firsts[w]);
+    }
+    p.first[request] = first;
+    p.heirs[request] = own;
+  }
+}
+
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 1) rank_kernel(const __grid_constant__ Plan p) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  Shared& sm = *reinterpret_cast<Shared*>(smem);
+  const int rank = int(cluster_rank()), requests = int(p.c.requests);
+  const int share = (requests + kCluster - 1) / kCluster, begin = min(rank * share, requests), end = min(begin + share, requests);
+  wait_for_predecessor();
+  let_successor_start();
+  int wishes = 0;
+  for (int request = begin + int(threadIdx.x); request < end; request += kThreads) wishes += p.heirs[request];
+  wishes = block_sum(sm, wishes);
+  cluster_barrier();  // (all blocks run)
+  tell(sm, 0, rank, wishes);
+  rank_wishes(p, sm, rank, begin, end);
+  if (rank == 0 && threadIdx.x == 0) *p.free = in_all(sm, 1);
+  cluster_barrier();  // (nobody leaves while others are told)
+}
+
+__global__ void __launch_bounds__(kRowThreads) give_kernel(const __grid_constant__ Plan p) {
+  wait_for_predecessor();
+  let_successor_start();
+  const int request = blockIdx.x, own = p.heirs[request];
+  if (own > 0) give(p, request, threadIdx.x, kRowThreads, p.ranks[request], own, p.first[request], *p.free);
 }
 
 // ---- fork -----------------------------------------------------------------------------------------------------------
@@ -288,7 +378,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 1) 
   for (int request = rank * kWarps + warp; request < requests; request += kCluster * kWarps) {
     const Extent extent = extent_of(p, request, p.c.lengths[request], lane == 0);
     const int heirs = __ldcg(p.heirs + request), filled = int(extent.rows % p.c.page_rows);
-    each_entry(p.c.table_in + int64_t(request) * entries, entries, [&](int i, int page) {
+    each_entry(p.c.table_in + int64_t(request) * entries, entries, lane, 32, [&](int i, int page) {
       const int more = (i >= extent.entries ? 0 : i == extent.entries - 1 && filled != 0 ? min(heirs, 1) : heirs) - 1;
       if (more != 0 && names_page(p, page)) atomicAdd(p.c.counts_out + page, more);
     });
@@ -297,7 +387,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 1) 
   for (int tile = begin; tile < end; tile += kThreads) {
     const int child = tile + int(threadIdx.x);
     const bool wants = child < end && wants_page(child, &source, &rows);
-    int total, page = -2;  // -2: as the parent has it
+    int total, page = kShared;
     const int place = rank_of_tile + block_rank(sm, wants, &total);
     rank_of_tile += total;
     if (wants && place < free) {
@@ -308,19 +398,21 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 1) 
       page = -1;
       report(p.c.status, SPARSE_MLA_STATUS_NO_PAGE, child, extent_of(p, p.parents[child], p.c.lengths[p.parents[child]], false).entries - 1);
     }
-    // rows of the new table, 32 of them by each warp
-    for (int k = 0; k < 32 && tile + warp * 32 + k < end; ++k) {
-      const int own = tile + warp * 32 + k, parent = p.parents[own], last_page = __shfl_sync(0xffffffffu, page, k);
-      const int counted = unsigned(parent) < unsigned(requests) ? extent_of(p, parent, p.c.lengths[parent], false).entries : 0;
-      int32_t* out = p.c.table_out + int64_t(own) * entries;
-      if (counted > 0)
-        each_entry(p.c.table_in + int64_t(parent) * entries, counted, [&](int i, int entry) {
-          if (i == counted - 1 && last_page != -2) entry = last_page;
-          out[i] = names_page(p, entry) ? entry : -1;
-        });
-      for (int i = counted + lane; i < entries; i += 32) out[i] = -1;
-    }
+    if (child < end) p.ranks[child] = page;
   }
+}
+
+// Row `child` of the new table.
+__device__ __forceinline__ void write_row(const Plan& p, int child, int thread, int threads) {
+  const int entries = int(p.c.entries), parent = p.parents[child], last_page = p.ranks[child];
+  const int counted = unsigned(parent) < unsigned(p.c.requests) ? extent_of(p, parent, p.c.lengths[parent], false).entries : 0;
+  int32_t* out = p.c.table_out + int64_t(child) * entries;
+  if (counted > 0)
+    each_entry(p.c.table_in + int64_t(parent) * entries, counted, thread, threads, [&](int i, int entry) {
+      if (i == counted - 1 && last_page != kShared) entry = last_page;
+      out[i] = names_page(p, entry) ? entry : -1;
+    });
+  for (int i = counted + thread; i < entries; i += threads) out[i] = -1;
 }
 
 // ---- compact --------------------------------------------------------------------------------------------------------
@@ -371,15 +463,13 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 1) 
 
 // ---- copies ---------------------------------------------------------------------------------------------------------
 
-constexpr int kCopyThreads = 256, kUnitBytes = 16384, kCopyBlocks = 6;  // per SM
+constexpr int kCopyThreads = 256, kUnitBytes = 16384, kCopyBlocks = 5;  // per SM
 
 struct Copies {
-  const int4* copies;
-  const int32_t* count;
-  const int32_t *table_in, *places;  // a table whose entries get their new numbers, or NULL
-  int32_t* table_out;
-  int64_t entries, page_rows;
-  int32_t blocks, tensors, units;  // units of all tensors, for one copy
+  Plan plan;       // fork: whose rows are written besides; compact: whose table gets new numbers
+  int64_t entries;  // of that, fork: 0
+  int64_t page_rows;
+  int32_t tensors, units;  // units of all tensors, for one copy
   struct {
     char* memory;
     int64_t page_bytes;
@@ -397,13 +487,13 @@ __device__ __forceinline__ uint4 load_once(const uint4* at) {
 __global__ void __launch_bounds__(kCopyThreads, kCopyBlocks) copy_kernel(const __grid_constant__ Copies p) {
   wait_for_predecessor();
   let_successor_start();
-  if (p.table_out != nullptr) {
-    for (int64_t i = int64_t(blockIdx.x) * kCopyThreads + threadIdx.x; i < p.entries; i += int64_t(gridDim.x) * kCopyThreads) {
-      const int page = p.table_in[i];
-      p.table_out[i] = unsigned(page) < unsigned(p.blocks) ? p.places[page] : page;
-    }
+  const Plan& plan = p.plan;
+  for (int child = blockIdx.x; child < plan.children; child += gridDim.x) write_row(plan, child, threadIdx.x, kCopyThreads);
+  for (int64_t i = int64_t(blockIdx.x) * kCopyThreads + threadIdx.x; i < p.entries; i += int64_t(gridDim.x) * kCopyThreads) {
+    const int page = plan.c.table_in[i];
+    plan.c.table_out[i] = names_page(plan, page) ? plan.places[page] : page;
   }
-  const int64_t items = int64_t(*p.count) * p.units;
+  const int64_t items = int64_t(*plan.copy_count) * p.units;
   for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
     const int which = int(item / p.units), unit = int(item - int64_t(which) * p.units);
     int tensor = 0;
@@ -411,7 +501,7 @@ __global__ void __launch_bounds__(kCopyThreads, kCopyBlocks) copy_kernel(const _
       const int middle = (tensor + high) >> 1;
       if (p.tensor[middle].first_unit <= unit) tensor = middle; else high = middle;
     }
-    const int4 copy = p.copies[which];
+    const int4 copy = plan.copies[which];
     const int64_t page_bytes = p.tensor[tensor].page_bytes, rows = p.tensor[tensor].rows;
     const int64_t first = int64_t(unit - p.tensor[tensor].first_unit) * kUnitBytes;
     const int64_t filled = (copy.z * rows + p.page_rows - 1) / p.page_rows * (page_bytes / rows);  // bytes of the page to copy
@@ -478,12 +568,11 @@ int fill_tensors(Copies* copies, const pages_call& c, const pages_tensor* tensor
   copies->tensors = int32_t(count);
   copies->units = int32_t(units);
   copies->page_rows = c.page_rows;
-  copies->blocks = int32_t(c.blocks);
   return 0;
 }
 
 int launch_copies(const Copies& copies, int64_t most, cudaStream_t stream) {
-  const int64_t items = std::max(most * copies.units, copies.table_out != nullptr ? (copies.entries + kCopyThreads - 1) / kCopyThreads : 0);
+  const int64_t items = std::max({most * copies.units, int64_t(copies.plan.children), (copies.entries + kCopyThreads - 1) / kCopyThreads});
   if (items == 0) return 0;
   const int grid = int(std::min<int64_t>(items, int64_t(latent::multiprocessors()) * kCopyBlocks));
   return int(launch_overlapped(copy_kernel, grid, kCopyThreads, 0, stream, copies));
@@ -501,8 +590,7 @@ int workspace_size_pages_resize(uint64_t* bytes, const pages_call* call) {
   if (bytes == nullptr || call == nullptr || !fits(*call)) return -1;
   Layout layout;
   layout.take(4 * call->blocks);
-  layout.take(4 * call->requests);
-  layout.take(4 * call->requests);
+  for (int i = 0; i < 3; ++i) layout.take(4 * call->requests);
   *bytes = layout.bytes;
   return 0;
 }
@@ -519,8 +607,18 @@ int launch_pages_resize(void* stream, const pages_call* call) {
   p.numbers = reinterpret_cast<int32_t*>(workspace + layout.take(4 * call->blocks));
   p.first = reinterpret_cast<int32_t*>(workspace + layout.take(4 * call->requests));
   p.heirs = reinterpret_cast<int32_t*>(workspace + layout.take(4 * call->requests));
+  p.ranks = reinterpret_cast<int32_t*>(workspace + layout.take(4 * call->requests));
+  p.free = reinterpret_cast<int32_t*>(workspace);
   p.words = words_of(*call);
-  return launch_plan(resize_kernel, p, static_cast<cudaStream_t>(stream));
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (call->requests * call->entries <= kSmallTable) return launch_plan(resize_kernel, p, s);
+  if (call->counts_in != call->counts_out && call->blocks > 0) {
+    const int64_t grid = std::min<int64_t>((call->blocks + kRowThreads * 8 - 1) / (kRowThreads * 8), latent::multiprocessors() * 4);
+    if (const cudaError_t error = launch_overlapped(copy_counts_kernel, int(grid), kRowThreads, 0, s, p)) return int(error);
+  }
+  if (const cudaError_t error = launch_overlapped(release_kernel, int(call->requests), kRowThreads, 0, s, p)) return int(error);
+  if (const int status = launch_plan(rank_kernel, p, s)) return status;
+  return int(launch_overlapped(give_kernel, int(call->requests), kRowThreads, 0, s, p));
 }
 
 int workspace_size_pages_fork(uint64_t* bytes, const pages_fork_call* call) {
@@ -531,6 +629,7 @@ int workspace_size_pages_fork(uint64_t* bytes, const pages_fork_call* call) {
   layout.take(4 * call->pages.requests);
   layout.take(4 * call->pages.requests);
   layout.take(16 * call->children);
+  layout.take(4 * call->children);
   *bytes = layout.bytes;
   return 0;
 }
@@ -554,10 +653,10 @@ int launch_pages_fork(void* stream, const pages_fork_call* call) {
   p.first = reinterpret_cast<int32_t*>(workspace + layout.take(4 * c.requests));
   p.heirs = reinterpret_cast<int32_t*>(workspace + layout.take(4 * c.requests));
   p.copies = reinterpret_cast<int4*>(workspace + layout.take(16 * call->children));
+  p.ranks = reinterpret_cast<int32_t*>(workspace + layout.take(4 * call->children));
   p.copy_count = reinterpret_cast<int32_t*>(workspace);
   p.words = words_of(c);
-  copies.copies = p.copies;
-  copies.count = p.copy_count;
+  copies.plan = p;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (const int status = launch_plan(fork_kernel, p, s)) return status;
   return launch_copies(copies, call->children > 0 ? call->children - 1 : 0, s);
@@ -589,12 +688,8 @@ int launch_pages_compact(void* stream, const pages_compact_call* call) {
   p.copies = reinterpret_cast<int4*>(workspace + layout.take(16 * (c.blocks / 2 + 1)));  // (no more moves than free pages, or than pages in use)
   p.copy_count = reinterpret_cast<int32_t*>(workspace);
   p.words = words_of(c);
-  copies.copies = p.copies;
-  copies.count = p.copy_count;
-  copies.places = call->places;
-  copies.table_in = c.table_in;
-  copies.table_out = table ? c.table_out : nullptr;
-  copies.entries = c.requests * c.entries;
+  copies.plan = p;
+  copies.entries = table ? c.requests * c.entries : 0;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (const int status = launch_plan(compact_kernel, p, s)) return status;
   return launch_copies(copies, c.blocks / 2, s);

@@ -66,6 +66,7 @@ def _check_scales(cache, scales, others):
 def _check_append8(latent, rope, cache, scales, block_table, cu_seqlens_q, seqused_kv, inv_freq, halves, amplitude):
     _check_append(latent, rope, cache, block_table, cu_seqlens_q, seqused_kv, inv_freq, halves, amplitude, HELD)
     require(cache.shape[3] % 16 == 0, "cache: rows must be a multiple of 16 features")
+    require(block_table.shape[0] <= 1 << 26, "block_table: too many requests")
     _check_scales(cache, scales, (latent, rope, cache, block_table, cu_seqlens_q, seqused_kv, inv_freq))
 
 
