@@ -356,18 +356,24 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 1) 
     }
   }
   cluster_barrier();
-  // Who wants a page: all but the first to continue a request whose last page is partly filled.
-  auto wants_page = [&](int child, int* source, int* rows) {
+  // Who wants a page: where the last page is partly filled, all but the first to continue a request, and that one too if others have named the page. (Told now: the
+  // counts change below.)
+  auto tail_of = [&](int child, int* rows) {  // the partly filled page and its rows, or -1
     const int parent = p.parents[child];
-    if (unsigned(parent) >= unsigned(requests) || __ldcg(p.first + parent) == child) return false;
+    if (unsigned(parent) >= unsigned(requests)) return -1;
     const Extent extent = extent_of(p, parent, p.c.lengths[parent], false);
     *rows = int(extent.rows % p.c.page_rows);
-    if (*rows == 0) return false;
-    *source = p.c.table_in[int64_t(parent) * entries + extent.entries - 1];
-    return names_page(p, *source);
+    if (*rows == 0) return -1;
+    const int page = p.c.table_in[int64_t(parent) * entries + extent.entries - 1];
+    return names_page(p, page) ? page : -1;
   };
-  int wishes = 0, source, rows;
-  for (int child = begin + int(threadIdx.x); child < end; child += kThreads) wishes += wants_page(child, &source, &rows);
+  int wishes = 0, rows = 0;
+  for (int child = begin + int(threadIdx.x); child < end; child += kThreads) {
+    const int source = tail_of(child, &rows);
+    const bool wants = source >= 0 && (__ldcg(p.first + p.parents[child]) != child || p.c.counts_in[source] != 1);
+    p.ranks[child] = wants ? -1 : kShared;
+    wishes += wants;
+  }
   wishes = block_sum(sm, wishes);
   tell(sm, 1, rank, wishes);
   const int free = in_all(sm, 0);
@@ -378,27 +384,27 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 1) 
   for (int request = rank * kWarps + warp; request < requests; request += kCluster * kWarps) {
     const Extent extent = extent_of(p, request, p.c.lengths[request], lane == 0);
     const int heirs = __ldcg(p.heirs + request), filled = int(extent.rows % p.c.page_rows);
+    const int keeps = heirs > 0 && __ldcg(p.ranks + __ldcg(p.first + request)) == kShared;  // its first child, the last page
     each_entry(p.c.table_in + int64_t(request) * entries, entries, lane, 32, [&](int i, int page) {
-      const int more = (i >= extent.entries ? 0 : i == extent.entries - 1 && filled != 0 ? min(heirs, 1) : heirs) - 1;
+      const int more = (i >= extent.entries ? 0 : i == extent.entries - 1 && filled != 0 ? keeps : heirs) - 1;
       if (more != 0 && names_page(p, page)) atomicAdd(p.c.counts_out + page, more);
     });
   }
   int rank_of_tile = in_front(sm, 1, rank);
   for (int tile = begin; tile < end; tile += kThreads) {
     const int child = tile + int(threadIdx.x);
-    const bool wants = child < end && wants_page(child, &source, &rows);
-    int total, page = kShared;
+    const bool wants = child < end && p.ranks[child] != kShared;
+    int total;
     const int place = rank_of_tile + block_rank(sm, wants, &total);
     rank_of_tile += total;
     if (wants && place < free) {
-      page = __ldcg(p.numbers + place);
+      const int page = __ldcg(p.numbers + place), source = tail_of(child, &rows);
+      p.ranks[child] = page;
       p.c.counts_out[page] = 1;
       p.copies[place] = make_int4(source, page, rows, 0);
     } else if (wants) {
-      page = -1;
       report(p.c.status, SPARSE_MLA_STATUS_NO_PAGE, child, extent_of(p, p.parents[child], p.c.lengths[p.parents[child]], false).entries - 1);
     }
-    if (child < end) p.ranks[child] = page;
   }
 }
 
@@ -659,7 +665,7 @@ int launch_pages_fork(void* stream, const pages_fork_call* call) {
   copies.plan = p;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (const int status = launch_plan(fork_kernel, p, s)) return status;
-  return launch_copies(copies, call->children > 0 ? call->children - 1 : 0, s);
+  return launch_copies(copies, call->children, s);
 }
 
 int workspace_size_pages_compact(uint64_t* bytes, const pages_compact_call* call) {

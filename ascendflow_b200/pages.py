@@ -28,7 +28,8 @@ def resize(block_table, counts, lengths, *, page_rows, out=None):
     """Request b gets the pages of `lengths[b]` rows: its first ceil(lengths[b] / page_rows) entries keep their page or, where empty, get a free one; the pages of
     its other entries are given back (and free at once, if nobody else has them). Returns (block_table, counts).
 
-    Lengths may grow (a step's new rows, a new prompt), shrink (drafts that were not taken) or be 0 (a request that ended).
+    Lengths may grow (a step's new rows, a new prompt), shrink (drafts that were not taken) or be 0 (a request that ended; another may begin there with the next call). Pages stay
+    shared: a request that shrinks to less than it had when it was forked, and goes on, is to be forked at that length first.
     """
     table_out, counts_out = _outputs(out, block_table, counts)
     arguments = (block_table, counts, lengths, page_rows, table_out, counts_out)
@@ -40,9 +41,9 @@ def resize(block_table, counts, lengths, *, page_rows, out=None):
 def fork(caches, block_table, counts, parents, lengths, *, page_rows, out=None):
     """A table of len(parents) rows, row i continuing request `parents[i]` of `block_table` at its length `lengths[parents[i]]`. Returns (block_table, counts).
 
-    A request may be continued by any number of rows: they share its full pages, and each but the first has a copy of the partly filled last one, so that all can be appended to. A
-    request that no row continues gives its pages back; a row whose parent is no request (-1) is empty. Only the entries that the length counts go on. The new
-    lengths are `lengths[parents]`.
+    A request may be continued by any number of rows: they share its full pages, and each but the first has a copy of the partly filled last one, so that all can be appended to (the first
+    too, if that page's count is above 1 because others name it). A request that no row continues gives its pages back; a row whose parent is no request (-1) is empty. Only the
+    entries that the length counts go on. The new lengths are `lengths[parents]`.
     caches: tensors `[BLOCKS, R, ...]` of any type whose pages the table names, R a divisor of page_rows (a cache of 16 or 8 bits, its scales; of all layers, up to
     128). Their filled rows are copied. The given table is not changed, and `out`'s must not overlap with it.
     """
