@@ -162,55 +162,87 @@ bool list_of(PyObject* object, std::vector<Tensor>* tensors) {
   return true;
 }
 
-// (block_table, counts, lengths, page_rows, table_out, counts_out)
+// Outputs that are given, or new ones (an int32 tensor of `sizes` on the device of `like`) where None is.
+struct Output {
+  const Tensor* given = nullptr;
+  Tensor made;
+  bool from(PyObject* object) { return optional_of(object, &given); }
+  const Tensor& tensor(const Tensor& like, at::IntArrayRef sizes) {
+    if (given != nullptr) return *given;
+    made = at::empty(sizes, at::TensorOptions(at::kInt).device(like.device()));
+    return made;
+  }
+  const Tensor* written() const { return given != nullptr ? given : &made; }
+};
+// A tuple of the outputs, False for a refused call, or an error.
+template <size_t N>
+PyObject* results(int status, const std::array<Output*, N>& outs) {
+  if (status == kRefused) Py_RETURN_FALSE;
+  if (status != 0) return raise_launch_status(status);
+  PyObject* tuple = PyTuple_New(Py_ssize_t(N));
+  for (size_t i = 0; i < N; ++i) {
+    count_up(outs[i]->given);
+    PyTuple_SET_ITEM(tuple, Py_ssize_t(i), THPVariable_Wrap(*outs[i]->written()));
+  }
+  return tuple;
+}
+bool plain_cuda(const Tensor& t, int64_t dims) { return t.defined() && t.is_cuda() && t.dim() == dims; }
+
+// (block_table, counts, lengths, page_rows, table_out or None, counts_out or None): (table, counts)
 PyObject* call_resize(PyObject*, PyObject* const* arguments, Py_ssize_t count) {
   HANDLE_TH_ERRORS
   std::array<const Tensor*, 3> t;
-  std::array<const Tensor*, 2> out;
+  Output table, counts;
   int64_t page_rows;
-  if (count != 6 || !tensors_of(arguments, &t) || !whole_of(arguments[3], &page_rows) || !tensors_of(arguments + 4, &out)) Py_RETURN_FALSE;
+  if (count != 6 || !tensors_of(arguments, &t) || !whole_of(arguments[3], &page_rows) || !table.from(arguments[4]) || !counts.from(arguments[5])) Py_RETURN_FALSE;
+  if (!plain_cuda(*t[0], 2) || !plain_cuda(*t[1], 1)) Py_RETURN_FALSE;
   int status;
   {
     pybind11::gil_scoped_release no_gil;  // the caller holds references to all of them
-    status = resize(*t[0], *t[1], *t[2], page_rows, *out[0], *out[1]);
+    status = resize(*t[0], *t[1], *t[2], page_rows, table.tensor(*t[0], t[0]->sizes()), counts.tensor(*t[1], t[1]->sizes()));
   }
-  return finished(status, {out[0], out[1]});
+  return results<2>(status, {&table, &counts});
   END_HANDLE_TH_ERRORS
 }
 
-// (caches, block_table, counts, parents, lengths, page_rows, table_out, counts_out)
+// (caches, block_table, counts, parents, lengths, page_rows, table_out or None, counts_out or None): (table, counts)
 PyObject* call_fork(PyObject*, PyObject* const* arguments, Py_ssize_t count) {
   HANDLE_TH_ERRORS
   std::vector<Tensor> caches;
   std::array<const Tensor*, 4> t;
-  std::array<const Tensor*, 2> out;
+  Output table, counts;
   int64_t page_rows;
-  if (count != 8 || !list_of(arguments[0], &caches) || !tensors_of(arguments + 1, &t) || !whole_of(arguments[5], &page_rows) || !tensors_of(arguments + 6, &out)) Py_RETURN_FALSE;
+  if (count != 8 || !list_of(arguments[0], &caches) || !tensors_of(arguments + 1, &t) || !whole_of(arguments[5], &page_rows) || !table.from(arguments[6]) || !counts.from(arguments[7]))
+    Py_RETURN_FALSE;
+  if (!plain_cuda(*t[0], 2) || !plain_cuda(*t[1], 1) || !plain_cuda(*t[2], 1)) Py_RETURN_FALSE;
   int status;
   {
     pybind11::gil_scoped_release no_gil;
-    status = fork(caches, *t[0], *t[1], *t[2], *t[3], page_rows, *out[0], *out[1]);
+    status = fork(caches, *t[0], *t[1], *t[2], *t[3], page_rows, table.tensor(*t[0], {t[2]->size(0), t[0]->size(1)}), counts.tensor(*t[1], t[1]->sizes()));
   }
   if (status == 0)
     for (const Tensor& cache : caches) count_up(&cache);
-  return finished(status, {out[0], out[1]});
+  return results<2>(status, {&table, &counts});
   END_HANDLE_TH_ERRORS
 }
 
-// (caches, block_table, counts, table_out, counts_out, places)
+// (caches, block_table, counts, table_out or None, counts_out or None, places or None): (table, counts, places)
 PyObject* call_compact(PyObject*, PyObject* const* arguments, Py_ssize_t count) {
   HANDLE_TH_ERRORS
   std::vector<Tensor> caches;
-  std::array<const Tensor*, 5> t;
-  if (count != 6 || !list_of(arguments[0], &caches) || !tensors_of(arguments + 1, &t)) Py_RETURN_FALSE;
+  std::array<const Tensor*, 2> t;
+  Output table, counts, places;
+  if (count != 6 || !list_of(arguments[0], &caches) || !tensors_of(arguments + 1, &t) || !table.from(arguments[3]) || !counts.from(arguments[4]) || !places.from(arguments[5]))
+    Py_RETURN_FALSE;
+  if (!plain_cuda(*t[0], 2) || !plain_cuda(*t[1], 1)) Py_RETURN_FALSE;
   int status;
   {
     pybind11::gil_scoped_release no_gil;
-    status = compact(caches, *t[0], *t[1], *t[2], *t[3], *t[4]);
+    status = compact(caches, *t[0], *t[1], table.tensor(*t[0], t[0]->sizes()), counts.tensor(*t[1], t[1]->sizes()), places.tensor(*t[1], t[1]->sizes()));
   }
   if (status == 0)
     for (const Tensor& cache : caches) count_up(&cache);
-  return finished(status, {t[2], t[3], t[4]});
+  return results<3>(status, {&table, &counts, &places});
   END_HANDLE_TH_ERRORS
 }
 

@@ -31,11 +31,12 @@ def resize(block_table, counts, lengths, *, page_rows, out=None):
     Lengths may grow (a step's new rows, a new prompt), shrink (drafts that were not taken) or be 0 (a request that ended; another may begin there with the next call). Pages stay
     shared: a request that shrinks to less than it had when it was forked, and goes on, is to be forked at that length first.
     """
-    table_out, counts_out = _outputs(out, block_table, counts)
-    arguments = (block_table, counts, lengths, page_rows, table_out, counts_out)
-    if is_compiling() or not _resize(*arguments):
-        _otherwise("pages_resize", arguments)
-    return table_out, counts_out
+    given = _given(out)
+    if not is_compiling() and (result := _resize(block_table, counts, lengths, page_rows, *given)):
+        return result
+    outputs = _outputs(given, block_table, counts)
+    _otherwise("pages_resize", (block_table, counts, lengths, page_rows, *outputs))
+    return outputs
 
 
 def fork(caches, block_table, counts, parents, lengths, *, page_rows, out=None):
@@ -47,13 +48,13 @@ def fork(caches, block_table, counts, parents, lengths, *, page_rows, out=None):
     caches: tensors `[BLOCKS, R, ...]` of any type whose pages the table names, R a divisor of page_rows (a cache of 16 or 8 bits, its scales; of all layers, up to
     128). Their filled rows are copied. The given table is not changed, and `out`'s must not overlap with it.
     """
-    require(isinstance(block_table, torch.Tensor) and block_table.dim() == 2 and isinstance(parents, torch.Tensor) and parents.dim() == 1,
-            "expected block_table [B, PAGES] and parents [N]")
-    table_out, counts_out = _outputs(out, block_table, counts, rows=parents.shape[0])
-    arguments = (_listed(caches), block_table, counts, parents, lengths, page_rows, table_out, counts_out)
-    if is_compiling() or not _fork(*arguments):
-        _otherwise("pages_fork", arguments)
-    return table_out, counts_out
+    given = _given(out)
+    if not is_compiling() and (result := _fork(caches, block_table, counts, parents, lengths, page_rows, *given)):
+        return result
+    require(isinstance(parents, torch.Tensor) and parents.dim() == 1, "parents: expected [N]")
+    outputs = _outputs(given, block_table, counts, rows=parents.shape[0])
+    _otherwise("pages_fork", (_listed(caches), block_table, counts, parents, lengths, page_rows, *outputs))
+    return outputs
 
 
 def compact(caches, block_table, counts, *, out=None, places=None):
@@ -61,20 +62,24 @@ def compact(caches, block_table, counts, *, out=None, places=None):
     in front. Returns (block_table, counts, places); `places` `[BLOCKS]` int32 has every page's new number, -1 for free pages, for whoever else keeps
     numbers. Pages from U on are free then and may be given back to the system.
     """
-    table_out, counts_out = _outputs(out, block_table, counts)
-    if places is None:
-        places = torch.empty_like(counts)
-    arguments = (_listed(caches), block_table, counts, table_out, counts_out, places)
-    if is_compiling() or not _compact(*arguments):
-        _otherwise("pages_compact", arguments)
-    return table_out, counts_out, places
+    given = _given(out)
+    if not is_compiling() and (result := _compact(caches, block_table, counts, *given, places)):
+        return result
+    outputs = (*_outputs(given, block_table, counts), torch.empty_like(counts) if places is None else places)
+    _otherwise("pages_compact", (_listed(caches), block_table, counts, *outputs))
+    return outputs
 
 
-def _outputs(out, block_table, counts, rows=None):
-    if out is not None:
-        require(isinstance(out, (tuple, list)) and len(out) == 2, "out: expected (block_table, counts)")
-        return tuple(out)
-    require(isinstance(block_table, torch.Tensor) and isinstance(counts, torch.Tensor), "block_table, counts: expected Torch tensors")
+def _given(out):
+    require(out is None or isinstance(out, (tuple, list)) and len(out) == 2 and all(t is not None for t in out), "out: expected (block_table, counts)")
+    return (None, None) if out is None else tuple(out)
+
+
+def _outputs(given, block_table, counts, rows=None):
+    """Given outputs, or new ones, where the native side does not make them."""
+    if given[0] is not None:
+        return given
+    require(isinstance(block_table, torch.Tensor) and block_table.dim() == 2 and isinstance(counts, torch.Tensor), "block_table, counts: expected [B, PAGES] and [BLOCKS]")
     table = torch.empty_like(block_table) if rows is None else torch.empty((rows, block_table.shape[1]), dtype=block_table.dtype, device=block_table.device)
     return table, torch.empty_like(counts)
 
