@@ -33,6 +33,7 @@ struct Plan {
   int32_t *first, *heirs;      // resize: a request's first entry that wishes, its number of wishes; fork: its first child, its number of children
   int32_t *ranks;              // resize: wishes in front of a request's; fork: the page that a child has of its own, -1: none was left, kShared
   int32_t *free;               // pages in `numbers`
+  uint32_t *marks;             // [8 words] of all blocks, where they have been made in front
   int4* copies;                // source, target, rows
   int32_t* copy_count;
   int32_t words;               // of 32 pages, per block
@@ -115,6 +116,17 @@ __device__ __forceinline__ int mark_pages(const Plan& p, Shared& sm, int rank, c
     }
   }
   return block_sum(sm, lane == 0 ? found : 0);
+}
+
+// The same of marks that have been made.
+__device__ __forceinline__ int fetch_marks(const Plan& p, Shared& sm, int rank) {
+  int found = 0;
+  for (int word = threadIdx.x; word < p.words; word += kThreads) {
+    const uint32_t marks = p.marks[rank * p.words + word];
+    sm.marks[word] = marks;
+    found += __popc(marks);
+  }
+  return block_sum(sm, found);
 }
 
 // Calls list(rank, page) for the marked pages of this block (behind a filter of words), ranks from `rank` on; stops at `most`.
@@ -225,9 +237,8 @@ __device__ __forceinline__ void give(const Plan& p, int request, int thread, int
   }
 }
 
-// Marks of the free pages and their list; the requests' ranks. By the cluster, behind everybody's releases; The blocks' wishes are in totals[0] behind the next cluster barrier.
-__device__ __forceinline__ void rank_wishes(const Plan& p, Shared& sm, int rank, int begin, int end) {
-  const int free_here = mark_pages<false>(p, sm, rank, p.c.counts_out, nullptr);
+// The list of the free pages, which are marked; the requests' ranks. By the cluster. The blocks' wishes are in totals[0] behind the next meeting.
+__device__ __forceinline__ void rank_wishes(const Plan& p, Shared& sm, int rank, int begin, int end, int free_here) {
   tell(sm, 1, rank, free_here);
   meet();
   list_marked(p, sm, rank, in_front(sm, 1, rank), in_all(sm, 0), [](uint32_t marks, int) { return marks; }, [&](int at, int page) { p.numbers[at] = page; });
@@ -265,7 +276,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 1) 
   wishes = block_sum(sm, lane == 0 ? wishes : 0);
   tell(sm, 0, rank, wishes);
   meet();
-  rank_wishes(p, sm, rank, begin, end);
+  rank_wishes(p, sm, rank, begin, end, mark_pages<false>(p, sm, rank, p.c.counts_out, nullptr));
   meet();  // (the last: nobody is told anything behind it)
   const int free = in_all(sm, 1);
   for (int request = begin + warp; request < end; request += kWarps) {
@@ -274,7 +285,8 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 1) 
   }
 }
 
-// A large table: a block to each request in front and behind, the cluster between. (1024 requests of 2049 entries, 700 K pages: 192 us by the cluster alone.)
+// A large table: a block to each request in front and behind, the cluster between. (1024 requests of 2049 entries, 700 K pages: 192 us by the cluster alone;
+// 128 requests of 129 entries 10.2 by the cluster, 64 of 513 13.4.)
 constexpr int kRowThreads = 256;
 constexpr int64_t kSmallTable = 1 << 16;
 
@@ -307,6 +319,22 @@ __global__ void __launch_bounds__(kRowThreads) release_kernel(const __grid_const
   }
 }
 
+// Marks of all pages, eight words by a warp, where there are many (700 K pages 39.3 / 29.1 us; 81 K 14.4 / 16.2).
+constexpr int kWordsPerWarp = 8, kManyPages = 1 << 18;
+__global__ void __launch_bounds__(kRowThreads) mark_kernel(const __grid_constant__ Plan p) {
+  wait_for_predecessor();
+  let_successor_start();
+  const int lane = threadIdx.x & 31, first = (int(blockIdx.x) * (kRowThreads / 32) + int(threadIdx.x >> 5)) * kWordsPerWarp;
+  int count[kWordsPerWarp];
+#pragma unroll
+  for (int n = 0; n < kWordsPerWarp; ++n) count[n] = (first + n) * 32 + lane < int(p.c.blocks) ? p.c.counts_out[(first + n) * 32 + lane] : 1;
+#pragma unroll
+  for (int n = 0; n < kWordsPerWarp; ++n) {
+    const uint32_t marks = __ballot_sync(0xffffffffu, count[n] == 0);
+    if (lane == n && first + n < kCluster * p.words) p.marks[first + n] = marks;
+  }
+}
+
 __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 1) rank_kernel(const __grid_constant__ Plan p) {
   extern __shared__ __align__(16) unsigned char smem[];
   Shared& sm = *reinterpret_cast<Shared*>(smem);
@@ -318,9 +346,10 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 1) 
   int wishes = 0;
   for (int request = begin + int(threadIdx.x); request < end; request += kThreads) wishes += p.heirs[request];
   wishes = block_sum(sm, wishes);
+  const int free_here = p.marks != nullptr ? fetch_marks(p, sm, rank) : mark_pages<false>(p, sm, rank, p.c.counts_out, nullptr);
   cluster_wait();  // (all blocks run)
   tell(sm, 0, rank, wishes);
-  rank_wishes(p, sm, rank, begin, end);
+  rank_wishes(p, sm, rank, begin, end, free_here);
   if (rank == 0 && threadIdx.x == 0) *p.free = in_all(sm, 1);
   meet();  // (nobody leaves while others are told)
 }
@@ -337,8 +366,9 @@ __global__ void __launch_bounds__(kRowThreads) give_kernel(const __grid_constant
 constexpr int kCopyThreads = 256, kUnitBytes = 16384, kCopyBlocks = 5;  // per SM
 
 struct Copies {
-  Plan plan;       // fork: whose rows are written besides; compact: whose table gets new numbers
-  int64_t entries;  // of that, fork: 0
+  Plan plan;
+  bool forks;
+  int64_t entries;  // of a table that gets new numbers
   int64_t page_rows;
   int32_t tensors, units;  // units of all tensors, for one copy
   struct {
@@ -367,11 +397,26 @@ __device__ __forceinline__ void write_row(const Plan& p, int child, int thread, 
   for (int i = counted + thread; i < entries; i += threads) out[i] = -1;
 }
 
-// What there is to do besides the plan: a fork's rows, a compacted table's numbers; copies. By `workers` times kCopyThreads threads. 16 KiB of a page go at a time, 64 bytes by a
+// A request's entries as they were: one reference less, and one more for each row that has them. (Other pages than those that are given out.)
+__device__ __forceinline__ void count_entries(const Plan& p, int request, int thread, int threads) {
+  const int entries = int(p.c.entries);
+  const Extent extent = extent_of(p, request, p.c.lengths[request], thread == 0);
+  const int heirs = __ldcg(p.heirs + request), filled = int(extent.rows % p.c.page_rows);
+  const int keeps = heirs > 0 && __ldcg(p.ranks + __ldcg(p.first + request)) == kShared;  // its first child, the last page
+  each_entry(p.c.table_in + int64_t(request) * entries, entries, thread, threads, [&](int i, int page) {
+    const int more = (i >= extent.entries ? 0 : i == extent.entries - 1 && filled != 0 ? keeps : heirs) - 1;
+    if (more != 0 && names_page(p, page)) atomicAdd(p.c.counts_out + page, more);
+  });
+}
+
+// What there is to do besides the plan: a fork's rows and counts, a compacted table's numbers; copies. By `workers` times kCopyThreads threads. 16 KiB of a page go at a time, 64 bytes by a
 // thread with all loads in flight; what is not 16-byte aligned byte by byte (scales of a few bytes).
 __device__ __forceinline__ void write_and_copy(const Copies& all, int worker, int workers, int thread) {
   const Plan& plan = all.plan;
-  for (int child = worker; child < plan.children; child += workers) write_row(plan, child, thread, kCopyThreads);
+  if (all.forks) {
+    for (int child = worker; child < plan.children; child += workers) write_row(plan, child, thread, kCopyThreads);
+    for (int request = worker; request < int(plan.c.requests); request += workers) count_entries(plan, request, thread, kCopyThreads);
+  }
   for (int64_t i = int64_t(worker) * kCopyThreads + thread; i < all.entries; i += int64_t(workers) * kCopyThreads) {
     const int page = plan.c.table_in[i];
     plan.c.table_out[i] = names_page(plan, page) ? __ldcg(plan.places + page) : page;
@@ -431,7 +476,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 1) 
   const Plan& p = all.plan;
   extern __shared__ __align__(16) unsigned char smem[];
   Shared& sm = *reinterpret_cast<Shared*>(smem);
-  const int rank = int(cluster_rank()), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int rank = int(cluster_rank());
   const int requests = int(p.c.requests), entries = int(p.c.entries), children = p.children;
   const int share = (children + kCluster - 1) / kCluster, begin = min(rank * share, children), end = min(begin + share, children);
   wait_for_predecessor();
@@ -476,16 +521,6 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 1) 
   list_marked(p, sm, rank, in_front(sm, 0, rank), children, [](uint32_t marks, int) { return marks; }, [&](int at, int page) { p.numbers[at] = page; });
   meet();  // (the last: nobody is told anything behind it)
   if (rank == 0 && threadIdx.x == 0) *p.copy_count = min(in_all(sm, 1), free);
-  // Entries of the table as it was: one reference less, and one more for each row that has them. (Other pages than those that are given out.)
-  for (int request = rank * kWarps + warp; request < requests; request += kCluster * kWarps) {
-    const Extent extent = extent_of(p, request, p.c.lengths[request], lane == 0);
-    const int heirs = __ldcg(p.heirs + request), filled = int(extent.rows % p.c.page_rows);
-    const int keeps = heirs > 0 && __ldcg(p.ranks + __ldcg(p.first + request)) == kShared;  // its first child, the last page
-    each_entry(p.c.table_in + int64_t(request) * entries, entries, lane, 32, [&](int i, int page) {
-      const int more = (i >= extent.entries ? 0 : i == extent.entries - 1 && filled != 0 ? keeps : heirs) - 1;
-      if (more != 0 && names_page(p, page)) atomicAdd(p.c.counts_out + page, more);
-    });
-  }
   int rank_of_tile = in_front(sm, 1, rank);
   for (int tile = begin; tile < end; tile += kThreads) {
     const int child = tile + int(threadIdx.x);
@@ -608,7 +643,7 @@ int64_t copied_bytes(const Copies& copies, int64_t most) {
 }
 
 int launch_copies(const Copies& copies, int64_t most, cudaStream_t stream) {
-  const int64_t items = std::max({most * copies.units, int64_t(copies.plan.children), (copies.entries + kCopyThreads - 1) / kCopyThreads});
+  const int64_t items = std::max({most * copies.units, copies.forks ? std::max<int64_t>(copies.plan.children, copies.plan.c.requests) : 0, (copies.entries + kCopyThreads - 1) / kCopyThreads});
   if (items == 0) return 0;
   const int grid = int(std::min<int64_t>(items, int64_t(latent::multiprocessors()) * kCopyBlocks));
   return int(launch_overlapped(copy_kernel, grid, kCopyThreads, 0, stream, copies));
@@ -627,6 +662,7 @@ int workspace_size_pages_resize(uint64_t* bytes, const pages_call* call) {
   Layout layout;
   layout.take(4 * call->blocks);
   for (int i = 0; i < 3; ++i) layout.take(4 * call->requests);
+  layout.take(4 * kCluster * int64_t(words_of(*call)));
   *bytes = layout.bytes;
   return 0;
 }
@@ -644,6 +680,7 @@ int launch_pages_resize(void* stream, const pages_call* call) {
   p.first = reinterpret_cast<int32_t*>(workspace + layout.take(4 * call->requests));
   p.heirs = reinterpret_cast<int32_t*>(workspace + layout.take(4 * call->requests));
   p.ranks = reinterpret_cast<int32_t*>(workspace + layout.take(4 * call->requests));
+  p.marks = reinterpret_cast<uint32_t*>(workspace + layout.take(4 * kCluster * int64_t(words_of(*call))));
   p.free = reinterpret_cast<int32_t*>(workspace);
   const int64_t entries = call->requests * call->entries;
   p.words = words_of(*call);
@@ -654,6 +691,12 @@ int launch_pages_resize(void* stream, const pages_call* call) {
     if (const cudaError_t error = launch_overlapped(copy_counts_kernel, int(grid), kRowThreads, 0, s, p)) return int(error);
   }
   if (const cudaError_t error = launch_overlapped(release_kernel, int(call->requests), kRowThreads, 0, s, p)) return int(error);
+  if (call->blocks > kManyPages) {
+    const int grid = (kCluster * p.words + kRowThreads / 32 * kWordsPerWarp - 1) / (kRowThreads / 32 * kWordsPerWarp);
+    if (const cudaError_t error = launch_overlapped(mark_kernel, grid, kRowThreads, 0, s, p)) return int(error);
+  } else {
+    p.marks = nullptr;
+  }
   if (const int status = launch_plan(rank_kernel, p, p, s)) return status;
   return int(launch_overlapped(give_kernel, int(call->requests), kRowThreads, 0, s, p));
 }
@@ -696,6 +739,7 @@ int launch_pages_fork(void* stream, const pages_fork_call* call) {
   const bool few = copied_bytes(copies, call->children) <= kFewBytes && entries <= kSmallTable;
   p.words = words_of(c);
   copies.plan = p;
+  copies.forks = true;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (few) return launch_plan(fork_kernel<true>, copies, p, s);
   if (const int status = launch_plan(fork_kernel<false>, copies, p, s)) return status;
