@@ -35,6 +35,8 @@
 #include "latent_parts.cuh"
 #include "latent_ptx.cuh"
 
+#include <type_traits>
+
 namespace latent {
 namespace absorbed {
 
@@ -119,6 +121,7 @@ __device__ __forceinline__ int over(int x, const Divisor& by) { return int(uint6
 
 struct Params {
   CUtensorMap cache;
+  CUtensorMap rest;  // rows in 8 bits: their last 64 features
   const char* q;
   const int32_t *table, *cu, *lengths;
   const float* sinks;
@@ -957,6 +960,7 @@ __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
 }  // namespace latent
 
 #include "latent_held8.cuh"
+#include "latent_turned8.cuh"
 
 namespace latent {
 namespace absorbed {
@@ -1049,7 +1053,8 @@ __global__ void __launch_bounds__(kHeld8 ? kThreads8 : kThreads, 1) attention_ke
 // (8 requests of 8192 keys, one token, 64 heads, 18 parts each: 4.0 us, and 8.7 with eight warps for every half row and statistics in front of the sums.)
 constexpr int kMostBlocks = 256, kUnits = LATENT_VALUES / kUnitFeatures;
 
-template <int kFormat>
+// kTurned: a slot's sums lie row by row (latent_turned8.cuh).
+template <int kFormat, bool kTurned>
 __global__ void __launch_bounds__(kCombineThreads, 2) combine_kernel(const __grid_constant__ Params p, int blocks) {
   struct Tile {
     int64_t row;
@@ -1103,7 +1108,7 @@ __global__ void __launch_bounds__(kCombineThreads, 2) combine_kernel(const __gri
     auto slot_of = [&](int part) { return size_t(part == 0 ? 2 * tile.block + 1 : 2 * (tile.block + part)); };
     join_parts<kFormat>(
         shared, warps, tile.parts, rows, tile.rows,
-        [&](int part, int row) { return p.sums + slot_of(part) * kSlotFloats + sums_place(row, feature_of(lane)); },
+        [&](int part, int row) { return p.sums + slot_of(part) * kSlotFloats + (kTurned ? row * LATENT_VALUES + feature_of(lane) : sums_place(row, feature_of(lane))); },
         [&](int part, int row) { return p.statistics + slot_of(part) * kRows + row; },
         [&](int row, int owner) { return p.out + ((tile.row + row) * LATENT_VALUES + feature_of(owner)) * 2; },
         [&](int row, float reference, float sum, bool first_of_row) {  // what the row's sums are multiplied with
@@ -1121,16 +1126,28 @@ int grid() { const int count = multiprocessors(); return count < kMostBlocks ? c
 
 template <int kFormat, int kWidth, bool kHeld8>
 int launch(const Params& p, int blocks, cudaStream_t stream) {
-  using L = Layout<kWidth>;
+  // Rows in 8 bits: bfloat16 queries are the other kernel's (64 requests of 32K, one token: TODO).
+  constexpr bool kTurned = kHeld8 && kFormat == 1;
+  void (*kernel)(Params) = nullptr;
+  int shared_bytes = 0, threads = 0;
+  if constexpr (kTurned) {
+    kernel = turned::attention_kernel<kWidth>;
+    shared_bytes = turned::Layout<kWidth>::kSmemBytes;
+    threads = turned::kThreads;
+  } else {
+    kernel = attention_kernel<kFormat, kWidth, kHeld8>;
+    shared_bytes = Layout<kWidth>::kSmemBytes;
+    threads = kHeld8 ? kThreads8 : kThreads;
+  }
   static bool configured[64] = {false};  // a per-device setting: plain words written with the same value by whoever gets there first
   int device = 0;
   if (const cudaError_t error = cudaGetDevice(&device)) return int(error);
   if (device < 0 || device >= 64) return -1;
   if (!configured[device]) {
-    if (const cudaError_t error = cudaFuncSetAttribute(attention_kernel<kFormat, kWidth, kHeld8>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmemBytes)) return int(error);
+    if (const cudaError_t error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared_bytes)) return int(error);
     configured[device] = true;
   }
-  if (const cudaError_t error = launch_overlapped(attention_kernel<kFormat, kWidth, kHeld8>, blocks, kHeld8 ? kThreads8 : kThreads, L::kSmemBytes, stream, p)) return int(error);
+  if (const cudaError_t error = launch_overlapped(kernel, blocks, threads, shared_bytes, stream, p)) return int(error);
   cudaLaunchAttribute overlap = {};
   overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   overlap.val.programmaticStreamSerializationAllowed = 1;
@@ -1140,7 +1157,7 @@ int launch(const Params& p, int blocks, cudaStream_t stream) {
   config.stream = stream;
   config.attrs = &overlap;
   config.numAttrs = 1;
-  return int(cudaLaunchKernelEx(&config, combine_kernel<kFormat>, p, blocks));
+  return int(cudaLaunchKernelEx(&config, combine_kernel<kFormat, kTurned>, p, blocks));
 }
 
 }  // namespace absorbed
@@ -1173,6 +1190,12 @@ int launch_call(void* stream, const latent_attention_call& c, const uint8_t* sca
   const int blocks = grid();
   Params p = {};
   if constexpr (kHeld8) {
+    const int64_t rows = c.blocks > 0 ? c.blocks * c.page_rows : 1;  // (without pages nothing is copied)
+    const void* base = c.blocks > 0 ? c.cache : c.q;
+    if (c.type == LATENT_BF16) {
+      if (const int e = turned::encode_map8(&p.cache, base, c.width, rows, 128)) return e;
+      if (const int e = turned::encode_map8(&p.rest, base, c.width, rows, 64)) return e;
+    }
     p.held = static_cast<const char*>(c.cache);
     p.scales = scales;
     while ((int64_t(1) << p.block_shift) < block_rows) ++p.block_shift;
