@@ -3,8 +3,8 @@
 // k = least whole number with max|v| <= 448 2^k over the block's new rows, and not below the block's own where older rows precede them; c = v 2^-k rounded
 // to e4m3. As scales are powers of two, a division by one is exact: a number is rounded once (and once more where its block's scale grows and it becomes a
 // subnormal one). Bound by latency: four rows to a warp, all of whose loads are on their way together, and which stay in registers between the maximum and the
-// numbers (rows of more than 512 features in front or 32 pairs are read twice). A block's warps meet once. 8192 rows in blocks of 64 (14 MB): 14.6 us with eight rows to a warp that
-// were read twice.
+// numbers (rows of more than 512 features in front or 32 pairs are read twice). A block's warps meet once. 8192 rows in blocks of 64 (14 MB) 7.1 us, 14.6
+// with eight rows to a warp that were read twice.
 #include "latent_common.cuh"
 
 #include <algorithm>

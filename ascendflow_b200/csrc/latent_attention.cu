@@ -35,6 +35,7 @@
 #include "latent_parts.cuh"
 #include "latent_ptx.cuh"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace latent {
@@ -1124,10 +1125,13 @@ __global__ void __launch_bounds__(kCombineThreads, 2) combine_kernel(const __gri
 // One block per SM; no more than `combine_kernel` has room for.
 int grid() { const int count = multiprocessors(); return count < kMostBlocks ? count : kMostBlocks - 1; }
 
-template <int kFormat, int kWidth, bool kHeld8>
+// How a call is worked out: rows in 16 bits; rows in 8 bits, widened to 16-bit tiles; rows in 8 bits, the other way round (latent_turned8.cuh).
+enum Form { kWide, kHeld, kTurnedRound };
+
+template <int kFormat, int kWidth, int kForm>
 int launch(const Params& p, int blocks, cudaStream_t stream) {
-  // Rows in 8 bits: bfloat16 queries are the other kernel's (64 requests of 32K, one token: TODO).
-  constexpr bool kTurned = kHeld8 && kFormat == 1;
+  constexpr bool kHeld8 = kForm != kWide, kTurned = kForm == kTurnedRound;
+  static_assert(!kTurned || kFormat == 1, "a query of half has more bits than two numbers of 8");
   void (*kernel)(Params) = nullptr;
   int shared_bytes = 0, threads = 0;
   if constexpr (kTurned) {
@@ -1178,6 +1182,12 @@ namespace latent {
 namespace absorbed {
 namespace {
 
+// From so many chunks to a block on bfloat16 queries over rows in 8 bits go the other way round, whose start takes 6 us longer and whose chunks 8 per cent less. The other way
+// round / not, us, of 64 heads (chunks): one token of 8K rows (0.9) 23.8 / 18.4; 16 of them (14) 42.5 / 41.3; 64 at 2K (14) 48.9 / 47.1; 24 at 8K (21) 53.7 / 55.1;
+// 8 x 6 at 4K (21) 52.8 / 49.4; 32 at 8K (28) 63.4 / 66.7; 16 x 6 at 4K (42) 84.4 / 85.4; 64 at 8K (55) 102.9 / 117.0; 500 tokens of 16 heads at 8K (108) 165 / 175. (The
+// host knows the table's width only, which is the longest that requests may be: hence not from 24 on.)
+constexpr int64_t kTurnedChunks = 32;
+
 template <bool kHeld8>
 int launch_call(void* stream, const latent_attention_call& c, const uint8_t* scales, int64_t block_rows) {
   if ((c.type != LATENT_F16 && c.type != LATENT_BF16) || (c.width != 512 && c.width != 576) || !scale_fits(c.scale)) return -1;
@@ -1227,8 +1237,15 @@ int launch_call(void* stream, const latent_attention_call& c, const uint8_t* sca
   p.by_page = divisor_of(p.page_rows / kChunk);
   p.scale_log2 = float(c.scale * 1.4426950408889634);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (c.type == LATENT_BF16) return c.width == 576 ? launch<1, 576, kHeld8>(p, blocks, s) : launch<1, 512, kHeld8>(p, blocks, s);
-  return c.width == 576 ? launch<0, 576, kHeld8>(p, blocks, s) : launch<0, 512, kHeld8>(p, blocks, s);
+  constexpr Form kForm = kHeld8 ? kHeld : kWide;
+  if constexpr (kHeld8) {
+    // Chunks to a block, if requests are as long as the table.
+    const int64_t tiles = std::max((c.tokens * c.heads + kRows - 1) / kRows, std::min(c.batches, c.tokens));
+    const int64_t chunks = tiles * std::min(c.pages, c.blocks) * (c.page_rows / kChunk) / blocks;
+    if (c.type == LATENT_BF16 && chunks >= kTurnedChunks) return c.width == 576 ? launch<1, 576, kTurnedRound>(p, blocks, s) : launch<1, 512, kTurnedRound>(p, blocks, s);
+  }
+  if (c.type == LATENT_BF16) return c.width == 576 ? launch<1, 576, kForm>(p, blocks, s) : launch<1, 512, kForm>(p, blocks, s);
+  return c.width == 576 ? launch<0, 576, kForm>(p, blocks, s) : launch<0, 512, kForm>(p, blocks, s);
 }
 
 }  // namespace

@@ -5,6 +5,11 @@
 // 2^-120 (subnormal numbers too), and to s.0eeee.mmm0000000, as half, times 2^-8; one multiplication of a pair by the scale times 2^120 or 2^8 does the
 // rest: a permutation, a shift, a mask and a product for two values.
 //
+// What bounds it: shared memory. Of the 2.7 k cycles of a chunk its ports are busy for 2.5 k: bytes in, bytes out, values over them, the two products' operands. Half queries, and
+// bfloat16 ones in small calls (latent_turned8.cuh has the others). 64 requests of 64 heads at 32K 411 us, 32 x 6 at 16K 535, one token at 8K 17.5 (its 16 us are the chain
+// that latent_attention.cu describes). With bytes by plain loads into registers 427 and 566, with two groups of warps in turn 459 and 589, tiles widened as a whole 431 and 568 (now
+// halves: 64 keys wait for 32), quarters as halves; conversions of e4m3 to half by the converter are no faster than the four instructions.
+//
 //   warps 8-11   Q of the next piece from global to tensor memory (a subpartition each)
 //   warp 6       brings chunks (64 rows of W bytes, contiguous) by bulk copies, and asks for the rows behind them in L2
 //   warps 12-19  a group of eight of the chunk's rows each: e4m3 numbers out of shared memory, values over them

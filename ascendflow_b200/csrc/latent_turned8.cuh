@@ -16,6 +16,12 @@
 //   warps 8-15   Q of the next piece, split, to tensor memory (its last 64 features to shared memory)
 //   warps 16-23  X^T, every other 16 keys by four of them, into two buffers in tensor memory
 //
+// What bounds it: the board's power (990 W) where a call is large. 64 requests of 64 heads at 32K, 1.22 GB: 379-385 us at 1.44 GHz, where the 16-bit products alone take 212 at the
+// power limit's rate and reading at that rate as much energy as 155 us of it; 32 x 6 at 16K: 489-496 us at 1.63 GHz, 0.9 PFLOP/s. A chunk takes 2.3 k cycles: 18 products
+// of 8 bits, 33 cycles each, 16 of 16 bits, and between those the chain of storing 16 widened keys to a buffer that has just become free. Against latent_held8.cuh
+// (shared memory, 2.7 k cycles): 64 x 1 411 -> 379 us, 32 x 6 535 -> 489 on one board. Softmax by two groups of warps that take turns came down to 2.2 k cycles per chunk and
+// took 388 and 508 us, since its instructions take power as well; waits that poll, or that are given a time, were slower.
+//
 // Tensor memory: columns 0-255 O^T (features' numbers modulo 4, 64 rows each), 256-383 Q's first 512 features, 384-447 scores, 448-511 X^T (two of 16 keys).
 #pragma once
 
@@ -27,12 +33,15 @@ constexpr int kQueryWarp0 = 8, kQueryWarps = 8, kConvertWarp0 = 16, kConvertWarp
 constexpr int kRing = 5, kWideBoxBytes = kChunk * 128, kRestBoxBytes = kChunk * 64;
 constexpr uint32_t kColumnsX = 448;
 constexpr float kSecond = 16.f;  // q2 is held times this
+constexpr int kLargeScale = 227, kSmallScale = 64, kBack = 20;
 
 // What is said of a chunk's rows besides: factors of their scores (two halves, a bank apart), multipliers of their values for pairs of keys, and second ones.
 struct Rows {
   float factors[2][kChunk / 2 + 4];
   uint32_t multipliers[kChunk / 2], again[kChunk / 2];
-  int live, twice, pad[2];
+  int live, twice;
+  float back;  // times this: 1 unless the scales are so large that sums of products times them do not fit FP32, or so small that they are subnormal, where the query's size may bring them back
+  int pad;
 };
 
 template <int kWidth>
@@ -145,15 +154,17 @@ __device__ void copy_role(const Params& p, const Shared& sm) {
       if (use > 0 && !warp_wait(sm.bar(kFree0 + stage), (use - 1) & 1, abort_flag)) { given_up = true; break; }
       Rows* about = rows_of<kWidth>(sm, stage);
       // What is behind the request's length, or in no page, has values of zero: as bits any byte is a finite number.
-      auto factor_of = [](int byte) { return byte == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float(uint32_t(byte) << 23); };  // (2^-127: zero)
+      const int most = __reduce_max_sync(0xffffffffu, max(low == 255 ? 0 : low, high == 255 ? 0 : high)), up = most > kLargeScale ? -kBack : most < kSmallScale ? kBack : 0;
+      // (what comes out as zero lies 60 binades below another scale of the chunk)
+      auto factor_of = [&](int byte) { return __uint_as_float(byte == 255 ? 0x7fc00000u : uint32_t(max(byte + up, 0)) << 23); };
       *reinterpret_cast<float2*>(&about->factors[lane >> 4][2 * (lane & 15)]) = make_float2(factor_of(low), factor_of(high));
       const uint32_t first_one = 2 * lane < valid ? multiplier_of<1>(low) & 0xffffu : 0u, second_one = 2 * lane + 1 < valid ? multiplier_of<1>(high) << 16 : 0u;
       about->multipliers[lane] = first_one | second_one;
       about->again[lane] = (second_multiplier_of<1>(low) & 0xffffu) | second_multiplier_of<1>(high) << 16;
-      const bool twice = __any_sync(0xffffffffu, (low != 255 && low > kMostInOne) || (high != 255 && high > kMostInOne));
       if (lane == 0) {
         about->live = valid;
-        about->twice = twice;
+        about->twice = most > kMostInOne;
+        about->back = __uint_as_float(uint32_t(127 - up) << 23);
         if (first < 0) report(p.status, SPARSE_MLA_STATUS_BAD_PAGE, int(piece.row / p.heads), chunk * kChunk);
       }
       __syncwarp();
@@ -198,49 +209,46 @@ __device__ __forceinline__ void split8(const uint4& words, float by, uint2* one,
   *two = make_uint2(second[0] | second[1] << 16, second[2] | second[3] << 16);
 }
 
-// As the 16-bit form's `query_role`: a subpartition's 16 rows are shared by two warps, segments of 64 bytes, a thread has 16 bytes of rows t / 4 and t / 4 + 8. The rows' greatest
-// magnitudes first; half of the segments stay in registers for that, the others are read again.
+// As in the 16-bit form a subpartition's 16 rows are shared by two warps, segments of 64 bytes, a thread has 16 bytes of rows t / 4 and t / 4 + 8. The rows'
+// greatest magnitudes first; then three segments at a time are read again (a loop: code that runs once per piece comes from far).
 template <int kWidth>
 __device__ void query_role(const Params& p, const Shared& sm, uint32_t tmem) {
   using L = Layout<kWidth>;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, subpartition = warp & 3, part = (warp - kQueryWarp0) >> 2;
+  const int warp = (threadIdx.x >> 5) - kQueryWarp0, lane = threadIdx.x & 31, subpartition = warp & 3, part = warp >> 2;
   volatile int* abort_flag = sm.abort_flag();
-  const uint32_t lanes = uint32_t(subpartition * 32) << 16;
-  constexpr int kOwn = kWidth / 64, kKept = 4;  // segments of this warp; of them in registers
+  constexpr int kOwn = kWidth / 64, kTogether = 3;  // segments of this warp; of them at a time
   const int row = subpartition * 16 + (lane >> 2);
-  uint32_t* most = reinterpret_cast<uint32_t*>(sm.ptr + L::kSmemMost);
-  float* sizes = reinterpret_cast<float*>(sm.ptr + L::kSmemSize);
-  unsigned char* rest = sm.ptr + L::kSmemRest;
   uint32_t loads = 0;
   Walk walk(sm);
   for (; walk.next_of_warp(); walk.done_of_warp()) {
     const Piece& piece = walk.piece;
     if (piece.first == piece.last) continue;  // sees nothing
     const char* source = p.q + (piece.row + row) * (kWidth * 2) + (lane & 3) * 16;
+    const int rows = piece.rows;
     auto fetch16 = [&](int s, int k) {
       const int segment = s < 8 ? part * 8 + s : 16 + part;
       uint4 words = make_uint4(0, 0, 0, 0);
-      if (row + 8 * k < piece.rows) words = *reinterpret_cast<const uint4*>(source + k * 8 * (kWidth * 2) + segment * 64);
+      if (row + 8 * k < rows && s < kOwn) words = *reinterpret_cast<const uint4*>(source + k * 8 * (kWidth * 2) + segment * 64);
       return words;
     };
     uint32_t greatest[2] = {0, 0};
-    auto see = [&](const uint4& words, int k) {
+#pragma unroll 1
+    for (int s0 = 0; s0 < kOwn; s0 += 5) {
+      uint4 words[5][2];
 #pragma unroll
-      for (const uint32_t w : {words.x, words.y, words.z, words.w}) greatest[k] = max(greatest[k], max(w & 0x7fffu, w >> 16 & 0x7fffu));  // (bits of bfloat16 numbers grow with them)
-    };
+      for (int s = 0; s < 5; ++s)
 #pragma unroll
-    for (int s = kKept; s < kOwn; ++s)
+        for (int k = 0; k < 2; ++k) words[s][k] = fetch16(s0 + s, k);
 #pragma unroll
-      for (int k = 0; k < 2; ++k) see(fetch16(s, k), k);
-    uint4 kept[kKept][2];
+      for (int s = 0; s < 5; ++s)
 #pragma unroll
-    for (int s = 0; s < kKept; ++s)
+        for (int k = 0; k < 2; ++k)
 #pragma unroll
-      for (int k = 0; k < 2; ++k) kept[s][k] = fetch16(s, k);
-#pragma unroll
-    for (int s = 0; s < kKept; ++s)
-#pragma unroll
-      for (int k = 0; k < 2; ++k) see(kept[s][k], k);
+          for (const uint32_t w : {words[s][k].x, words[s][k].y, words[s][k].z, words[s][k].w})
+            greatest[k] = max(greatest[k], max(w & 0x7fffu, w >> 16 & 0x7fffu));  // (bits of bfloat16 numbers grow with them)
+    }
+    uint32_t* most = reinterpret_cast<uint32_t*>(sm.ptr + L::kSmemMost);
+    float* sizes = reinterpret_cast<float*>(sm.ptr + L::kSmemSize);
     const uint32_t parity = loads & 1;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -250,6 +258,11 @@ __device__ void query_role(const Params& p, const Shared& sm, uint32_t tmem) {
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(sm.bar(kMost0 + subpartition));
+    uint4 words[kTogether][2];
+#pragma unroll
+    for (int s = 0; s < kTogether; ++s)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) words[s][k] = fetch16(s, k);
     if (!warp_wait(sm.bar(kMost0 + subpartition), parity, abort_flag, kLongWait)) return;
     float by[2], size[2];
 #pragma unroll
@@ -270,34 +283,38 @@ __device__ void query_role(const Params& p, const Shared& sm, uint32_t tmem) {
       __syncwarp();
       if (lane == 0) mbar_arrive(sm.bar(kSizes0 + parity));
     }
-    auto put = [&](int s, const uint4& a, const uint4& b) {
-      uint2 a1, a2, b1, b2;
-      split8(a, by[0], &a1, &a2);
-      split8(b, by[1], &b1, &b2);
-      if (s < 8) {
-        const uint32_t at = tmem + lanes + kColumnsQ + (part * 8 + s) * 8;
-        tmem_st_8(at, a1.x, a1.y, b1.x, b1.y);
-        tmem_st_8(at + kHighLanes, a2.x, a2.y, b2.x, b2.y);
-      } else {  // rows of 64 bytes, swizzled by 64
-        auto place = [&](int lane_of) { return reinterpret_cast<uint2*>(rest + lane_of * 64 + (((part * 2 + ((lane & 3) >> 1)) ^ (lane_of >> 1 & 3)) << 4) + (lane & 1) * 8); };
-        const int low = subpartition * 32 + (lane >> 2);
-        *place(low) = a1;
-        *place(low + 8) = b1;
-        *place(low + 16) = a2;
-        *place(low + 24) = b2;
+#pragma unroll 1
+    for (int s0 = 0; s0 < kOwn; s0 += kTogether) {
+      uint4 next[kTogether][2];
+#pragma unroll
+      for (int s = 0; s < kTogether; ++s)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) next[s][k] = fetch16(s0 + kTogether + s, k);
+#pragma unroll
+      for (int s = 0; s < kTogether; ++s) {
+        uint2 a1, a2, b1, b2;
+        split8(words[s][0], by[0], &a1, &a2);
+        split8(words[s][1], by[1], &b1, &b2);
+        if (s0 + s < 8) {
+          const uint32_t at = tmem + (uint32_t(subpartition * 32) << 16) + kColumnsQ + (part * 8 + s0 + s) * 8;
+          tmem_st_8(at, a1.x, a1.y, b1.x, b1.y);
+          tmem_st_8(at + kHighLanes, a2.x, a2.y, b2.x, b2.y);
+        } else if (kOwn > 8 && s0 + s == 8) {  // rows of 64 bytes, swizzled by 64
+          auto place = [&](int lane_of) {
+            return reinterpret_cast<uint2*>(sm.ptr + L::kSmemRest + lane_of * 64 + (((part * 2 + ((lane & 3) >> 1)) ^ (lane_of >> 1 & 3)) << 4) + (lane & 1) * 8);
+          };
+          const int low = subpartition * 32 + (lane >> 2);
+          *place(low) = a1;
+          *place(low + 8) = b1;
+          *place(low + 16) = a2;
+          *place(low + 24) = b2;
+        }
       }
-    };
 #pragma unroll
-    for (int s = 0; s < kKept; ++s) put(s, kept[s][0], kept[s][1]);
+      for (int s = 0; s < kTogether; ++s)
 #pragma unroll
-    for (int s = 0; s < kKept; ++s)
-      if (s + kKept < kOwn)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) kept[s][k] = fetch16(s + kKept, k);
-#pragma unroll
-    for (int s = 0; s < kKept; ++s)
-      if (s + kKept < kOwn) put(s + kKept, kept[s][0], kept[s][1]);
-    if constexpr (kOwn > 2 * kKept) put(8, fetch16(8, 0), fetch16(8, 1));
+        for (int k = 0; k < 2; ++k) words[s][k] = next[s][k];
+    }
     tmem_wait_st();
     fence_proxy_async();  // products read the last features through the async proxy
     tc_fence_before_sync();
@@ -474,10 +491,10 @@ __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
     const int chunks = piece.last - piece.first;
     const int end = row < piece.rows ? piece.base + over(piece.head + row, p.by_heads) + piece.token : INT32_MAX;  // this row sees keys below
     const int warp_end = __reduce_min_sync(0xffffffffu, end);
-    float reference = -INFINITY, sum = 0.f, scale_log2 = 0.f;
+    float reference = -INFINITY, sum = 0.f, size = 0.f;
     if (chunks > 0) {
       if (!warp_wait(sm.bar(kSizes0 + (loads & 1)), (loads >> 1) & 1, abort_flag, kLongWait)) { failed = true; meet(true); return; }
-      scale_log2 = p.scale_log2 * sizes[(loads++ & 1) * kRows + row];
+      size = sizes[(loads++ & 1) * kRows + row];
     }
     for (int i = 0; i < chunks; ++i, ++count) {
       const uint32_t stage = count % kRing;
@@ -486,6 +503,7 @@ __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
       tc_fence_after_sync();
       const Rows* about = rows_of<kWidth>(sm, stage);
       const int key = (piece.first + i) * kChunk, live = about->live;
+      const float scale_log2 = p.scale_log2 * (size * about->back);
       float2 s[16];
       {
         uint32_t low_a[16], low_b[16], high_a[16], high_b[16];

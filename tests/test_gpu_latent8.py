@@ -150,18 +150,31 @@ CASES = [
 ]
 
 
+def large(heads, tokens, table, page_rows):
+    """So many pages, of a cache and of a table, that a call of bfloat16 queries goes the other way round: 32 chunks to each of 148 blocks if requests are as long as the table."""
+    tiles = max(-(-tokens * heads // 64), min(len(table), tokens))
+    return -(-33 * 148 // (max(tiles, 1) * (page_rows // 64)))
+
+
 @pytest.mark.parametrize("case", range(len(CASES)))
-@pytest.mark.parametrize("dtype,width,block", [(BF16, 576, 1), (BF16, 512, 64), (F16, 576, 16), (F16, 512, 1), (BF16, 576, 32), (F16, 576, 64)])
-def test_attention(case, dtype, width, block):
+@pytest.mark.parametrize("dtype,width,block,turned", [(BF16, 576, 1, False), (BF16, 512, 64, False), (F16, 576, 16, False), (F16, 512, 1, False), (BF16, 576, 32, False), (F16, 576, 64, False),
+                                                      (BF16, 576, 1, True), (BF16, 512, 64, True), (BF16, 576, 16, True), (BF16, 512, 1, True)])
+def test_attention(case, dtype, width, block, turned):
     counts, lengths, heads, page_rows = CASES[case]
     table, blocks = tables(case, lengths, page_rows)
-    cache, scales = held(case, blocks, page_rows, width, block, 117, 123)
     tokens = sum(counts) + 3  # three behind the last request
+    if turned:
+        pages = large(heads, tokens, table, page_rows)
+        blocks = max(blocks, pages)
+        table = torch.cat([table, torch.full((len(table), max(pages - table.shape[1], 0)), -1, dtype=torch.int32, device="cuda")], 1)
+    cache, scales = held(case, blocks, page_rows, width, block, 117, 123)
     q = normal(20 + case, tokens, heads, width, dtype=dtype, spread=0.3)
+    q[0] *= 2.0 ** -40  # rows of other sizes, and of few numbers
+    q[min(1, tokens - 1), :, 1:] *= 2.0 ** -12
     sinks = normal(30, heads) if case % 2 else None
     (out, lse), (out16, lse16) = both(q, cache, scales, table, starts(counts), i32(lengths), scale=width ** -0.5, sinks=sinks)
     assert ops.status()[0] == 0
-    if dtype == F16:
+    if not turned:  # the products are the same
         assert torch.equal(out, out16) and torch.equal(lse, lse16)
     assert (out[-3:] == 7).all() and (lse[-3:] == 7).all()
     wide, token = E.values(cache, scales), 0
@@ -169,38 +182,111 @@ def test_attention(case, dtype, width, block):
         own = wide[table[b, : -(-length // page_rows)].long()].view(1, -1, width)[:, :length]
         seen = torch.arange(length, device="cuda") < (length - n + 1 + torch.arange(n, device="cuda"))[:, None]
         expected, expected_lse, error, lse_error = R.attention(q[token : token + n], own, own[..., :512], seen, width ** -0.5, sinks)
+        if turned and length:  # a query is held by two numbers of 8 bits: to 2^-22 of its greatest, and half of that
+            split = 1.5 * 2.0 ** -22 * width ** -0.5 * q[token : token + n].double().abs().amax(-1, keepdim=True) * own.abs().sum(-1).amax()
+            lse_error = lse_error + split[..., 0]
+            error = error + 2 * split * own[..., :512].abs().amax()
         R.within(out[token : token + n], expected, error, f"request {b}")
         R.within(lse[token : token + n], expected_lse, lse_error, f"request {b}, lse")
         token += n
 
 
+@pytest.mark.parametrize("spread", [1.0, 30.0])
+def test_long_rows_the_other_way_round(spread):
+    """Many chunks to a block, pieces that begin and end within tiles, references that move (queries of a spread of 30: scores of hundreds)."""
+    counts, lengths, heads, page_rows = [1, 2, 1, 3, 1, 1], [40000, 23456, 1, 30011, 64, 51000], 64, 128
+    table, blocks = tables(9, lengths, page_rows)
+    cache, scales = held(19, blocks, page_rows, 576, 8, 117, 121)
+    q = normal(29, sum(counts), heads, 576, dtype=BF16, spread=0.3 * spread)
+    lse = torch.empty(q.shape[:2], device="cuda")
+    out = latent8.latent_attention8(q, cache, scales, table, starts(counts), i32(lengths), scale=576 ** -0.5, lse=lse)
+    assert torch.equal(out, latent8.latent_attention8(q, cache, scales, table, starts(counts), i32(lengths), scale=576 ** -0.5)) and ops.status()[0] == 0
+    wide, token = E.values(cache, scales), 0
+    for b, (n, length) in enumerate(zip(counts, lengths)):
+        own = wide[table[b, : -(-length // page_rows)].long()].view(1, -1, 576)[:, :length]
+        seen = torch.arange(length, device="cuda") < (length - n + 1 + torch.arange(n, device="cuda"))[:, None]
+        expected, expected_lse, error, lse_error = R.attention(q[token : token + n], own, own[..., :512], seen, 576 ** -0.5)
+        split = 1.5 * 2.0 ** -22 * 576 ** -0.5 * q[token : token + n].double().abs().amax(-1, keepdim=True) * own.abs().sum(-1).amax()
+        R.within(out[token : token + n], expected, error + 2 * split * own[..., :512].abs().amax(), b)
+        R.within(lse[token : token + n], expected_lse, lse_error + split[..., 0], b)
+        token += n
+
+
+@pytest.mark.parametrize("blocks", [9, 2500])  # (2500: the other way round)
 @pytest.mark.parametrize("dtype,low,high", [(BF16, 0, 40), (BF16, 130, 140), (BF16, 120, 200), (F16, 104, 112), (F16, 130, 137)])
-def test_scales_of_the_whole_range(dtype, low, high):
+def test_scales_of_the_whole_range(dtype, low, high, blocks):
     """Also those above 2^7, whose multiplication takes two steps, and those that leave subnormal numbers; values are kept where both types hold them."""
-    cache, scales = held(8, 9, 64, 576, 4, low, high)
+    cache, scales = held(8, blocks, 64, 576, 4, low, high)
     wide = E.values(cache, scales)
-    fits = (wide.to(dtype).double() == wide).view(9, 16, -1).all(-1)
+    fits = (wide.to(dtype).double() == wide).view(blocks, 16, -1).all(-1)
     cache = torch.where(fits.repeat_interleave(4, 1)[..., None, None], cache.view(torch.uint8), torch.zeros_like(cache.view(torch.uint8))).view(E.HELD)
     q = normal(9, 6, 64, 576, dtype=dtype)
     scale = 2.0 ** -max(high - 127, 0) * 576 ** -0.5 / 448
-    table, lengths = i32([[8, 1, 2], [3, 7, 5]]), [130, 192]
+    table, lengths = torch.full((2, blocks), -1, dtype=torch.int32, device="cuda"), [130, 192]
+    table[:, :3] = i32([[8, 1, 2], [3, 7, 5]])
     (out, lse), (out16, lse16) = both(q, cache, scales, table, i32([0, 3, 6]), i32(lengths), scale=scale)
     assert torch.isfinite(out).all()
-    if dtype == F16:
+    if dtype == F16 or blocks == 9:
         assert torch.equal(out, out16) and torch.equal(lse, lse16)
     for b, length in enumerate(lengths):
-        own = E.values(cache, scales)[table[b].long()].view(1, -1, 576)[:, :length]
+        own = E.values(cache, scales)[table[b, :3].long()].view(1, -1, 576)[:, :length]
         seen = torch.arange(length, device="cuda") < (length - 2 + torch.arange(3, device="cuda"))[:, None]
         expected, expected_lse, error, lse_error = R.attention(q[3 * b : 3 * b + 3], own, own[..., :512], seen, scale)
+        split = 1.5 * 2.0 ** -22 * scale * q[3 * b : 3 * b + 3].double().abs().amax(-1, keepdim=True) * own.abs().sum(-1).amax() * (blocks > 9)
         # (what is below the smallest normal number counts as zero in FP32 sums: one for every key)
-        R.within(out[3 * b : 3 * b + 3], expected, error + 2.0 ** -126 * length, b)
-        R.within(lse[3 * b : 3 * b + 3], expected_lse, lse_error, b)
+        R.within(out[3 * b : 3 * b + 3], expected, error + 2 * split * own[..., :512].abs().amax() + 2.0 ** -126 * length, b)
+        R.within(lse[3 * b : 3 * b + 3], expected_lse, lse_error + split[..., 0], b)
 
 
-def test_what_lies_behind_the_rows_may_be_anything():
+@pytest.mark.parametrize("blocks", [9, 2500])
+@pytest.mark.parametrize("exponent,low,high", [(-100, 228, 236), (100, 0, 6), (100, 25, 35), (-110, 228, 231)])
+def test_queries_that_bring_scales_back(exponent, low, high, blocks):
+    """Scores of ordinary size out of tiny queries and large scales, or the other way round: sums of products with either alone would not fit."""
+    cache, scales = held(28, blocks, 64, 576, 2, low, high)
+    q = normal(38, 4, 64, 576, dtype=BF16) * 2.0 ** exponent
+    scale = 2.0 ** (127 - high - exponent - 8) * 576 ** -0.5
+    if not 2.0 ** -100 <= scale <= 2.0 ** 100:
+        scale = 0.5
+    lengths, table = [100, 128], torch.full((2, blocks), -1, dtype=torch.int32, device="cuda")
+    table[:, :2] = i32([[8, 1], [3, 7]])
+    lse = torch.empty((4, 64), device="cuda")
+    out = latent8.latent_attention8(q, cache, scales, table, i32([0, 2, 4]), i32(lengths), scale=scale, lse=lse)
+    for b, length in enumerate(lengths):
+        own = E.values(cache, scales)[table[b, :2].long()].view(1, -1, 576)[:, :length]
+        seen = torch.arange(length, device="cuda") < (length - 1 + torch.arange(2, device="cuda"))[:, None]
+        expected, expected_lse, error, lse_error = R.attention(q[2 * b : 2 * b + 2], own, own[..., :512], seen, scale)
+        split = 1.5 * 2.0 ** -22 * scale * q[2 * b : 2 * b + 2].double().abs().amax(-1, keepdim=True) * own.abs().sum(-1).amax()
+        R.within(out[2 * b : 2 * b + 2], expected, error + 2 * split * own[..., :512].abs().amax() + 2.0 ** -126 * length, b)
+        R.within(lse[2 * b : 2 * b + 2], expected_lse, lse_error + split[..., 0], b)
+
+
+@pytest.mark.parametrize("columns", [4, 2500])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_a_query_without_a_number_spoils_its_row(value, columns):
+    lengths, page_rows = [200, 250], 64
+    table, blocks = tables(6, lengths, page_rows, columns)
+    table = torch.cat([table, torch.full((2, columns), -1, dtype=torch.int32, device="cuda")], 1)
+    cache, scales = held(16, blocks, page_rows, 576, 8)
+    q = normal(17, 2, 64, 576, dtype=BF16)
+    arguments = (cache, scales, table, i32([0, 1, 2]), i32(lengths))
+    clean = latent8.latent_attention8(q, *arguments, scale=0.04)
+    for feature in (3, 511, 575):
+        spoilt, lse = q.clone(), torch.empty((2, 64), device="cuda")
+        spoilt[0, 5, feature] = spoilt[1, 63, feature] = value
+        out = latent8.latent_attention8(spoilt, *arguments, scale=0.04, lse=lse)
+        assert torch.isnan(out[0, 5]).all() and torch.isnan(out[1, 63]).all() and torch.isnan(lse[0, 5]) and torch.isnan(lse[1, 63])
+        keep = torch.ones((2, 64), dtype=torch.bool, device="cuda")
+        keep[0, 5] = keep[1, 63] = False
+        assert torch.equal(out[keep], clean[keep]) and torch.isfinite(lse[keep]).all()
+
+
+@pytest.mark.parametrize("turned", [False, True])
+def test_what_lies_behind_the_rows_may_be_anything(turned):
     """NaN numbers and scales behind a request's length and in pages that are nobody's."""
     lengths, page_rows, block = [70, 1, 200, 128], 128, 16
-    table, blocks = tables(3, lengths, page_rows)
+    table, blocks = tables(3, lengths, page_rows, 700 if turned else 3)
+    if turned:
+        table = torch.cat([table, torch.full((4, 700), -1, dtype=torch.int32, device="cuda")], 1)
     cache, scales = held(11, blocks, page_rows, 576, block)
     q = normal(12, 4, 64, 576, dtype=BF16)
     clean = latent8.latent_attention8(q, cache, scales, table, starts([1] * 4), i32(lengths), scale=0.01)
@@ -213,9 +299,12 @@ def test_what_lies_behind_the_rows_may_be_anything():
     assert torch.equal(latent8.latent_attention8(q, cache, scales, table, starts([1] * 4), i32(lengths), scale=0.01), clean)
 
 
-def test_a_scale_without_a_number_spoils_what_sees_it_and_nothing_else():
+@pytest.mark.parametrize("turned", [False, True])
+def test_a_scale_without_a_number_spoils_what_sees_it_and_nothing_else(turned):
     lengths, page_rows = [100, 100, 30], 64
-    table, blocks = tables(5, lengths, page_rows)
+    table, blocks = tables(5, lengths, page_rows, 2500 if turned else 3)
+    if turned:
+        table = torch.cat([table, torch.full((3, 2500), -1, dtype=torch.int32, device="cuda")], 1)
     cache, scales = held(13, blocks, page_rows, 576, 1)
     q, cu = normal(14, 6, 16, 576, dtype=BF16), starts([2, 2, 2])
     clean = latent8.latent_attention8(q, cache, scales, table, cu, i32(lengths), scale=0.01)
@@ -224,10 +313,13 @@ def test_a_scale_without_a_number_spoils_what_sees_it_and_nothing_else():
     assert torch.equal(out[[0, 1, 4, 5]], clean[[0, 1, 4, 5]]) and torch.isnan(out[3]).all()
 
 
-def test_pages_outside_of_the_cache_are_masked_and_reported():
-    cache, scales = held(15, 6, 64, 576, 16)
+@pytest.mark.parametrize("turned", [False, True])
+def test_pages_outside_of_the_cache_are_masked_and_reported(turned):
+    cache, scales = held(15, 2000 if turned else 6, 64, 576, 16)
     q, cu = normal(16, 3, 64, 576, dtype=BF16), i32([0, 1, 2, 3])
-    table = i32([[0, 1, 2], [3, 99, 4], [-1, -5, 6]])
+    table = i32([[0, 1, 2], [3, 9999, 4], [-1, -5, 2000]])
+    if turned:
+        table = torch.cat([table, torch.full((3, 2000), -1, dtype=torch.int32, device="cuda")], 1)
     ops.status()
     out = latent8.latent_attention8(q, cache, scales, table, cu, i32([150, 150, 150]), scale=0.01)
     assert ops.status()[0] == 1
