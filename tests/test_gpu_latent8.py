@@ -341,18 +341,26 @@ def test_offsets_behind_32_bits():
     scales = torch.full((blocks, 8), 127, dtype=torch.uint8, device="cuda").view(E.SCALE)
     table, inv_freq = i32([[69999, 5, 69998]]), latent.rotary_frequencies(64)
     rows = normal(17, 300, 576, dtype=BF16)
-    small = torch.zeros((3, 128, 1, 576), dtype=torch.uint8, device="cuda").view(E.HELD), torch.zeros((3, 8), dtype=torch.uint8, device="cuda").view(E.SCALE)
+    small = torch.zeros((2500, 128, 1, 576), dtype=torch.uint8, device="cuda").view(E.HELD), torch.zeros((2500, 8), dtype=torch.uint8, device="cuda").view(E.SCALE)
     for c, s, t in ((cache, scales, table), (*small, i32([[0, 1, 2]]))):
         latent8.rotary_append8(rows[:, :512], rows[:, 512:], c, s, t, i32([0, 300]), i32([300]), inv_freq)
     q = normal(18, 2, 64, 576, dtype=BF16)
     outs = [latent8.latent_attention8(q, c, s, t, i32([0, 2]), i32([300]), scale=0.05) for c, s, t in ((cache, scales, table), (*small, i32([[0, 1, 2]])))]
     assert torch.equal(*outs) and ops.status()[0] == 0
+    more = torch.full((1, 2497), -1, dtype=torch.int32, device="cuda")  # the other way round
+    tables_ = torch.cat([table, more], 1), torch.cat([i32([[0, 1, 2]]), more], 1)
+    turned = [latent8.latent_attention8(q, c, s, t, i32([0, 2]), i32([300]), scale=0.05) for c, s, t in ((cache, scales, tables_[0]), (*small, tables_[1]))]
+    assert torch.equal(*turned) and not torch.equal(turned[0], outs[0]) and ops.status()[0] == 0
+    # weights and outputs are rounded by half a step, 2^-8, in either form; both are averages of values that the rows bound
+    assert (turned[0].double() - outs[0].double()).abs().max() < 4.1 * 2.0 ** -8 * E.values(*small).abs().max()
 
 
 # ---- how calls are made --------------------------------------------------------------------------------------------------
 
-def arguments():
-    table, blocks = tables(1, [100, 200], 64)
+def arguments(turned=False):
+    table, blocks = tables(1, [100, 200], 64, 2500 if turned else 3)
+    if turned:
+        table = torch.cat([table, torch.full((2, 2500), -1, dtype=torch.int32, device="cuda")], 1)
     cache, scales = held(1, blocks, 64, 576, 16)
     return {"q": normal(2, 4, 8, 576, dtype=BF16), "cache": cache, "scales": scales, "block_table": table, "cu_seqlens_q": i32([0, 2, 4]), "seqused_kv": i32([100, 200]), "scale": 0.04}
 
@@ -396,9 +404,10 @@ def test_refused_append_calls():
     assert ops.status()[0] == 0
 
 
-def test_two_streams_and_two_graphs():
+@pytest.mark.parametrize("turned", [False, True])
+def test_two_streams_and_two_graphs(turned):
     """Calls that run at the same time, captured ones among them, have workspaces of their own."""
-    own = [arguments() for _ in range(2)]
+    own = [arguments(turned) for _ in range(2)]
     for k, a in enumerate(own):
         a["q"] = normal(40 + k, 4, 8, 576, dtype=BF16)
     expected = [latent8.latent_attention8(**a) for a in own]
@@ -423,9 +432,12 @@ def test_two_streams_and_two_graphs():
         assert all(torch.equal(e, out) for out in captured + called)
 
 
-def test_a_captured_step_replays_with_new_lengths():
+@pytest.mark.parametrize("turned", [False, True])
+def test_a_captured_step_replays_with_new_lengths(turned):
     """Append and attention in a graph whose lengths the program moves on between replays."""
-    table, blocks = tables(2, [64, 130], 64)
+    table, blocks = tables(2, [64, 130], 64, 2500 if turned else 3)
+    if turned:
+        table = torch.cat([table, torch.full((2, 2500), -1, dtype=torch.int32, device="cuda")], 1)
     cache, scales = held(21, blocks, 64, 576, 16)
     rows, q, lengths, cu, inv_freq = normal(22, 2, 576, dtype=BF16), normal(23, 2, 8, 576, dtype=BF16), i32([9, 100]), i32([0, 1, 2]), latent.rotary_frequencies(64)
     out = torch.empty((2, 8, 512), dtype=BF16, device="cuda")
