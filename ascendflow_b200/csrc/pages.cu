@@ -94,7 +94,7 @@ __device__ __forceinline__ int block_rank(Shared& sm, int value, int* total) {
 // Marks of this block's pages: bit i of word w for page 32 (rank * words + w) + i. Free pages (kUsed: those in use); their number. Copies the counts where there are two.
 template <bool kUsed>
 __device__ __forceinline__ int mark_pages(const Plan& p, Shared& sm, int rank, const int32_t* counts, int32_t* copy) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, blocks = int(p.c.blocks);
+  const int lane = threadIdx.x & 31, warp = kWarps - 1 - (threadIdx.x >> 5), blocks = int(p.c.blocks);  // (the first warps may have more to do)
   constexpr int kInFlight = 8;
   int found = 0;
   for (int word = warp; word < p.words; word += kWarps * kInFlight) {
@@ -120,24 +120,53 @@ __device__ __forceinline__ int mark_pages(const Plan& p, Shared& sm, int rank, c
 
 // The same of marks that have been made.
 __device__ __forceinline__ int fetch_marks(const Plan& p, Shared& sm, int rank) {
+  constexpr int kInFlight = 4;
   int found = 0;
-  for (int word = threadIdx.x; word < p.words; word += kThreads) {
-    const uint32_t marks = p.marks[rank * p.words + word];
-    sm.marks[word] = marks;
-    found += __popc(marks);
+  for (int word = threadIdx.x; word < p.words; word += kThreads * kInFlight) {
+    uint32_t marks[kInFlight];
+#pragma unroll
+    for (int n = 0; n < kInFlight; ++n) marks[n] = word + n * kThreads < p.words ? p.marks[rank * p.words + word + n * kThreads] : 0;
+#pragma unroll
+    for (int n = 0; n < kInFlight; ++n) {
+      if (word + n * kThreads < p.words) sm.marks[word + n * kThreads] = marks[n];
+      found += __popc(marks[n]);
+    }
   }
   return block_sum(sm, found);
 }
 
-// Calls list(rank, page) for the marked pages of this block (behind a filter of words), ranks from `rank` on; stops at `most`.
+// Calls list(rank, page) for the marked pages of this block (behind a filter of words), ranks from `rank` on; stops at `most`. A warp goes through its words one by one, a
+// page to a lane, so that what is listed is stored side by side, or, where there are fewer marks in each word than such words, a word to a
+// lane; with room for them (`staged`), up to kStaged of a warp's pages go through shared memory instead
+// (a large table's: 73 K pages, seven to a word, are listed in 10 us by either of the others, and in 4 so).
+constexpr int kStaged = 512;
 template <class Filter, class List>
-__device__ __forceinline__ void list_marked(const Plan& p, Shared& sm, int block_rank_, int rank, int most, Filter filter, List list) {
+__device__ __forceinline__ void list_marked(const Plan& p, Shared& sm, int block_rank_, int rank, int most, Filter filter, List list, uint16_t (*staged)[kStaged] = nullptr) {
   for (int word0 = 0; word0 < p.words && rank < most; word0 += kThreads) {
     const int word = word0 + int(threadIdx.x);
-    const int page0 = (block_rank_ * p.words + word) * 32;
-    uint32_t marks = word < p.words ? filter(sm.marks[word], page0) : 0u;
+    const int page0 = (block_rank_ * p.words + word) * 32, lane = threadIdx.x & 31;
+    const uint32_t marks = word < p.words ? filter(sm.marks[word], page0) : 0u;
     int total, own = rank + block_rank(sm, __popc(marks), &total);
-    for (; marks != 0 && own < most; marks &= marks - 1, ++own) list(own, page0 + __ffs(marks) - 1);
+    uint32_t left = __ballot_sync(0xffffffffu, marks != 0 && own < most);
+    if (const int all = __reduce_add_sync(0xffffffffu, __popc(marks)); staged != nullptr && all <= kStaged) {
+      const int first = __shfl_sync(0xffffffffu, own, 0), page_of_warp = __shfl_sync(0xffffffffu, page0, 0);
+      uint16_t* const found = staged[threadIdx.x >> 5];
+      int at = own - first;
+      for (uint32_t mine = marks; mine != 0; mine &= mine - 1) found[at++] = uint16_t(lane * 32 + __ffs(mine) - 1);
+      __syncwarp();
+      for (int i = lane; i < min(all, most - first); i += 32) list(first + i, page_of_warp + found[i]);
+      __syncwarp();
+      left = 0;
+    } else if (int(__reduce_max_sync(0xffffffffu, uint32_t(__popc(marks)))) < __popc(left)) {
+      for (uint32_t mine = marks; mine != 0 && own < most; mine &= mine - 1, ++own) list(own, page0 + __ffs(mine) - 1);
+      left = 0;
+    }
+    for (; left != 0; left &= left - 1) {
+      const int from = __ffs(left) - 1, page = __shfl_sync(0xffffffffu, page0, from) + lane;
+      const uint32_t theirs = __shfl_sync(0xffffffffu, marks, from);
+      const int place = __shfl_sync(0xffffffffu, own, from) + __popc(theirs & ((1u << lane) - 1u));
+      if ((theirs >> lane & 1) && place < most) list(place, page);
+    }
     rank += total;
   }
 }
@@ -238,10 +267,10 @@ __device__ __forceinline__ void give(const Plan& p, int request, int thread, int
 }
 
 // The list of the free pages, which are marked; the requests' ranks. By the cluster. The blocks' wishes are in totals[0] behind the next meeting.
-__device__ __forceinline__ void rank_wishes(const Plan& p, Shared& sm, int rank, int begin, int end, int free_here) {
+__device__ __forceinline__ void rank_wishes(const Plan& p, Shared& sm, int rank, int begin, int end, int free_here, uint16_t (*staged)[kStaged] = nullptr) {
   tell(sm, 1, rank, free_here);
   meet();
-  list_marked(p, sm, rank, in_front(sm, 1, rank), in_all(sm, 0), [](uint32_t marks, int) { return marks; }, [&](int at, int page) { p.numbers[at] = page; });
+  list_marked(p, sm, rank, in_front(sm, 1, rank), in_all(sm, 0), [](uint32_t marks, int) { return marks; }, [&](int at, int page) { p.numbers[at] = page; }, staged);
   int rank_of_tile = in_front(sm, 0, rank);
   for (int tile = begin; tile < end; tile += kThreads) {
     const int request = tile + int(threadIdx.x), own = request < end ? p.heirs[request] : 0;
@@ -285,7 +314,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 1) 
   }
 }
 
-// A large table: a block to each request in front and behind, the cluster between. (1024 requests of 2049 entries, 700 K pages: 192 us by the cluster alone;
+// A large table: a block to each request in front and behind, the cluster between. (1024 requests of 2049 entries, 700 K pages: 192 us by the cluster alone, 24 so;
 // 128 requests of 129 entries 10.2 by the cluster, 64 of 513 13.4.)
 constexpr int kRowThreads = 256;
 constexpr int64_t kSmallTable = 1 << 16;
@@ -319,7 +348,7 @@ __global__ void __launch_bounds__(kRowThreads) release_kernel(const __grid_const
   }
 }
 
-// Marks of all pages, eight words by a warp, where there are many (700 K pages 39.3 / 29.1 us; 81 K 14.4 / 16.2).
+// Marks of all pages, eight words by a warp, where there are many (without / with: 700 K pages 39.3 / 29.1 us; 81 K 14.4 / 16.2; before listing went through shared memory).
 constexpr int kWordsPerWarp = 8, kManyPages = 1 << 18;
 __global__ void __launch_bounds__(kRowThreads) mark_kernel(const __grid_constant__ Plan p) {
   wait_for_predecessor();
@@ -337,6 +366,7 @@ __global__ void __launch_bounds__(kRowThreads) mark_kernel(const __grid_constant
 
 __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 1) rank_kernel(const __grid_constant__ Plan p) {
   extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ uint16_t staged[kWarps][kStaged];
   Shared& sm = *reinterpret_cast<Shared*>(smem);
   const int rank = int(cluster_rank()), requests = int(p.c.requests);
   const int share = (requests + kCluster - 1) / kCluster, begin = min(rank * share, requests), end = min(begin + share, requests);
@@ -349,7 +379,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 1) 
   const int free_here = p.marks != nullptr ? fetch_marks(p, sm, rank) : mark_pages<false>(p, sm, rank, p.c.counts_out, nullptr);
   cluster_wait();  // (all blocks run)
   tell(sm, 0, rank, wishes);
-  rank_wishes(p, sm, rank, begin, end, free_here);
+  rank_wishes(p, sm, rank, begin, end, free_here, staged);
   if (rank == 0 && threadIdx.x == 0) *p.free = in_all(sm, 1);
   meet();  // (nobody leaves while others are told)
 }
@@ -486,11 +516,32 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 1) 
     p.heirs[request] = 0;
   }
   cluster_arrive();
+  struct Tail {
+    int parent;      // or -1
+    int page, rows;  // the partly filled page, or -1, and its rows
+    int count;       // of entries that name it
+  };
+  auto tail_of = [&](int child) {
+    Tail tail = {p.parents[child], -1, 0, 0};
+    if (unsigned(tail.parent) >= unsigned(requests)) tail.parent = -1;
+    if (tail.parent < 0) return tail;
+    const Extent extent = extent_of(p, tail.parent, p.c.lengths[tail.parent], false);
+    tail.rows = int(extent.rows % p.c.page_rows);
+    if (tail.rows == 0) return tail;
+    const int page = p.c.table_in[int64_t(tail.parent) * entries + extent.entries - 1];
+    if (!names_page(p, page)) return tail;
+    tail.page = page;
+    tail.count = p.c.counts_in[page];
+    return tail;
+  };
+  // A thread's first child's: a chain of four loads, beside those of the marks.
+  const int own = begin + int(threadIdx.x);
+  const Tail of_own = own < end ? tail_of(own) : Tail{-1, -1, 0, 0};
   const int free_here = mark_pages<false>(p, sm, rank, p.c.counts_in, p.c.counts_in != p.c.counts_out ? p.c.counts_out : nullptr);
   cluster_wait();  // (all blocks run, and have written the above)
   tell(sm, 0, rank, free_here);
-  for (int child = begin + int(threadIdx.x); child < end; child += kThreads) {
-    const int parent = p.parents[child];
+  for (int child = own; child < end; child += kThreads) {
+    const int parent = child == own ? of_own.parent : p.parents[child];
     if (unsigned(parent) < unsigned(requests)) {
       atomicMin(p.first + parent, child);
       atomicAdd(p.heirs + parent, 1);
@@ -499,19 +550,10 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 1) 
   meet();
   // Who wants a page: where the last page is partly filled, all but the first to continue a request, and that one too if others have named the page. (Told now: the
   // counts change below.)
-  auto tail_of = [&](int child, int* rows) {  // the partly filled page and its rows, or -1
-    const int parent = p.parents[child];
-    if (unsigned(parent) >= unsigned(requests)) return -1;
-    const Extent extent = extent_of(p, parent, p.c.lengths[parent], false);
-    *rows = int(extent.rows % p.c.page_rows);
-    if (*rows == 0) return -1;
-    const int page = p.c.table_in[int64_t(parent) * entries + extent.entries - 1];
-    return names_page(p, page) ? page : -1;
-  };
-  int wishes = 0, rows = 0;
-  for (int child = begin + int(threadIdx.x); child < end; child += kThreads) {
-    const int source = tail_of(child, &rows);
-    const bool wants = source >= 0 && (__ldcg(p.first + p.parents[child]) != child || p.c.counts_in[source] != 1);
+  int wishes = 0;
+  for (int child = own; child < end; child += kThreads) {
+    const Tail tail = child == own ? of_own : tail_of(child);
+    const bool wants = tail.page >= 0 && (__ldcg(p.first + tail.parent) != child || tail.count != 1);
     p.ranks[child] = wants ? -1 : kShared;
     wishes += wants;
   }
@@ -529,10 +571,11 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 1) 
     const int place = rank_of_tile + block_rank(sm, wants, &total);
     rank_of_tile += total;
     if (wants && place < free) {
-      const int page = __ldcg(p.numbers + place), source = tail_of(child, &rows);
+      const int page = __ldcg(p.numbers + place);
+      const Tail tail = child == own ? of_own : tail_of(child);
       p.ranks[child] = page;
       p.c.counts_out[page] = 1;
-      p.copies[place] = make_int4(source, page, rows, 0);
+      p.copies[place] = make_int4(tail.page, page, tail.rows, 0);
     } else if (wants) {
       report(p.c.status, SPARSE_MLA_STATUS_NO_PAGE, child, extent_of(p, p.parents[child], p.c.lengths[p.parents[child]], false).entries - 1);
     }
@@ -560,16 +603,15 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 1) 
   auto movers = [&](uint32_t marks, int page0) { return marks & ~below(page0, border); };
   auto holes = [&](uint32_t marks, int page0) { return ~marks & below(page0, border); };  // (border <= blocks)
   int staying = 0;
-  for (int word = threadIdx.x; word < p.words; word += kThreads) {
+  const int lane = threadIdx.x & 31;
+  for (int word = threadIdx.x >> 5; word < p.words; word += kWarps) {
     const uint32_t marks = sm.marks[word];
-    const int page0 = (rank * p.words + word) * 32;
-    staying += __popc(marks & below(page0, border));
-    for (int i = 0; i < 32 && page0 + i < blocks; ++i) {
-      const bool used = marks >> i & 1;
-      if (!used || page0 + i < border) p.places[page0 + i] = used ? page0 + i : -1;
-    }
+    const int first = (rank * p.words + word) * 32, page = first + lane;
+    staying += __popc(marks & below(first, border));
+    const bool used = marks >> lane & 1;
+    if (page < blocks && (!used || page < border)) p.places[page] = used ? page : -1;
   }
-  staying = block_sum(sm, staying);
+  staying = block_sum(sm, lane == 0 ? staying : 0);
   tell(sm, 1, rank, staying);
   int* const lists = reinterpret_cast<int*>(p.copies);
   // (pages in front of this block's that are free and in front of the border: all of those in front of the border but the ones in use)
@@ -608,13 +650,13 @@ struct Layout {
 };
 
 int words_of(const pages_call& c) { return int((c.blocks + 32 * kCluster - 1) / (32 * kCluster)); }
-// Up to so many bytes (in the worst case) the planning blocks copy by themselves, which spares a launch: 16 rows of four beams, 0.3 MB, 14.0 / 11.9 us; a cache of 70 pages 13.2 / 11.4.
+// Up to so many bytes (in the worst case) the planning blocks copy by themselves, which spares a launch: 16 rows of four beams, 0.3 MB, 14.0 / 11.9 us; a cache of 70 pages 13.2 / 11.4 (by now 10.6 and 8.9).
 constexpr int64_t kFewBytes = 2 << 20;
 
 template <class Arguments>
 int launch_plan(void (*kernel)(const Arguments), const Arguments& arguments, const Plan& p, cudaStream_t stream) {
   const size_t shared = sizeof(Shared) + size_t(p.words) * sizeof(uint32_t);
-  if (shared > 48 * 1024)  // (a per-device setting; always the same value)
+  if (shared + sizeof(uint16_t) * kWarps * kStaged > 48 * 1024)  // (a per-device setting; always the same value)
     if (const cudaError_t error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(Shared) + PAGES_MOST_BLOCKS / 8 / kCluster))) return int(error);
   return int(launch_overlapped(kernel, kCluster, kThreads, shared, stream, arguments));
 }

@@ -44,6 +44,7 @@ def latent_attention8(q, cache, scales, block_table, cu_seqlens_q, seqused_kv, *
     """Causal attention of q `[T, H, W]` (bf16 or f16), W 512 or 576, over the paged `cache` and its `scales`: returns out `[T, H, 512]` in the type of q.
 
     As `latent.latent_attention` over a cache that holds the numbers times their scales (in the type of q: for f16 they have to be finite there, and scales up to 2^22).
+    In large calls bf16 queries are split into two numbers of 8 bits, which leaves out what is below 2^-22 of a row's greatest.
     Rows behind a request's length may hold anything; a number NaN among the others is not looked for, a scale NaN makes what sees its rows NaN.
     """
     if out is None:

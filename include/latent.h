@@ -108,7 +108,8 @@ typedef struct {
 int launch_latent_append8(void* stream, const latent_append8_call* call);
 
 /* Attention as launch_latent_attention over such a cache; its workspace is as large as that one's. Held values are taken as they are (in the type of q, which holds them exactly
- * where they are finite and normal numbers there; for half: scales up to 2^22). NaN among the numbers of rows that are seen is not looked for; scales that are NaN make what sees them NaN. */
+ * where they are finite and normal numbers there; for half: scales up to 2^22). bfloat16 queries may be split into
+ * two numbers of 8 bits, which leaves out what is below 2^-22 of a row's greatest (large calls). NaN among the numbers of rows that are seen is not looked for; scales that are NaN make what sees them NaN. */
 typedef struct {
   latent_attention_call attention; /* cache: e4m3 */
   const uint8_t* scales;

@@ -231,6 +231,43 @@ def test_a_cache_of_millions_of_pages():
         pages.resize(i32([[-1]]), torch.zeros(blocks + 1, dtype=torch.int32, device="cuda"), i32([4]), page_rows=1)
 
 
+@pytest.mark.parametrize("in_place", [False, True])
+def test_a_fork_of_many_rows(in_place):
+    """More rows than the planning threads; about half of them get a page of their own before there are no more."""
+    requests, entries, blocks, page_rows, children = 9, 3, 12000, 16, 20000
+    rng = random.Random(77)
+    table, counts, lengths = state_of(rng, requests, entries, blocks, page_rows)
+    parents = [rng.randrange(-1, requests) for _ in range(children)]
+    caches = [torch.randint(0, 256, (blocks, page_rows, 3), dtype=torch.uint8, device="cuda", generator=torch.Generator(device="cuda").manual_seed(7))]
+    expected = forked(caches, table, counts, parents, lengths, page_rows)
+    given = i32(counts)
+    out = (torch.empty((children, entries), dtype=torch.int32, device="cuda"), given) if in_place else None
+    got = pages.fork(caches, tensor(table, entries), given, i32(parents), i32(lengths), page_rows=page_rows, out=out)
+    same(got, *expected[:2], entries)
+    assert equal(caches, expected[2])
+    ops.status()
+
+
+@pytest.mark.parametrize("blocks", [100000, 500000])
+@pytest.mark.parametrize("one_in", [1, 2, 5, 40, 3000])
+def test_free_pages_lie_close_or_far_apart(blocks, one_in):
+    """A large table's wishes are listed out of marks of every density, whole words of free pages and of used ones among them; nothing is left in the end."""
+    requests, entries = 90, 1000
+    generator = torch.Generator().manual_seed(one_in)
+    free = torch.randint(0, one_in, (blocks,), generator=generator) == 0
+    free[5000:9000], free[20000:60000] = True, False
+    lengths = torch.randint(0, 64 * entries, (requests,), generator=generator, dtype=torch.int32)
+    wishes = (torch.arange(entries) < (lengths[:, None] + 63) // 64)
+    pages_ = free.nonzero()[:, 0].int()[: int(wishes.sum())]
+    expected = torch.full((requests * entries,), -1, dtype=torch.int32)
+    expected[wishes.flatten().nonzero()[: len(pages_), 0]] = pages_
+    counts = (~free).int()
+    got = pages.resize(torch.full((requests, entries), -1, dtype=torch.int32, device="cuda"), counts.cuda(), lengths.cuda(), page_rows=64)
+    counts[pages_.long()] = 1
+    assert torch.equal(got[0].cpu().flatten(), expected) and torch.equal(got[1].cpu(), counts)
+    assert ops.status()[0] == (3 if len(pages_) < int(wishes.sum()) else 0)
+
+
 def test_many_tensors():
     caches = [torch.full((6, 4, 24), k, dtype=torch.int16, device="cuda") + torch.arange(6, dtype=torch.int16, device="cuda").view(6, 1, 1) for k in range(pages.MOST_CACHES)]
     expected = forked(caches, [[2]], [0, 0, 1, 0, 0, 0], [0, 0, 0], [7], 8)
