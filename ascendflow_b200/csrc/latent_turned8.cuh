@@ -503,7 +503,7 @@ __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
       tc_fence_after_sync();
       const Rows* about = rows_of<kWidth>(sm, stage);
       const int key = (piece.first + i) * kChunk, live = about->live;
-      const float scale_log2 = p.scale_log2 * (size * about->back);
+      float scale_log2 = p.scale_log2 * (size * about->back);
       float2 s[16];
       {
         uint32_t low_a[16], low_b[16], high_a[16], high_b[16];
@@ -528,6 +528,13 @@ __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
         const float4 f = *reinterpret_cast<const float4*>(&about->factors[half][2 * e]);
         s[e] = multiply2(s[e], make_float2(f.x, f.y));
         s[e + 1] = multiply2(s[e + 1], make_float2(f.z, f.w));
+      }
+      // A multiplier that FP32 holds as no normal number (queries of zeros and tiny ones; as zero it would make NaNs of masked scores): the scores take the query's size first. What is lost
+      // so is below 2^-126, or beyond FP32 already.
+      if (scale_log2 < FLT_MIN || scale_log2 > FLT_MAX) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] = multiply2(s[e], make_float2(size, size));
+        scale_log2 = p.scale_log2 * about->back;
       }
       if (live < kChunk || key + kChunk > warp_end) {
         const int seen = min(end - key, live) - half * 32;
