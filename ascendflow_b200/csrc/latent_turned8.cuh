@@ -268,10 +268,11 @@ __device__ void query_role(const Params& p, const Shared& sm, uint32_t tmem) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const uint32_t bits = max(greatest[k], most[(parity * 2 + (part ^ 1)) * kRows + row + 8 * k]) << 16;
-      // 2^e: the least with |q| <= 448 2^e (and a normal number as its inverse is); no number where q has one that is none
+      // 2^e: the least with |q| <= 448 2^e (and a normal number as its inverse is). A row with what is no number, or infinite, has none: all of its scores are NaN, and only those of keys
+      // that it sees are taken.
       const int e = min(max(int(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u), 1), 253);
-      by[k] = __uint_as_float(uint32_t(254 - e) << 23);
-      size[k] = bits >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __uint_as_float(uint32_t(e) << 23);
+      by[k] = bits >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __uint_as_float(uint32_t(254 - e) << 23);
+      size[k] = __uint_as_float(uint32_t(e) << 23);
     }
     if (loads > 0 && !warp_wait(sm.bar(kQFree), (loads - 1) & 1, abort_flag, kLongWait)) return;
     tc_fence_after_sync();

@@ -1,5 +1,7 @@
 """Attention over a latent cache in 8 bits at the ends of what queries, scales and masks may be, against the definition in 64 bits."""
 
+import math
+
 import pytest
 import torch
 
@@ -99,3 +101,20 @@ def test_tiny_queries_of_large_scales(turned):
     cache, scales = held(11, blocks, 64, 576, 2, 224, 228)
     q = (normal(12, sum(counts), heads, 576) * 2.0 ** -118).bfloat16()
     check(attend(q, cache, scales, table, counts, lengths, 2.0 ** -4), q, cache, scales, table, counts, lengths, 2.0 ** -4, turned)
+
+
+# ---- what is masked ---------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype,turned", FORMS)
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_a_query_without_a_number_that_sees_no_key(dtype, turned, value):
+    """Its output is zeros, whatever it holds, beside tokens of the same tile that see some."""
+    counts, lengths, heads = [5, 3], [3, 100], 8
+    table, blocks = pages_for(13, counts, lengths, heads, turned)
+    cache, scales = held(14, blocks, 64, 576, 8, 117, 123)
+    q = normal(15, 8, heads, 576, spread=0.3).to(dtype)
+    clean = attend(q, cache, scales, table, counts, lengths, 0.04)
+    q[0, :, 7] = q[1, 3] = value  # the first request's first two tokens see nothing
+    out, lse = attend(q, cache, scales, table, counts, lengths, 0.04)
+    assert (out[:2] == 0).all() and (lse[:2] == -math.inf).all()
+    assert torch.equal(out, clean[0]) and torch.equal(lse, clean[1])
