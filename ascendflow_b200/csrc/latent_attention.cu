@@ -150,6 +150,7 @@ struct Shared {
   __device__ __forceinline__ uint32_t* tmem_slot() const { return reinterpret_cast<uint32_t*>(ptr + misc); }
   __device__ __forceinline__ volatile int* abort_flag() const { return reinterpret_cast<volatile int*>(ptr + misc + 4); }
   __device__ __forceinline__ volatile int* live(uint32_t stage) const { return reinterpret_cast<volatile int*>(ptr + misc + 8 + stage * 4); }
+  __device__ __forceinline__ volatile int* spoilt(uint32_t stage) const { return reinterpret_cast<volatile int*>(ptr + misc + 20 + stage * 4); }  // rows in 8 bits: scales that are NaN
   __device__ __forceinline__ int64_t* scan() const { return reinterpret_cast<int64_t*>(ptr); }  // (before the first tile lands)
 };
 
@@ -762,7 +763,7 @@ __device__ __forceinline__ float inverse_of(float reference, float sum, float si
   return sum == 0.f ? 0.f : share / (total * sum);
 }
 
-template <int kFormat, int kWidth>
+template <int kFormat, int kWidth, bool kHeld8>
 __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
   using L = Layout<kWidth>;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = lane >> 4;
@@ -819,6 +820,16 @@ __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
                       make_float2(__uint_as_float(high_a[2 * e]), __uint_as_float(high_a[2 * e + 1])));
           s[8 + e] = add2(make_float2(__uint_as_float(low_b[2 * e]), __uint_as_float(low_b[2 * e + 1])),
                           make_float2(__uint_as_float(high_b[2 * e]), __uint_as_float(high_b[2 * e + 1])));
+        }
+      }
+      if constexpr (kHeld8) {
+        if (*sm.spoilt(stage)) {  // keys whose scales are NaN: their values are zeros here
+          const unsigned char* scales = sm.ptr + L::kSmemScales + stage * kChunk + half * 32;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            if (scales[2 * e] == 255) s[e].x = __uint_as_float(0x7fc00000u);
+            if (scales[2 * e + 1] == 255) s[e].y = __uint_as_float(0x7fc00000u);
+          }
         }
       }
       if (live < kChunk || key + kChunk > warp_end) {
@@ -1024,7 +1035,7 @@ __global__ void __launch_bounds__(kHeld8 ? kThreads8 : kThreads, 1) attention_ke
   if constexpr (kHeld8) {
     if (warp < kSoftmaxWarps) {
       take_128_registers();
-      softmax_role<kFormat, kWidth>(p, sm, tmem);
+      softmax_role<kFormat, kWidth, kHeld8>(p, sm, tmem);
     } else if (warp < kConvertWarp0) {
       keep_64_registers();
       if (warp == kScoreWarp || warp == kValueWarp) issue();
@@ -1036,7 +1047,7 @@ __global__ void __launch_bounds__(kHeld8 ? kThreads8 : kThreads, 1) attention_ke
       convert_role<kFormat, kWidth>(p, sm);
     }
   } else {
-    if (warp < kSoftmaxWarps) softmax_role<kFormat, kWidth>(p, sm, tmem);
+    if (warp < kSoftmaxWarps) softmax_role<kFormat, kWidth, kHeld8>(p, sm, tmem);
     else if (warp == kScoreWarp || warp == kValueWarp) issue();
     else if (warp == kCopyWarp) copy_role<kWidth>(p, sm);
     else if (warp == kPlanWarp) plan();

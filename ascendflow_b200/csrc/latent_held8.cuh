@@ -22,7 +22,7 @@ constexpr int kQueryWarps8 = 4, kConvertWarp0 = kQueryWarp0 + kQueryWarps8, kCon
 constexpr int kThreads8 = 32 * (kConvertWarp0 + kConvertWarps);
 
 // A scale's byte: 2^(byte - 127), 255: NaN. The multiplier (twice, for a pair) is 2^(byte - kBias); what is above the type's largest power of two is
-// left for a second one.
+// left for a second one. With NaN the values are zeros and the scores become NaN, for as values NaN would reach all rows of a tile, by weights of zero too.
 template <int kFormat> constexpr int kBias = kFormat == 1 ? 7 : 119;
 constexpr int kMostInOne = 134;  // 2^127 in bfloat16, 2^15 in half
 template <int kFormat>
@@ -34,7 +34,7 @@ __device__ __forceinline__ uint32_t power_of_two(int exponent) {  // (below the 
 }
 template <int kFormat>
 __device__ __forceinline__ uint32_t multiplier_of(int byte) {
-  if (byte == 255) return 0x7fff7fffu;  // NaN in either type
+  if (byte == 255) return 0u;
   return power_of_two<kFormat>(min(byte, kMostInOne) - kBias<kFormat>);
 }
 // (half: values times such scales are finite up to 2^22 only, where this is 2^15)
@@ -131,8 +131,10 @@ __device__ void copy_role8(const Params& p, const Shared& sm) {
         }
         if (half == 0) {
           // (what the chunk before says has been read: its second product has begun)
+          const bool spoilt = __any_sync(0xffffffffu, (low == 255 && lane < valid) || (high == 255 && lane + 32 < valid));
           if (lane == 0) {
             *sm.live(stage) = valid;
+            *sm.spoilt(stage) = spoilt;
             if (first < 0) report(p.status, SPARSE_MLA_STATUS_BAD_PAGE, int(piece.row / p.heads), chunk * kChunk);
           }
           unsigned char* scales = sm.ptr + L::kSmemScales + stage * kChunk;

@@ -118,3 +118,25 @@ def test_a_query_without_a_number_that_sees_no_key(dtype, turned, value):
     out, lse = attend(q, cache, scales, table, counts, lengths, 0.04)
     assert (out[:2] == 0).all() and (lse[:2] == -math.inf).all()
     assert torch.equal(out, clean[0]) and torch.equal(lse, clean[1])
+
+
+@pytest.mark.parametrize("dtype,turned", FORMS)
+@pytest.mark.parametrize("block", [1, 8, 64])
+@pytest.mark.parametrize("width,heads", [(576, 16), (512, 64)])
+def test_a_scale_without_a_number_leaves_alone_what_does_not_see_it(dtype, turned, block, width, heads):
+    """The last block of rows of every other request: a draft that overflowed. Tokens in front of it, in the same tile, do not see it."""
+    counts, lengths = [7, 2, 4, 1, 3, 66], [70, 100, 3, 64, 3009, 130]
+    table, blocks = pages_for(16, counts, lengths, heads, turned)
+    cache, scales = held(17, blocks, 64, width, block, 117, 123)
+    q = normal(18, sum(counts), heads, width, spread=0.3).to(dtype)
+    clean = attend(q, cache, scales, table, counts, lengths, width ** -0.5)
+    spoilt, token = torch.zeros(sum(counts), dtype=torch.bool, device="cuda"), 0
+    for b, (n, length) in enumerate(zip(counts, lengths)):
+        if b % 2 == 0 or b == 5:
+            first = (length - 1) // block * block  # of the block's rows
+            scales.view(torch.uint8)[table[b, first // 64], first % 64 // block] = 255
+            spoilt[token : token + n] = length - n + 1 + torch.arange(n, device="cuda") > first
+        token += n
+    out, lse = attend(q, cache, scales, table, counts, lengths, width ** -0.5)
+    assert torch.equal(out[~spoilt], clean[0][~spoilt]) and torch.equal(lse[~spoilt], clean[1][~spoilt])
+    assert torch.isnan(out[spoilt]).all() and torch.isnan(lse[spoilt]).all() and 0 < int(spoilt.sum()) < len(spoilt)
