@@ -153,8 +153,9 @@ __device__ void copy_role(const Params& p, const Shared& sm) {
       const uint32_t stage = count % kRing, use = count / kRing, target = sm.base + stage * L::kTileBytes, bar = sm.bar(kFull0 + stage);
       if (use > 0 && !warp_wait(sm.bar(kFree0 + stage), (use - 1) & 1, abort_flag)) { given_up = true; break; }
       Rows* about = rows_of<kWidth>(sm, stage);
-      // What is behind the request's length, or in no page, has values of zero: as bits any byte is a finite number.
-      const int most = __reduce_max_sync(0xffffffffu, max(low == 255 ? 0 : low, high == 255 ? 0 : high)), up = most > kLargeScale ? -kBack : most < kSmallScale ? kBack : 0;
+      // What is behind the request's length, or in no page, has values of zero (as bits any byte is a finite number), and its scales count for nothing.
+      const int most = __reduce_max_sync(0xffffffffu, max(low == 255 || 2 * lane >= valid ? 0 : low, high == 255 || 2 * lane + 1 >= valid ? 0 : high));
+      const int up = most > kLargeScale ? -kBack : most < kSmallScale ? kBack : 0;
       // (what comes out as zero lies 60 binades below another scale of the chunk)
       auto factor_of = [&](int byte) { return __uint_as_float(byte == 255 ? 0x7fc00000u : uint32_t(max(byte + up, 0)) << 23); };
       *reinterpret_cast<float2*>(&about->factors[lane >> 4][2 * (lane & 15)]) = make_float2(factor_of(low), factor_of(high));

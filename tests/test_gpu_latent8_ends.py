@@ -140,3 +140,21 @@ def test_a_scale_without_a_number_leaves_alone_what_does_not_see_it(dtype, turne
     out, lse = attend(q, cache, scales, table, counts, lengths, width ** -0.5)
     assert torch.equal(out[~spoilt], clean[0][~spoilt]) and torch.equal(lse[~spoilt], clean[1][~spoilt])
     assert torch.isnan(out[spoilt]).all() and torch.isnan(lse[spoilt]).all() and 0 < int(spoilt.sum()) < len(spoilt)
+
+
+@pytest.mark.parametrize("turned", [False, True])
+@pytest.mark.parametrize("low,exponent", [(6, 110), (0, 118), (230, -100)])
+@pytest.mark.parametrize("behind", [0, 64, 127, 254, 255])
+def test_scales_behind_the_rows_may_be_anything(turned, low, exponent, behind):
+    """What an earlier request has left there does not move the scales of rows that count."""
+    counts, lengths, heads = [1, 2, 1], [70, 2, 129], 16
+    table, blocks = pages_for(19, counts, lengths, heads, turned)
+    cache, scales = held(20, blocks, 64, 576, 1, low, low + 4)
+    cache = torch.where(cache.float().abs() < 2, 2.0, cache.float()).to(E.HELD)  # (normal numbers of bfloat16 with every scale)
+    q = (normal(21, 4, heads, 576) * 2.0 ** exponent).bfloat16()
+    clean = attend(q, cache, scales, table, counts, lengths, 0.02)
+    for b, length in enumerate(lengths):
+        scales.view(torch.uint8)[table[b, length // 64], length % 64 :] = behind
+    out, lse = attend(q, cache, scales, table, counts, lengths, 0.02)
+    assert torch.isfinite(lse).all() and (lse.amax(1) != lse.amin(1)).all()  # (scores that count)
+    assert torch.equal(out, clean[0]) and torch.equal(lse, clean[1])
