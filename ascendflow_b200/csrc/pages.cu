@@ -712,7 +712,7 @@ int workspace_size_pages_resize(uint64_t* bytes, const pages_call* call) {
 int launch_pages_resize(void* stream, const pages_call* call) {
   using namespace pages;
   if (call == nullptr || !fits(*call)) return -1;
-  if ((call->requests == 0 || call->entries == 0) && (call->blocks == 0 || call->counts_in == call->counts_out)) return 0;
+  if (call->requests == 0 && (call->blocks == 0 || call->counts_in == call->counts_out)) return 0;  // (requests of a table without entries may have lengths to report)
   if (!usable(*call)) return -1;
   char* workspace = static_cast<char*>(call->workspace);
   Plan p = {};
@@ -763,7 +763,7 @@ int launch_pages_fork(void* stream, const pages_fork_call* call) {
   if (c.entries > 0 && call->children > INT_MAX / c.entries) return -1;
   Copies copies = {};
   if (const int status = fill_tensors(&copies, c, call->tensors, call->tensor_count)) return status;
-  if ((c.requests == 0 || c.entries == 0) && (call->children == 0 || c.entries == 0) && (c.blocks == 0 || c.counts_in == c.counts_out)) return 0;
+  if (c.requests == 0 && (call->children == 0 || c.entries == 0) && (c.blocks == 0 || c.counts_in == c.counts_out)) return 0;
   if (!usable(c)) return -1;
   char* workspace = static_cast<char*>(c.workspace);
   Plan p = {};
