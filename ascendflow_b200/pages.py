@@ -44,7 +44,8 @@ def fork(caches, block_table, counts, parents, lengths, *, page_rows, out=None):
 
     A request may be continued by any number of rows: they share its full pages, and each but the first has a copy of the partly filled last one, so that all can be appended to (the first
     too, if that page's count is above 1 because others name it). A request that no row continues gives its pages back; a row whose parent is no request (-1) is empty. Only the
-    entries that the length counts go on. The new lengths are `lengths[parents]`.
+    entries that the length counts go on. The new lengths are `lengths[parents]` where every parent is a request; a row without one has length 0:
+    `torch.where((parents >= 0) & (parents < B), lengths[parents.clamp(0, B - 1)], 0)`. (As an index -1 is the last request, whose length would be the empty row's, and a number of B or more an error on the device.)
     caches: tensors `[BLOCKS, R, ...]` of any type whose pages the table names, R a divisor of page_rows (a cache of 16 or 8 bits, its scales; of all layers, up to
     128). Their filled rows are copied. The given table is not changed, and `out`'s must not overlap with it.
     """

@@ -50,7 +50,7 @@ int workspace_size_pages_resize(uint64_t* bytes, const pages_call* call);
 int launch_pages_resize(void* stream, const pages_call* call);
 
 /* Row i of table_out continues request parents[i]: it has the entries that this one's length counts, the others are empty; so are all of a row whose
- * parent is no request. A last page that is partly filled goes on in one row: the first that continues the request keeps it if its count is 1 (nobody else names it), and every
+ * parent is no request (whose length from then on is 0). A last page that is partly filled goes on in one row: the first that continues the request keeps it if its count is 1 (nobody else names it), and every
  * other gets one of the pages that are free before the call (lowest numbers first, in the order of the rows) with a copy of the filled rows in every tensor (parts that are
  * filled in part are copied whole). So rows may be appended to, also where a length is shorter than the request was when it shared its pages. counts_out counts the entries of table_out instead of those of table_in. Sources and targets of copies are different pages. */
 typedef struct {
