@@ -1,11 +1,13 @@
-"""The pages of a cache at the ends of what the calls allow."""
+"""The pages of a cache at the ends of what the calls allow: tables of no columns, rows without a parent, the most pages, none left, caches behind 32 bits."""
+
+import random
 
 import pytest
 import torch
 
 from ascendflow_b200 import latent8, ops, pages
 from tests import latent8_reference as E
-from tests.test_gpu_pages import i32
+from tests.test_gpu_pages import counted, forked, i32, same, state_of, tensor
 
 pytestmark = pytest.mark.gpu
 
@@ -41,3 +43,59 @@ def test_rows_without_a_parent_go_on_as_empty_ones():
     lse = torch.empty((7, 8), device="cuda")
     out = latent8.latent_attention8(q, cache, scales, table, i32(range(8)), lengths, scale=0.04, lse=lse)
     assert (out == 0).all() and (lse[~heirs] == -float("inf")).all() and torch.isfinite(lse[heirs]).all() and ops.status()[0] == 0
+
+
+def test_the_last_pages_of_a_large_cache_go_to_the_front_in_order():
+    """Pages in use in all eight parts that blocks of threads share out."""
+    blocks = pages.MOST_BLOCKS
+    used = [7, *(blocks // 8 * k + 11 * k for k in range(1, 8)), blocks - 1]
+    counts = torch.zeros(blocks, dtype=torch.int32, device="cuda")
+    counts[used] = i32(range(1, 10))
+    cache = torch.zeros((blocks, 2), dtype=torch.uint8, device="cuda")
+    cache[used, 1] = torch.arange(1, 10, dtype=torch.uint8, device="cuda")
+    table, counts, places = pages.compact([cache], i32([used]), counts)
+    order = [7, 0, 1, 2, 3, 4, 5, 6, 8]  # page 7 is in front already; the others take the free ones in front, in order
+    assert table.tolist() == [order] and places[used].tolist() == order and int((places >= 0).sum()) == 9
+    expected = [order.index(p) + 1 for p in range(9)]
+    assert counts[:9].tolist() == expected and int((counts != 0).sum()) == 9
+    assert cache[:9, 1].tolist() == expected and ops.status()[0] == 0
+
+
+def test_rows_that_get_no_page_in_a_fork_are_reported():
+    requests, entries, blocks, page_rows, children = 9, 3, 12000, 16, 20000
+    rng = random.Random(77)
+    table, counts, lengths = state_of(rng, requests, entries, blocks, page_rows)
+    parents = [rng.randrange(-1, requests) for _ in range(children)]
+    expected = forked([], table, counts, parents, lengths, page_rows)
+    ops.status()
+    got = pages.fork([], tensor(table, entries), i32(counts), i32(parents), i32(lengths), page_rows=page_rows)
+    same(got, *expected[:2], entries)
+    without = {(r, n - 1) for r, p in enumerate(parents) if p >= 0 and (n := counted(lengths[p], page_rows, entries)) and expected[0][r][n - 1] < 0 <= table[p][n - 1]}
+    status = ops.status()
+    assert status[0] == 3 and (status[1], status[2]) in without
+
+
+def test_pages_behind_32_bits():
+    """A cache of 5 GB: pages of its end copied there and moved to its front."""
+    blocks = 70000
+    cache = torch.zeros((blocks, 64, 1152), dtype=torch.uint8, device="cuda")
+    own = torch.randint(1, 256, (4, 64, 1152), dtype=torch.uint8, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    cache[blocks - 4 :] = own
+    counts = torch.ones(blocks, dtype=torch.int32, device="cuda")  # pages that somebody else keeps, but for four
+    counts[[3, 60000, blocks - 6, blocks - 5]] = 0
+    table = i32([[blocks - 1, blocks - 2], [blocks - 3, blocks - 4]])
+    table, counts = pages.fork([cache], table, counts, i32([0, 0, 1, 1, 1]), i32([64 + 9, 128]), page_rows=64)
+    last = [blocks - 1, blocks - 2], [blocks - 3, blocks - 4]
+    assert table.tolist() == [last[0], [blocks - 1, 3], last[1], last[1], last[1]]
+    assert torch.equal(cache[3, :9], own[2, :9]) and not cache[3, 9:].any() and torch.equal(cache[blocks - 4 :], own)
+    table, counts = pages.fork([cache], table, counts, i32([0, 0, 1, 2]), i32([64 + 9, 64 + 9, 0, 0, 0]), page_rows=64)
+    assert table.tolist() == [last[0], [blocks - 1, 60000], [blocks - 1, 3], [-1, -1]]
+    assert torch.equal(cache[60000, :9], own[2, :9]) and not cache[60000, 9:].any()
+    counts[5 : blocks - 8] = 0
+    counts[[0, 1, 2, 4]] = 0
+    table = torch.where((table >= 5) & (table < blocks - 8), -1, table)
+    table, counts, places = pages.compact([cache], table, counts)
+    used = [3, blocks - 8, blocks - 7, blocks - 2, blocks - 1]
+    assert places[used].tolist() == [3, 0, 1, 2, 4] and int((places >= 0).sum()) == 5
+    assert table.tolist() == [[4, 2], [4, -1], [4, 3], [-1, -1]]
+    assert torch.equal(cache[2], own[2]) and torch.equal(cache[4], own[3]) and not cache[:2].any() and ops.status()[0] == 0
