@@ -49,6 +49,7 @@ constexpr int kThreads = 32 * (kQueryWarp0 + kQueryWarps);
 constexpr int kBoxBytes = kChunk * 128;  // 64 features of a chunk
 constexpr int kStages = 3;
 constexpr int kPieces = 4;               // pieces announced ahead
+constexpr int kSpoilt = 128;             // see Shared::marked
 
 constexpr uint32_t kColumnsQ = 256, kColumnsScores = 384, kColumnsPlaces = 448, kColumnsQRest = 464;
 constexpr uint32_t kHighLanes = 16u << 16;
@@ -150,7 +151,9 @@ struct Shared {
   __device__ __forceinline__ uint32_t* tmem_slot() const { return reinterpret_cast<uint32_t*>(ptr + misc); }
   __device__ __forceinline__ volatile int* abort_flag() const { return reinterpret_cast<volatile int*>(ptr + misc + 4); }
   __device__ __forceinline__ volatile int* live(uint32_t stage) const { return reinterpret_cast<volatile int*>(ptr + misc + 8 + stage * 4); }
-  __device__ __forceinline__ volatile int* spoilt(uint32_t stage) const { return reinterpret_cast<volatile int*>(ptr + misc + 20 + stage * 4); }  // rows in 8 bits: scales that are NaN
+  // Rows in 8 bits: the same, less kSpoilt where a scale among them is NaN (so that what looks out for a chunk's end finds it); which, of keys 32 half .. + 31.
+  __device__ __forceinline__ volatile int* marked(uint32_t stage) const { return reinterpret_cast<volatile int*>(ptr + misc + 20 + stage * 4); }
+  __device__ __forceinline__ volatile uint32_t* spoilt(uint32_t stage, int half) const { return reinterpret_cast<volatile uint32_t*>(ptr + misc + 32 + (stage * 2 + half) * 4); }
   __device__ __forceinline__ int64_t* scan() const { return reinterpret_cast<int64_t*>(ptr); }  // (before the first tile lands)
 };
 
@@ -801,7 +804,8 @@ __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
       // (the tile has landed when its scores are there; this wait makes what was written about it visible)
       if (!warp_wait(sm.bar(kScoresFull), count & 1, abort_flag) || !warp_wait(sm.bar(kFull0 + stage), (count / kStages) & 1, abort_flag)) { failed = true; meet(true); return; }
       tc_fence_after_sync();
-      const int key = (piece.first + i) * kChunk, live = *sm.live(stage);
+      const int key = (piece.first + i) * kChunk;
+      int live = kHeld8 ? *sm.marked(stage) : *sm.live(stage);
       float2 s[16];
       {
         // Both partial sums of a score come straight to the thread that owns it.
@@ -822,17 +826,16 @@ __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
                           make_float2(__uint_as_float(high_b[2 * e]), __uint_as_float(high_b[2 * e + 1])));
         }
       }
-      if constexpr (kHeld8) {
-        if (*sm.spoilt(stage)) {  // keys whose scales are NaN: their values are zeros here
-          const unsigned char* scales = sm.ptr + L::kSmemScales + stage * kChunk + half * 32;
+      if (live < kChunk || key + kChunk > warp_end) {
+        if (kHeld8 && live < 0) {  // keys whose scales are NaN: their values are zeros here
+          live += kSpoilt;
+          const uint32_t spoilt = *sm.spoilt(stage, half);
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            if (scales[2 * e] == 255) s[e].x = __uint_as_float(0x7fc00000u);
-            if (scales[2 * e + 1] == 255) s[e].y = __uint_as_float(0x7fc00000u);
+            if (spoilt >> 2 * e & 1) s[e].x = __uint_as_float(0x7fc00000u);
+            if (spoilt >> 2 * e & 2) s[e].y = __uint_as_float(0x7fc00000u);
           }
         }
-      }
-      if (live < kChunk || key + kChunk > warp_end) {
         const int seen = min(end - key, live) - half * 32;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {

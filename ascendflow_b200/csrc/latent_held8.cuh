@@ -131,16 +131,22 @@ __device__ void copy_role8(const Params& p, const Shared& sm) {
         }
         if (half == 0) {
           // (what the chunk before says has been read: its second product has begun)
-          const bool spoilt = __any_sync(0xffffffffu, (low == 255 && lane < valid) || (high == 255 && lane + 32 < valid));
           if (lane == 0) {
             *sm.live(stage) = valid;
-            *sm.spoilt(stage) = spoilt;
             if (first < 0) report(p.status, SPARSE_MLA_STATUS_BAD_PAGE, int(piece.row / p.heads), chunk * kChunk);
           }
           unsigned char* scales = sm.ptr + L::kSmemScales + stage * kChunk;
           scales[lane] = static_cast<unsigned char>(low);
           scales[lane + 32] = static_cast<unsigned char>(high);
           __syncwarp();
+        }
+        if (half == 1) {  // (nobody waits for this yet)
+          const uint32_t spoilt[2] = {__ballot_sync(0xffffffffu, low == 255 && lane < valid), __ballot_sync(0xffffffffu, high == 255 && lane + 32 < valid)};
+          if (lane == 0) {
+            *sm.marked(stage) = (spoilt[0] | spoilt[1]) != 0 ? valid - kSpoilt : valid;
+            *sm.spoilt(stage, 0) = spoilt[0];
+            *sm.spoilt(stage, 1) = spoilt[1];
+          }
         }
         if (lane == 0) mbar_arrive_expect(bar, min(max(valid - half * 32, 0), 32) * kWidth);
         __syncwarp();

@@ -218,7 +218,7 @@ __device__ void query_role(const Params& p, const Shared& sm, uint32_t tmem) {
   const int warp = (threadIdx.x >> 5) - kQueryWarp0, lane = threadIdx.x & 31, subpartition = warp & 3, part = warp >> 2;
   volatile int* abort_flag = sm.abort_flag();
   constexpr int kOwn = kWidth / 64, kTogether = 3;  // segments of this warp; of them at a time
-  const int row = subpartition * 16 + (lane >> 2);
+  const int row = subpartition * 16 + (lane >> 2), least = max(128 - int(__float_as_uint(p.scale_log2) >> 23), 1);
   uint32_t loads = 0;
   Walk walk(sm);
   for (; walk.next_of_warp(); walk.done_of_warp()) {
@@ -269,9 +269,9 @@ __device__ void query_role(const Params& p, const Shared& sm, uint32_t tmem) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const uint32_t bits = max(greatest[k], most[(parity * 2 + (part ^ 1)) * kRows + row + 8 * k]) << 16;
-      // 2^e: the least with |q| <= 448 2^e (and a normal number as its inverse is). A row with what is no number, or infinite, has none: all of its scores are NaN, and only those of keys
-      // that it sees are taken.
-      const int e = min(max(int(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u), 1), 253);
+      // 2^e: the least with |q| <= 448 2^e, a normal number as its inverse is, and the product with the scores' scale (rows of zeros, tiny ones: what is left out of these moves scores by less
+      // than 2^-138 of the keys' magnitudes). A row with what is no number, or infinite, has none: all of its scores are NaN, and only those of keys that it sees are taken.
+      const int e = min(max(int(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u), least), 253);
       by[k] = bits >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __uint_as_float(uint32_t(254 - e) << 23);
       size[k] = __uint_as_float(uint32_t(e) << 23);
     }
@@ -493,10 +493,10 @@ __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
     const int chunks = piece.last - piece.first;
     const int end = row < piece.rows ? piece.base + over(piece.head + row, p.by_heads) + piece.token : INT32_MAX;  // this row sees keys below
     const int warp_end = __reduce_min_sync(0xffffffffu, end);
-    float reference = -INFINITY, sum = 0.f, size = 0.f;
+    float reference = -INFINITY, sum = 0.f, scale = 0.f;
     if (chunks > 0) {
       if (!warp_wait(sm.bar(kSizes0 + (loads & 1)), (loads >> 1) & 1, abort_flag, kLongWait)) { failed = true; meet(true); return; }
-      size = sizes[(loads++ & 1) * kRows + row];
+      scale = fminf(p.scale_log2 * sizes[(loads++ & 1) * kRows + row], FLT_MAX);
     }
     for (int i = 0; i < chunks; ++i, ++count) {
       const uint32_t stage = count % kRing;
@@ -505,7 +505,8 @@ __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
       tc_fence_after_sync();
       const Rows* about = rows_of<kWidth>(sm, stage);
       const int key = (piece.first + i) * kChunk, live = about->live;
-      float scale_log2 = p.scale_log2 * (size * about->back);
+      // (a positive number, for masked scores and zeros are multiplied by it, too; what the bounds move are scores below 2^-140, or beyond FP32)
+      const float scale_log2 = fminf(fmaxf(scale * about->back, FLT_MIN), FLT_MAX);
       float2 s[16];
       {
         uint32_t low_a[16], low_b[16], high_a[16], high_b[16];
@@ -530,13 +531,6 @@ __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
         const float4 f = *reinterpret_cast<const float4*>(&about->factors[half][2 * e]);
         s[e] = multiply2(s[e], make_float2(f.x, f.y));
         s[e + 1] = multiply2(s[e + 1], make_float2(f.z, f.w));
-      }
-      // A multiplier that FP32 holds as no normal number (queries of zeros and tiny ones; as zero it would make NaNs of masked scores): the scores take the query's size first. What is lost
-      // so is below 2^-126, or beyond FP32 already.
-      if (scale_log2 < FLT_MIN || scale_log2 > FLT_MAX) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) s[e] = multiply2(s[e], make_float2(size, size));
-        scale_log2 = p.scale_log2 * about->back;
       }
       if (live < kChunk || key + kChunk > warp_end) {
         const int seen = min(end - key, live) - half * 32;
@@ -571,7 +565,7 @@ __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
       __syncwarp();
       if (lane == 0) mbar_arrive(sm.bar(kMoved0 + (count & 1)));
       const float shift = reference == -INFINITY ? 0.f : -reference;
-      const float2 scale = make_float2(scale_log2, scale_log2), shifts = make_float2(shift, shift);
+      const float2 scales = make_float2(scale_log2, scale_log2), shifts = make_float2(shift, shift);
       float2 sum_a = make_float2(0.f, 0.f), sum_b = sum_a;
       uint4 packed[4];
 #pragma unroll
@@ -580,7 +574,7 @@ __device__ void softmax_role(const Params& p, const Shared& sm, uint32_t tmem) {
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           const int e = 4 * u + w;
-          float2 weight = fma2(s[e], scale, shifts);
+          float2 weight = fma2(s[e], scales, shifts);
           weight.x = exp2f(weight.x);
           weight.y = exp2f(weight.y);
           if (e & 1) sum_b = add2(sum_b, weight); else sum_a = add2(sum_a, weight);
