@@ -650,8 +650,11 @@ struct Layout {
 };
 
 int words_of(const pages_call& c) { return int((c.blocks + 32 * kCluster - 1) / (32 * kCluster)); }
-// Up to so many bytes (in the worst case) the planning blocks copy by themselves, which spares a launch: 16 rows of four beams, 0.3 MB, 14.0 / 11.9 us; a cache of 70 pages 13.2 / 11.4 (by now 10.6 and 8.9).
-constexpr int64_t kFewBytes = 2 << 20;
+// Up to so many units of a copy (in the worst case) the planning blocks copy by themselves, one after the other by 32 groups of threads, which spares the host a launch. By them /
+// by a second kernel, called eagerly, us (in brackets replayed from a graph, where a launch costs less than their copies): rows of one beam, none to copy 9.1 / 10.2 (9.2 / 9.3); 16 rows of four
+// beams, 48 units 11.9 / 10.8 (11.9 / 9.4); compaction of a cache of 70 pages, 105 units 9.3 / 10.3 (9.2 / 6.8), of 100 pages, 150 units 10.6 / 10.4 (10.5 / 6.8); 192 units, fork 14.4 / 11.1, 420,
+// compaction 15.0 / 11.0, 1000 of 1152 bytes 23.9 / 10.5.
+constexpr int64_t kFewUnits = 160;
 
 template <class Arguments>
 int launch_plan(void (*kernel)(const Arguments), const Arguments& arguments, const Plan& p, cudaStream_t stream) {
@@ -675,13 +678,6 @@ int fill_tensors(Copies* copies, const pages_call& c, const pages_tensor* tensor
   copies->units = int32_t(units);
   copies->page_rows = c.page_rows;
   return 0;
-}
-
-// Bytes of `most` copied pages.
-int64_t copied_bytes(const Copies& copies, int64_t most) {
-  int64_t each = 0;
-  for (int t = 0; t < copies.tensors; ++t) each += copies.tensor[t].page_bytes;
-  return each > 0 && most > INT64_MAX / each ? INT64_MAX : most * each;
 }
 
 int launch_copies(const Copies& copies, int64_t most, cudaStream_t stream) {
@@ -778,7 +774,7 @@ int launch_pages_fork(void* stream, const pages_fork_call* call) {
   p.ranks = reinterpret_cast<int32_t*>(workspace + layout.take(4 * call->children));
   p.copy_count = reinterpret_cast<int32_t*>(workspace);
   const int64_t entries = std::max(c.requests, call->children) * std::max<int64_t>(c.entries, 1);
-  const bool few = copied_bytes(copies, call->children) <= kFewBytes && entries <= kSmallTable;
+  const bool few = call->children * copies.units <= kFewUnits && entries <= kSmallTable;
   p.words = words_of(c);
   copies.plan = p;
   copies.forks = true;
@@ -816,7 +812,7 @@ int launch_pages_compact(void* stream, const pages_compact_call* call) {
   p.numbers = reinterpret_cast<int32_t*>(workspace + layout.take(4 * c.blocks));
   p.copy_count = reinterpret_cast<int32_t*>(workspace);
   copies.entries = table ? c.requests * c.entries : 0;
-  const bool few = copied_bytes(copies, c.blocks / 2) <= kFewBytes && copies.entries <= kSmallTable;
+  const bool few = c.blocks / 2 * copies.units <= kFewUnits && copies.entries <= kSmallTable;
   p.words = words_of(c);
   copies.plan = p;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -7,7 +7,7 @@ import torch
 
 from ascendflow_b200 import latent8, ops, pages
 from tests import latent8_reference as E
-from tests.test_gpu_pages import counted, forked, i32, same, state_of, tensor
+from tests.test_gpu_pages import compacted, counted, equal, forked, i32, same, state_of, tensor
 
 pytestmark = pytest.mark.gpu
 
@@ -99,3 +99,24 @@ def test_pages_behind_32_bits():
     assert places[used].tolist() == [3, 0, 1, 2, 4] and int((places >= 0).sum()) == 5
     assert table.tolist() == [[4, 2], [4, -1], [4, 3], [-1, -1]]
     assert torch.equal(cache[2], own[2]) and torch.equal(cache[4], own[3]) and not cache[:2].any() and ops.status()[0] == 0
+
+
+@pytest.mark.parametrize("units", [159, 160, 161, 162])
+def test_copies_by_the_plan_and_by_a_kernel_of_their_own(units):
+    """Calls on both sides of the number of units from which copies are the second kernel's."""
+    rng, generator = random.Random(units), torch.Generator(device="cuda").manual_seed(units)
+
+    def cache_of(blocks, rows):
+        return torch.randint(0, 256, (blocks, rows, 96), dtype=torch.uint8, device="cuda", generator=generator)
+
+    table, counts, lengths = state_of(rng, 30, 7, 400, 64)
+    caches, parents = [cache_of(400, 64)], [rng.randrange(-1, 30) for _ in range(units)]
+    expected = forked(caches, table, counts, parents, lengths, 64)
+    same(pages.fork(caches, tensor(table, 7), i32(counts), i32(parents), i32(lengths), page_rows=64), *expected[:2], 7)
+    assert equal(caches, expected[2])
+    table, counts, _ = state_of(rng, 40, 5, 2 * units, 64)
+    caches = [cache_of(2 * units, 3)]
+    expected = compacted(caches, table, counts)
+    got = pages.compact(caches, tensor(table, 5), i32(counts))
+    same(got[:2], *expected[:2], 5)
+    assert got[2].tolist() == expected[2] and equal(caches, expected[3]) and ops.status()[0] in (0, 3)
