@@ -348,8 +348,10 @@ __global__ void __launch_bounds__(kRowThreads) release_kernel(const __grid_const
   }
 }
 
-// Marks of all pages, eight words by a warp, where there are many (without / with: 700 K pages 39.3 / 29.1 us; 81 K 14.4 / 16.2; before listing went through shared memory).
-constexpr int kWordsPerWarp = 8, kManyPages = 1 << 18;
+// Marks of all pages, eight words by a warp, where there are many. Without / with, called eagerly, us (in brackets replayed from a graph), 256 requests with 256 to 10 K wishes: 80 K pages
+// 14.2-15.8 / 15.4-16.0 (12.6-14.3 / 12.0-13.7), 131 K 14.7-18.5 / 15.5-17.3 (12.9-16.6 / 12.0-15.7), 200 K 16.8-21.2 / 16.2-18.2 (15.1-19.6 / 12.2-16.7), 262 K 17.5-21.5 / 15.5-17.8, 700 K
+// 27.4-31.5 / 15.5-19.6.
+constexpr int kWordsPerWarp = 8, kManyPages = 1 << 17;
 __global__ void __launch_bounds__(kRowThreads) mark_kernel(const __grid_constant__ Plan p) {
   wait_for_predecessor();
   let_successor_start();
