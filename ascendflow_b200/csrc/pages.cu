@@ -314,10 +314,11 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 1) 
   }
 }
 
-// A large table: a block to each request in front and behind, the cluster between. (1024 requests of 2049 entries, 700 K pages: 192 us by the cluster alone, 24 so;
-// 128 requests of 129 entries 10.2 by the cluster, 64 of 513 13.4.)
+// A large table, or long rows: a block to each request in front and behind, the cluster between. By the cluster alone / so, called eagerly, us (in brackets replayed from a graph): 128 requests of
+// 129 entries 9.7 / 13.1 (9.6 / 10.1), 64 of 513 10.8 / 13.5 (10.4 / 10.5), 128 of 513 12.7 / 13.3 (12.3 / 11.3), 512 of 129 14.3 / 13.7, 1024 of 129 20.8 / 16.3; 1024 of 2049, 700 K pages 192 / 24. A warp goes
+// through a row alone: 16 rows of 1025 11.1 / 13.2, one of 2049 13.0 / 13.0, 4 of 8193 28.0 / 14.5, one of 32769 84 / 23.
 constexpr int kRowThreads = 256;
-constexpr int64_t kSmallTable = 1 << 16;
+constexpr int64_t kSmallTable = 1 << 16, kShortRow = 1 << 11;
 
 __global__ void __launch_bounds__(kRowThreads) copy_counts_kernel(const __grid_constant__ Plan p) {
   wait_for_predecessor();
@@ -725,7 +726,7 @@ int launch_pages_resize(void* stream, const pages_call* call) {
   const int64_t entries = call->requests * call->entries;
   p.words = words_of(*call);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (entries <= kSmallTable) return launch_plan(resize_kernel, p, p, s);
+  if (entries <= kSmallTable && call->entries <= kShortRow) return launch_plan(resize_kernel, p, p, s);
   if (call->counts_in != call->counts_out && call->blocks > 0) {
     const int64_t grid = std::min<int64_t>((call->blocks + kRowThreads * 8 - 1) / (kRowThreads * 8), latent::multiprocessors() * 4);
     if (const cudaError_t error = launch_overlapped(copy_counts_kernel, int(grid), kRowThreads, 0, s, p)) return int(error);

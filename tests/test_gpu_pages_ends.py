@@ -7,7 +7,7 @@ import torch
 
 from ascendflow_b200 import latent8, ops, pages
 from tests import latent8_reference as E
-from tests.test_gpu_pages import compacted, counted, equal, forked, i32, same, state_of, tensor
+from tests.test_gpu_pages import compacted, counted, equal, forked, i32, resized, same, state_of, tensor
 
 pytestmark = pytest.mark.gpu
 
@@ -120,3 +120,18 @@ def test_copies_by_the_plan_and_by_a_kernel_of_their_own(units):
     got = pages.compact(caches, tensor(table, 5), i32(counts))
     same(got[:2], *expected[:2], 5)
     assert got[2].tolist() == expected[2] and equal(caches, expected[3]) and ops.status()[0] in (0, 3)
+
+
+@pytest.mark.parametrize("requests,entries", [(1, 2048), (1, 2049), (5, 2049), (32, 2048), (2, 9001)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_long_rows_are_resized_by_blocks_of_their_own(requests, entries, in_place):
+    """Rows on both sides of the length from which a warp does not go through them alone."""
+    rng = random.Random(entries)
+    table, counts, lengths = state_of(rng, requests, entries, requests * entries + 9, 16)
+    for _ in range(2):
+        lengths = [min(max(length + rng.choice([-300, -1, 0, 1, 700, 40000]), 0), 16 * entries) for length in lengths]
+        given = tensor(table, entries), i32(counts)
+        got = pages.resize(*given, i32(lengths), page_rows=16, out=given if in_place else None)
+        table, counts = resized(table, counts, lengths, 16)
+        same(got, table, counts, entries)
+        assert ops.status()[0] == 0
