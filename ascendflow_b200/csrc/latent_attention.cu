@@ -1199,7 +1199,8 @@ namespace {
 // From so many chunks to a block on bfloat16 queries over rows in 8 bits go the other way round, whose start takes 6 us longer and whose chunks 8 per cent less. The other way
 // round / not, us, of 64 heads (chunks): one token of 8K rows (0.9) 23.8 / 18.4; 16 of them (14) 42.5 / 41.3; 64 at 2K (14) 48.9 / 47.1; 24 at 8K (21) 53.7 / 55.1;
 // 8 x 6 at 4K (21) 52.8 / 49.4; 32 at 8K (28) 63.4 / 66.7; 16 x 6 at 4K (42) 84.4 / 85.4; 64 at 8K (55) 102.9 / 117.0; 500 tokens of 16 heads at 8K (108) 165 / 175. (The
-// host knows the table's width only, which is the longest that requests may be: hence not from 24 on.)
+// host knows the table's width only, which is the longest that requests may be: hence not from 24 on. Short requests under a wide table pay for it: 8 at 2K under one for 128K 26.5 / 19.1, 32 at 2K
+// 33.9 / 28.5, 8 at 8K 34.0 / 27.7, 64 at 2K 48.7 / 47.4.)
 constexpr int64_t kTurnedChunks = 32;
 
 template <bool kHeld8>

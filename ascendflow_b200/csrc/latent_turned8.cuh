@@ -1,7 +1,7 @@
 // Attention of bfloat16 queries over rows in 8 bits (included by latent_attention.cu): nothing of 16 bits goes through shared memory but the weights.
 //
 // Scores are products of 8-bit numbers. A query is split in two of them, q = 2^e (q1 + q2 / 16): four significant bits each make up bfloat16's eight, so what is
-// left out is below 2^-22 of the row's greatest. Lanes 0-15 of a subpartition hold q1 of 16 rows, lanes 16-31 q2, so that one product M = 128, N = 64 of 8 bits takes both; the
+// left out is at most 2^-14 of 2^e, below 2^-21.8 of the row's greatest (448 2^e >= |q| > 224 2^e; e is not below -126, nor where the product with the scores' scale is no normal number). Lanes 0-15 of a subpartition hold q1 of 16 rows, lanes 16-31 q2, so that one product M = 128, N = 64 of 8 bits takes both; the
 // softmax warps add the two sums and multiply by the key's scale and 2^e.
 //
 // The accumulator is turned: O^T = X^T P^T, features over the lanes and rows over the columns. X^T in 16 bits is the A operand, which the tensor core takes from tensor

@@ -28,7 +28,8 @@ def rotary_append8(latent, rope, cache, scales, block_table, cu_seqlens_q, sequs
     Arguments as `latent.rotary_append`'s; `latent` and `rope` are bf16 or f16, W is a multiple of 16. A block's scale becomes the least power of two s with
     |v| <= 448 s for all its new rows, and not less than it was where rows in front of the new ones share the block: where it grows, their numbers are divided by the growth (exact
     but for subnormal ones). A block that begins with a new row forgets its scale. Rows are worked out in FP32 and rounded once, to nearest. Of f16 rows,
-    what is beyond 61440 is held as that (the next number would not fit f16). A row that is not finite makes its block's scale NaN.
+    what is beyond 61440 is held as that (the next number would not fit f16). A row that is not finite makes its block's scale NaN, also for the rows in front of it.
+    What a row does to its block stays when the row is given up (a draft that was not taken): scales do not shrink before a new row begins the block. With G = 1 rows do nothing to each other.
     The page of a row that is appended must not be shared with another request (`pages.fork` sees to that).
     """
     halves = _HALVES.get(layout)
@@ -44,8 +45,9 @@ def latent_attention8(q, cache, scales, block_table, cu_seqlens_q, seqused_kv, *
     """Causal attention of q `[T, H, W]` (bf16 or f16), W 512 or 576, over the paged `cache` and its `scales`: returns out `[T, H, 512]` in the type of q.
 
     As `latent.latent_attention` over a cache that holds the numbers times their scales (in the type of q: for f16 they have to be finite there, and scales up to 2^22).
-    In large calls bf16 queries are split into two numbers of 8 bits, which leaves out what is below 2^-22 of a row's greatest.
-    Rows behind a request's length may hold anything; a number NaN among the others is not looked for, a scale NaN makes what sees its rows NaN.
+    In large calls bf16 queries are split into two numbers of 8 bits, which leaves out what is below 2^-21.8 of a row's greatest. What is large is told by the table: its columns are
+    the longest that requests may be (or the cache's pages, where those are fewer), so short requests under a wide table are worked out in this way too and have other bits than under a narrow one.
+    Rows behind a request's length may hold anything; a number NaN among the others is not looked for, a scale NaN makes what sees its rows NaN and nothing else.
     """
     if out is None:
         require(isinstance(q, torch.Tensor) and q.dim() == 3, "q: expected a [T, H, W] Torch tensor")

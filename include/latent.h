@@ -99,7 +99,8 @@ int launch_latent_attention(void* stream, const latent_attention_call* call);
  * rounded once: numbers to the nearest e4m3 number after the division by the scale. A block's scale is the least power of two s with |v| <= 448 s for
  * all its new rows v, and, unless the first of these begins the block, not below the scale that the block has: where that grows, the numbers of the rows in front of the
  * new ones are divided by the growth and rounded to nearest. From half rows, values beyond 61440 (the greatest whose number times its scale half holds) are taken
- * as that. A row that is not finite makes its block's scale NaN. Values below 2^-126 count as zero. */
+ * as that. A row that is not finite makes its block's scale NaN, also for the rows in front of it. What a row has done to its block's scale and to the numbers in front of it stays when
+ * the row is given up (a shorter length in the next call), until a new row begins the block. Values below 2^-126 count as zero. */
 typedef struct {
   latent_append_call append; /* cache: e4m3 */
   uint8_t* scales;
@@ -108,8 +109,10 @@ typedef struct {
 int launch_latent_append8(void* stream, const latent_append8_call* call);
 
 /* Attention as launch_latent_attention over such a cache; its workspace is as large as that one's. Held values are taken as they are (in the type of q, which holds them exactly
- * where they are finite and normal numbers there; for half: scales up to 2^22). bfloat16 queries may be split into
- * two numbers of 8 bits, which leaves out what is below 2^-22 of a row's greatest (large calls). NaN among the numbers of rows that are seen is not looked for; scales that are NaN make what sees them NaN. */
+ * where they are finite and normal numbers there; for half: scales up to 2^22). In calls that are large if requests are as long as the table, bfloat16 queries are split into
+ * two numbers of 8 bits, which leaves out what is below 2^-21.8 of a row's greatest (of 2^-118 where that is less), and scores of rows whose scale is less than 2^-62 of another's of
+ * their 64 rows may count as zero: results have other bits than under a narrower table. NaN among the numbers of rows that are seen is not looked for. Scales that are NaN make what
+ * sees their rows NaN, and leave alone what does not. */
 typedef struct {
   latent_attention_call attention; /* cache: e4m3 */
   const uint8_t* scales;
