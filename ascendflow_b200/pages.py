@@ -7,7 +7,7 @@ table. Results are the same for the same inputs, whatever the timing: the free p
 
 The calls return new tables and counts; with `out=` they write given ones, `counts` in place if that is what is given (and the table too, for `resize` and `compact`).
 They launch on torch's current stream and never wait, so a step that includes them may be captured in a CUDA graph (an `out=` of the inputs
-makes every replay continue where the last one ended). Reports go to `ops.status()`: 3, request, entry where no free page was left (the entry stays empty, and what is appended
+makes every replay continue where the last one ended). Reports go to `ops.status()`: 3, request (`fork`: row of the new table), entry where no free page was left (the entry stays empty, and what is appended
 there is reported in turn); 1, request, length for a length behind the table. While a graph is traced they are
 `torch.ops.ascendflow_b200.pages_resize`, `pages_fork` and `pages_compact`.
 """

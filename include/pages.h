@@ -10,7 +10,7 @@
  * synchronise; 0 is success, -1 a call outside of what is stated here (nothing is enqueued), anything else the CUDA error code of the failed enqueue.
  * `workspace` (16-byte aligned, of the size that the functions of that name give): its contents matter to nobody between calls, but calls that may run at the same time need one each.
  *
- * `status`: SPARSE_MLA_STATUS_WORDS int32 words (sparse_mla.h), set to the first report if word 0 is zero: SPARSE_MLA_STATUS_NO_PAGE, request, entry where no free page was
+ * `status`: SPARSE_MLA_STATUS_WORDS int32 words (sparse_mla.h), set to the first report if word 0 is zero: SPARSE_MLA_STATUS_NO_PAGE, request (fork: row of table_out), entry where no free page was
  * left, whose entry stays empty; SPARSE_MLA_STATUS_BAD_PAGE, request, length for a length behind the table.
  */
 #ifndef ASCENDFLOW_B200_PAGES_H_
