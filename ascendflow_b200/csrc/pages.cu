@@ -653,11 +653,11 @@ struct Layout {
 };
 
 int words_of(const pages_call& c) { return int((c.blocks + 32 * kCluster - 1) / (32 * kCluster)); }
-// Up to so many units of a copy (in the worst case) the planning blocks copy by themselves, one after the other by 32 groups of threads, which spares the host a launch. By them /
+// Up to so many units of a copy (in the worst case), and rows of a fork's tables, the planning blocks work through by themselves, one after the other by 32 groups of threads, which spares the host a launch. By them /
 // by a second kernel, called eagerly, us (in brackets replayed from a graph, where a launch costs less than their copies): rows of one beam, none to copy 9.1 / 10.2 (9.2 / 9.3); 16 rows of four
 // beams, 48 units 11.9 / 10.8 (11.9 / 9.4); compaction of a cache of 70 pages, 105 units 9.3 / 10.3 (9.2 / 6.8), of 100 pages, 150 units 10.6 / 10.4 (10.5 / 6.8); 192 units, fork 14.4 / 11.1, 420,
-// compaction 15.0 / 11.0, 1000 of 1152 bytes 23.9 / 10.5.
-constexpr int64_t kFewUnits = 160;
+// compaction 15.0 / 11.0, 1000 of 1152 bytes 23.9 / 10.5. Rows alone, 32 of 32 requests 9.4 / 10.4, 64 of 64 11.6 / 10.7, 256 of 256 25.7 / 11.9, 2000 of 2000 141 / 18.6; 48 units, 16 of 512 24.2 / 10.8.
+constexpr int64_t kFewItems = 160;
 
 template <class Arguments>
 int launch_plan(void (*kernel)(const Arguments), const Arguments& arguments, const Plan& p, cudaStream_t stream) {
@@ -777,7 +777,7 @@ int launch_pages_fork(void* stream, const pages_fork_call* call) {
   p.ranks = reinterpret_cast<int32_t*>(workspace + layout.take(4 * call->children));
   p.copy_count = reinterpret_cast<int32_t*>(workspace);
   const int64_t entries = std::max(c.requests, call->children) * std::max<int64_t>(c.entries, 1);
-  const bool few = call->children * copies.units <= kFewUnits && entries <= kSmallTable;
+  const bool few = call->children * copies.units + call->children + c.requests <= kFewItems && entries <= kSmallTable;
   p.words = words_of(c);
   copies.plan = p;
   copies.forks = true;
@@ -815,7 +815,7 @@ int launch_pages_compact(void* stream, const pages_compact_call* call) {
   p.numbers = reinterpret_cast<int32_t*>(workspace + layout.take(4 * c.blocks));
   p.copy_count = reinterpret_cast<int32_t*>(workspace);
   copies.entries = table ? c.requests * c.entries : 0;
-  const bool few = c.blocks / 2 * copies.units <= kFewUnits && copies.entries <= kSmallTable;
+  const bool few = c.blocks / 2 * copies.units <= kFewItems && copies.entries <= kSmallTable;
   p.words = words_of(c);
   copies.plan = p;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);

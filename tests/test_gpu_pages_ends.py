@@ -101,6 +101,18 @@ def test_pages_behind_32_bits():
     assert torch.equal(cache[2], own[2]) and torch.equal(cache[4], own[3]) and not cache[:2].any() and ops.status()[0] == 0
 
 
+@pytest.mark.parametrize("requests,children", [(40, 40), (10, 60), (80, 80), (81, 80), (159, 1), (160, 1), (1, 159), (700, 3), (3, 700)])
+@pytest.mark.parametrize("tensors", [0, 2])
+def test_rows_by_the_plan_and_by_a_kernel_of_their_own(requests, children, tensors):
+    """Forks on both sides of the number of rows from which these are the second kernel's, with and without pages to copy."""
+    rng, generator = random.Random(requests), torch.Generator(device="cuda").manual_seed(children)
+    table, counts, lengths = state_of(rng, requests, 6, 6 * requests + 400, 64)
+    caches, parents = [torch.randint(0, 256, (len(counts), 64, 24), dtype=torch.uint8, device="cuda", generator=generator) for _ in range(tensors)], [rng.randrange(-1, requests) for _ in range(children)]
+    expected = forked(caches, table, counts, parents, lengths, 64)
+    same(pages.fork(caches, tensor(table, 6), i32(counts), i32(parents), i32(lengths), page_rows=64), *expected[:2], 6)
+    assert equal(caches, expected[2]) and ops.status()[0] in (0, 3)
+
+
 @pytest.mark.parametrize("units", [159, 160, 161, 162])
 def test_copies_by_the_plan_and_by_a_kernel_of_their_own(units):
     """Calls on both sides of the number of units from which copies are the second kernel's."""
